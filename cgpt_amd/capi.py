@@ -62,6 +62,11 @@ PROTOTYPES = {
                                                     _sz, _sz, _f, _i, _sz, _i, _i, _vp],
     "cgptx_flash_gqa_attention_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _f, _i,
                                            _sz, _i, _i, _vp],
+    "cgptx_layernorm_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _f, _i, _vp],
+    "cgptx_dropout_backward": [_vp, _vp, _sz, _f, _u64, _u64, _vp, _i, _i, _vp],
+    "cgptx_differential_attention_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz,
+                                              _f, _i, _sz, _i, _i, _vp],
+    "cgptx_differential_lambda_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _i, _vp],
     "cgptx_adamw_workspace_create": [ctypes.POINTER(_vp)],
     "cgptx_adamw_workspace_destroy": [_vp],
     "cgptx_adamw_step_many_async": [_vp, ctypes.POINTER(AdamWEntry), _sz, ctypes.POINTER(AdamWOptions), _u64, _vp],
@@ -78,6 +83,10 @@ PROTOTYPES = {
     "cgptx_linear_backward_weights_stacked": [_vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _i, _vp],
     "cgptx_embedding_forward": [_vp, _vp, _sz, _vp, _sz, _sz, _i, _vp],
     "cgptx_flash_gqa_attention_forward": [_vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _f, _i, _sz, _i, _vp],
+    "cgptx_layernorm_forward": [_vp, _vp, _vp, _vp, _sz, _sz, _f, _i, _vp],
+    "cgptx_dropout_forward": [_vp, _vp, _vp, _sz, _f, _u64, _u64, _vp, _i, _vp],
+    "cgptx_differential_attention_forward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _f, _i, _sz, _i, _vp],
+    "cgptx_differential_lambda_forward": [_vp, _vp, _vp, _vp, _vp, _f, _sz, _sz, _sz, _i, _vp],
     "cgptx_add": [_vp, _vp, _vp, _sz, _i, _vp],
     "cgptx_model_create": [ctypes.POINTER(_vp), ctypes.POINTER(ModelConfig), _sz, _sz, _u64],
     "cgptx_model_destroy": [_vp],

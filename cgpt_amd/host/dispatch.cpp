@@ -6,6 +6,7 @@
 // rmsnorm_backward 8.3 -> 5.9 (two launches), linear_backward 6.0 -> 3.6, attention 6.5 -> 3.2; a block of 128 tokens, forward and
 // backward, 212.6 -> 169.7.
 #include <Python.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -205,6 +206,20 @@ struct Call {
     float number(PyObject* o) {
         if (!need(ok && PyFloat_CheckExact(o) && std::fabs(PyFloat_AS_DOUBLE(o)) <= std::numeric_limits<float>::max())) return 0.0f;
         return static_cast<float>(PyFloat_AS_DOUBLE(o));
+    }
+    // Whether the tensors (null: none) are on the device that the library launches on.
+    bool here(std::initializer_list<const at::Tensor*> tensors) {
+        if (!ok) return false;
+        const auto current = c10::impl::VirtualGuardImpl(c10::DeviceType::CUDA).getDevice().index();
+        for (const at::Tensor* t : tensors) need(t == nullptr || t->device().index() == current);
+        return ok;
+    }
+    // One 64-bit number on the device, or null for None.
+    const at::Tensor* counter(int i) {
+        if (!ok || args[i] == Py_None) return nullptr;
+        const at::Tensor* t = other(i, at::ScalarType::Long, at::ScalarType::UInt64);
+        need(ok && t->numel() == 1);
+        return t;
     }
     float positive(int i) {
         const float value = number(args[i]);
@@ -503,6 +518,136 @@ PyObject* cut_cross_entropy_forward_backward(Call c) {  // loss, input_gradient,
     });
 }
 
+bool is_row(const at::Tensor* t, const at::Tensor* x) { return t == nullptr || (t->dim() == 1 && t->size(0) == x->size(1)); }
+
+PyObject* layernorm_forward(Call c) {  // output, input, weight, bias or None, epsilon, stream
+    const at::Tensor *y = c.tensor(0), *x = c.tensor(1), *w = c.tensor(2), *b = c.tensor(3, true);
+    const float epsilon = c.positive(4);
+    if (!c.need(c.ok && x->dim() == 2 && same(y, x) && is_row(w, x) && is_row(b, x)) || !c.here({y, x, w, b})) return none();
+    const auto stream = stream_of(c, 5);
+    return finish(c, [&] { return cgptx_layernorm_forward(data(y), data(x), data(w), data(b), at(x, 0), at(x, 1), epsilon, c.code, stream); });
+}
+
+PyObject* layernorm_backward(Call c) {  // grad_input, grad_weight, grad_bias or None, grad_output, input, weight, residual or None, epsilon, stream
+    const at::Tensor *dx = c.tensor(0), *dw = c.tensor(1), *db = c.tensor(2, true), *dy = c.tensor(3), *x = c.tensor(4), *w = c.tensor(5),
+                     *residual = c.tensor(6, true);
+    const float epsilon = c.positive(7);
+    if (!c.need(c.ok && x->dim() == 2 && same(x, dy) && same(x, dx) && (residual == nullptr || same(x, residual)) && is_row(w, x) &&
+                is_row(dw, x) && is_row(db, x)) ||
+        !c.here({dx, dw, db, dy, x, w, residual}))
+        return none();
+    const auto stream = stream_of(c, 8);
+    return finish(c, [&] {
+        return cgptx_layernorm_backward(data(dx), data(dw), data(db), data(dy), data(x), data(w), data(residual), at(x, 0), at(x, 1),
+                                        epsilon, c.code, stream);
+    });
+}
+
+float share(Call& c, int i) {
+    const float value = c.number(c.args[i]);
+    c.need(value >= 0.0f && value <= 1.0f);
+    return value;
+}
+
+PyObject* dropout_forward(Call c) {  // output, input, residual or None, probability, seed, offset, counter or None, stream
+    const at::Tensor *y = c.tensor(0), *x = c.tensor(1), *residual = c.tensor(2, true);
+    const float probability = share(c, 3);
+    const size_t seed = c.size(4), offset = c.size(5);
+    const at::Tensor* counter = c.counter(6);
+    if (!c.need(c.ok && same(x, y) && (residual == nullptr || same(x, residual))) || !c.here({y, x, residual, counter})) return none();
+    const auto stream = stream_of(c, 7);
+    return finish(c, [&] {
+        return cgptx_dropout_forward(data(y), data(x), data(residual), static_cast<size_t>(x->numel()), probability, seed, offset,
+                                     static_cast<const uint64_t*>(data(counter)), c.code, stream);
+    });
+}
+
+PyObject* dropout_backward(Call c) {  // grad_input, grad_output, probability, seed, offset, counter or None, accumulate, stream
+    const at::Tensor *dx = c.tensor(0), *dy = c.tensor(1);
+    const float probability = share(c, 2);
+    const size_t seed = c.size(3), offset = c.size(4);
+    const at::Tensor* counter = c.counter(5);
+    const int accumulate = c.flag(6);
+    if (!c.need(c.ok && same(dx, dy)) || !c.here({dx, dy, counter})) return none();
+    const auto stream = stream_of(c, 7);
+    return finish(c, [&] {
+        return cgptx_dropout_backward(data(dx), data(dy), static_cast<size_t>(dy->numel()), probability, seed, offset,
+                                      static_cast<const uint64_t*>(data(counter)), accumulate, c.code, stream);
+    });
+}
+
+bool differential(const Attention& a, const at::Tensor* lambdas, const at::Tensor* lse, const at::Tensor* q) {
+    return a.head_dim % 2 == 0 && lambdas->dim() == 1 && at(lambdas, 0) == a.query_heads &&
+           (lse == nullptr || (lse->dim() == 4 && lse->size(0) == 2 && lse->sizes().slice(1) == q->sizes().slice(0, 3)));
+}
+
+PyObject* differential_attention_forward(Call c) {  // output, second or None, logsumexp or None, query, key, value, lambdas, options, stream
+    const at::Tensor *o = c.tensor(0), *o2 = c.tensor(1, true), *q = c.tensor(3), *k = c.tensor(4), *v = c.tensor(5);
+    const at::Tensor *lse = c.args[2] != Py_None ? c.f32(2) : nullptr, *lambdas = c.f32(6);
+    if (!c.ok) return none();
+    const Attention a(c, c.args[7]);
+    if (!c.need(c.ok && a.fits(q, k, v) && same(o, q) && (o2 == nullptr || same(o2, q)) && differential(a, lambdas, lse, q)) ||
+        !c.here({o, o2, lse, q, k, v, lambdas}))
+        return none();
+    const auto stream = stream_of(c, 8);
+    return finish(c, [&] {
+        return cgptx_differential_attention_forward(data(o), data(o2), static_cast<float*>(data(lse)), data(q), data(k), data(v),
+                                                    static_cast<const float*>(data(lambdas)), at(q, 0), at(q, 1), at(k, 1), a.query_heads,
+                                                    a.kv_heads, a.head_dim, a.scale, a.causal, a.offset, c.code, stream);
+    });
+}
+
+PyObject* differential_attention_backward(Call c) {  // grad_query, grad_key, grad_value, grad_lambdas, grad_output, output, second, logsumexp, query, key, value, lambdas, options, accumulate, stream
+    const at::Tensor *dq = c.tensor(0), *dk = c.tensor(1), *dv = c.tensor(2), *d_o = c.tensor(4), *o = c.tensor(5), *o2 = c.tensor(6),
+                     *q = c.tensor(8), *k = c.tensor(9), *v = c.tensor(10);
+    const at::Tensor *dlambdas = c.f32(3), *lse = c.f32(7), *lambdas = c.f32(11);
+    if (!c.ok) return none();
+    const Attention a(c, c.args[12]);
+    const int accumulate = c.flag(13);
+    if (!c.need(c.ok && a.fits(q, k, v) && same(q, d_o) && same(q, dq) && same(q, o) && same(q, o2) && same(k, dk) && same(k, dv) &&
+                differential(a, lambdas, lse, q) && same(dlambdas, lambdas)) ||
+        !c.here({dq, dk, dv, dlambdas, d_o, o, o2, lse, q, k, v, lambdas}))
+        return none();
+    const auto stream = stream_of(c, 14);
+    return finish(c, [&] {
+        return cgptx_differential_attention_backward(data(dq), data(dk), data(dv), static_cast<float*>(data(dlambdas)), data(d_o), data(o),
+                                                     data(o2), static_cast<const float*>(data(lse)), data(q), data(k), data(v),
+                                                     static_cast<const float*>(data(lambdas)), at(q, 0), at(q, 1), at(k, 1), a.query_heads,
+                                                     a.kv_heads, a.head_dim, a.scale, a.causal, a.offset, accumulate, c.code, stream);
+    });
+}
+
+// Vectors [sets, width] of lambdas [heads].
+bool weighs(const at::Tensor* lambdas, std::initializer_list<const at::Tensor*> vectors) {
+    const at::Tensor* first = *vectors.begin();
+    if (lambdas->dim() != 1 || first->dim() != 2 || (first->size(0) != 1 && first->size(0) != lambdas->size(0))) return false;
+    for (const at::Tensor* v : vectors)
+        if (!same(first, v)) return false;
+    return true;
+}
+
+PyObject* differential_lambda_forward(Call c) {  // lambdas, query1, key1, query2, key2, initial, stream
+    const at::Tensor *q1 = c.tensor(1), *k1 = c.tensor(2), *q2 = c.tensor(3), *k2 = c.tensor(4), *lambdas = c.f32(0);
+    const float initial = c.number(c.args[5]);
+    if (!c.need(c.ok && weighs(lambdas, {q1, k1, q2, k2})) || !c.here({lambdas, q1, k1, q2, k2})) return none();
+    const auto stream = stream_of(c, 6);
+    return finish(c, [&] {
+        return cgptx_differential_lambda_forward(static_cast<float*>(data(lambdas)), data(q1), data(k1), data(q2), data(k2), initial, at(q1, 0),
+                                                 at(lambdas, 0), at(q1, 1), c.code, stream);
+    });
+}
+
+PyObject* differential_lambda_backward(Call c) {  // four gradients, grad_lambdas, query1, key1, query2, key2, stream
+    const at::Tensor *g1 = c.tensor(0), *g2 = c.tensor(1), *g3 = c.tensor(2), *g4 = c.tensor(3), *q1 = c.tensor(5), *k1 = c.tensor(6),
+                     *q2 = c.tensor(7), *k2 = c.tensor(8), *dlambdas = c.f32(4);
+    if (!c.need(c.ok && weighs(dlambdas, {q1, k1, q2, k2, g1, g2, g3, g4})) || !c.here({g1, g2, g3, g4, dlambdas, q1, k1, q2, k2})) return none();
+    const auto stream = stream_of(c, 9);
+    return finish(c, [&] {
+        return cgptx_differential_lambda_backward(data(g1), data(g2), data(g3), data(g4), static_cast<const float*>(data(dlambdas)), data(q1),
+                                                  data(k1), data(q2), data(k2), at(q1, 0), at(dlambdas, 0), at(q1, 1), c.code, stream);
+    });
+}
+
 // A tensor that refuses to say what it is makes the call one that is not taken.
 template <PyObject* (*Function)(Call), int COUNT>
 PyObject* operation(PyObject*, PyObject* const* args, Py_ssize_t count) {
@@ -537,6 +682,14 @@ PyMethodDef methods[] = {
     method<cross_entropy_forward_backward, 7>("cross_entropy_forward_backward"),
     method<cross_entropy_forward, 5>("cross_entropy_forward"),
     method<cut_cross_entropy_forward_backward, 10>("cut_cross_entropy_forward_backward"),
+    method<layernorm_forward, 6>("layernorm_forward"),
+    method<layernorm_backward, 9>("layernorm_backward"),
+    method<dropout_forward, 8>("dropout_forward"),
+    method<dropout_backward, 8>("dropout_backward"),
+    method<differential_attention_forward, 9>("differential_attention_forward"),
+    method<differential_attention_backward, 15>("differential_attention_backward"),
+    method<differential_lambda_forward, 7>("differential_lambda_forward"),
+    method<differential_lambda_backward, 10>("differential_lambda_backward"),
     {"tensors", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(call<tensors>)), METH_FASTCALL, "(dtype code, pointers) or None"},
     {"same_shape", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(call<same_shape>)), METH_FASTCALL, "whether all shapes are equal"},
     {"adamw_entries", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(call<adamw_entries>)), METH_FASTCALL, "fills an entry array"},

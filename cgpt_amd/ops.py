@@ -108,6 +108,14 @@ def _reject(name: str, *tensors):
     return (_code(present[0]), *(_ptr(t) for t in tensors))
 
 
+def _on_current_device(name: str, *tensors) -> None:
+    """The library launches on the current device and takes its working memory there."""
+    current = _current_device()
+    for t in tensors:
+        if t is not None and t.device.index != current:
+            raise ValueError(f"{name}: tensors must be on the current device")
+
+
 def _ids(name: str, ids: torch.Tensor, count: int) -> None:
     if ids is None or ids.device.type != "cuda" or ids.dtype not in (torch.int32, torch.uint32) or ids.numel() < count:
         raise ValueError(f"{name}: token ids must be a device uint32 buffer with at least token_count entries")
@@ -154,6 +162,18 @@ class EmbeddingBackwardOptions:  # include/ops/backward/embedding_backward.h:6-1
     block_size: int = 0
     bounds_check: bool = True
     accumulate_weight: bool = False
+
+
+@dataclasses.dataclass
+class DropoutOptions:
+    """Which mask (cgptx_dropout_forward in include/cgptx.h): of how many elements, from which key, from which counter value on. A
+    call uses up (count + 7) // 8 counter values. counter: device int64 tensor of one element, added to the offset when the call
+    runs."""
+
+    probability: float = 0.1
+    seed: int = 0
+    offset: int = 0
+    counter: Optional[torch.Tensor] = None
 
 
 @dataclasses.dataclass
@@ -430,6 +450,119 @@ def flash_gqa_attention_backward(grad_query, grad_key, grad_value, grad_output, 
         raise ValueError(f"{name}: gradient shapes must match their tensors")
     capi.call("cgptx_flash_gqa_attention_backward", dq, dk, dv, do, q, k, v, *sizes, options.attention_scale,
               int(options.causal), options.query_position_offset, int(accumulate_grads), code, _stream(stream))
+
+
+def layernorm_backward(grad_input, grad_weight, grad_bias, grad_output, input, weight, epsilon, stream=None, residual=None):
+    """Gradients of layernorm_forward; grad_bias may be None. residual ([rows, hidden]; may be grad_input) is added to grad_input: the
+    gradient that reaches the input past the norm."""
+    status = _native.layernorm_backward(grad_input, grad_weight, grad_bias, grad_output, input, weight, residual, epsilon, stream)
+    if status == 0:
+        return
+    if status:
+        capi.check(status)
+    name = "layernorm_backward"
+    if not (math.isfinite(epsilon) and epsilon > 0):
+        raise ValueError(f"{name}: epsilon must be finite and positive")
+    tensors = (grad_input, grad_weight, grad_bias, grad_output, input, weight, residual)
+    code, dx, dw, db, dy, x, w, res = _tensors(*tensors) or _reject(name, *tensors)
+    _on_current_device(name, *tensors)
+    if input.dim() != 2 or not _same_shape(input, grad_output, grad_input) or (residual is not None and not _same_shape(input, residual)):
+        raise ValueError(f"{name}: input, grad_output, grad_input and residual must have shape [rows, hidden]")
+    rows, hidden = input.shape
+    if any(t is not None and tuple(t.shape) != (hidden,) for t in (weight, grad_weight, grad_bias)):
+        raise ValueError(f"{name}: weight, grad_weight and grad_bias must have shape [hidden]")
+    capi.call("cgptx_layernorm_backward", dx, dw, db, dy, x, w, res, rows, hidden, epsilon, code, _stream(stream))
+
+
+def _dropout_check(name, options: DropoutOptions):
+    if not 0.0 <= options.probability <= 1.0:
+        raise ValueError(f"{name}: the probability must be between 0 and 1")
+    for value in (options.seed, options.offset):
+        if not 0 <= value < 2**64:
+            raise ValueError(f"{name}: seed and offset must be unsigned 64-bit numbers")
+    counter = options.counter
+    if counter is not None and (counter.device.type != "cuda" or counter.dtype not in (torch.int64, torch.uint64) or counter.numel() != 1):
+        raise ValueError(f"{name}: the counter must be a device int64 tensor of one element")
+
+
+def dropout_backward(grad_input, grad_output, stream=None, options: DropoutOptions = DropoutOptions(), accumulate: bool = False):
+    """grad_input = grad_output under the mask that dropout_forward had of the same options (added to grad_input with accumulate)."""
+    status = _native.dropout_backward(grad_input, grad_output, options.probability, options.seed, options.offset, options.counter,
+                                      accumulate, stream)
+    if status == 0:
+        return
+    if status:
+        capi.check(status)
+    name = "dropout_backward"
+    code, dx, dy = _tensors(grad_input, grad_output) or _reject(name, grad_input, grad_output)
+    _dropout_check(name, options)
+    _on_current_device(name, grad_input, grad_output, options.counter)
+    if not _same_shape(grad_input, grad_output):
+        raise ValueError(f"{name}: shape mismatch")
+    capi.call("cgptx_dropout_backward", dx, dy, grad_output.numel(), options.probability, options.seed, options.offset,
+              _ptr(options.counter), int(accumulate), code, _stream(stream))
+
+
+def _differential_check(name, q, k, v, lambdas, options):
+    sizes = _attention_check(name, q, k, v, options)
+    if options.head_dim % 2:
+        raise ValueError(f"{name}: head_dim must be even")
+    if lambdas.dtype != torch.float32 or tuple(lambdas.shape) != (options.num_query_heads,):
+        raise ValueError(f"{name}: lambdas must be a device F32 tensor with shape [query_heads]")
+    return sizes
+
+
+def differential_attention_backward(grad_query, grad_key, grad_value, grad_lambdas, grad_output, output, second, logsumexp, query, key,
+                                    value, lambdas, stream=None, options: FlashAttentionOptions = FlashAttentionOptions(),
+                                    accumulate_grads: bool = False):
+    """Gradients of differential_attention_forward, which leaves output, second and logsumexp; grad_lambdas F32 [query_heads]."""
+    status = _native.differential_attention_backward(grad_query, grad_key, grad_value, grad_lambdas, grad_output, output, second, logsumexp,
+                                                     query, key, value, lambdas, options, accumulate_grads, stream)
+    if status == 0:
+        return
+    if status:
+        capi.check(status)
+    name = "differential_attention_backward"
+    tensors = (grad_query, grad_key, grad_value, grad_output, output, second, query, key, value)
+    code, dq, dk, dv, do, o, o2, q, k, v = _tensors(*tensors) or _reject(name, *tensors)
+    _require_device(name, grad_lambdas, logsumexp, lambdas)
+    _on_current_device(name, *tensors, grad_lambdas, logsumexp, lambdas)
+    sizes = _differential_check(name, query, key, value, lambdas, options)
+    if not _same_shape(query, grad_output, grad_query, output, second) or not _same_shape(key, grad_key, grad_value):
+        raise ValueError(f"{name}: gradient shapes must match their tensors")
+    if logsumexp.dtype != torch.float32 or tuple(logsumexp.shape) != (2, *query.shape[:3]):
+        raise ValueError(f"{name}: invalid logsumexp")
+    if grad_lambdas.dtype != torch.float32 or not _same_shape(lambdas, grad_lambdas):
+        raise ValueError(f"{name}: grad_lambdas must match lambdas")
+    capi.call("cgptx_differential_attention_backward", dq, dk, dv, grad_lambdas.data_ptr(), do, o, o2, logsumexp.data_ptr(), q, k, v,
+              lambdas.data_ptr(), *sizes, options.attention_scale, int(options.causal), options.query_position_offset,
+              int(accumulate_grads), code, _stream(stream))
+
+
+def _lambda_check(name, lambdas, *vectors):
+    first = vectors[0]
+    if first.dim() != 2 or not _same_shape(*vectors):
+        raise ValueError(f"{name}: vectors must all have the shape [heads or 1, width]")
+    if lambdas.dtype != torch.float32 or lambdas.dim() != 1 or first.shape[0] not in (1, lambdas.shape[0]):
+        raise ValueError(f"{name}: lambdas must be F32 with shape [heads], the vectors one set for all heads or one for each")
+    return first.shape[0], lambdas.shape[0], first.shape[1]
+
+
+def differential_lambda_backward(grad_query1, grad_key1, grad_query2, grad_key2, grad_lambdas, query1, key1, query2, key2, stream=None):
+    """Gradients of differential_lambda_forward's vectors; a set that all heads share gets the sum over the heads."""
+    status = _native.differential_lambda_backward(grad_query1, grad_key1, grad_query2, grad_key2, grad_lambdas, query1, key1, query2, key2,
+                                                  stream)
+    if status == 0:
+        return
+    if status:
+        capi.check(status)
+    name = "differential_lambda_backward"
+    tensors = (grad_query1, grad_key1, grad_query2, grad_key2, query1, key1, query2, key2)
+    code, g1, g2, g3, g4, q1, k1, q2, k2 = _tensors(*tensors) or _reject(name, *tensors)
+    _require_device(name, grad_lambdas)
+    _on_current_device(name, *tensors, grad_lambdas)
+    sizes = _lambda_check(name, grad_lambdas, *tensors)
+    capi.call("cgptx_differential_lambda_backward", g1, g2, g3, g4, grad_lambdas.data_ptr(), q1, k1, q2, k2, *sizes, code, _stream(stream))
 
 
 # ------------------------------------------------------------------------------ AdamW
@@ -748,3 +881,84 @@ def add_tensors(output, a, b, stream=None):
     if not _same_shape(a, output, b):
         raise ValueError(f"{name}: shape mismatch")
     capi.call("cgptx_add", y, x1, x2, a.numel(), code, _stream(stream))
+
+
+def layernorm_forward(output, input, weight, bias, epsilon, stream=None):
+    """y = (x - mean) / sqrt(variance + epsilon) * weight + bias over the rows of [rows, hidden]; bias may be None."""
+    status = _native.layernorm_forward(output, input, weight, bias, epsilon, stream)
+    if status == 0:
+        return
+    if status:
+        capi.check(status)
+    name = "layernorm_forward"
+    if not (math.isfinite(epsilon) and epsilon > 0):
+        raise ValueError(f"{name}: epsilon must be finite and positive")
+    code, y, x, w, b = _tensors(output, input, weight, bias) or _reject(name, output, input, weight, bias)
+    _on_current_device(name, output, input, weight, bias)
+    if input.dim() != 2 or not _same_shape(output, input) or \
+            any(t is not None and tuple(t.shape) != (input.shape[1],) for t in (weight, bias)):
+        raise ValueError(f"{name}: incompatible shapes")
+    rows, hidden = input.shape
+    capi.call("cgptx_layernorm_forward", y, x, w, b, rows, hidden, epsilon, code, _stream(stream))
+
+
+def dropout_forward(output, input, residual=None, stream=None, options: DropoutOptions = DropoutOptions()):
+    """output = residual + input under a mask that is made of the options alone and never stored (include/cgptx.h); residual may be None,
+    output may be input or residual."""
+    status = _native.dropout_forward(output, input, residual, options.probability, options.seed, options.offset, options.counter, stream)
+    if status == 0:
+        return
+    if status:
+        capi.check(status)
+    name = "dropout_forward"
+    code, y, x, res = _tensors(output, input, residual) or _reject(name, output, input, residual)
+    _dropout_check(name, options)
+    _on_current_device(name, output, input, residual, options.counter)
+    if not _same_shape(input, output) or (residual is not None and not _same_shape(input, residual)):
+        raise ValueError(f"{name}: shape mismatch")
+    capi.call("cgptx_dropout_forward", y, x, res, input.numel(), options.probability, options.seed, options.offset, _ptr(options.counter),
+              code, _stream(stream))
+
+
+def differential_attention_forward(output, second, logsumexp, query, key, value, lambdas, stream=None,
+                                   options: FlashAttentionOptions = FlashAttentionOptions()):
+    """output = softmax(s q1 k1') v - lambda softmax(s q2 k2') v per query head: query and key [batch, sequence, heads, head_dim] hold the
+    two maps' halves side by side, value is head_dim wide, lambdas F32 [query_heads], s = 1/sqrt(head_dim/2) unless given. second (like
+    output) = softmax(s q2 k2') v and logsumexp F32 [2, batch, query sequence, query heads] are what the backward pass needs; None where it
+    is not run."""
+    status = _native.differential_attention_forward(output, second, logsumexp, query, key, value, lambdas, options, stream)
+    if status == 0:
+        return
+    if status:
+        capi.check(status)
+    name = "differential_attention_forward"
+    tensors = (output, second, query, key, value)
+    code, o, o2, q, k, v = _tensors(*tensors) or _reject(name, *tensors)
+    _require_device(name, lambdas)
+    if logsumexp is not None:
+        _require_device(name, logsumexp)
+    _on_current_device(name, *tensors, logsumexp, lambdas)
+    sizes = _differential_check(name, query, key, value, lambdas, options)
+    if not _same_shape(output, query) or (second is not None and not _same_shape(second, query)):
+        raise ValueError(f"{name}: output and second must match query")
+    if logsumexp is not None and (logsumexp.dtype != torch.float32 or tuple(logsumexp.shape) != (2, *query.shape[:3])):
+        raise ValueError(f"{name}: invalid logsumexp tensor")
+    capi.call("cgptx_differential_attention_forward", o, o2, _ptr(logsumexp), q, k, v, lambdas.data_ptr(), *sizes, options.attention_scale,
+              int(options.causal), options.query_position_offset, code, _stream(stream))
+
+
+def differential_lambda_forward(lambdas, query1, key1, query2, key2, initial, stream=None):
+    """lambdas[h] = exp(q1.k1) - exp(q2.k2) + initial, F32 [heads], from learned vectors [heads or 1, width] (1: all heads share them)."""
+    status = _native.differential_lambda_forward(lambdas, query1, key1, query2, key2, initial, stream)
+    if status == 0:
+        return
+    if status:
+        capi.check(status)
+    name = "differential_lambda_forward"
+    code, q1, k1, q2, k2 = _tensors(query1, key1, query2, key2) or _reject(name, query1, key1, query2, key2)
+    _require_device(name, lambdas)
+    _on_current_device(name, lambdas, query1, key1, query2, key2)
+    sizes = _lambda_check(name, lambdas, query1, key1, query2, key2)
+    if not math.isfinite(initial):
+        raise ValueError(f"{name}: the initial value must be finite")
+    capi.call("cgptx_differential_lambda_forward", lambdas.data_ptr(), q1, k1, q2, k2, initial, *sizes, code, _stream(stream))

@@ -186,6 +186,47 @@ int cgptx_flash_gqa_attention_backward(
     size_t query_position_offset, int accumulate_grads, int dtype,
     cgptx_stream stream);
 
+/* Layer norm's gradient (no counterpart in the reference, whose models have RMS norms only; the manner is
+ * rmsnorm_backward's). x, dy, dx, residual: [rows, hidden]; weight, grad_weight, grad_bias: [hidden]; all of `dtype`.
+ * With xh = (x - mean)/sqrt(mean((x - mean)^2) + eps) and g = dy*w:
+ * dx = (g - mean(g) - xh*mean(g*xh))/sqrt(...) + residual, grad_weight = sum_rows dy*xh, grad_bias = sum_rows dy.
+ * residual is the gradient that reaches x past the norm; it may be NULL and may be grad_input. grad_bias may be NULL.
+ * Outputs are overwritten. */
+int cgptx_layernorm_backward(void* grad_input, void* grad_weight, void* grad_bias,
+                             const void* grad_output, const void* input,
+                             const void* weight, const void* residual, size_t rows,
+                             size_t hidden, float epsilon, int dtype,
+                             cgptx_stream stream);
+
+/* Dropout's gradient with the mask of the forward call of the same probability, seed, offset, counter and count (see
+ * cgptx_dropout_forward): grad_input = grad_output*mask, added to what grad_input holds with `accumulate`.
+ * grad_input may be grad_output (without accumulate). */
+int cgptx_dropout_backward(void* grad_input, const void* grad_output, size_t count,
+                           float probability, uint64_t seed, uint64_t offset,
+                           const uint64_t* counter, int accumulate, int dtype,
+                           cgptx_stream stream);
+
+/* Gradients of differential attention (see cgptx_differential_attention_forward, which leaves output, second and
+ * logsumexp). grad_lambda: fp32 [query_heads]. accumulate_grads adds to all four. The workgroups' parts of every sum meet
+ * in an order that the sizes fix: results do not depend on scheduling. */
+int cgptx_differential_attention_backward(
+    void* grad_query, void* grad_key, void* grad_value, float* grad_lambda,
+    const void* grad_output, const void* output, const void* second,
+    const float* logsumexp, const void* query, const void* key, const void* value,
+    const float* lambda, size_t batch, size_t query_sequence, size_t kv_sequence,
+    size_t query_heads, size_t kv_heads, size_t head_dim, float attention_scale,
+    int causal, size_t query_position_offset, int accumulate_grads, int dtype,
+    cgptx_stream stream);
+
+/* Gradients of differential_lambda's vectors from grad_lambda (fp32 [heads]), in their shapes and dtype; one set for all
+ * heads gets the sum over the heads. */
+int cgptx_differential_lambda_backward(void* grad_query1, void* grad_key1,
+                                       void* grad_query2, void* grad_key2,
+                                       const float* grad_lambda, const void* query1,
+                                       const void* key1, const void* query2,
+                                       const void* key2, size_t sets, size_t heads,
+                                       size_t width, int dtype, cgptx_stream stream);
+
 /* ------------------------------------------------------------------- AdamW */
 
 /* AdamWOptions — include/optim/adamw.h:12-27. */
@@ -321,6 +362,45 @@ int cgptx_flash_gqa_attention_forward(
     const void* value, size_t batch, size_t query_sequence, size_t kv_sequence,
     size_t query_heads, size_t kv_heads, size_t head_dim, float attention_scale,
     int causal, size_t query_position_offset, int dtype, cgptx_stream stream);
+
+/* Layer norm: y = (x - mean(x))/sqrt(mean((x - mean)^2) + eps)*w + b over rows of `hidden` values; bias may be NULL.
+ * No counterpart in the reference (RMS norms only). */
+int cgptx_layernorm_forward(void* output, const void* input, const void* weight,
+                            const void* bias, size_t rows, size_t hidden,
+                            float epsilon, int dtype, cgptx_stream stream);
+
+/* Dropout onto a residual stream: output = residual + input*mask, mask = 0 with the given probability and the inverse of
+ * the share kept otherwise. No counterpart in the reference. residual may be NULL; output may be input or residual.
+ * The mask is never stored. Elements 8j .. 8j + 7 take the eight 16-bit numbers (low halves first) of Philox 4x32-10
+ * with key `seed` at counter offset + j (+ *counter, read on the device when the call runs, where counter is not NULL: a
+ * replayed graph draws new masks as a program moves it on); an element is dropped where its number is below
+ * round(65536*probability). A call uses up (count + 7)/8 counter values: the next one's offset starts behind them.
+ * 0 <= probability <= 1, in steps of 2^-16; count 0 does nothing. */
+int cgptx_dropout_forward(void* output, const void* input, const void* residual,
+                          size_t count, float probability, uint64_t seed,
+                          uint64_t offset, const uint64_t* counter, int dtype,
+                          cgptx_stream stream);
+
+/* Differential attention (no counterpart in the reference; tensors, options and checks are flash_gqa_attention's). A head's
+ * query and key are two halves of head_dim/2, values are head_dim wide:
+ *   output = softmax(s q1 k1') v - lambda[head] softmax(s q2 k2') v.
+ * head_dim: even, at most 128; attention_scale <= 0 selects s = 1/sqrt(head_dim/2); lambda: fp32 [query_heads], on the
+ * device. For the backward pass: second [batch, query_sequence, query_heads, head_dim] = softmax(s q2 k2') v, logsumexp
+ * fp32 [2, batch, query_sequence, query_heads] of both maps; either may be NULL. */
+int cgptx_differential_attention_forward(
+    void* output, void* second, float* logsumexp, const void* query,
+    const void* key, const void* value, const float* lambda, size_t batch,
+    size_t query_sequence, size_t kv_sequence, size_t query_heads,
+    size_t kv_heads, size_t head_dim, float attention_scale, int causal,
+    size_t query_position_offset, int dtype, cgptx_stream stream);
+
+/* The weights of differential attention's second maps: lambda[h] = exp(q1.k1) - exp(q2.k2) + initial, fp32 [heads], from
+ * learned vectors [sets, width] of `dtype`; sets = heads, or 1: one set for all heads. */
+int cgptx_differential_lambda_forward(float* lambda, const void* query1,
+                                      const void* key1, const void* query2,
+                                      const void* key2, float initial, size_t sets,
+                                      size_t heads, size_t width, int dtype,
+                                      cgptx_stream stream);
 
 /* Residual helpers used by the block (src/core/transformer_block.cu:134-144, 242-248):
  * out = a + b, and out += b, elementwise over `count` values. */
