@@ -36,11 +36,11 @@ DEVICE_FLAGS = [
 ]
 
 
-# Per-file additions. attention.hip: MFMA results in vector registers (the softmax arithmetic reads them in
+# Per-file additions. The attention kernels: MFMA results in vector registers (the softmax arithmetic reads them in
 # place). The option belongs to the compiler's backend, not to its documented interface: it is probed once and
 # left out, with a warning, when this hipcc does not know it (the kernels are correct either way, the
 # accumulators are then copied between the two register files).
-FILE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+FILE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("attention.hip", "differential_attention_mfma.hip")}
 _probed_flags: dict[tuple[str, ...], bool] = {}
 
 

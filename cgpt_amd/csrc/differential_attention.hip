@@ -12,12 +12,14 @@
 // dlambda cancels over rows and keys, and it is fp32: the dQ pass corrects the delta2 that it takes from the rounded O2 by
 // rowsum(dS2), which is what that rounding left (the rows of P2 sum to one).
 //
-// One wavefront per output row, fp32 arithmetic, lane l holding elements l and l + 64 of the head. No atomics: every row has one
+// This file holds the entries and the kernels that take every call: fp32 storage, head widths that are not multiples of 16, tensors off
+// 16-byte boundaries. One wavefront per output row, fp32 arithmetic, lane l holding elements l and l + 64 of the head. No atomics: every row has one
 // owner that adds its terms in a fixed order.
-#include "common.hpp"
+#include "differential_attention.hpp"
 
+#include <algorithm>
 #include <cmath>
-#include <limits>
+#include <initializer_list>
 
 namespace cgptx {
 namespace {
@@ -25,20 +27,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kScalarWaves = kThreads / kWave;
 
-struct Params {
-    void *out, *second;  // O and O2 (which may be null)
-    float* lse_out;      // [2][batch, qs, hq], or null
-    void *dq, *dk, *dv;
-    float* dlambda;
-    const void *q, *k, *v, *dout, *o, *o2;
-    const float *lambda, *lse;
-    float* delta;           // [2][batch, qs, hq]
-    float* lambda_partial;  // [hq][parts]
-    int batch, qs, ks, hq, hkv, d;
-    float scale;
-    int causal, offset, accumulate;
-    long rows() const { return static_cast<long>(batch) * qs * hq; }
-};
+using Params = DifferentialArgs;
 
 template <typename T>
 struct RowPair {
@@ -303,10 +292,18 @@ Params make_params(const Shape& s, const void* q, const void* k, const void* v, 
     p.scale = s.scale > 0.0f ? s.scale : 1.0f / std::sqrt(static_cast<float>(s.d / 2));
     p.causal = s.causal ? 1 : 0;
     p.offset = s.causal ? static_cast<int>(s.offset) : 0;
+    p.dtype = s.dtype;
     return p;
 }
 
 unsigned int scalar_blocks(std::size_t rows) { return static_cast<unsigned int>((rows + kScalarWaves - 1) / kScalarWaves); }
+
+// The matrix kernels' calls; everything else runs on the scalar ones.
+bool on_matrix_cores(const Params& p, std::initializer_list<const void*> tensors) {
+    for (const void* t : tensors)
+        if (!is_aligned16(t)) return false;  // an absent one is
+    return differential_mfma_takes(p);
+}
 
 int validate_lambda(const char* name, std::size_t sets, std::size_t heads, std::size_t width, int dtype) {
     const std::string n(name);
@@ -319,6 +316,14 @@ int validate_lambda(const char* name, std::size_t sets, std::size_t heads, std::
 }
 
 }  // namespace
+
+int differential_dlambda(const DifferentialArgs& a, long parts, hipStream_t stream) {
+    hipLaunchKernelGGL(differential_dlambda_kernel, dim3(static_cast<unsigned int>(a.hq)), dim3(kLambdaThreads), 0, stream, a.dlambda,
+                       a.lambda_partial, parts, a.accumulate);
+    CGPTX_LAUNCH_CHECK();
+    return CGPTX_OK;
+}
+
 }  // namespace cgptx
 
 extern "C" int cgptx_differential_lambda_forward(float* lambda, const void* query1, const void* key1, const void* query2,
@@ -378,6 +383,7 @@ extern "C" int cgptx_differential_attention_forward(void* output, void* second, 
     p.out = output;
     p.second = second;
     p.lse_out = logsumexp;
+    if (on_matrix_cores(p, {output, second, query, key, value})) return differential_mfma_forward(p, static_cast<hipStream_t>(stream));
     return dispatch_dtype(dtype, [&]<typename T>() -> int {
         hipLaunchKernelGGL((differential_forward_scalar_kernel<T>), dim3(scalar_blocks(batch * query_sequence * query_heads)),
                            dim3(kThreads), 0, static_cast<hipStream_t>(stream), p);
@@ -415,6 +421,10 @@ extern "C" int cgptx_differential_attention_backward(void* grad_query, void* gra
     p.accumulate = accumulate_grads != 0;
     const std::size_t rows = batch * query_sequence * query_heads;
     void* mem = nullptr;
+    if (on_matrix_cores(p, {grad_query, grad_key, grad_value, grad_output, output, second, query, key, value})) {
+        if (int st = scratch(stream, differential_mfma_scratch(p), &mem)) return st;
+        return differential_mfma_backward(p, mem, stream);
+    }
     if (int st = scratch(stream, 3 * rows * sizeof(float), &mem)) return st;
     p.delta = static_cast<float*>(mem);
     p.lambda_partial = p.delta + 2 * rows;
@@ -424,9 +434,6 @@ extern "C" int cgptx_differential_attention_backward(void* grad_query, void* gra
         hipLaunchKernelGGL((differential_dkv_scalar_kernel<T>), dim3(scalar_blocks(batch * kv_sequence * kv_heads)), dim3(kThreads), 0,
                            stream, p);
         CGPTX_LAUNCH_CHECK();
-        hipLaunchKernelGGL(differential_dlambda_kernel, dim3(static_cast<unsigned int>(query_heads)), dim3(kLambdaThreads), 0, stream,
-                           grad_lambda, p.lambda_partial, static_cast<long>(batch * query_sequence), p.accumulate);
-        CGPTX_LAUNCH_CHECK();
-        return CGPTX_OK;
+        return differential_dlambda(p, static_cast<long>(batch * query_sequence), stream);
     });
 }

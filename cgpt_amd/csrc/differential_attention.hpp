@@ -1,0 +1,34 @@
+// What the kernels of differential attention share: the call, and the entries of the 16-bit matrix-core kernels.
+#pragma once
+
+#include "common.hpp"
+
+namespace cgptx {
+
+struct DifferentialArgs {
+    void *out, *second;  // O and O2 (which may be null)
+    float* lse_out;      // [2][batch, qs, hq], or null
+    void *dq, *dk, *dv;
+    float* dlambda;
+    const void *q, *k, *v, *dout, *o, *o2;
+    const float *lambda, *lse;
+    float* delta;           // scalar kernels [2][batch, qs, hq]: delta1, delta2; matrix kernels [4]: those behind both LSE·log2 e
+    float* lambda_partial;  // [hq][parts]: what a head's dlambda is the sum of
+    int batch, qs, ks, hq, hkv, d;
+    float scale;
+    int causal, offset, accumulate;
+    int dtype;
+};
+
+// Whether the 16-bit matrix kernels serve a call's types and sizes: halves of a head in multiples of 8 (128-bit chunks of a row), and
+// 64 rows of a tensor within 1 GiB, which their 32-bit offsets within a tile reach. Their tensors lie on 16-byte boundaries.
+bool differential_mfma_takes(const DifferentialArgs& args);
+int differential_mfma_forward(const DifferentialArgs& args, hipStream_t stream);
+// Bytes behind args.delta that a backward call works in; it sets delta and lambda_partial in them itself. *parts: of args.lambda_partial.
+std::size_t differential_mfma_scratch(const DifferentialArgs& args);
+int differential_mfma_backward(DifferentialArgs args, void* memory, hipStream_t stream);
+
+// dlambda from its parts.
+int differential_dlambda(const DifferentialArgs& args, long parts, hipStream_t stream);
+
+}  // namespace cgptx

@@ -1,0 +1,784 @@
+// Differential attention on the matrix cores, 16-bit storage (formulas: differential_attention.hip; operand layouts and the
+// streaming of tiles: attention.hip, attention_tiles.hpp).
+//
+// A head's row of q or k is kept in LDS and registers as two halves of W/2 columns, each padded with zeros from D/2: the score
+// tile of a map is the product over its half, and both maps' score gradients meet the other operand's halves in one accumulator
+// of width W. So the tiles, fragments and register counts are those of plain attention with heads of W, and what the maps add
+// is a second set of exponentials and, in the forward pass, a second product with v (the maps' sums are known only at its end).
+//
+//   forward : block = 128 queries of one (batch, q-head), wave = 32 queries; streams 64-key K/V tiles; per tile and map Sᵀ = K·Qᵀ
+//             and its softmax, then Oᵀ_i += Vᵀ·Pᵀ_i for both maps from the same fragments of V.
+//   dQ      : same shape; Sᵀ_i = K_i·Qᵀ_i, Gᵀ = V·dOᵀ, dQᵀ_i += Kᵀ_i·dSᵀ_i. Leaves LSE·log2 e and delta of both maps for the
+//             dK/dV pass, and dlambda's parts.
+//   dK/dV   : block = 128 keys of one (batch, kv-head), wave = 32 keys; streams 64-query Q/dO tiles of every q-head of the group.
+#include "attention_tiles.hpp"
+#include "differential_attention.hpp"
+
+#include <algorithm>
+
+namespace cgptx {
+namespace {
+
+// Rows of a [.., sequence, heads, d] tensor from one (batch, head) on, streamed in 64-row tiles. A tile's buffer starts at its first
+// row, so that 32 bits hold every offset in it however long the sequence is; rows past the end and padding columns are zeros.
+struct RowStream {
+    const char* base;
+    long bytes;     // from base to the end of the last row's part that belongs to it
+    int row_bytes;  // between consecutive sequence positions
+    int voffset;    // of a lane's 16 bytes in the first load of a tile
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t at(int row0) const {
+        const long skipped = static_cast<long>(row0) * row_bytes;
+        const long left = min(bytes - skipped, 1l << 30);
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + skipped), 0, static_cast<int>(left), 0x00020000);
+    }
+};
+// Column of the tensor's row that padded column `c` (a multiple of 8) of a tile holds, or -1. HALVES: two halves of W/2 (q, k).
+template <int W, bool HALVES>
+__device__ __forceinline__ int source_column(int c, int d) {
+    if constexpr (HALVES) {
+        const int half = c / (W / 2), within = c % (W / 2);
+        return within < d / 2 ? half * (d / 2) + within : -1;
+    } else {
+        return c < d ? c : -1;
+    }
+}
+template <typename T, int W, bool HALVES>
+__device__ __forceinline__ RowStream make_stream(const void* tensor, long offset, long row_stride, int rows, int d, int wave, long last_row) {
+    constexpr int kChunks = W / 8, kRowsPerLoad = 64 / kChunks;
+    const int lane = threadIdx.x & 63;
+    RowStream s;
+    s.base = static_cast<const char*>(tensor) + offset * static_cast<long>(sizeof(T));
+    s.row_bytes = static_cast<int>(row_stride * sizeof(T));
+    s.bytes = ((rows - 1) * row_stride + last_row) * static_cast<long>(sizeof(T));
+    const int r = wave * kRowsPerLoad + lane / kChunks;
+    const int column = source_column<W, HALVES>(((lane % kChunks) ^ swizzle<W>(r)) * 8, d);
+    s.voffset = column >= 0 ? r * s.row_bytes + column * static_cast<int>(sizeof(T)) : (1 << 30);
+    return s;
+}
+template <typename T, int W>
+__device__ __forceinline__ void stream_rows(const RowStream& s, int row0, T* tile, int wave) {
+    constexpr int kRowsPerLoad = 64 / (W / 8), kLoads = kStream / (4 * kRowsPerLoad);
+    const __amdgpu_buffer_rsrc_t rsrc = s.at(row0);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_ptr)(tile + (i * 4 + wave) * kRowsPerLoad * W), 16, s.voffset,
+                                                 i * 4 * kRowsPerLoad * s.row_bytes, 0, 0);
+}
+
+// Element offsets in LDS of a lane's fragments of a tile that starts at element `tile` (a multiple of 512). The offsets of a tile differ by
+// bits that the swizzle only flips, so one register per kind of read stands for all of them: row-wise ones of step s, and
+// transposed ones of column block t, whose second read (see wide_transposed_offset) lies eight rows further with bit 4 flipped.
+template <int W>
+struct TileOffsets {
+    int direct, transposed;
+    __device__ __forceinline__ TileOffsets(int lane) : direct(wide_direct_offset<W>(lane, 0)), transposed(wide_transposed_offset<W>(lane, 0, 0)) {}
+    __device__ __forceinline__ TileOffsets at(int tile) const {
+        TileOffsets o = *this;
+        o.direct += tile;
+        o.transposed += tile;
+        asm volatile("" : "+v"(o.direct), "+v"(o.transposed));  // derived anew for each tile: no registers for all of them
+        return o;
+    }
+    template <typename T>
+    __device__ __forceinline__ typename Mma<T>::frag row(const T* lds, int block, int step) const {
+        return *reinterpret_cast<const typename Mma<T>::frag*>(lds + block * W + (direct ^ (16 * step)));
+    }
+    template <typename T>
+    __device__ __forceinline__ typename Mma<T>::frag columns(const T* lds, int block, int t) const {
+        return wide_transposed_frag<T>(lds + block * W, transposed ^ (32 * t), (transposed ^ (32 * t) ^ 16) + 8 * W);
+    }
+};
+
+// The operand that stays in registers, from global memory: lane -> row lane%32, padded columns 16*step + 8*(lane/32) .. + 7.
+template <typename T, int W, bool HALVES>
+__device__ __forceinline__ typename Mma<T>::frag row_frag(const T* row, bool live, int step, int d) {
+    using frag = typename Mma<T>::frag;
+    const int column = source_column<W, HALVES>(step * 16 + ((threadIdx.x & 63) >> 5) * 8, d);
+    if (live && column >= 0) return *reinterpret_cast<const frag*>(row + column);
+    return frag(static_cast<T>(0.0f));
+}
+
+// Stores a wavefront's transposed accumulators (lane = row, registers = padded columns) times a factor, four elements at a time.
+// value(t, g, e) is element e of quad g of column block t.
+template <typename T, int W, bool HALVES, typename Value>
+__device__ __forceinline__ void store_columns(T* row, int d, bool accumulate, Value&& value) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int t = 0; t < W / 32; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = t * 32 + g * 8, column = source_column<W, HALVES>(c, d);
+            if (column < 0) continue;
+            T* to = row + column + (lane >> 5) * 4;
+            vec_t<float, 4> v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = value(t, 4 * g + e);
+            if (accumulate) v += vec_to_f32<T, 4>(load_vec<T, 4>(to));
+            store_vec<T, 4>(to, vec_from_f32<T, 4>(v));
+        }
+}
+
+// Whether a 64-row tile holds an Inf or a NaN (the same answer in all lanes): the largest exponent and fraction of any sign.
+template <typename T, int W>
+__device__ __forceinline__ bool not_finite(const T* tile) {
+    using halves = vec_t<unsigned short, 8>;
+    constexpr unsigned short kInfinite = __is_same(T, f16_t) ? 0x7C00 : 0x7F80;
+    halves top(0);
+#pragma unroll
+    for (int i = 0; i < W / 8; ++i) {
+        const halves v = *reinterpret_cast<const halves*>(tile + (i * kWave + (threadIdx.x & 63)) * 8);
+        top = __builtin_elementwise_max(top, v & static_cast<unsigned short>(0x7FFF));
+    }
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) any |= top[e] >= kInfinite;
+    return __any(any);
+}
+// A hidden key's probability is 0, but 0 x Inf is NaN in the matrix instruction: a tile on the causal diagonal (at most two of a
+// wavefront's) that is not finite is left out of the products and added key by key behind the walk, by the lanes that see the key.
+struct LeftOut {
+    int first, tiles = 0;  // first tile with a key that a row of the wavefront does not see; bits of those from there on
+    __device__ __forceinline__ LeftOut(const DifferentialArgs& p, int wave_first_q)
+        : first(p.causal ? (p.offset + wave_first_q + 1) / kStream : 1 << 30) {}
+    // Whether tile j is one of them (the wavefront's causal mask allows it and the tile's values are not finite).
+    template <typename T, int W>
+    __device__ __forceinline__ bool out(int j, const T* tile) {
+        if (j < first || !not_finite<T, W>(tile)) return false;
+        tiles |= 1 << (j - first);
+        return true;
+    }
+    template <typename Use>
+    __device__ __forceinline__ void each_key(int ks, Use&& use) const {
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+            if ((tiles >> i & 1) == 0) continue;
+#pragma unroll 1
+            for (int key = (first + i) * kStream; key < min(ks, (first + i + 1) * kStream); ++key) use(key);
+        }
+    }
+};
+// The accumulators in the lane's own memory, where code that runs once in a blue moon takes no registers from the walk.
+template <int COUNT>
+struct Parked {
+    volatile float values[COUNT * 16];
+    __device__ __forceinline__ void put(int t, const acc_t& sums) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) values[t * 16 + e] = sums[e];
+    }
+    __device__ __forceinline__ void get(int t, acc_t& sums) const {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sums[e] = values[t * 16 + e];
+    }
+};
+// Product of columns from .. from + count - 1 of two rows.
+template <typename T>
+__device__ __noinline__ float row_product(const T* a, const T* b, int count) {
+    float sum = 0.0f;
+    for (int c = 0; c < count; ++c) sum = fmaf(to_f32(a[c]), to_f32(b[c]), sum);
+    return sum;
+}
+// Column of a row that register `index` of a lane's accumulators (16 to a block of 32 columns) stands for, or -1.
+template <int W, bool HALVES>
+__device__ __forceinline__ int register_column(int index, int d) {
+    const int block = source_column<W, HALVES>(index / 16 * 32 + (index % 16 >> 2) * 8, d);
+    return block < 0 ? -1 : block + ((threadIdx.x & 63) >> 5) * 4 + (index & 3);
+}
+
+struct RowTiles {
+    int b, h, kvh, q_block, row_wave, part, q_row;
+    bool live;
+    template <int PARTS>
+    __device__ __forceinline__ static RowTiles of(const DifferentialArgs& p, int wave) {
+        constexpr int kRows = kBlockRows / PARTS;
+        const BlockCoordinates where = block_coordinates<kRows>(p.hkv);
+        RowTiles r;
+        r.b = where.b;
+        r.h = where.h;
+        r.kvh = where.h / (p.hq / p.hkv);
+        r.q_block = where.q_block;
+        r.row_wave = wave % (4 / PARTS);
+        r.part = wave / (4 / PARTS);
+        r.q_row = r.q_block + r.row_wave * 32 + static_cast<int>(threadIdx.x & 31);
+        r.live = r.q_row < p.qs;
+        return r;
+    }
+};
+
+template <typename T, int W, int PARTS>
+__global__ __launch_bounds__(kThreads, 2) void differential_forward_kernel(DifferentialArgs p) {
+    using frag = typename Mma<T>::frag;
+    constexpr int STEPS = W / 16, HALF = STEPS / 2, DT = W / 32;
+    T* const lds = wide_stages<T, W, PARTS>();  // [stage][part][K | V]
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const RowTiles at = RowTiles::of<PARTS>(p, wave);
+    const long q_stride = static_cast<long>(p.hq) * p.d, kv_stride = static_cast<long>(p.hkv) * p.d;
+    const long q_offset = (static_cast<long>(at.b) * p.qs + at.q_row) * q_stride + at.h * p.d;
+    const long kv_offset = static_cast<long>(at.b) * p.ks * kv_stride + at.kvh * p.d;
+    const RowStream k_src = make_stream<T, W, true>(p.k, kv_offset, kv_stride, p.ks, p.d, wave, p.d);
+    const RowStream v_src = make_stream<T, W, false>(p.v, kv_offset, kv_stride, p.ks, p.d, wave, p.d);
+
+    const int last_q_block = min(at.q_block + kBlockRows / PARTS, p.qs) - 1;
+    const int k_end = p.causal ? min(p.ks, p.offset + last_q_block + 1) : p.ks;
+    const int tiles = (k_end + kStream - 1) / kStream;
+    auto request = [&](int j, T* stage) __attribute__((always_inline)) {
+#pragma unroll
+        for (int g = 0; g < PARTS; ++g) {
+            if (j + g >= tiles) break;
+            stream_rows<T, W>(k_src, (j + g) * kStream, stage + 2 * g * kWideTile<W>, wave);
+            stream_rows<T, W>(v_src, (j + g) * kStream, stage + (2 * g + 1) * kWideTile<W>, wave);
+        }
+    };
+    request(0, lds);
+
+    frag qf[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) qf[s] = row_frag<T, W, true>(static_cast<const T*>(p.q) + q_offset, at.live, s, p.d);
+    const TileOffsets<W> offsets(lane);
+
+    // Both maps' sums, and their running maxima m of the raw scores (the scale is positive) as in attention.hip: mb = m * scale2, 0 while
+    // m is -inf; it follows the maximum only when that has moved by more than 2^8 in probability.
+    acc_t o[2][DT];
+    float m[2], mb[2], l[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[i][t] = acc_t(0.0f);
+        m[i] = -INFINITY;
+        mb[i] = 0.0f;
+        l[i] = 0.0f;
+    }
+    const float scale2 = p.scale * kLog2e;
+    const int wave_first_q = at.q_block + at.row_wave * 32;
+    const int wave_last_q = min(wave_first_q + 31, p.qs - 1);
+    const bool wave_live = wave_first_q < p.qs;
+    const int q_limit = p.causal ? p.offset + at.q_row : p.ks;  // largest visible key of this lane's query
+    const int clear_limit = p.causal ? min(p.ks - 1, p.offset + wave_first_q) : p.ks - 1;  // tiles up to here need no mask
+
+    LeftOut left(p, wave_first_q);
+    for (int first = 0; first < tiles; first += PARTS) {
+        const int j = first + at.part, k0 = j * kStream, stage = (first / PARTS) & 1;
+        const int tile = (stage * PARTS + at.part) * 2 * kWideTile<W>;  // K's; V's is the next
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's part of the tiles is in LDS
+        __syncthreads();                     // ... and everybody else's; the other stage is free
+        request(first + PARTS, lds + (stage ^ 1) * PARTS * 2 * kWideTile<W>);
+        if (PARTS > 1 && j >= tiles) continue;
+        if (!wave_live || (p.causal && k0 > p.offset + wave_last_q) || left.out<T, W>(j, lds + tile + kWideTile<W>)) continue;
+        const bool masked = k0 + kStream - 1 > clear_limit;
+        const int bound = min(q_limit, p.ks - 1) - k0 - 4 * (lane >> 5);  // of the tile's keys, what this lane's query sees
+
+        const TileOffsets<W> here = offsets.at(tile);
+        frag pf[2][2][2];  // [map][32 keys][16 keys]
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            acc_t st[2] = {acc_t(0.0f), acc_t(0.0f)};
+            {
+                frag ka[2][HALF];
+#pragma unroll
+                for (int s = 0; s < HALF; ++s) {
+                    ka[0][s] = here.row(lds, 0, i * HALF + s);
+                    ka[1][s] = here.row(lds, 32, i * HALF + s);
+                }
+#pragma unroll
+                for (int s = 0; s < HALF; ++s) {
+                    st[0] = Mma<T>::run(ka[0][s], qf[i * HALF + s], st[0]);
+                    st[1] = Mma<T>::run(ka[1][s], qf[i * HALF + s], st[1]);
+                }
+                sched_reads_under_mfmas<2 * HALF, 2 * HALF, 4>();
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (masked) {
+                asm volatile("" ::: "memory");  // keeps the masking out of the common path (no if-conversion)
+#pragma unroll
+                for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        st[sub][e] = (sub * 32 + 8 * (e >> 2) + (e & 3) <= bound) ? st[sub][e] : -INFINITY;
+            }
+            float top = max3(st[0][0], st[1][0], st[0][1]);
+            top = max3(top, st[1][1], st[0][2]);
+#pragma unroll
+            for (int e = 2; e < 16; ++e) top = max3(top, st[1][e], e + 1 < 16 ? st[0][e + 1] : st[1][e]);
+            top = fmaxf(top, other_half(top));
+            if (__any(top > m[i] && (top - m[i]) * scale2 > kRescaleThreshold)) {
+                const float next = fmaxf(m[i], top);
+                const float next_b = next == -INFINITY ? 0.0f : next * scale2;
+                const float alpha = __builtin_amdgcn_exp2f(m[i] == -INFINITY ? -INFINITY : m[i] * scale2 - next_b);
+                l[i] *= alpha;
+#pragma unroll
+                for (int t = 0; t < DT; ++t) o[i][t] *= alpha;
+                m[i] = next;
+                mb[i] = next_b;
+            }
+            float sum = 0.0f;
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float prob = __builtin_amdgcn_exp2f(fmaf(st[sub][e], scale2, -mb[i]));
+                    st[sub][e] = prob;
+                    sum += prob;
+                }
+            l[i] += sum;
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) pf[i][sub][s] = acc_frag<T>(st[sub], s);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                frag vt[DT];
+#pragma unroll
+                for (int t = 0; t < DT; ++t) vt[t] = here.columns(lds, kStream + sub * 32 + s * 16, t);
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    o[0][t] = Mma<T>::run(vt[t], pf[0][sub][s], o[0][t]);
+                    o[1][t] = Mma<T>::run(vt[t], pf[1][sub][s], o[1][t]);
+                }
+            }
+        sched_reads_under_mfmas<8 * DT, 8 * DT, 8>();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    if (left.tiles != 0) {
+        Parked<2 * DT> sums;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+            sums.put(t, o[0][t]);
+            sums.put(DT + t, o[1][t]);
+        }
+        const T* q_row = static_cast<const T*>(p.q) + q_offset;
+        left.each_key(p.ks, [&](int key) {
+            if (!at.live || key > q_limit) return;
+            const T* k_row = static_cast<const T*>(p.k) + kv_offset + key * kv_stride;
+            const T* v_row = static_cast<const T*>(p.v) + kv_offset + key * kv_stride;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float score = row_product(q_row + i * (p.d / 2), k_row + i * (p.d / 2), p.d / 2);
+                const float next = fmaxf(m[i], score), next_b = next == -INFINITY ? 0.0f : next * scale2;
+                const float alpha = __builtin_amdgcn_exp2f(m[i] == -INFINITY ? -INFINITY : mb[i] - next_b);
+                const float e = __builtin_amdgcn_exp2f(fmaf(score, scale2, -next_b));
+                l[i] = fmaf(l[i], alpha, lane < 32 ? e : 0.0f);  // a row's sum is that of its two lanes'
+                m[i] = next;
+                mb[i] = next_b;
+#pragma unroll 1
+                for (int r = 0; r < DT * 16; ++r) {
+                    const int column = register_column<W, false>(r, p.d);
+                    if (column >= 0) sums.values[i * DT * 16 + r] = fmaf(e, to_f32(v_row[column]), sums.values[i * DT * 16 + r] * alpha);
+                }
+            }
+        });
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+            sums.get(t, o[0][t]);
+            sums.get(DT + t, o[1][t]);
+        }
+    }
+    if constexpr (PARTS > 1) {
+        // The second part's sums are brought to the common maximum and added to the first's.
+        constexpr int kWords = 2 * (4 * DT + 1);
+        auto* meet = reinterpret_cast<vec_t<float, 4>*>(lds) + at.row_wave * kWords * kWave + lane;
+        __syncthreads();
+        if (at.part != 0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                deposit_sums<DT>(meet + i * (4 * DT + 1) * kWave, o[i]);
+                meet[(i * (4 * DT + 1) + 4 * DT) * kWave] = vec_t<float, 4>{m[i], l[i], 0.0f, 0.0f};
+            }
+        }
+        __syncthreads();
+        if (at.part != 0) return;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const vec_t<float, 4> theirs = meet[(i * (4 * DT + 1) + 4 * DT) * kWave];
+            const float top = fmaxf(m[i], theirs[0]);
+            const float top_b = top == -INFINITY ? 0.0f : top * scale2;
+            const float mine = m[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mb[i] - top_b);
+            const float other = theirs[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(theirs[0] * scale2 - top_b);
+            l[i] = fmaf(l[i], mine, theirs[1] * other);
+            add_sums<DT>(meet + i * (4 * DT + 1) * kWave, o[i], mine, other);
+            mb[i] = top_b;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) l[i] += other_half(l[i]);
+    if (!at.live) return;
+    const float lambda = p.lambda[at.h];
+    const float inverse1 = 1.0f / l[0], inverse2 = 1.0f / l[1];
+    store_columns<T, W, false>(static_cast<T*>(p.out) + q_offset, p.d, false,
+                               [&](int t, int e) { return fmaf(-lambda, o[1][t][e] * inverse2, o[0][t][e] * inverse1); });
+    if (p.second != nullptr)
+        store_columns<T, W, false>(static_cast<T*>(p.second) + q_offset, p.d, false, [&](int t, int e) { return o[1][t][e] * inverse2; });
+    if (p.lse_out != nullptr) {  // one map from either half of the wavefront
+        const long rows = static_cast<long>(p.batch) * p.qs * p.hq, row = (static_cast<long>(at.b) * p.qs + at.q_row) * p.hq + at.h;
+        const bool second = lane >= 32;
+        p.lse_out[(second ? rows : 0) + row] = ((second ? mb[1] : mb[0]) + log2f(second ? l[1] : l[0])) * kLn2;
+    }
+}
+
+template <typename T, int W, int PARTS>
+__global__ __launch_bounds__(kThreads, 2) void differential_dq_kernel(DifferentialArgs p) {
+    using frag = typename Mma<T>::frag;
+    constexpr int STEPS = W / 16, HALF = STEPS / 2, DT = W / 32;
+    T* const lds = wide_stages<T, W, PARTS>();  // [stage][part][K | V]
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const RowTiles at = RowTiles::of<PARTS>(p, wave);
+    const long q_stride = static_cast<long>(p.hq) * p.d, kv_stride = static_cast<long>(p.hkv) * p.d;
+    const long q_offset = (static_cast<long>(at.b) * p.qs + at.q_row) * q_stride + at.h * p.d;
+    const long kv_offset = static_cast<long>(at.b) * p.ks * kv_stride + at.kvh * p.d;
+    const RowStream k_src = make_stream<T, W, true>(p.k, kv_offset, kv_stride, p.ks, p.d, wave, p.d);
+    const RowStream v_src = make_stream<T, W, false>(p.v, kv_offset, kv_stride, p.ks, p.d, wave, p.d);
+
+    const int last_q_block = min(at.q_block + kBlockRows / PARTS, p.qs) - 1;
+    const int k_end = p.causal ? min(p.ks, p.offset + last_q_block + 1) : p.ks;
+    const int tiles = (k_end + kStream - 1) / kStream;
+    auto request = [&](int j, T* stage) __attribute__((always_inline)) {
+#pragma unroll
+        for (int g = 0; g < PARTS; ++g) {
+            if (j + g >= tiles) break;
+            stream_rows<T, W>(k_src, (j + g) * kStream, stage + 2 * g * kWideTile<W>, wave);
+            stream_rows<T, W>(v_src, (j + g) * kStream, stage + (2 * g + 1) * kWideTile<W>, wave);
+        }
+    };
+    request(0, lds);
+
+    frag qf[STEPS], dof[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        qf[s] = row_frag<T, W, true>(static_cast<const T*>(p.q) + q_offset, at.live, s, p.d);
+        dof[s] = row_frag<T, W, false>(static_cast<const T*>(p.dout) + q_offset, at.live, s, p.d);
+    }
+    const float lambda = p.lambda[at.h];
+    const long rows = static_cast<long>(p.batch) * p.qs * p.hq, row = (static_cast<long>(at.b) * p.qs + at.q_row) * p.hq + at.h;
+    const float delta2 = row_delta<T, STEPS>(dof, static_cast<const T*>(p.o2) + q_offset, at.live, p.d);
+    const float delta1 = fmaf(lambda, delta2, row_delta<T, STEPS>(dof, static_cast<const T*>(p.o) + q_offset, at.live, p.d));
+    const float lse1 = at.live ? p.lse[row] * kLog2e : 0.0f, lse2 = at.live ? p.lse[rows + row] * kLog2e : 0.0f;
+    if (at.live && at.part == 0 && lane < 32) {
+        p.delta[row] = lse1;
+        p.delta[rows + row] = lse2;
+        p.delta[2 * rows + row] = delta1;
+        p.delta[3 * rows + row] = delta2;
+    }
+    int k_off[STEPS], kt_off[DT][2];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) k_off[s] = wide_direct_offset<W>(lane, s);
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+        kt_off[t][0] = wide_transposed_offset<W>(lane, t, 0);
+        kt_off[t][1] = wide_transposed_offset<W>(lane, t, 1);
+    }
+
+    acc_t dq[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) dq[t] = acc_t(0.0f);
+    float rest = 0.0f;  // rowsum(P2 (G - delta2)): what the rounding of O2 left in delta2
+    const float scale2 = p.scale * kLog2e;
+    const int wave_first_q = at.q_block + at.row_wave * 32;
+    const int wave_last_q = min(wave_first_q + 31, p.qs - 1);
+    const bool wave_live = wave_first_q < p.qs;
+    const int q_limit = p.causal ? p.offset + at.q_row : p.ks;
+    const int clear_limit = p.causal ? min(p.ks - 1, p.offset + wave_first_q) : p.ks - 1;
+
+    LeftOut left(p, wave_first_q);
+    for (int first = 0; first < tiles; first += PARTS) {
+        const int j = first + at.part, k0 = j * kStream, stage = (first / PARTS) & 1;
+        const T* k_tile = lds + (stage * PARTS + at.part) * 2 * kWideTile<W>;
+        const T* v_tile = k_tile + kWideTile<W>;
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's part of the tiles is in LDS
+        __syncthreads();                     // ... and everybody else's; the other stage is free
+        request(first + PARTS, lds + (stage ^ 1) * PARTS * 2 * kWideTile<W>);
+        if (PARTS > 1 && j >= tiles) continue;
+        if (!wave_live || (p.causal && k0 > p.offset + wave_last_q) || left.out<T, W>(j, k_tile)) continue;
+        const bool masked = k0 + kStream - 1 > clear_limit;
+        const int bound = min(q_limit, p.ks - 1) - k0 - 4 * (lane >> 5);
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+            acc_t st[2] = {acc_t(0.0f), acc_t(0.0f)}, g(0.0f);
+            {
+                frag ka[STEPS], va[STEPS];
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) {
+                    ka[s] = *reinterpret_cast<const frag*>(k_tile + sub * 32 * W + k_off[s]);
+                    va[s] = *reinterpret_cast<const frag*>(v_tile + sub * 32 * W + k_off[s]);
+                }
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) {
+                    st[s / HALF] = Mma<T>::run(ka[s], qf[s], st[s / HALF]);
+                    g = Mma<T>::run(va[s], dof[s], g);
+                }
+                sched_reads_under_mfmas<2 * STEPS, 2 * STEPS, 4>();
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                st[0][e] = __builtin_amdgcn_exp2f(fmaf(st[0][e], scale2, -lse1)) * (g[e] - delta1);
+                st[1][e] = __builtin_amdgcn_exp2f(fmaf(st[1][e], scale2, -lse2)) * (g[e] - delta2);
+            }
+            if (masked) {
+                asm volatile("" ::: "memory");  // keeps the masking out of the common path (no if-conversion)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const bool visible = sub * 32 + 8 * (e >> 2) + (e & 3) <= bound;
+                    st[0][e] = visible ? st[0][e] : 0.0f;
+                    st[1][e] = visible ? st[1][e] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) rest += st[1][e];
+            __builtin_amdgcn_sched_barrier(0);
+            {
+                frag dsf[2][2], kt[2][DT];
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    dsf[0][s] = acc_frag<T>(st[0], s);
+                    dsf[1][s] = acc_frag<T>(st[1], s);
+                    const T* block = k_tile + (sub * 32 + s * 16) * W;
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) kt[s][t] = wide_transposed_frag<T>(block, kt_off[t][0], kt_off[t][1]);
+                }
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) dq[t] = Mma<T>::run(kt[s][t], dsf[t / (DT / 2)][s], dq[t]);
+                sched_reads_under_mfmas<2 * DT, 4 * DT, 6>();
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    if (left.tiles != 0) {
+        Parked<DT> sums;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) sums.put(t, dq[t]);
+        const T *q_row = static_cast<const T*>(p.q) + q_offset, *do_row = static_cast<const T*>(p.dout) + q_offset;
+        left.each_key(p.ks, [&](int key) {
+            if (!at.live || key > q_limit) return;
+            const T* k_row = static_cast<const T*>(p.k) + kv_offset + key * kv_stride;
+            const float g = row_product(do_row, static_cast<const T*>(p.v) + kv_offset + key * kv_stride, p.d);
+            const float s1 = row_product(q_row, k_row, p.d / 2), s2 = row_product(q_row + p.d / 2, k_row + p.d / 2, p.d / 2);
+            const float ds1 = __builtin_amdgcn_exp2f(fmaf(s1, scale2, -lse1)) * (g - delta1);
+            const float ds2 = __builtin_amdgcn_exp2f(fmaf(s2, scale2, -lse2)) * (g - delta2);
+            if (lane < 32) rest += ds2;  // a row's rest is the sum of its two lanes'
+#pragma unroll 1
+            for (int r = 0; r < DT * 16; ++r) {
+                const int column = register_column<W, true>(r, p.d);
+                if (column >= 0) sums.values[r] = fmaf(r < DT * 8 ? ds1 : ds2, to_f32(k_row[column]), sums.values[r]);
+            }
+        });
+#pragma unroll
+        for (int t = 0; t < DT; ++t) sums.get(t, dq[t]);
+    }
+    if constexpr (PARTS > 1) {
+        auto* meet = reinterpret_cast<vec_t<float, 4>*>(lds) + at.row_wave * (4 * DT + 1) * kWave + lane;
+        __syncthreads();
+        if (at.part != 0) {
+            deposit_sums<DT>(meet, dq);
+            meet[4 * DT * kWave] = vec_t<float, 4>{rest, 0.0f, 0.0f, 0.0f};
+        }
+        __syncthreads();
+        if (at.part != 0) return;
+        add_sums<DT>(meet, dq, 1.0f, 1.0f);
+        rest += meet[4 * DT * kWave][0];
+    }
+    {
+        // -(delta2 + rest) of the wavefront's rows.
+        const float mine = at.live ? rest + (lane < 32 ? delta2 : 0.0f) : 0.0f;
+        const float sum = wave_sum(mine);
+        constexpr int kRowWaves = 4 / PARTS;
+        const long blocks = gridDim.x, part = (static_cast<long>(at.b) * blocks + at.q_block / (kBlockRows / PARTS)) * kRowWaves + at.row_wave;
+        if (lane == 0) p.lambda_partial[at.h * (blocks * p.batch * kRowWaves) + part] = -sum;
+    }
+    if (!at.live) return;
+    const float factor[2] = {p.scale, -lambda * p.scale};
+    store_columns<T, W, true>(static_cast<T*>(p.dq) + q_offset, p.d, p.accumulate != 0,
+                              [&](int t, int e) { return dq[t][e] * factor[t / (DT / 2)]; });
+}
+
+// As the register-staged dK/dV kernel of attention.hip walks its queries, on LDS-direct tiles.
+template <int W>
+constexpr int kDkvSmem = 4 * kWideTile<W> * 2 + 8 * kStream * static_cast<int>(sizeof(float));
+
+template <typename T, int W>
+__global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(DifferentialArgs p) {
+    using frag = typename Mma<T>::frag;
+    constexpr int STEPS = W / 16, HALF = STEPS / 2, DT = W / 32;
+    extern __shared__ __align__(1024) unsigned char wide_smem[];
+    T* lds = reinterpret_cast<T*>(wide_smem);                                           // [stage][Q | dO]
+    float* stats = reinterpret_cast<float*>(wide_smem + 4 * kWideTile<W> * sizeof(T));  // [stage][lse1, lse2, delta1, delta2][64]
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.z, kvh = blockIdx.y, group = p.hq / p.hkv;
+    const int k_block = blockIdx.x * kBlockRows, k_row = k_block + wave * 32 + (lane & 31);
+    const bool live = k_row < p.ks;
+    const long q_stride = static_cast<long>(p.hq) * p.d, kv_stride = static_cast<long>(p.hkv) * p.d;
+    const long k_offset = (static_cast<long>(b) * p.ks + k_row) * kv_stride + kvh * p.d;
+    const long q_batch = static_cast<long>(b) * p.qs * q_stride, rows = static_cast<long>(p.batch) * p.qs * p.hq;
+    frag kf[STEPS], vf[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        kf[s] = row_frag<T, W, true>(static_cast<const T*>(p.k) + k_offset, live, s, p.d);
+        vf[s] = row_frag<T, W, false>(static_cast<const T*>(p.v) + k_offset, live, s, p.d);
+    }
+    int q_off[STEPS], t_off[DT][2];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) q_off[s] = wide_direct_offset<W>(lane, s);
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+        t_off[t][0] = wide_transposed_offset<W>(lane, t, 0);
+        t_off[t][1] = wide_transposed_offset<W>(lane, t, 1);
+    }
+    acc_t dk[DT], dv[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) dk[t] = dv[t] = acc_t(0.0f);
+    const float scale2 = p.scale * kLog2e;
+    const int q_begin = p.causal ? max(0, k_block - p.offset) / kStream * kStream : 0;  // first tile that sees a key of the block
+    const int tiles_per_head = q_begin < p.qs ? (p.qs - q_begin + kStream - 1) / kStream : 0;
+    const int tiles = tiles_per_head * group;
+    const RowStream q_src = make_stream<T, W, true>(p.q, q_batch + kvh * group * p.d, q_stride, p.qs, p.d, wave, p.d);
+    const RowStream do_src = make_stream<T, W, false>(p.dout, q_batch + kvh * group * p.d, q_stride, p.qs, p.d, wave, p.d);
+    auto request = [&](int tile) {
+        if (tile >= tiles) return;
+        const int head = tile / tiles_per_head, q0 = q_begin + (tile - head * tiles_per_head) * kStream;
+        T* stage = lds + (tile & 1) * 2 * kWideTile<W>;
+        RowStream of_head = q_src;
+        of_head.base += head * p.d * static_cast<int>(sizeof(T));
+        stream_rows<T, W>(of_head, q0, stage, wave);
+        of_head = do_src;
+        of_head.base += head * p.d * static_cast<int>(sizeof(T));
+        stream_rows<T, W>(of_head, q0, stage + kWideTile<W>, wave);
+        const float* from = p.delta + wave * rows + static_cast<long>(b) * p.qs * p.hq + kvh * group + head;
+        const int q = q0 + lane;
+        stats[((tile & 1) * 4 + wave) * kStream + lane] = q < p.qs ? from[static_cast<long>(q) * p.hq] : 0.0f;
+    };
+    request(0);
+    for (int tile = 0; tile < tiles; ++tile) {
+        const int head = tile / tiles_per_head, q0 = q_begin + (tile - head * tiles_per_head) * kStream;
+        const float lambda = p.lambda[kvh * group + head];
+        const T* q_tile = lds + (tile & 1) * 2 * kWideTile<W>;
+        const T* do_tile = q_tile + kWideTile<W>;
+        const float* stat = stats + (tile & 1) * 4 * kStream;
+        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
+        __syncthreads();
+        request(tile + 1);
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+            acc_t st[2] = {acc_t(0.0f), acc_t(0.0f)}, g(0.0f), ds[2];
+            {
+                frag qa[STEPS], da[STEPS];
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) {
+                    qa[s] = *reinterpret_cast<const frag*>(q_tile + sub * 32 * W + q_off[s]);
+                    da[s] = *reinterpret_cast<const frag*>(do_tile + sub * 32 * W + q_off[s]);
+                }
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) {
+                    st[s / HALF] = Mma<T>::run(qa[s], kf[s], st[s / HALF]);
+                    g = Mma<T>::run(da[s], vf[s], g);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int local = sub * 32 + acc_row(e), q = q0 + local;
+                const bool visible = live && q < p.qs && (!p.causal || k_row <= p.offset + q);
+                const float p1 = visible ? __builtin_amdgcn_exp2f(fmaf(st[0][e], scale2, -stat[local])) : 0.0f;
+                const float p2 = visible ? -lambda * __builtin_amdgcn_exp2f(fmaf(st[1][e], scale2, -stat[kStream + local])) : 0.0f;
+                ds[0][e] = p1 * (g[e] - stat[2 * kStream + local]);
+                ds[1][e] = p2 * (g[e] - stat[3 * kStream + local]);
+                st[0][e] = p1 + p2;
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const frag pf = acc_frag<T>(st[0], s), dsf[2] = {acc_frag<T>(ds[0], s), acc_frag<T>(ds[1], s)};
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    const int block = (sub * 32 + s * 16) * W;
+                    dv[t] = Mma<T>::run(wide_transposed_frag<T>(do_tile + block, t_off[t][0], t_off[t][1]), pf, dv[t]);
+                    dk[t] = Mma<T>::run(wide_transposed_frag<T>(q_tile + block, t_off[t][0], t_off[t][1]), dsf[t / (DT / 2)], dk[t]);
+                }
+            }
+        }
+    }
+    if (!live) return;
+    store_columns<T, W, true>(static_cast<T*>(p.dk) + k_offset, p.d, p.accumulate != 0, [&](int t, int e) { return dk[t][e] * p.scale; });
+    store_columns<T, W, false>(static_cast<T*>(p.dv) + k_offset, p.d, p.accumulate != 0, [&](int t, int e) { return dv[t][e]; });
+}
+
+template <typename Fn>
+int dispatch(const DifferentialArgs& a, Fn&& fn) {
+    const bool narrow = a.d <= 64;
+    if (a.dtype == CGPTX_F16) return narrow ? fn.template operator()<f16_t, 64>() : fn.template operator()<f16_t, 128>();
+    return narrow ? fn.template operator()<bf16_t, 64>() : fn.template operator()<bf16_t, 128>();
+}
+
+// Whether forward and dQ run in two parts: blocks of 64 rows that all find a place on the chip at once (two per CU with heads of 64),
+// and more than one key tile.
+bool two_parts(const DifferentialArgs& a) {
+    const long blocks = (static_cast<long>(a.qs) + kBlockRows / 2 - 1) / (kBlockRows / 2) * a.hq * a.batch;
+    return a.ks > kStream && blocks <= static_cast<long>(compute_units()) * (a.d <= 64 ? 2 : 1);
+}
+template <auto Kernel, int W, int PARTS>
+int launch_rows(const DifferentialArgs& a, hipStream_t stream) {
+    constexpr int smem = PARTS == 1 ? 0 : 8 * kWideTile<W> * 2;  // [stage][part][K | V] of 16-bit elements
+    if constexpr (PARTS > 1) {
+        static const hipError_t status =
+            hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+        CGPTX_HIP(status);
+    }
+    const dim3 grid(static_cast<unsigned int>((a.qs + kBlockRows / PARTS - 1) / (kBlockRows / PARTS)), static_cast<unsigned int>(a.hq),
+                    static_cast<unsigned int>(a.batch));
+    hipLaunchKernelGGL(Kernel, grid, dim3(kThreads), smem, stream, a);
+    CGPTX_LAUNCH_CHECK();
+    return CGPTX_OK;
+}
+
+// Row wavefronts of a dQ launch per head: the parts of a head's dlambda.
+long lambda_parts(const DifferentialArgs& a) {
+    const int block = two_parts(a) ? kBlockRows / 2 : kBlockRows;
+    return (static_cast<long>(a.qs) + block - 1) / block * (block / 32) * a.batch;
+}
+std::size_t statistics_bytes(const DifferentialArgs& a) {
+    return (4 * static_cast<std::size_t>(a.batch) * a.qs * a.hq * sizeof(float) + 255) & ~std::size_t{255};
+}
+
+}  // namespace
+
+bool differential_mfma_takes(const DifferentialArgs& a) {
+    const std::size_t row = static_cast<std::size_t>(std::max(a.hq, a.hkv)) * a.d * 2;
+    return a.dtype != CGPTX_F32 && a.d % 16 == 0 && kStream * row <= (std::size_t{1} << 30);
+}
+
+int differential_mfma_forward(const DifferentialArgs& a, hipStream_t stream) {
+    return dispatch(a, [&]<typename T, int W>() -> int {
+        return two_parts(a) ? launch_rows<differential_forward_kernel<T, W, 2>, W, 2>(a, stream)
+                            : launch_rows<differential_forward_kernel<T, W, 1>, W, 1>(a, stream);
+    });
+}
+
+std::size_t differential_mfma_scratch(const DifferentialArgs& a) {
+    return statistics_bytes(a) + static_cast<std::size_t>(lambda_parts(a)) * a.hq * sizeof(float);
+}
+
+int differential_mfma_backward(DifferentialArgs a, void* memory, hipStream_t stream) {
+    a.delta = static_cast<float*>(memory);
+    a.lambda_partial = reinterpret_cast<float*>(static_cast<char*>(memory) + statistics_bytes(a));
+    if (int st = dispatch(a, [&]<typename T, int W>() -> int {
+            if (int s = two_parts(a) ? launch_rows<differential_dq_kernel<T, W, 2>, W, 2>(a, stream)
+                                     : launch_rows<differential_dq_kernel<T, W, 1>, W, 1>(a, stream))
+                return s;
+            constexpr auto kernel = differential_dkv_kernel<T, W>;
+            static const hipError_t status =
+                hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kDkvSmem<W>);
+            CGPTX_HIP(status);
+            const dim3 grid(static_cast<unsigned int>((a.ks + kBlockRows - 1) / kBlockRows), static_cast<unsigned int>(a.hkv),
+                            static_cast<unsigned int>(a.batch));
+            hipLaunchKernelGGL(kernel, grid, dim3(kThreads), kDkvSmem<W>, stream, a);
+            CGPTX_LAUNCH_CHECK();
+            return CGPTX_OK;
+        }))
+        return st;
+    return differential_dlambda(a, lambda_parts(a), stream);
+}
+
+}  // namespace cgptx
