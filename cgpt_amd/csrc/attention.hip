@@ -1256,31 +1256,6 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 2 : 1) void attention_dkv_wide_
     }
 }
 
-// dK and dV from the parts of shared key blocks, added in the order of the parts; four elements per thread.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void attention_dkv_reduce_kernel(T* __restrict__ dk, T* __restrict__ dv,
-                                                                       const float* __restrict__ partial, long count,
-                                                                       int splits, int accumulate) {
-    const long quad = static_cast<long>(blockIdx.x) * kThreads + threadIdx.x;
-    if (quad >= count / 2) return;  // count elements of dK, then of dV
-    const bool second = quad >= count / 4;
-    const long at = (second ? quad - count / 4 : quad) * 4;
-    const float* source = partial + (second ? count : 0) + at;
-    vec_t<float, 4> sum = load_vec<float, 4>(source);
-    int s = 1;
-    for (; s + 3 < splits; s += 4) {
-        vec_t<float, 4> v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = load_vec<float, 4>(source + 2 * (s + i) * count);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum += v[i];
-    }
-    for (; s < splits; ++s) sum += load_vec<float, 4>(source + 2 * s * count);
-    T* out = (second ? dv : dk) + at;
-    if (accumulate) sum += vec_to_f32<T, 4>(load_vec<T, 4>(out));
-    store_vec<T, 4>(out, vec_from_f32<T, 4>(sum));
-}
-
 // ============================================================================================
 // Scalar family: head dimensions that are not multiples of 8 (16-bit storage) or 4 (fp32), and tensors that are
 // not 16-byte aligned — what the reference serves with its warp-per-row kernels
@@ -1505,33 +1480,20 @@ unsigned int scalar_blocks(std::size_t rows) { return static_cast<unsigned int>(
 int dkv_splits(const Shape& s) {
     const bool f32 = s.dtype == CGPTX_F32;
     if (!f32 && !wide_path(s)) return 1;
-    const std::size_t block_rows = f32 ? 16 : kBlockRows, stream_rows = f32 ? 16 : kStream;
-    const long waves = f32 ? 8 : 1;  // that walk tiles of their own
-    const long units = compute_units(), group = static_cast<long>(s.hq / s.hkv);
-    const long key_blocks = static_cast<long>((s.ks + block_rows - 1) / block_rows), pairs = static_cast<long>(s.hkv * s.batch);
-    long longest = 0, total = 0;
-    for (long i = 0; i < key_blocks; ++i) {
-        const long rows = static_cast<long>(stream_rows), skipped = i * static_cast<long>(block_rows) - static_cast<long>(s.offset);
-        const long begin = s.causal ? std::max<long>(0, skipped) / rows * rows : 0;
-        const long walked = begin < static_cast<long>(s.qs) ? (static_cast<long>(s.qs) - begin + rows - 1) / rows * group : 0;
-        const long tiles = (walked + waves - 1) / waves;
-        longest = std::max(longest, tiles);
-        total += tiles * pairs;
-        if (total > 16 * units * std::max<long>(longest, 1)) return 1;  // a full chip many times over
-    }
-    const double tile_us = f32 ? 8.0 : s.d <= 64 ? 0.9 : 1.75;
-    const double megabytes = static_cast<double>(s.batch * s.ks * s.hkv * s.d) * 8e-6;
-    int best = 1;
-    double best_us = 0.0;
-    for (int parts = 1; parts <= 16 && parts <= std::max<long>(longest, 1); ++parts) {
-        const double busiest = std::max<double>(std::ceil(static_cast<double>(longest) / parts), static_cast<double>(total) / static_cast<double>(units));
-        const double us = busiest * tile_us + (parts > 1 ? 5.0 + 0.4 * megabytes * parts : 0.0);
-        if (parts == 1 || us < best_us) {
-            best = parts;
-            best_us = us;
-        }
-    }
-    return best;
+    KeyWalk walk{};
+    walk.batch = static_cast<long>(s.batch);
+    walk.qs = static_cast<long>(s.qs);
+    walk.ks = static_cast<long>(s.ks);
+    walk.hkv = static_cast<long>(s.hkv);
+    walk.group = static_cast<long>(s.hq / s.hkv);
+    walk.d = static_cast<long>(s.d);
+    walk.causal = s.causal;
+    walk.offset = static_cast<long>(s.offset);
+    walk.block_rows = f32 ? 16 : kBlockRows;
+    walk.stream_rows = f32 ? 16 : kStream;
+    walk.waves = f32 ? 8 : 1;
+    walk.tile_us = f32 ? 8.0 : s.d <= 64 ? 0.9 : 1.75;
+    return key_block_parts(walk);
 }
 
 // Whether forward and dQ run in two parts: blocks of 64 rows that all find a place on the chip at once (two per CU with
@@ -1550,15 +1512,6 @@ int launch_two_parts(const Shape& s, const Params& p, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned int>((s.qs + kBlockRows / 2 - 1) / (kBlockRows / 2)), static_cast<unsigned int>(s.hq),
                     static_cast<unsigned int>(s.batch));
     hipLaunchKernelGGL(Kernel, grid, dim3(kThreads), smem, stream, p);
-    CGPTX_LAUNCH_CHECK();
-    return CGPTX_OK;
-}
-
-template <typename T>
-int launch_dkv_reduce(const Shape& s, void* dk, void* dv, const float* partial, int splits, int accumulate, hipStream_t stream) {
-    const long count = static_cast<long>(s.batch * s.ks * s.hkv * s.d);
-    hipLaunchKernelGGL((attention_dkv_reduce_kernel<T>), dim3(static_cast<unsigned int>((count / 2 + kThreads - 1) / kThreads)),
-                       dim3(kThreads), 0, stream, static_cast<T*>(dk), static_cast<T*>(dv), partial, count, splits, accumulate);
     CGPTX_LAUNCH_CHECK();
     return CGPTX_OK;
 }
@@ -1660,7 +1613,7 @@ int launch_backward(const Shape& s, Params p, void* dq, void* dk, void* dv, cons
         a.parts = room.splits;
         a.partial = reinterpret_cast<float*>(room.mem + 2 * stat_bytes);
         if (int st = attention_f32_backward(a, stream)) return st;
-        return a.parts > 1 ? launch_dkv_reduce<float>(s, dk, dv, a.partial, a.parts, accumulate, stream) : CGPTX_OK;
+        return a.parts > 1 ? launch_dkv_reduce<float>(static_cast<long>(s.batch * s.ks * s.hkv * s.d), dk, dv, a.partial, a.parts, accumulate, stream) : CGPTX_OK;
     }
     if (scalar) {
         const std::size_t key_rows = s.batch * s.ks * s.hkv;
@@ -1732,7 +1685,7 @@ int launch_backward(const Shape& s, Params p, void* dq, void* dk, void* dv, cons
                 if (int st = s.d <= 64 ? launch.template operator()<64>() : launch.template operator()<128>()) return st;
                 if (pk.splits > 1) {
                     CGPTX_LAUNCH_CHECK();
-                    if (int st = launch_dkv_reduce<T>(s, dk, dv, pk.partial, pk.splits, accumulate, stream)) return st;
+                    if (int st = launch_dkv_reduce<T>(static_cast<long>(s.batch * s.ks * s.hkv * s.d), dk, dv, pk.partial, pk.splits, accumulate, stream)) return st;
                 }
             } else {
                 const dim3 k_grid(key_blocks, static_cast<unsigned int>(s.hkv), static_cast<unsigned int>(s.batch));

@@ -4,6 +4,7 @@
 
 #include "common.hpp"
 
+#include <algorithm>
 #include <cmath>
 
 namespace cgptx {
@@ -292,6 +293,72 @@ __device__ __forceinline__ void add_sums(const vec_t<float, 4>* from, acc_t (&su
 #pragma unroll
             for (int e = 0; e < 4; ++e) sums[t][4 * q + e] = fmaf(sums[t][4 * q + e], mine, v[e] * other);
         }
+}
+
+// dK and dV from the parts of shared key blocks, added in the order of the parts; four elements per thread.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void attention_dkv_reduce_kernel(T* __restrict__ dk, T* __restrict__ dv,
+                                                                       const float* __restrict__ partial, long count,
+                                                                       int splits, int accumulate) {
+    const long quad = static_cast<long>(blockIdx.x) * kThreads + threadIdx.x;
+    if (quad >= count / 2) return;  // count elements of dK, then of dV
+    const bool second = quad >= count / 4;
+    const long at = (second ? quad - count / 4 : quad) * 4;
+    const float* source = partial + (second ? count : 0) + at;
+    vec_t<float, 4> sum = load_vec<float, 4>(source);
+    int s = 1;
+    for (; s + 3 < splits; s += 4) {
+        vec_t<float, 4> v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = load_vec<float, 4>(source + 2 * (s + i) * count);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += v[i];
+    }
+    for (; s < splits; ++s) sum += load_vec<float, 4>(source + 2 * s * count);
+    T* out = (second ? dv : dk) + at;
+    if (accumulate) sum += vec_to_f32<T, 4>(load_vec<T, 4>(out));
+    store_vec<T, 4>(out, vec_from_f32<T, 4>(sum));
+}
+
+template <typename T>
+int launch_dkv_reduce(long count, void* dk, void* dv, const float* partial, int splits, int accumulate, hipStream_t stream) {
+    hipLaunchKernelGGL((attention_dkv_reduce_kernel<T>), dim3(static_cast<unsigned int>((count / 2 + kThreads - 1) / kThreads)),
+                       dim3(kThreads), 0, stream, static_cast<T*>(dk), static_cast<T*>(dv), partial, count, splits, accumulate);
+    CGPTX_LAUNCH_CHECK();
+    return CGPTX_OK;
+}
+
+// What decides how many workgroups share a key block in a dK/dV pass whose workgroups hold `block_rows` keys of one kv head, of which
+// `waves` wavefronts walk tiles of `stream_rows` queries of their own, `tile_us` each.
+struct KeyWalk {
+    long batch, qs, ks, hkv, group, d;
+    int causal;
+    long offset, block_rows, stream_rows, waves;
+    double tile_us;
+};
+inline int key_block_parts(const KeyWalk& k) {
+    const long units = compute_units(), key_blocks = (k.ks + k.block_rows - 1) / k.block_rows, pairs = k.hkv * k.batch;
+    long longest = 0, total = 0;
+    for (long i = 0; i < key_blocks; ++i) {
+        const long begin = k.causal ? std::max<long>(0, i * k.block_rows - k.offset) / k.stream_rows * k.stream_rows : 0;
+        const long walked = begin < k.qs ? (k.qs - begin + k.stream_rows - 1) / k.stream_rows * k.group : 0;
+        const long tiles = (walked + k.waves - 1) / k.waves;
+        longest = std::max(longest, tiles);
+        total += tiles * pairs;
+        if (total > 16 * units * std::max<long>(longest, 1)) return 1;  // a full chip many times over
+    }
+    const double megabytes = static_cast<double>(k.batch * k.ks * k.hkv * k.d) * 8e-6;
+    int best = 1;
+    double best_us = 0.0;
+    for (int parts = 1; parts <= 16 && parts <= std::max<long>(longest, 1); ++parts) {
+        const double busiest = std::max<double>(std::ceil(static_cast<double>(longest) / parts), static_cast<double>(total) / static_cast<double>(units));
+        const double us = busiest * k.tile_us + (parts > 1 ? 5.0 + 0.4 * megabytes * parts : 0.0);
+        if (parts == 1 || us < best_us) {
+            best = parts;
+            best_us = us;
+        }
+    }
+    return best;
 }
 
 }  // namespace cgptx

@@ -419,12 +419,10 @@ extern "C" int cgptx_differential_attention_backward(void* grad_query, void* gra
     p.dv = grad_value;
     p.dlambda = grad_lambda;
     p.accumulate = accumulate_grads != 0;
+    if (on_matrix_cores(p, {grad_query, grad_key, grad_value, grad_output, output, second, query, key, value}))
+        return differential_mfma_backward(p, stream);
     const std::size_t rows = batch * query_sequence * query_heads;
     void* mem = nullptr;
-    if (on_matrix_cores(p, {grad_query, grad_key, grad_value, grad_output, output, second, query, key, value})) {
-        if (int st = scratch(stream, differential_mfma_scratch(p), &mem)) return st;
-        return differential_mfma_backward(p, mem, stream);
-    }
     if (int st = scratch(stream, 3 * rows * sizeof(float), &mem)) return st;
     p.delta = static_cast<float*>(mem);
     p.lambda_partial = p.delta + 2 * rows;

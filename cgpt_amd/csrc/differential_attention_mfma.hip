@@ -15,6 +15,7 @@
 #include "differential_attention.hpp"
 
 #include <algorithm>
+#include <utility>
 
 namespace cgptx {
 namespace {
@@ -55,14 +56,17 @@ __device__ __forceinline__ RowStream make_stream(const void* tensor, long offset
     s.voffset = column >= 0 ? r * s.row_bytes + column * static_cast<int>(sizeof(T)) : (1 << 30);
     return s;
 }
+// 16 bytes per lane, 1 KiB in all, straight into LDS.
+__device__ __forceinline__ void load_chunks(__amdgpu_buffer_rsrc_t rsrc, void* to, int voffset, int soffset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_ptr)(to), 16, voffset, soffset, 0, 0);
+}
 template <typename T, int W>
 __device__ __forceinline__ void stream_rows(const RowStream& s, int row0, T* tile, int wave) {
     constexpr int kRowsPerLoad = 64 / (W / 8), kLoads = kStream / (4 * kRowsPerLoad);
     const __amdgpu_buffer_rsrc_t rsrc = s.at(row0);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_ptr)(tile + (i * 4 + wave) * kRowsPerLoad * W), 16, s.voffset,
-                                                 i * 4 * kRowsPerLoad * s.row_bytes, 0, 0);
+        load_chunks(rsrc, tile + (i * 4 + wave) * kRowsPerLoad * W, s.voffset, i * 4 * kRowsPerLoad * s.row_bytes);
 }
 
 // Element offsets in LDS of a lane's fragments of a tile that starts at element `tile` (a multiple of 512). The offsets of a tile differ by
@@ -596,9 +600,42 @@ __global__ __launch_bounds__(kThreads, 2) void differential_dq_kernel(Differenti
                               [&](int t, int e) { return dq[t][e] * factor[t / (DT / 2)]; });
 }
 
-// As the register-staged dK/dV kernel of attention.hip walks its queries, on LDS-direct tiles.
+// dK/dV: keys are stationary, 32 per wavefront with their K and V fragments and accumulators in registers; 64-query Q/dO tiles of
+// every q-head of the group pass through two LDS stages with their statistics. A tile is 4 N matrix instructions (N = W/8), in slots
+// of one with a scheduling fence after each: what else a tile has to do runs in the shadow of instructions that it does not depend
+// on, if it stands between them. With H = N/2, halves of 32 queries in brackets:
+//   Sᵀ(0) H | Gᵀ(0), Sᵀ(1) by turns 2H | Gᵀ(1), dV(0) by turns 2H | dV(1) H | dK(0) H | dK(1) H
+// The exponentials and the packed P1 - lambda P2 of a half run from the end of its scores to its dV, its score gradients from there
+// to its dK: two maps' worth take about as long as the matrix instructions (plain attention's half of that), so they are dealt out
+// over all slots between.
 template <int W>
 constexpr int kDkvSmem = 4 * kWideTile<W> * 2 + 8 * kStream * static_cast<int>(sizeof(float));
+
+// Where a 64-query tile comes from and goes to.
+template <typename T>
+struct QueryTile {
+    bool live;
+    __amdgpu_buffer_rsrc_t q, dout, stat;
+    T* stage;
+    float* stat_stage;
+};
+
+enum class Product { scores, grads, values, keys };
+struct Slot {
+    Product product;
+    int half, index;
+};
+constexpr Slot dkv_slot(int k, int h) {
+    if (k < h) return {Product::scores, 0, k};
+    if (k < 3 * h) return (k - h) % 2 == 0 ? Slot{Product::grads, 0, (k - h) / 2} : Slot{Product::scores, 1, (k - h) / 2};
+    if (k < 5 * h) return (k - h) % 2 == 0 ? Slot{Product::grads, 1, (k - 3 * h) / 2} : Slot{Product::values, 0, (k - 3 * h) / 2};
+    if (k < 6 * h) return {Product::values, 1, k - 5 * h};
+    if (k < 7 * h) return {Product::keys, 0, k - 6 * h};
+    return {Product::keys, 1, k - 7 * h};
+}
+// Slot in which step n of 8 of a half's exponentials (or score gradients) runs.
+constexpr int exponential_slot(int half, int n, int h) { return (half == 0 ? h + 2 : 3 * h + 2) + n * (2 * h - 2) / 8; }
+constexpr int gradient_slot(int half, int n, int h) { return (half == 0 ? 4 * h + h / 2 : 6 * h - h / 4) + n * (half == 0 ? 3 * h / 2 : 5 * h / 4) / 8; }
 
 template <typename T, int W>
 __global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(DifferentialArgs p) {
@@ -609,100 +646,227 @@ __global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(Different
     float* stats = reinterpret_cast<float*>(wide_smem + 4 * kWideTile<W> * sizeof(T));  // [stage][lse1, lse2, delta1, delta2][64]
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int b = blockIdx.z, kvh = blockIdx.y, group = p.hq / p.hkv;
-    const int k_block = blockIdx.x * kBlockRows, k_row = k_block + wave * 32 + (lane & 31);
-    const bool live = k_row < p.ks;
-    const long q_stride = static_cast<long>(p.hq) * p.d, kv_stride = static_cast<long>(p.hkv) * p.d;
-    const long k_offset = (static_cast<long>(b) * p.ks + k_row) * kv_stride + kvh * p.d;
-    const long q_batch = static_cast<long>(b) * p.qs * q_stride, rows = static_cast<long>(p.batch) * p.qs * p.hq;
-    frag kf[STEPS], vf[STEPS];
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-        kf[s] = row_frag<T, W, true>(static_cast<const T*>(p.k) + k_offset, live, s, p.d);
-        vf[s] = row_frag<T, W, false>(static_cast<const T*>(p.v) + k_offset, live, s, p.d);
-    }
-    int q_off[STEPS], t_off[DT][2];
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) q_off[s] = wide_direct_offset<W>(lane, s);
-#pragma unroll
-    for (int t = 0; t < DT; ++t) {
-        t_off[t][0] = wide_transposed_offset<W>(lane, t, 0);
-        t_off[t][1] = wide_transposed_offset<W>(lane, t, 1);
-    }
-    acc_t dk[DT], dv[DT];
-#pragma unroll
-    for (int t = 0; t < DT; ++t) dk[t] = dv[t] = acc_t(0.0f);
-    const float scale2 = p.scale * kLog2e;
-    const int q_begin = p.causal ? max(0, k_block - p.offset) / kStream * kStream : 0;  // first tile that sees a key of the block
-    const int tiles_per_head = q_begin < p.qs ? (p.qs - q_begin + kStream - 1) / kStream : 0;
-    const int tiles = tiles_per_head * group;
-    const RowStream q_src = make_stream<T, W, true>(p.q, q_batch + kvh * group * p.d, q_stride, p.qs, p.d, wave, p.d);
-    const RowStream do_src = make_stream<T, W, false>(p.dout, q_batch + kvh * group * p.d, q_stride, p.qs, p.d, wave, p.d);
-    auto request = [&](int tile) {
-        if (tile >= tiles) return;
-        const int head = tile / tiles_per_head, q0 = q_begin + (tile - head * tiles_per_head) * kStream;
-        T* stage = lds + (tile & 1) * 2 * kWideTile<W>;
-        RowStream of_head = q_src;
-        of_head.base += head * p.d * static_cast<int>(sizeof(T));
-        stream_rows<T, W>(of_head, q0, stage, wave);
-        of_head = do_src;
-        of_head.base += head * p.d * static_cast<int>(sizeof(T));
-        stream_rows<T, W>(of_head, q0, stage + kWideTile<W>, wave);
-        const float* from = p.delta + wave * rows + static_cast<long>(b) * p.qs * p.hq + kvh * group + head;
-        const int q = q0 + lane;
-        stats[((tile & 1) * 4 + wave) * kStream + lane] = q < p.qs ? from[static_cast<long>(q) * p.hq] : 0.0f;
-    };
-    request(0);
-    for (int tile = 0; tile < tiles; ++tile) {
-        const int head = tile / tiles_per_head, q0 = q_begin + (tile - head * tiles_per_head) * kStream;
-        const float lambda = p.lambda[kvh * group + head];
-        const T* q_tile = lds + (tile & 1) * 2 * kWideTile<W>;
-        const T* do_tile = q_tile + kWideTile<W>;
-        const float* stat = stats + (tile & 1) * 4 * kStream;
-        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
-        __syncthreads();
-        request(tile + 1);
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-            acc_t st[2] = {acc_t(0.0f), acc_t(0.0f)}, g(0.0f), ds[2];
-            {
-                frag qa[STEPS], da[STEPS];
-#pragma unroll
-                for (int s = 0; s < STEPS; ++s) {
-                    qa[s] = *reinterpret_cast<const frag*>(q_tile + sub * 32 * W + q_off[s]);
-                    da[s] = *reinterpret_cast<const frag*>(do_tile + sub * 32 * W + q_off[s]);
-                }
-#pragma unroll
-                for (int s = 0; s < STEPS; ++s) {
-                    st[s / HALF] = Mma<T>::run(qa[s], kf[s], st[s / HALF]);
-                    g = Mma<T>::run(da[s], vf[s], g);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int local = sub * 32 + acc_row(e), q = q0 + local;
-                const bool visible = live && q < p.qs && (!p.causal || k_row <= p.offset + q);
-                const float p1 = visible ? __builtin_amdgcn_exp2f(fmaf(st[0][e], scale2, -stat[local])) : 0.0f;
-                const float p2 = visible ? -lambda * __builtin_amdgcn_exp2f(fmaf(st[1][e], scale2, -stat[kStream + local])) : 0.0f;
-                ds[0][e] = p1 * (g[e] - stat[2 * kStream + local]);
-                ds[1][e] = p2 * (g[e] - stat[3 * kStream + local]);
-                st[0][e] = p1 + p2;
-            }
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const frag pf = acc_frag<T>(st[0], s), dsf[2] = {acc_frag<T>(ds[0], s), acc_frag<T>(ds[1], s)};
-#pragma unroll
-                for (int t = 0; t < DT; ++t) {
-                    const int block = (sub * 32 + s * 16) * W;
-                    dv[t] = Mma<T>::run(wide_transposed_frag<T>(do_tile + block, t_off[t][0], t_off[t][1]), pf, dv[t]);
-                    dk[t] = Mma<T>::run(wide_transposed_frag<T>(q_tile + block, t_off[t][0], t_off[t][1]), dsf[t / (DT / 2)], dk[t]);
-                }
-            }
+    // Workgroup -> (key block or pair of them, kv head, batch entry), as in attention.hip's dK/dV: the owners of an XCD's workgroups
+    // stream the same Q and dO.
+    int block = static_cast<int>(blockIdx.x), b = static_cast<int>(blockIdx.z), kvh = static_cast<int>(blockIdx.y);
+    {
+        constexpr unsigned int kXcds = 8;
+        const unsigned int linear = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z);
+        const unsigned int owners = gridDim.y * gridDim.z;
+        const unsigned int xcds = owners % kXcds == 0 ? kXcds : 1;
+        if (xcds > 1 || p.by_block) {
+            const unsigned int xcd = linear % xcds, local = linear / xcds, mine = owners / xcds;
+            const unsigned int owner = xcd + xcds * (p.by_block ? local % mine : local / gridDim.x);
+            block = static_cast<int>(p.by_block ? local / mine : local % gridDim.x);
+            kvh = static_cast<int>(owner % gridDim.y);
+            b = static_cast<int>(owner / gridDim.y);
         }
     }
-    if (!live) return;
-    store_columns<T, W, true>(static_cast<T*>(p.dk) + k_offset, p.d, p.accumulate != 0, [&](int t, int e) { return dk[t][e] * p.scale; });
-    store_columns<T, W, false>(static_cast<T*>(p.dv) + k_offset, p.d, p.accumulate != 0, [&](int t, int e) { return dv[t][e]; });
+    const int group = p.hq / p.hkv;
+    const long q_stride = static_cast<long>(p.hq) * p.d, kv_stride = static_cast<long>(p.hkv) * p.d;
+    const long rows = static_cast<long>(p.batch) * p.qs * p.hq;
+    const float scale2 = p.scale * kLog2e;
+    const long q_batch = static_cast<long>(b) * p.qs * q_stride + kvh * group * p.d;
+    const RowStream q_src = make_stream<T, W, true>(p.q, q_batch, q_stride, p.qs, p.d, wave, p.d);
+    const RowStream do_src = make_stream<T, W, false>(p.dout, q_batch, q_stride, p.qs, p.d, wave, p.d);
+    const TileOffsets<W> offsets(lane);
+
+    const int key_blocks = (p.ks + kBlockRows - 1) / kBlockRows;
+    const int part = p.splits > 1 ? block % p.splits : 0;
+    if (p.splits > 1) block /= p.splits;
+    for (int turn = 0; turn < (p.paired ? 2 : 1); ++turn) {
+        const int block_index = turn == 0 ? block : key_blocks - 1 - block;
+        if (turn == 1 && block_index <= block) break;
+        const int k_block = block_index * kBlockRows;
+        const int k_row = k_block + wave * 32 + (lane & 31);
+        const bool k_live = k_row < p.ks;
+        const long k_offset = (static_cast<long>(b) * p.ks + k_row) * kv_stride + kvh * p.d;
+        frag kf[STEPS], vf[STEPS];
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            kf[s] = row_frag<T, W, true>(static_cast<const T*>(p.k) + k_offset, k_live, s, p.d);
+            vf[s] = row_frag<T, W, false>(static_cast<const T*>(p.v) + k_offset, k_live, s, p.d);
+        }
+        acc_t dk[DT], dv[DT];
+#pragma unroll
+        for (int t = 0; t < DT; ++t) dk[t] = dv[t] = acc_t(0.0f);
+        // First query tile that sees a key of this block; the (head of the group, query tile) pairs form one sequence.
+        const int q_begin = p.causal ? max(0, k_block - p.offset) / kStream * kStream : 0;
+        const int tiles_per_head = q_begin < p.qs ? (p.qs - q_begin + kStream - 1) / kStream : 0;
+        const long all_tiles = static_cast<long>(tiles_per_head) * group;
+        const int first_index = p.splits > 1 ? static_cast<int>(part * all_tiles / p.splits) : 0;
+        const int total_tiles = static_cast<int>(p.splits > 1 ? (part + 1) * all_tiles / p.splits : all_tiles);  // end of the part
+        const int wave_last_key = k_block + wave * 32 + 31;
+
+        constexpr int kRowsPerLoad = 64 / (W / 8), kLoads = kStream / (4 * kRowsPerLoad);
+        using NextTile = QueryTile<T>;
+        auto next_tile = [&](int tile) {
+            NextTile n;
+            n.live = tile < total_tiles;
+            const int head = min(tile / max(tiles_per_head, 1), group - 1);
+            const int q0 = q_begin + (tile - head * tiles_per_head) * kStream;
+            RowStream of_head = q_src;
+            of_head.base += head * p.d * static_cast<int>(sizeof(T));
+            n.q = of_head.at(n.live ? q0 : 0);
+            of_head = do_src;
+            of_head.base += head * p.d * static_cast<int>(sizeof(T));
+            n.dout = of_head.at(n.live ? q0 : 0);
+            // One float per query and statistic: wavefront w brings statistic w.
+            const float* from = p.delta + wave * rows + (static_cast<long>(b) * p.qs + q0) * p.hq + kvh * group + head;
+            const long left = ((static_cast<long>(p.qs) - 1 - q0) * p.hq + 1) * static_cast<long>(sizeof(float));
+            n.stat = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(from), 0, static_cast<int>(min(left, 1l << 30)), 0x00020000);
+            n.stage = lds + (tile & 1) * 2 * kWideTile<W>;
+            n.stat_stage = stats + ((tile & 1) * 4 + wave) * kStream;
+            return n;
+        };
+        const int stat_voffset = lane * p.hq * static_cast<int>(sizeof(float));
+        auto request_part = [&](const NextTile& n, int i) {
+            if (!n.live) return;
+            if (i < kLoads) {
+                const int soffset = i * 4 * kRowsPerLoad * q_src.row_bytes;
+                T* to = n.stage + (i * 4 + wave) * kRowsPerLoad * W;
+                load_chunks(n.q, to, q_src.voffset, soffset);
+                load_chunks(n.dout, to + kWideTile<W>, do_src.voffset, soffset);
+            } else if (i == kLoads) {
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(n.stat, (lds_void_ptr)(n.stat_stage), 4, stat_voffset, 0, 0, 0);
+            }
+        };
+
+        // MASKED: some (query, key) pairs of this wavefront are hidden (causal mask, keys past the end); first = first visible register
+        // coordinate for this lane's key. Queries past the end need nothing: their dO rows, delta and lse are zeros.
+        auto tile_body = [&]<bool MASKED>(int stage, float minus_lambda, int first, const NextTile& next) {
+            constexpr int H = W / 16, kSlots = 8 * H, kLookAhead = W == 64 ? 2 : 4;
+            const TileOffsets<W> here = offsets.at(stage * 2 * kWideTile<W>);
+            const float* stat = stats + stage * 4 * kStream + 4 * (lane >> 5);
+            acc_t s_acc[2][2], g_acc[2];                        // [half][map]
+            vec_t<unsigned int, 4> p_words[2][2], ds_words[2][2][2];  // [half][16-query step], [half][map][step]: k-operands of dV, dK
+            vec_t<float, 4> lse_q[2][4][2], delta_q[2][4][2];
+            frag operand[kSlots];
+            auto read_operand = [&]<int K>() {
+                constexpr Slot at = dkv_slot(K, H);
+                if constexpr (at.product == Product::scores) operand[K] = here.row(lds, at.half * 32, at.index % 2 * HALF + at.index / 2);
+                else if constexpr (at.product == Product::grads) operand[K] = here.row(lds, kStream + at.half * 32, at.index);
+                else operand[K] = here.columns(lds, (at.product == Product::values ? kStream : 0) + at.half * 32 + at.index / DT * 16, at.index % DT);
+            };
+            auto multiply = [&]<int K>() {
+                constexpr Slot at = dkv_slot(K, H);
+                if constexpr (at.product == Product::scores) {
+                    constexpr int map = at.index % 2, s = at.index / 2;
+                    s_acc[at.half][map] = Mma<T>::run(operand[K], kf[map * HALF + s], s == 0 ? acc_t(0.0f) : s_acc[at.half][map]);
+                } else if constexpr (at.product == Product::grads) {
+                    g_acc[at.half] = Mma<T>::run(operand[K], vf[at.index], at.index == 0 ? acc_t(0.0f) : g_acc[at.half]);
+                } else {
+                    constexpr int s = at.index / DT, t = at.index % DT;
+                    if constexpr (at.product == Product::values) dv[t] = Mma<T>::run(operand[K], __builtin_bit_cast(frag, p_words[at.half][s]), dv[t]);
+                    else dk[t] = Mma<T>::run(operand[K], __builtin_bit_cast(frag, ds_words[at.half][t / (DT / 2)][s]), dk[t]);
+                }
+            };
+            // Statistics of steps N and N + 1 (N even), read a few slots ahead of them.
+            auto read_statistics = [&]<int HALF_TILE, int N, bool DELTA>() {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const auto v = *reinterpret_cast<const vec_t<float, 4>*>(stat + (i + (DELTA ? 2 : 0)) * kStream + HALF_TILE * 32 + 4 * N);
+                    if constexpr (DELTA) delta_q[HALF_TILE][N / 2][i] = v;
+                    else lse_q[HALF_TILE][N / 2][i] = v;
+                }
+            };
+            // Step N of 8 of a half: scores 2 N and 2 N + 1.
+            auto exponentials = [&]<int HALF_TILE, int N>() {
+                vec_t<float, 2> map;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    constexpr int i0 = 2 * N;
+                    float p1 = __builtin_amdgcn_exp2f(fmaf(s_acc[HALF_TILE][0][i0 + e], scale2, -lse_q[HALF_TILE][N / 2][0][(i0 & 3) + e]));
+                    float p2 = minus_lambda * __builtin_amdgcn_exp2f(fmaf(s_acc[HALF_TILE][1][i0 + e], scale2, -lse_q[HALF_TILE][N / 2][1][(i0 & 3) + e]));
+                    if constexpr (MASKED) {
+                        const bool visible = HALF_TILE * 32 + 8 * (i0 >> 2) + (i0 & 3) + e >= first;
+                        p1 = visible ? p1 : 0.0f;
+                        p2 = visible ? p2 : 0.0f;
+                    }
+                    s_acc[HALF_TILE][0][i0 + e] = p1;
+                    s_acc[HALF_TILE][1][i0 + e] = p2;
+                    map[e] = p1 + p2;
+                }
+                p_words[HALF_TILE][N / 4][N % 4] = __builtin_bit_cast(unsigned int, vec_from_f32<T, 2>(map));
+            };
+            auto gradients = [&]<int HALF_TILE, int N>() {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    vec_t<float, 2> ds;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        ds[e] = s_acc[HALF_TILE][i][2 * N + e] * (g_acc[HALF_TILE][2 * N + e] - delta_q[HALF_TILE][N / 2][i][(2 * N & 3) + e]);
+                    ds_words[HALF_TILE][i][N / 4][N % 4] = __builtin_bit_cast(unsigned int, vec_from_f32<T, 2>(ds));
+                }
+            };
+            auto beside = [&]<int K, int N>() {
+                if constexpr (N % 2 == 0) {
+                    constexpr int kAhead = W == 64 ? 1 : 3;
+                    if constexpr (exponential_slot(0, N, H) - kAhead == K) read_statistics.template operator()<0, N, false>();
+                    if constexpr (exponential_slot(1, N, H) - kAhead == K) read_statistics.template operator()<1, N, false>();
+                    if constexpr (gradient_slot(0, N, H) - kAhead == K) read_statistics.template operator()<0, N, true>();
+                    if constexpr (gradient_slot(1, N, H) - kAhead == K) read_statistics.template operator()<1, N, true>();
+                }
+                if constexpr (exponential_slot(0, N, H) == K) exponentials.template operator()<0, N>();
+                if constexpr (exponential_slot(1, N, H) == K) exponentials.template operator()<1, N>();
+                if constexpr (gradient_slot(0, N, H) == K) gradients.template operator()<0, N>();
+                if constexpr (gradient_slot(1, N, H) == K) gradients.template operator()<1, N>();
+            };
+            auto slot = [&]<int K>() {
+                if constexpr (K + kLookAhead < kSlots) read_operand.template operator()<K + kLookAhead>();
+                multiply.template operator()<K>();
+                if constexpr (K <= kLoads) request_part(next, K);
+                [&]<int... N>(std::integer_sequence<int, N...>) { (beside.template operator()<K, N>(), ...); }(std::make_integer_sequence<int, 8>{});
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            [&]<int... K>(std::integer_sequence<int, K...>) {
+                (read_operand.template operator()<K>(), ...);
+            }(std::make_integer_sequence<int, kLookAhead>{});
+            __builtin_amdgcn_sched_barrier(0);
+            [&]<int... K>(std::integer_sequence<int, K...>) { (slot.template operator()<K>(), ...); }(std::make_integer_sequence<int, kSlots>{});
+        };
+
+        // Every wavefront runs every tile; per head the tiles that need the mask come first: two loops with one straight-line body each.
+        int masked_per_head = 0;
+        if (wave_last_key >= p.ks) masked_per_head = tiles_per_head;
+        else if (p.causal) masked_per_head = min(tiles_per_head, max(0, (wave_last_key - p.offset - q_begin + kStream - 1) / kStream));
+        auto arrive = [&]() {
+            __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's part of the tile is in LDS
+            __syncthreads();                     // ... and everybody else's; the other stage is free
+        };
+        {
+            const NextTile first_tile = next_tile(first_index);
+#pragma unroll
+            for (int i = 0; i <= kLoads; ++i) request_part(first_tile, i);
+        }
+        for (int head = 0; head < group; ++head) {
+            const int tile0 = head * tiles_per_head;
+            const int begin = max(0, first_index - tile0), end = min(tiles_per_head, total_tiles - tile0);
+            if (begin >= end) continue;
+            const float minus_lambda = -p.lambda[kvh * group + head];
+            for (int t = begin; t < min(masked_per_head, end); ++t) {
+                const int tile = tile0 + t, q0 = q_begin + t * kStream;
+                arrive();
+                const int causal_first = p.causal ? k_row - p.offset - q0 - 4 * (lane >> 5) : -(1 << 30);
+                tile_body.template operator()<true>(tile & 1, minus_lambda, k_live ? causal_first : (1 << 30), next_tile(tile + 1));
+            }
+            for (int t = max(masked_per_head, begin); t < end; ++t) {
+                arrive();
+                tile_body.template operator()<false>((tile0 + t) & 1, minus_lambda, 0, next_tile(tile0 + t + 1));
+            }
+        }
+        __syncthreads();  // the next key block's first loads overwrite stage 0
+        if (!k_live) continue;
+        if (p.splits > 1) {
+            const long count = static_cast<long>(p.batch) * p.ks * kv_stride;
+            float* to = p.partial + 2 * part * count + k_offset;
+            store_columns<float, W, true>(to, p.d, false, [&](int t, int e) { return dk[t][e] * p.scale; });
+            store_columns<float, W, false>(to + count, p.d, false, [&](int t, int e) { return dv[t][e]; });
+        } else {
+            store_columns<T, W, true>(static_cast<T*>(p.dk) + k_offset, p.d, p.accumulate != 0, [&](int t, int e) { return dk[t][e] * p.scale; });
+            store_columns<T, W, false>(static_cast<T*>(p.dv) + k_offset, p.d, p.accumulate != 0, [&](int t, int e) { return dv[t][e]; });
+        }
+    }
 }
 
 template <typename Fn>
@@ -733,6 +897,44 @@ int launch_rows(const DifferentialArgs& a, hipStream_t stream) {
     return CGPTX_OK;
 }
 
+// Workgroups that share a key block: see attention.hip's dK/dV pass.
+int dkv_splits(const DifferentialArgs& a) {
+    KeyWalk walk{};
+    walk.batch = a.batch;
+    walk.qs = a.qs;
+    walk.ks = a.ks;
+    walk.hkv = a.hkv;
+    walk.group = a.hq / a.hkv;
+    walk.d = a.d;
+    walk.causal = a.causal;
+    walk.offset = a.offset;
+    walk.block_rows = kBlockRows;
+    walk.stream_rows = kStream;
+    walk.waves = 1;
+    walk.tile_us = a.d <= 64 ? 1.2 : 2.0;
+    return key_block_parts(walk);
+}
+long key_values(const DifferentialArgs& a) { return static_cast<long>(a.batch) * a.ks * a.hkv * a.d; }
+
+template <typename T, int W>
+int launch_dkv(DifferentialArgs a, hipStream_t stream) {
+    const auto kernel = differential_dkv_kernel<T, W>;
+    static const hipError_t status =
+        hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kDkvSmem<W>);
+    CGPTX_HIP(status);
+    const unsigned int key_blocks = static_cast<unsigned int>((a.ks + kBlockRows - 1) / kBlockRows);
+    const std::size_t blocks = static_cast<std::size_t>(key_blocks) * a.hkv * a.batch;
+    // Under a causal mask key blocks (i, last - i) together are as long as any other two; where the single blocks do not fill the chip
+    // their longest is shorter than a pair.
+    a.paired = a.splits == 1 && a.causal && blocks > static_cast<std::size_t>(compute_units());
+    a.by_block = a.splits > 1 && key_blocks * static_cast<unsigned int>(a.splits) < static_cast<unsigned int>(compute_units());
+    const dim3 grid(a.paired ? (key_blocks + 1) / 2 : key_blocks * static_cast<unsigned int>(a.splits), static_cast<unsigned int>(a.hkv),
+                    static_cast<unsigned int>(a.batch));
+    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), kDkvSmem<W>, stream, a);
+    CGPTX_LAUNCH_CHECK();
+    return a.splits > 1 ? launch_dkv_reduce<T>(key_values(a), a.dk, a.dv, a.partial, a.splits, a.accumulate, stream) : CGPTX_OK;
+}
+
 // Row wavefronts of a dQ launch per head: the parts of a head's dlambda.
 long lambda_parts(const DifferentialArgs& a) {
     const int block = two_parts(a) ? kBlockRows / 2 : kBlockRows;
@@ -756,26 +958,26 @@ int differential_mfma_forward(const DifferentialArgs& a, hipStream_t stream) {
     });
 }
 
-std::size_t differential_mfma_scratch(const DifferentialArgs& a) {
-    return statistics_bytes(a) + static_cast<std::size_t>(lambda_parts(a)) * a.hq * sizeof(float);
-}
-
-int differential_mfma_backward(DifferentialArgs a, void* memory, hipStream_t stream) {
+// [lse1, lse2, delta1, delta2 | dlambda's parts | parts of shared key blocks]. An arena that cannot grow shares key blocks between as
+// many workgroups as it has room for.
+int differential_mfma_backward(DifferentialArgs a, hipStream_t stream) {
+    const std::size_t lambda_bytes = (static_cast<std::size_t>(lambda_parts(a)) * a.hq * sizeof(float) + 255) & ~std::size_t{255};
+    const std::size_t fixed = statistics_bytes(a) + lambda_bytes, part = 2 * static_cast<std::size_t>(key_values(a)) * sizeof(float);
+    a.splits = dkv_splits(a);
+    auto wanted = [&] { return fixed + (a.splits > 1 ? a.splits * part : 0); };
+    void* memory = nullptr;
+    std::size_t held = 0;
+    if (int st = scratch_up_to(stream, wanted(), &memory, &held)) return st;
+    while (a.splits > 1 && held < wanted()) --a.splits;
+    if (int st = scratch(stream, wanted(), &memory)) return st;
     a.delta = static_cast<float*>(memory);
     a.lambda_partial = reinterpret_cast<float*>(static_cast<char*>(memory) + statistics_bytes(a));
+    a.partial = reinterpret_cast<float*>(static_cast<char*>(memory) + fixed);
     if (int st = dispatch(a, [&]<typename T, int W>() -> int {
             if (int s = two_parts(a) ? launch_rows<differential_dq_kernel<T, W, 2>, W, 2>(a, stream)
                                      : launch_rows<differential_dq_kernel<T, W, 1>, W, 1>(a, stream))
                 return s;
-            constexpr auto kernel = differential_dkv_kernel<T, W>;
-            static const hipError_t status =
-                hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kDkvSmem<W>);
-            CGPTX_HIP(status);
-            const dim3 grid(static_cast<unsigned int>((a.ks + kBlockRows - 1) / kBlockRows), static_cast<unsigned int>(a.hkv),
-                            static_cast<unsigned int>(a.batch));
-            hipLaunchKernelGGL(kernel, grid, dim3(kThreads), kDkvSmem<W>, stream, a);
-            CGPTX_LAUNCH_CHECK();
-            return CGPTX_OK;
+            return launch_dkv<T, W>(a, stream);
         }))
         return st;
     return differential_dlambda(a, lambda_parts(a), stream);
