@@ -347,5 +347,8 @@ struct ScratchWatch {
 
 // Number of compute units of the current device (cached).
 int compute_units();
+// Blocks of `kernel` (of `threads` threads, without dynamic LDS) that the device holds at once. Row kernels are grid-stride loops with
+// equal shares: launched with more blocks than fit, the surplus would run as a second, mostly idle round.
+int resident_blocks(const void* kernel, int threads);
 
 }  // namespace cgptx

@@ -7,8 +7,11 @@
 // would be rounding. Nothing is saved between the passes; the backward pass has the row at hand and takes its statistics
 // anew. All sums are fp32.
 //
-// One workgroup takes a row at a time and walks it as often as a sum needs (the row comes from the caches behind the
-// first walk); a second kernel walks columns for dw and db.
+// What bounds it is memory: x (and dy, residual) read once, y or dx written once. Rows of up to 16384 values stay in registers between
+// the sums and the store (layernorm_rows): a wavefront owns one or several rows, or several wavefronts one, the next row's
+// loads are in flight while a row is summed, and dw and db gather in the registers of the lanes that own their columns. Per-workgroup
+// partial sums of them go to scratch and a second launch adds them in a fixed order. Longer rows are walked as often as a sum
+// needs by a workgroup, and columns by a kernel of their own.
 #include "common.hpp"
 #include "reduce.hpp"
 
@@ -109,6 +112,234 @@ __global__ __launch_bounds__(kThreads) void layernorm_column_kernel(float* __res
     }
 }
 
+// ------------------------------------------------------------------------------------------------ rows in registers
+// 16 bytes of a row, at any element's address: a row's start is aligned as its width allows (the vector memory instructions
+// take any address).
+template <typename T>
+struct Unaligned {
+    typedef vec_t<T, kVec128<T>> type __attribute__((aligned(sizeof(T))));
+};
+// The first `count` elements from p on, zeros behind them.
+template <typename T>
+__device__ __forceinline__ vec_t<T, kVec128<T>> load_some(const T* p, int count) {
+    if (count >= kVec128<T>) return *reinterpret_cast<const typename Unaligned<T>::type*>(p);
+    vec_t<T, kVec128<T>> v(static_cast<T>(0.0f));
+#pragma unroll
+    for (int e = 0; e < kVec128<T> - 1; ++e)
+        if (e < count) v[e] = p[e];
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ void store_some(T* p, vec_t<T, kVec128<T>> v, int count) {
+    if (count >= kVec128<T>) {
+        *reinterpret_cast<typename Unaligned<T>::type*>(p) = v;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < kVec128<T> - 1; ++e)
+        if (e < count) p[e] = v[e];
+}
+
+// Sums over the LPR lanes, or the WAVES wavefronts, of a row; the same bits in all of its lanes.
+template <int LPR, int WAVES>
+__device__ __forceinline__ float row_sum(float v, float* stage) {
+    v = wave_sum<LPR>(v);
+    if constexpr (WAVES > 1) {
+        __syncthreads();
+        if ((threadIdx.x & (kWave - 1)) == 0) stage[threadIdx.x / kWave] = v;
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int s = 0; s < WAVES; ++s) v += stage[s];
+    }
+    return v;
+}
+
+// LPR lanes of a wavefront (WAVES = 1), or WAVES wavefronts, share a row; a lane holds K vectors of it.
+template <typename T, int LPR, int WAVES, int K, bool Backward>
+__global__ __launch_bounds__(WAVES > 4 ? WAVES * kWave : kThreads) void layernorm_rows_kernel(
+    T* out, float* __restrict__ partial /* [2][blocks][hidden]: dw, db */, const T* __restrict__ dy, const T* residual, const T* x,
+    const T* __restrict__ w, const T* __restrict__ bias, int rows, int hidden, float inv_hidden, float eps) {
+    constexpr int VEC = kVec128<T>;
+    constexpr int kBlockWaves = WAVES > 4 ? WAVES : kWavesPerBlock;
+    constexpr int kRowsPerWave = kWave / LPR;                                     // of WAVES = 1
+    constexpr int kRowsPerBlock = WAVES > 1 ? kBlockWaves / WAVES : kBlockWaves * kRowsPerWave;
+    static_assert(WAVES == 1 || kRowsPerBlock == 1, "the wavefronts of a row meet at the workgroup's barriers");
+    using F = vec_t<float, VEC>;
+    using V = vec_t<T, VEC>;
+    __shared__ float stage[WAVES];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int sub = WAVES > 1 ? static_cast<int>(threadIdx.x) : lane % LPR;
+    const int slot = WAVES > 1 ? 0 : wave * kRowsPerWave + lane / LPR;  // which of the workgroup's rows
+
+    int count[K];  // elements of the row that a lane's vectors hold
+    F wv[K], acc_w[K], acc_b[K], bv[K];
+#pragma unroll
+    for (int c = 0; c < K; ++c) {
+        const int col = (c * LPR * WAVES + sub) * VEC;
+        count[c] = hidden - col;
+        wv[c] = vec_to_f32<T, VEC>(load_some<T>(w + col, count[c]));
+        acc_w[c] = acc_b[c] = F(0.0f);
+        if constexpr (!Backward) bv[c] = bias != nullptr ? vec_to_f32<T, VEC>(load_some<T>(bias + col, count[c])) : F(0.0f);
+    }
+    struct Row {
+        V x[K], dy[K], residual[K];
+    };
+    auto fetch = [&](long row, Row& r) __attribute__((always_inline)) {
+        const std::size_t base = static_cast<std::size_t>(row) * hidden;
+#pragma unroll
+        for (int c = 0; c < K; ++c) {
+            const int col = (c * LPR * WAVES + sub) * VEC, n = row < rows ? count[c] : 0;
+            r.x[c] = load_some<T>(x + base + col, n);
+            if constexpr (Backward) {
+                r.dy[c] = load_some<T>(dy + base + col, n);
+                if (residual != nullptr) r.residual[c] = load_some<T>(residual + base + col, n);
+            }
+        }
+    };
+    const long stride = static_cast<long>(gridDim.x) * kRowsPerBlock;
+    Row now, next;
+    fetch(static_cast<long>(blockIdx.x) * kRowsPerBlock + slot, now);
+    for (long first = static_cast<long>(blockIdx.x) * kRowsPerBlock; first < rows; first += stride) {
+        const long row = first + slot;
+        if (first + stride < rows) fetch(row + stride, next);
+        const std::size_t base = static_cast<std::size_t>(row) * hidden;
+        F xc[K], g[K];
+        float sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < K; ++c) {
+            xc[c] = vec_to_f32<T, VEC>(now.x[c]);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) sum += xc[c][e];
+        }
+        const float mean = row_sum<LPR, WAVES>(sum, stage) * inv_hidden;
+        float squares = 0.0f;
+#pragma unroll
+        for (int c = 0; c < K; ++c)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                xc[c][e] = e < count[c] ? xc[c][e] - mean : 0.0f;
+                squares = fmaf(xc[c][e], xc[c][e], squares);
+            }
+        const float r = 1.0f / sqrtf(row_sum<LPR, WAVES>(squares, stage) * inv_hidden + eps);
+        if constexpr (Backward) {
+            float g_sum = 0.0f, gx_sum = 0.0f;
+#pragma unroll
+            for (int c = 0; c < K; ++c) {
+                g[c] = vec_to_f32<T, VEC>(now.dy[c]);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    xc[c][e] *= r;
+                    acc_w[c][e] = fmaf(g[c][e], xc[c][e], acc_w[c][e]);
+                    acc_b[c][e] += g[c][e];
+                    g[c][e] *= wv[c][e];
+                    g_sum += g[c][e];
+                    gx_sum = fmaf(g[c][e], xc[c][e], gx_sum);
+                }
+            }
+            const float g_mean = row_sum<LPR, WAVES>(g_sum, stage) * inv_hidden;
+            const float gx_mean = row_sum<LPR, WAVES>(gx_sum, stage) * inv_hidden;
+#pragma unroll
+            for (int c = 0; c < K; ++c) {
+                F v;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[e] = r * (g[c][e] - g_mean - xc[c][e] * gx_mean);
+                if (residual != nullptr) v += vec_to_f32<T, VEC>(now.residual[c]);
+                if (row < rows) store_some<T>(out + base + (c * LPR * WAVES + sub) * VEC, vec_from_f32<T, VEC>(v), count[c]);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < K; ++c) {
+                F v;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[e] = fmaf(xc[c][e] * r, wv[c][e], bv[c][e]);
+                if (row < rows) store_some<T>(out + base + (c * LPR * WAVES + sub) * VEC, vec_from_f32<T, VEC>(v), count[c]);
+            }
+        }
+        now = next;
+    }
+    if constexpr (Backward) {
+        float* const mine[2] = {partial + static_cast<std::size_t>(blockIdx.x) * hidden,
+                                partial + (static_cast<std::size_t>(gridDim.x) + blockIdx.x) * hidden};
+        if constexpr (WAVES > 1) {
+#pragma unroll
+            for (int c = 0; c < K; ++c) {
+                const int col = (c * LPR * WAVES + sub) * VEC;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (e < count[c]) {
+                        mine[0][col + e] = acc_w[c][e];
+                        mine[1][col + e] = acc_b[c][e];
+                    }
+            }
+        } else {
+            // The row slots of a wavefront, then the workgroup's wavefronts.
+            __shared__ float fold[kBlockWaves][LPR * K * VEC];
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                __syncthreads();
+#pragma unroll
+                for (int c = 0; c < K; ++c)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        float v = which == 0 ? acc_w[c][e] : acc_b[c][e];
+#pragma unroll
+                        for (int offset = LPR; offset < kWave; offset <<= 1) v += __shfl_xor(v, offset, kWave);
+                        if (lane < LPR) fold[wave][(c * LPR + sub) * VEC + e] = v;
+                    }
+                __syncthreads();
+                for (int col = threadIdx.x; col < hidden; col += kThreads) {
+                    float v = 0.0f;
+#pragma unroll
+                    for (int s = 0; s < kBlockWaves; ++s) v += fold[s][col];
+                    mine[which][col] = v;
+                }
+            }
+        }
+    }
+}
+
+// dw and, of a second row of workgroups, db from the workgroups' partial sums.
+template <typename T, int COLUMNS>
+__global__ __launch_bounds__(kFinishThreads) void layernorm_finish_kernel(T* __restrict__ dw, T* __restrict__ db,
+                                                                          const float* __restrict__ partial, int parts, int hidden, int units) {
+    __shared__ float folded[kFolded], stage[4 * COLUMNS];
+    column_partial_reduce_body<T, COLUMNS>(blockIdx.y == 0 ? dw : db, partial + blockIdx.y * static_cast<std::size_t>(parts) * hidden, parts,
+                                           hidden, 0, static_cast<int>(blockIdx.x), units, folded, stage);
+}
+
+// Kernel for rows of `hidden` values; rows of a workgroup; threads of one.
+template <typename T, bool Backward>
+struct RowPlan {
+    void (*kernel)(T*, float*, const T*, const T*, const T*, const T*, const T*, int, int, float, float) = nullptr;
+    int rows_per_block = 0, threads = 0;
+
+    template <int LPR, int WAVES, int K>
+    void take() {
+        kernel = layernorm_rows_kernel<T, LPR, WAVES, K, Backward>;
+        rows_per_block = WAVES > 1 ? 1 : kWavesPerBlock * kWave / LPR;
+        threads = WAVES > 4 ? WAVES * kWave : kThreads;
+    }
+    // Up to 32 values of a row in a lane where one wavefront has it, 16 where several do: the backward pass holds five of each.
+    explicit RowPlan(int hidden) {
+        const int vectors = (hidden + kVec128<T> - 1) / kVec128<T>;
+        constexpr bool kHalf = sizeof(T) == 2;
+        if (vectors <= 16) take<16, 1, 1>();
+        else if (vectors <= 32) take<32, 1, 1>();
+        else if (vectors <= 64) take<64, 1, 1>();
+        else if (vectors <= 128) take<64, 1, 2>();
+        else if (vectors <= 256) take<64, 1, 4>();
+        else if (vectors <= 512) take<64, 4, 2>();
+        else if (vectors <= 1024) take<64, kHalf ? 16 : 4, kHalf ? 1 : 4>();
+        else if (vectors <= 2048) take<64, 16, 2>();
+        else if (vectors <= 4096 && !kHalf) take<64, 16, kHalf ? 1 : 4>();
+    }
+    int blocks(int rows) const {
+        const int wanted = (rows + rows_per_block - 1) / rows_per_block, resident = resident_blocks(reinterpret_cast<const void*>(kernel), threads);
+        return wanted < resident ? wanted : resident;
+    }
+};
+
 int validate(const char* name, std::size_t rows, std::size_t hidden, float eps, int dtype) {
     const std::string n(name);
     if (!valid_dtype(dtype)) return fail(CGPTX_INVALID_ARGUMENT, n + ": unsupported dtype");
@@ -133,6 +364,13 @@ extern "C" int cgptx_layernorm_forward(void* output, const void* input, const vo
     auto stream = static_cast<hipStream_t>(stream_);
     const int r = static_cast<int>(rows), h = static_cast<int>(hidden);
     return dispatch_dtype(dtype, [&]<typename T>() -> int {
+        if (const RowPlan<T, false> plan(h); plan.kernel != nullptr) {
+            hipLaunchKernelGGL(plan.kernel, dim3(plan.blocks(r)), dim3(plan.threads), 0, stream, static_cast<T*>(output), nullptr, nullptr,
+                               nullptr, static_cast<const T*>(input), static_cast<const T*>(weight), static_cast<const T*>(bias), r, h,
+                               1.0f / static_cast<float>(h), epsilon);
+            CGPTX_LAUNCH_CHECK();
+            return CGPTX_OK;
+        }
         hipLaunchKernelGGL((layernorm_row_kernel<T, false>), dim3(row_blocks(r)), dim3(kThreads), 0, stream, static_cast<T*>(output),
                            nullptr, nullptr, nullptr, static_cast<const T*>(input), static_cast<const T*>(weight),
                            static_cast<const T*>(bias), r, h, 1.0f / static_cast<float>(h), epsilon);
@@ -153,6 +391,22 @@ extern "C" int cgptx_layernorm_backward(void* grad_input, void* grad_weight, voi
     return dispatch_dtype(dtype, [&]<typename T>() -> int {
         auto* dy = static_cast<const T*>(grad_output);
         auto* x = static_cast<const T*>(input);
+        if (const RowPlan<T, true> plan(h); plan.kernel != nullptr) {
+            const int blocks = plan.blocks(r);
+            void* mem = nullptr;
+            if (int s = scratch(stream, 2 * static_cast<std::size_t>(blocks) * hidden * sizeof(float), &mem)) return s;
+            auto* partial = static_cast<float*>(mem);
+            hipLaunchKernelGGL(plan.kernel, dim3(blocks), dim3(plan.threads), 0, stream, static_cast<T*>(grad_input), partial, dy,
+                               static_cast<const T*>(residual), x, static_cast<const T*>(weight), nullptr, r, h, 1.0f / static_cast<float>(h),
+                               epsilon);
+            CGPTX_LAUNCH_CHECK();
+            const int columns = finish_columns(h);
+            auto finish = columns == 16 ? layernorm_finish_kernel<T, 16> : layernorm_finish_kernel<T, 32>;
+            hipLaunchKernelGGL(finish, dim3((h + columns - 1) / columns, grad_bias != nullptr ? 2 : 1), dim3(kFinishThreads), 0, stream,
+                               static_cast<T*>(grad_weight), static_cast<T*>(grad_bias), partial, blocks, h, compute_units());
+            CGPTX_LAUNCH_CHECK();
+            return CGPTX_OK;
+        }
         const int slices = r < 256 ? 1 : (r < 65536 ? 64 : 256);
         const int rows_per_slice = (r + slices - 1) / slices;
         const std::size_t statistics_bytes = (2 * rows * sizeof(float) + 255) & ~std::size_t{255};

@@ -21,7 +21,6 @@
 #include <cmath>
 #include <limits>
 #include <mutex>
-#include <unordered_map>
 
 namespace cgptx {
 namespace {
@@ -679,30 +678,11 @@ const void* fast_kernel(const FastShape shape) {
     return nullptr;
 }
 
-// Blocks of `kernel` the device holds at once. The row kernels are grid-stride loops with equal
-// shares: launched with more blocks than fit, the surplus would run as a second, mostly idle round.
-int resident_blocks(const void* kernel) {
-    static std::mutex guard;
-    static std::unordered_map<const void*, int> known;
-    std::lock_guard<std::mutex> lock(guard);
-    auto found = known.find(kernel);
-    if (found == known.end()) {
-        int per_cu = 0;
-        if (kernel == nullptr || hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, kThreads, 0) != hipSuccess ||
-            per_cu < 1) {
-            (void)hipGetLastError();
-            per_cu = 1;
-        }
-        found = known.emplace(kernel, per_cu).first;
-    }
-    return found->second * compute_units();
-}
-
 int fast_blocks(const FastShape shape, int rows, const void* kernel) {
     const int rpw = kWave / shape.lpr;
     const long groups = (static_cast<long>(rows) + rpw - 1) / rpw;
     const long wanted = (groups + kWavesPerBlock - 1) / kWavesPerBlock;
-    const long cap = resident_blocks(kernel);
+    const long cap = resident_blocks(kernel, kThreads);
     return static_cast<int>(wanted < cap ? wanted : cap);
 }
 
@@ -811,7 +791,7 @@ struct PairPlan {
     int blocks_q, blocks_k;
     PairPlan(int rows_q, int rows_k, int head_dim, RopeArgs rope) : lanes(pair_lanes<T>(head_dim)), dense(rope_dense<T>(std::max(rows_q, rows_k), head_dim, rope) &&
                                                                                                          rows_q % 4 == 0 && rows_k % 4 == 0) {
-        const int cap = resident_blocks(reinterpret_cast<const void*>(pair_kernel<T, Backward>(lanes, dense, false)));
+        const int cap = resident_blocks(reinterpret_cast<const void*>(pair_kernel<T, Backward>(lanes, dense, false)), kThreads);
         blocks_q = std::min(pair_blocks(rows_q, lanes), cap);
         blocks_k = std::min(pair_blocks(rows_k, lanes), cap);
     }
@@ -1093,7 +1073,7 @@ std::size_t rmsnorm_backward_sink_bytes(NormPass pass, std::size_t rows, std::si
             if (lanes == 0) return CGPTX_OK;
             for (const bool dense : {false, true})
                 blocks = std::max(blocks, std::min(pair_blocks(r, lanes) + 1,
-                                                   2 * resident_blocks(reinterpret_cast<const void*>(pair_kernel<T, true>(lanes, dense, false)))));
+                                                   2 * resident_blocks(reinterpret_cast<const void*>(pair_kernel<T, true>(lanes, dense, false)), kThreads)));
         } else {
             const void* kernel = pass == NormPass::dual ? dual_kernel<T, true>(shape) : fast_kernel<T, true>(shape);
             if (kernel == nullptr) return CGPTX_OK;

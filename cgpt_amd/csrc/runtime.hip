@@ -3,6 +3,7 @@
 
 #include <map>
 #include <mutex>
+#include <unordered_map>
 #include <utility>
 #include <vector>
 
@@ -137,6 +138,23 @@ int compute_units() {
         return count;
     }();
     return cached;
+}
+
+int resident_blocks(const void* kernel, int threads) {
+    static std::mutex guard;
+    static std::unordered_map<const void*, int> known;
+    std::lock_guard<std::mutex> lock(guard);
+    auto found = known.find(kernel);
+    if (found == known.end()) {
+        int per_cu = 0;
+        if (kernel == nullptr || hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, threads, 0) != hipSuccess ||
+            per_cu < 1) {
+            (void)hipGetLastError();
+            per_cu = 1;
+        }
+        found = known.emplace(kernel, per_cu).first;
+    }
+    return found->second * compute_units();
 }
 
 }  // namespace cgptx
