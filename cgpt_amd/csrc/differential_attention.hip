@@ -12,8 +12,8 @@
 // dlambda cancels over rows and keys, and it is fp32: the dQ pass corrects the delta2 that it takes from the rounded O2 by
 // rowsum(dS2), which is what that rounding left (the rows of P2 sum to one).
 //
-// This file holds the entries and the kernels that take every call: fp32 storage, head widths that are not multiples of 16, tensors off
-// 16-byte boundaries. One wavefront per output row, fp32 arithmetic, lane l holding elements l and l + 64 of the head. No atomics: every row has one
+// This file holds the entries and the kernels that take every call: head widths that are not multiples of 16 (fp32: of 8), tensors off
+// 16-byte boundaries (differential_attention_mfma.hip and differential_attention_f32.hip have the others). One wavefront per output row, fp32 arithmetic, lane l holding elements l and l + 64 of the head. No atomics: every row has one
 // owner that adds its terms in a fixed order.
 #include "differential_attention.hpp"
 
@@ -24,7 +24,6 @@
 namespace cgptx {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kScalarWaves = kThreads / kWave;
 
 using Params = DifferentialArgs;
@@ -298,11 +297,10 @@ Params make_params(const Shape& s, const void* q, const void* k, const void* v, 
 
 unsigned int scalar_blocks(std::size_t rows) { return static_cast<unsigned int>((rows + kScalarWaves - 1) / kScalarWaves); }
 
-// The matrix kernels' calls; everything else runs on the scalar ones.
-bool on_matrix_cores(const Params& p, std::initializer_list<const void*> tensors) {
+bool aligned(std::initializer_list<const void*> tensors) {
     for (const void* t : tensors)
         if (!is_aligned16(t)) return false;  // an absent one is
-    return differential_mfma_takes(p);
+    return true;
 }
 
 int validate_lambda(const char* name, std::size_t sets, std::size_t heads, std::size_t width, int dtype) {
@@ -316,6 +314,37 @@ int validate_lambda(const char* name, std::size_t sets, std::size_t heads, std::
 }
 
 }  // namespace
+
+KeyWalk key_walk(const DifferentialArgs& a) {
+    KeyWalk walk{};
+    walk.batch = a.batch;
+    walk.qs = a.qs;
+    walk.ks = a.ks;
+    walk.hkv = a.hkv;
+    walk.group = a.hq / a.hkv;
+    walk.d = a.d;
+    walk.causal = a.causal;
+    walk.offset = a.offset;
+    return walk;
+}
+
+int differential_backward_scratch(DifferentialArgs& a, int statistics, long lambda_parts, int splits, hipStream_t stream) {
+    auto rounded = [](std::size_t bytes) { return (bytes + 255) & ~std::size_t{255}; };
+    const std::size_t first = rounded(static_cast<std::size_t>(statistics) * a.batch * a.qs * a.hq * sizeof(float));
+    const std::size_t fixed = first + rounded(static_cast<std::size_t>(lambda_parts) * a.hq * sizeof(float));
+    const std::size_t part = 2 * static_cast<std::size_t>(a.batch) * a.ks * a.hkv * a.d * sizeof(float);
+    a.splits = splits;
+    auto wanted = [&] { return fixed + (a.splits > 1 ? a.splits * part : 0); };
+    void* memory = nullptr;
+    std::size_t held = 0;
+    if (int st = scratch_up_to(stream, wanted(), &memory, &held)) return st;
+    while (a.splits > 1 && held < wanted()) --a.splits;
+    if (int st = scratch(stream, wanted(), &memory)) return st;
+    a.delta = static_cast<float*>(memory);
+    a.lambda_partial = reinterpret_cast<float*>(static_cast<char*>(memory) + first);
+    a.partial = reinterpret_cast<float*>(static_cast<char*>(memory) + fixed);
+    return CGPTX_OK;
+}
 
 int differential_dlambda(const DifferentialArgs& a, long parts, hipStream_t stream) {
     hipLaunchKernelGGL(differential_dlambda_kernel, dim3(static_cast<unsigned int>(a.hq)), dim3(kLambdaThreads), 0, stream, a.dlambda,
@@ -383,7 +412,10 @@ extern "C" int cgptx_differential_attention_forward(void* output, void* second, 
     p.out = output;
     p.second = second;
     p.lse_out = logsumexp;
-    if (on_matrix_cores(p, {output, second, query, key, value})) return differential_mfma_forward(p, static_cast<hipStream_t>(stream));
+    if (aligned({output, second, query, key, value})) {
+        if (differential_mfma_takes(p)) return differential_mfma_forward(p, static_cast<hipStream_t>(stream));
+        if (differential_f32_takes(p)) return differential_f32_forward(p, static_cast<hipStream_t>(stream));
+    }
     return dispatch_dtype(dtype, [&]<typename T>() -> int {
         hipLaunchKernelGGL((differential_forward_scalar_kernel<T>), dim3(scalar_blocks(batch * query_sequence * query_heads)),
                            dim3(kThreads), 0, static_cast<hipStream_t>(stream), p);
@@ -419,19 +451,19 @@ extern "C" int cgptx_differential_attention_backward(void* grad_query, void* gra
     p.dv = grad_value;
     p.dlambda = grad_lambda;
     p.accumulate = accumulate_grads != 0;
-    if (on_matrix_cores(p, {grad_query, grad_key, grad_value, grad_output, output, second, query, key, value}))
-        return differential_mfma_backward(p, stream);
+    if (aligned({grad_query, grad_key, grad_value, grad_output, output, second, query, key, value})) {
+        if (differential_mfma_takes(p)) return differential_mfma_backward(p, stream);
+        if (differential_f32_takes(p)) return differential_f32_backward(p, stream);
+    }
     const std::size_t rows = batch * query_sequence * query_heads;
-    void* mem = nullptr;
-    if (int st = scratch(stream, 3 * rows * sizeof(float), &mem)) return st;
-    p.delta = static_cast<float*>(mem);
-    p.lambda_partial = p.delta + 2 * rows;
+    const long lambda_parts = static_cast<long>(batch * query_sequence);
+    if (int st = differential_backward_scratch(p, 2, lambda_parts, 1, stream)) return st;
     return dispatch_dtype(dtype, [&]<typename T>() -> int {
         hipLaunchKernelGGL((differential_dq_scalar_kernel<T>), dim3(scalar_blocks(rows)), dim3(kThreads), 0, stream, p);
         CGPTX_LAUNCH_CHECK();
         hipLaunchKernelGGL((differential_dkv_scalar_kernel<T>), dim3(scalar_blocks(batch * kv_sequence * kv_heads)), dim3(kThreads), 0,
                            stream, p);
         CGPTX_LAUNCH_CHECK();
-        return differential_dlambda(p, static_cast<long>(batch * query_sequence), stream);
+        return differential_dlambda(p, lambda_parts, stream);
     });
 }

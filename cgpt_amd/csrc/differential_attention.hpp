@@ -1,7 +1,7 @@
 // What the kernels of differential attention share: the call, and the entries of the 16-bit matrix-core kernels.
 #pragma once
 
-#include "common.hpp"
+#include "attention_tiles.hpp"
 
 namespace cgptx {
 
@@ -18,7 +18,7 @@ struct DifferentialArgs {
     float scale;
     int causal, offset, accumulate;
     int dtype;
-    // dK/dV on the matrix cores, set by its launch:
+    // dK/dV on the matrix cores, set by its launch (fp32: splits only):
     int paired;      // a workgroup takes key blocks (i, last - i) instead of one
     int splits;      // workgroups that share a key block's query tiles (never with paired)
     int by_block;    // splits > 1: workgroups go out block by block over all (batch, kv-head) pairs
@@ -31,6 +31,16 @@ bool differential_mfma_takes(const DifferentialArgs& args);
 int differential_mfma_forward(const DifferentialArgs& args, hipStream_t stream);
 int differential_mfma_backward(DifferentialArgs args, hipStream_t stream);  // takes its scratch itself
 
+// The fp32 ones: halves of a head in multiples of 4, tensors on 16-byte boundaries.
+bool differential_f32_takes(const DifferentialArgs& args);
+int differential_f32_forward(const DifferentialArgs& args, hipStream_t stream);
+int differential_f32_backward(DifferentialArgs args, hipStream_t stream);
+
+// A call's part of what key_block_parts goes by.
+KeyWalk key_walk(const DifferentialArgs& args);
+// Takes a backward pass's scratch, [`statistics` floats per (batch, query, head) | dlambda's parts | parts of shared key blocks], and
+// sets args' pointers and splits: at most `splits`, as many as an arena that cannot grow has room for.
+int differential_backward_scratch(DifferentialArgs& args, int statistics, long lambda_parts, int splits, hipStream_t stream);
 // dlambda from its parts.
 int differential_dlambda(const DifferentialArgs& args, long parts, hipStream_t stream);
 

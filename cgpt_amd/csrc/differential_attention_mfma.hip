@@ -897,23 +897,6 @@ int launch_rows(const DifferentialArgs& a, hipStream_t stream) {
     return CGPTX_OK;
 }
 
-// Workgroups that share a key block: see attention.hip's dK/dV pass.
-int dkv_splits(const DifferentialArgs& a) {
-    KeyWalk walk{};
-    walk.batch = a.batch;
-    walk.qs = a.qs;
-    walk.ks = a.ks;
-    walk.hkv = a.hkv;
-    walk.group = a.hq / a.hkv;
-    walk.d = a.d;
-    walk.causal = a.causal;
-    walk.offset = a.offset;
-    walk.block_rows = kBlockRows;
-    walk.stream_rows = kStream;
-    walk.waves = 1;
-    walk.tile_us = a.d <= 64 ? 1.2 : 2.0;
-    return key_block_parts(walk);
-}
 long key_values(const DifferentialArgs& a) { return static_cast<long>(a.batch) * a.ks * a.hkv * a.d; }
 
 template <typename T, int W>
@@ -940,9 +923,6 @@ long lambda_parts(const DifferentialArgs& a) {
     const int block = two_parts(a) ? kBlockRows / 2 : kBlockRows;
     return (static_cast<long>(a.qs) + block - 1) / block * (block / 32) * a.batch;
 }
-std::size_t statistics_bytes(const DifferentialArgs& a) {
-    return (4 * static_cast<std::size_t>(a.batch) * a.qs * a.hq * sizeof(float) + 255) & ~std::size_t{255};
-}
 
 }  // namespace
 
@@ -958,21 +938,13 @@ int differential_mfma_forward(const DifferentialArgs& a, hipStream_t stream) {
     });
 }
 
-// [lse1, lse2, delta1, delta2 | dlambda's parts | parts of shared key blocks]. An arena that cannot grow shares key blocks between as
-// many workgroups as it has room for.
 int differential_mfma_backward(DifferentialArgs a, hipStream_t stream) {
-    const std::size_t lambda_bytes = (static_cast<std::size_t>(lambda_parts(a)) * a.hq * sizeof(float) + 255) & ~std::size_t{255};
-    const std::size_t fixed = statistics_bytes(a) + lambda_bytes, part = 2 * static_cast<std::size_t>(key_values(a)) * sizeof(float);
-    a.splits = dkv_splits(a);
-    auto wanted = [&] { return fixed + (a.splits > 1 ? a.splits * part : 0); };
-    void* memory = nullptr;
-    std::size_t held = 0;
-    if (int st = scratch_up_to(stream, wanted(), &memory, &held)) return st;
-    while (a.splits > 1 && held < wanted()) --a.splits;
-    if (int st = scratch(stream, wanted(), &memory)) return st;
-    a.delta = static_cast<float*>(memory);
-    a.lambda_partial = reinterpret_cast<float*>(static_cast<char*>(memory) + statistics_bytes(a));
-    a.partial = reinterpret_cast<float*>(static_cast<char*>(memory) + fixed);
+    KeyWalk walk = key_walk(a);
+    walk.block_rows = kBlockRows;
+    walk.stream_rows = kStream;
+    walk.waves = 1;
+    walk.tile_us = a.d <= 64 ? 1.2 : 2.0;
+    if (int st = differential_backward_scratch(a, 4, lambda_parts(a), key_block_parts(walk), stream)) return st;
     if (int st = dispatch(a, [&]<typename T, int W>() -> int {
             if (int s = two_parts(a) ? launch_rows<differential_dq_kernel<T, W, 2>, W, 2>(a, stream)
                                      : launch_rows<differential_dq_kernel<T, W, 1>, W, 1>(a, stream))
