@@ -56,6 +56,9 @@ __device__ __forceinline__ RowStream make_stream(const void* tensor, long offset
     s.voffset = column >= 0 ? r * s.row_bytes + column * static_cast<int>(sizeof(T)) : (1 << 30);
     return s;
 }
+__device__ __forceinline__ vec_t<unsigned int, 4> load_words(__amdgpu_buffer_rsrc_t rsrc, int voffset) {
+    return __builtin_bit_cast(vec_t<unsigned int, 4>, __builtin_amdgcn_raw_buffer_load_b128(rsrc, voffset, 0, 0));
+}
 // 16 bytes per lane, 1 KiB in all, straight into LDS.
 __device__ __forceinline__ void load_chunks(__amdgpu_buffer_rsrc_t rsrc, void* to, int voffset, int soffset) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_ptr)(to), 16, voffset, soffset, 0, 0);
@@ -93,61 +96,99 @@ struct TileOffsets {
     }
 };
 
-// The operand that stays in registers, from global memory: lane -> row lane%32, padded columns 16*step + 8*(lane/32) .. + 7.
+// The operand that stays in registers, from global memory: lane -> row row0 + lane%32 of a tensor's (batch, head), padded columns
+// 16*step + 8*(lane/32) .. + 7; rows past the end are zeros.
 template <typename T, int W, bool HALVES>
-__device__ __forceinline__ typename Mma<T>::frag row_frag(const T* row, bool live, int step, int d) {
+__device__ __forceinline__ void load_rows(typename Mma<T>::frag (&rows)[W / 16], const void* tensor, long offset, long row_stride, int count, int row0,
+                                          int d) {
     using frag = typename Mma<T>::frag;
-    const int column = source_column<W, HALVES>(step * 16 + ((threadIdx.x & 63) >> 5) * 8, d);
-    if (live && column >= 0) return *reinterpret_cast<const frag*>(row + column);
-    return frag(static_cast<T>(0.0f));
+    const int lane = threadIdx.x & 63;
+    RowStream s;
+    s.base = static_cast<const char*>(tensor) + offset * static_cast<long>(sizeof(T));
+    s.row_bytes = static_cast<int>(row_stride * sizeof(T));
+    s.bytes = ((count - 1) * row_stride + d) * static_cast<long>(sizeof(T));
+    const __amdgpu_buffer_rsrc_t rsrc = s.at(min(row0, count - 1));
+    const int row = row0 < count ? (lane & 31) * s.row_bytes : 1 << 30;
+#pragma unroll
+    for (int i = 0; i < W / 16; ++i) {
+        const int column = source_column<W, HALVES>(i * 16 + (lane >> 5) * 8, d);
+        rows[i] = __builtin_bit_cast(frag, load_words(rsrc, column >= 0 ? row + column * static_cast<int>(sizeof(T)) : 1 << 30));
+    }
 }
 
 // Stores a wavefront's transposed accumulators (lane = row, registers = padded columns) times a factor, four elements at a time.
-// value(t, g, e) is element e of quad g of column block t.
+// value(t, r) is register r of column block t. (fp32: parts, stored without adding.)
 template <typename T, int W, bool HALVES, typename Value>
 __device__ __forceinline__ void store_columns(T* row, int d, bool accumulate, Value&& value) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int t = 0; t < W / 32; ++t)
+    for (int t = 0; t < W / 32; ++t) {
+        if constexpr (sizeof(T) == 2) {
+            // A lane has quads of its row's columns, its partner in the other half of the wavefront the quads between: swapped, a lane has
+            // eight in a row of every other group.
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int c = t * 32 + g * 8, column = source_column<W, HALVES>(c, d);
-            if (column < 0) continue;
-            T* to = row + column + (lane >> 5) * 4;
-            vec_t<float, 4> v;
+            for (int g = 0; g < 4; g += 2) {
+                const int column = source_column<W, HALVES>(t * 32 + (g + (lane >> 5)) * 8, d);
+                float v[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = value(t, 4 * g + e);
-            if (accumulate) v += vec_to_f32<T, 4>(load_vec<T, 4>(to));
-            store_vec<T, 4>(to, vec_from_f32<T, 4>(v));
+                for (int e = 0; e < 4; ++e) {
+                    const auto swapped = __builtin_amdgcn_permlane32_swap(__float_as_uint(value(t, 4 * g + e)), __float_as_uint(value(t, 4 * g + 4 + e)),
+                                                                          false, false);
+                    v[e] = __uint_as_float(swapped[0]);
+                    v[4 + e] = __uint_as_float(swapped[1]);
+                }
+                if (column < 0) continue;
+                vec_t<float, 8> sum{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+                if (accumulate) sum += vec_to_f32<T, 8>(load_vec<T, 8>(row + column));
+                store_vec<T, 8>(row + column, vec_from_f32<T, 8>(sum));
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int column = source_column<W, HALVES>(t * 32 + g * 8, d);
+                if (column < 0) continue;
+                T* to = row + column + (lane >> 5) * 4;
+                vec_t<float, 4> v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = value(t, 4 * g + e);
+                store_vec<T, 4>(to, v);
+            }
         }
+    }
 }
 
-// Whether a 64-row tile holds an Inf or a NaN (the same answer in all lanes): the largest exponent and fraction of any sign.
+// Whether rows `from` .. 63 of a tile hold an Inf or a NaN (the same answer in all lanes): their products with 0 are not 0. Looked at in
+// halves of 32 rows.
 template <typename T, int W>
-__device__ __forceinline__ bool not_finite(const T* tile) {
-    using halves = vec_t<unsigned short, 8>;
-    constexpr unsigned short kInfinite = __is_same(T, f16_t) ? 0x7C00 : 0x7F80;
-    halves top(0);
+__device__ __forceinline__ bool not_finite(const T* tile, int from) {
+    using pair = vec_t<T, 2>;
+    float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < W / 8; ++i) {
-        const halves v = *reinterpret_cast<const halves*>(tile + (i * kWave + (threadIdx.x & 63)) * 8);
-        top = __builtin_elementwise_max(top, v & static_cast<unsigned short>(0x7FFF));
+    for (int half = 0; half < 2; ++half) {
+        if (half == 0 && from >= 32) continue;
+#pragma unroll
+        for (int i = 0; i < W / 16; ++i) {
+            const auto words = *reinterpret_cast<const vec_t<unsigned int, 4>*>(tile + ((half * (W / 16) + i) * kWave + (threadIdx.x & 63)) * 8);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const pair x = __builtin_bit_cast(pair, words[w]), zeros(static_cast<T>(0.0f));
+                if constexpr (__is_same(T, f16_t)) sum = __builtin_amdgcn_fdot2(x, zeros, sum, false);
+                else sum = __builtin_amdgcn_fdot2_f32_bf16(x, zeros, sum, false);
+            }
+        }
     }
-    bool any = false;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) any |= top[e] >= kInfinite;
-    return __any(any);
+    return __any(!(sum == 0.0f));
 }
 // A hidden key's probability is 0, but 0 x Inf is NaN in the matrix instruction: a tile on the causal diagonal (at most two of a
 // wavefront's) that is not finite is left out of the products and added key by key behind the walk, by the lanes that see the key.
 struct LeftOut {
-    int first, tiles = 0;  // first tile with a key that a row of the wavefront does not see; bits of those from there on
+    int hidden, first, tiles = 0;  // first key that a row of the wavefront does not see, its tile; bits of the tiles from there on
     __device__ __forceinline__ LeftOut(const DifferentialArgs& p, int wave_first_q)
-        : first(p.causal ? (p.offset + wave_first_q + 1) / kStream : 1 << 30) {}
+        : hidden(p.offset + wave_first_q + 1), first(p.causal ? hidden / kStream : 1 << 30) {}
     // Whether tile j is one of them (the wavefront's causal mask allows it and the tile's values are not finite).
     template <typename T, int W>
     __device__ __forceinline__ bool out(int j, const T* tile) {
-        if (j < first || !not_finite<T, W>(tile)) return false;
+        if (j < first || !not_finite<T, W>(tile, hidden - j * kStream)) return false;
         tiles |= 1 << (j - first);
         return true;
     }
@@ -236,8 +277,8 @@ __global__ __launch_bounds__(kThreads, 2) void differential_forward_kernel(Diffe
     request(0, lds);
 
     frag qf[STEPS];
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) qf[s] = row_frag<T, W, true>(static_cast<const T*>(p.q) + q_offset, at.live, s, p.d);
+    const long head = static_cast<long>(at.b) * p.qs * q_stride + at.h * p.d;
+    load_rows<T, W, true>(qf, p.q, head, q_stride, p.qs, at.q_block + at.row_wave * 32, p.d);
     const TileOffsets<W> offsets(lane);
 
     // Both maps' sums, and their running maxima m of the raw scores (the scale is positive) as in attention.hip: mb = m * scale2, 0 while
@@ -450,15 +491,19 @@ __global__ __launch_bounds__(kThreads, 2) void differential_dq_kernel(Differenti
     request(0, lds);
 
     frag qf[STEPS], dof[STEPS];
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-        qf[s] = row_frag<T, W, true>(static_cast<const T*>(p.q) + q_offset, at.live, s, p.d);
-        dof[s] = row_frag<T, W, false>(static_cast<const T*>(p.dout) + q_offset, at.live, s, p.d);
-    }
+    const long head = static_cast<long>(at.b) * p.qs * q_stride + at.h * p.d;
+    load_rows<T, W, true>(qf, p.q, head, q_stride, p.qs, at.q_block + at.row_wave * 32, p.d);
+    load_rows<T, W, false>(dof, p.dout, head, q_stride, p.qs, at.q_block + at.row_wave * 32, p.d);
     const float lambda = p.lambda[at.h];
     const long rows = static_cast<long>(p.batch) * p.qs * p.hq, row = (static_cast<long>(at.b) * p.qs + at.q_row) * p.hq + at.h;
-    const float delta2 = row_delta<T, STEPS>(dof, static_cast<const T*>(p.o2) + q_offset, at.live, p.d);
-    const float delta1 = fmaf(lambda, delta2, row_delta<T, STEPS>(dof, static_cast<const T*>(p.o) + q_offset, at.live, p.d));
+    float delta1, delta2;
+    {
+        frag of[STEPS], o2f[STEPS];
+        load_rows<T, W, false>(of, p.o, head, q_stride, p.qs, at.q_block + at.row_wave * 32, p.d);
+        load_rows<T, W, false>(o2f, p.o2, head, q_stride, p.qs, at.q_block + at.row_wave * 32, p.d);
+        delta2 = row_delta<T, STEPS>(dof, o2f);
+        delta1 = fmaf(lambda, delta2, row_delta<T, STEPS>(dof, of));
+    }
     const float lse1 = at.live ? p.lse[row] * kLog2e : 0.0f, lse2 = at.live ? p.lse[rows + row] * kLog2e : 0.0f;
     if (at.live && at.part == 0 && lane < 32) {
         p.delta[row] = lse1;
@@ -680,13 +725,10 @@ __global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(Different
         const int k_block = block_index * kBlockRows;
         const int k_row = k_block + wave * 32 + (lane & 31);
         const bool k_live = k_row < p.ks;
-        const long k_offset = (static_cast<long>(b) * p.ks + k_row) * kv_stride + kvh * p.d;
+        const long k_head = static_cast<long>(b) * p.ks * kv_stride + kvh * p.d, k_offset = k_head + k_row * kv_stride;
         frag kf[STEPS], vf[STEPS];
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            kf[s] = row_frag<T, W, true>(static_cast<const T*>(p.k) + k_offset, k_live, s, p.d);
-            vf[s] = row_frag<T, W, false>(static_cast<const T*>(p.v) + k_offset, k_live, s, p.d);
-        }
+        load_rows<T, W, true>(kf, p.k, k_head, kv_stride, p.ks, k_block + wave * 32, p.d);
+        load_rows<T, W, false>(vf, p.v, k_head, kv_stride, p.ks, k_block + wave * 32, p.d);
         acc_t dk[DT], dv[DT];
 #pragma unroll
         for (int t = 0; t < DT; ++t) dk[t] = dv[t] = acc_t(0.0f);
