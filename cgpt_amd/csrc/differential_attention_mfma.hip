@@ -8,8 +8,8 @@
 //
 //   forward : block = 128 queries of one (batch, q-head), wave = 32 queries; streams 64-key K/V tiles; per tile and map Sᵀ = K·Qᵀ
 //             and its softmax, then Oᵀ_i += Vᵀ·Pᵀ_i for both maps from the same fragments of V.
-//   dQ      : same shape; Sᵀ_i = K_i·Qᵀ_i, Gᵀ = V·dOᵀ, dQᵀ_i += Kᵀ_i·dSᵀ_i. Leaves LSE·log2 e and delta of both maps for the
-//             dK/dV pass, and dlambda's parts.
+//   dQ      : same shape; Sᵀ_i = K_i·Qᵀ_i, Gᵀ = V·dOᵀ, dQᵀ_i += Kᵀ_i·dSᵀ_i. Leaves both maps' statistics for the dK/dV pass, and
+//             dlambda's parts.
 //   dK/dV   : block = 128 keys of one (batch, kv-head), wave = 32 keys; streams 64-query Q/dO tiles of every q-head of the group.
 #include "attention_tiles.hpp"
 #include "differential_attention.hpp"
@@ -463,6 +463,9 @@ __global__ __launch_bounds__(kThreads, 2) void differential_forward_kernel(Diffe
     }
 }
 
+// The sign of -lambda.
+__device__ __forceinline__ float sign_of_second(float lambda) { return lambda > 0.0f ? -1.0f : 1.0f; }
+
 template <typename T, int W, int PARTS>
 __global__ __launch_bounds__(kThreads, 2) void differential_dq_kernel(DifferentialArgs p) {
     using frag = typename Mma<T>::frag;
@@ -506,10 +509,12 @@ __global__ __launch_bounds__(kThreads, 2) void differential_dq_kernel(Differenti
     }
     const float lse1 = at.live ? p.lse[row] * kLog2e : 0.0f, lse2 = at.live ? p.lse[rows + row] * kLog2e : 0.0f;
     if (at.live && at.part == 0 && lane < 32) {
+        // In the form that the dK/dV pass needs fewest instructions for: |lambda| inside the second map's exponent, and its sign, as
+        // that of -lambda, on what is left of its score gradient, whose G already has delta1 taken off.
         p.delta[row] = lse1;
-        p.delta[rows + row] = lse2;
-        p.delta[2 * rows + row] = delta1;
-        p.delta[3 * rows + row] = delta2;
+        p.delta[rows + row] = lse2 - log2f(fabsf(lambda));
+        p.delta[2 * rows + row] = -delta1;
+        p.delta[3 * rows + row] = sign_of_second(lambda) * (delta1 - delta2);
     }
     int k_off[STEPS], kt_off[DT][2];
 #pragma unroll
@@ -688,7 +693,7 @@ __global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(Different
     constexpr int STEPS = W / 16, HALF = STEPS / 2, DT = W / 32;
     extern __shared__ __align__(1024) unsigned char wide_smem[];
     T* lds = reinterpret_cast<T*>(wide_smem);                                           // [stage][Q | dO]
-    float* stats = reinterpret_cast<float*>(wide_smem + 4 * kWideTile<W> * sizeof(T));  // [stage][lse1, lse2, delta1, delta2][64]
+    float* stats = reinterpret_cast<float*>(wide_smem + 4 * kWideTile<W> * sizeof(T));  // [stage][the dQ pass's four][64]
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Workgroup -> (key block or pair of them, kv head, batch entry), as in attention.hip's dK/dV: the owners of an XCD's workgroups
@@ -776,13 +781,13 @@ __global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(Different
 
         // MASKED: some (query, key) pairs of this wavefront are hidden (causal mask, keys past the end); first = first visible register
         // coordinate for this lane's key. Queries past the end need nothing: their dO rows, delta and lse are zeros.
-        auto tile_body = [&]<bool MASKED>(int stage, float minus_lambda, int first, const NextTile& next) {
+        auto tile_body = [&]<bool MASKED>(int stage, float sign, int first, const NextTile& next) {
             constexpr int H = W / 16, kSlots = 8 * H, kLookAhead = W == 64 ? 2 : 4;
             const TileOffsets<W> here = offsets.at(stage * 2 * kWideTile<W>);
             const float* stat = stats + stage * 4 * kStream + 4 * (lane >> 5);
-            acc_t s_acc[2][2], g_acc[2];                        // [half][map]
+            acc_t s_acc[2][2], g_acc[2];                              // [half][map]
             vec_t<unsigned int, 4> p_words[2][2], ds_words[2][2][2];  // [half][16-query step], [half][map][step]: k-operands of dV, dK
-            vec_t<float, 4> lse_q[2][4][2], delta_q[2][4][2];
+            vec_t<float, 4> lse_q[2][4][2], delta_q[2][4];
             frag operand[kSlots];
             auto read_operand = [&]<int K>() {
                 constexpr Slot at = dkv_slot(K, H);
@@ -796,20 +801,26 @@ __global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(Different
                     constexpr int map = at.index % 2, s = at.index / 2;
                     s_acc[at.half][map] = Mma<T>::run(operand[K], kf[map * HALF + s], s == 0 ? acc_t(0.0f) : s_acc[at.half][map]);
                 } else if constexpr (at.product == Product::grads) {
-                    g_acc[at.half] = Mma<T>::run(operand[K], vf[at.index], at.index == 0 ? acc_t(0.0f) : g_acc[at.half]);
+                    g_acc[at.half] = Mma<T>::run(operand[K], vf[at.index], g_acc[at.half]);  // from -delta1 on
                 } else {
                     constexpr int s = at.index / DT, t = at.index % DT;
                     if constexpr (at.product == Product::values) dv[t] = Mma<T>::run(operand[K], __builtin_bit_cast(frag, p_words[at.half][s]), dv[t]);
                     else dk[t] = Mma<T>::run(operand[K], __builtin_bit_cast(frag, ds_words[at.half][t / (DT / 2)][s]), dk[t]);
                 }
             };
-            // Statistics of steps N and N + 1 (N even), read a few slots ahead of them.
-            auto read_statistics = [&]<int HALF_TILE, int N, bool DELTA>() {
+            // Statistics of steps N and N + 1 (N even), read a few slots ahead of them: KIND 0 both lse, 1 -delta1 (where G's sums
+            // start), 2 what the second map's score gradient differs by.
+            auto read_statistics = [&]<int HALF_TILE, int N, int KIND>() {
+                auto read = [&](int which) { return *reinterpret_cast<const vec_t<float, 4>*>(stat + which * kStream + HALF_TILE * 32 + 4 * N); };
+                if constexpr (KIND == 0) {
+                    lse_q[HALF_TILE][N / 2][0] = read(0);
+                    lse_q[HALF_TILE][N / 2][1] = read(1);
+                } else if constexpr (KIND == 1) {
+                    const vec_t<float, 4> v = read(2);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const auto v = *reinterpret_cast<const vec_t<float, 4>*>(stat + (i + (DELTA ? 2 : 0)) * kStream + HALF_TILE * 32 + 4 * N);
-                    if constexpr (DELTA) delta_q[HALF_TILE][N / 2][i] = v;
-                    else lse_q[HALF_TILE][N / 2][i] = v;
+                    for (int e = 0; e < 4; ++e) g_acc[HALF_TILE][2 * N + e] = v[e];
+                } else {
+                    delta_q[HALF_TILE][N / 2] = read(3);
                 }
             };
             // Step N of 8 of a half: scores 2 N and 2 N + 1.
@@ -819,7 +830,7 @@ __global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(Different
                 for (int e = 0; e < 2; ++e) {
                     constexpr int i0 = 2 * N;
                     float p1 = __builtin_amdgcn_exp2f(fmaf(s_acc[HALF_TILE][0][i0 + e], scale2, -lse_q[HALF_TILE][N / 2][0][(i0 & 3) + e]));
-                    float p2 = minus_lambda * __builtin_amdgcn_exp2f(fmaf(s_acc[HALF_TILE][1][i0 + e], scale2, -lse_q[HALF_TILE][N / 2][1][(i0 & 3) + e]));
+                    float p2 = __builtin_amdgcn_exp2f(fmaf(s_acc[HALF_TILE][1][i0 + e], scale2, -lse_q[HALF_TILE][N / 2][1][(i0 & 3) + e]));
                     if constexpr (MASKED) {
                         const bool visible = HALF_TILE * 32 + 8 * (i0 >> 2) + (i0 & 3) + e >= first;
                         p1 = visible ? p1 : 0.0f;
@@ -827,27 +838,30 @@ __global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(Different
                     }
                     s_acc[HALF_TILE][0][i0 + e] = p1;
                     s_acc[HALF_TILE][1][i0 + e] = p2;
-                    map[e] = p1 + p2;
+                    map[e] = fmaf(sign, p2, p1);
                 }
                 p_words[HALF_TILE][N / 4][N % 4] = __builtin_bit_cast(unsigned int, vec_from_f32<T, 2>(map));
             };
             auto gradients = [&]<int HALF_TILE, int N>() {
+                vec_t<float, 2> first_map, second_map;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    vec_t<float, 2> ds;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        ds[e] = s_acc[HALF_TILE][i][2 * N + e] * (g_acc[HALF_TILE][2 * N + e] - delta_q[HALF_TILE][N / 2][i][(2 * N & 3) + e]);
-                    ds_words[HALF_TILE][i][N / 4][N % 4] = __builtin_bit_cast(unsigned int, vec_from_f32<T, 2>(ds));
+                for (int e = 0; e < 2; ++e) {
+                    const float g = g_acc[HALF_TILE][2 * N + e];  // G - delta1
+                    first_map[e] = s_acc[HALF_TILE][0][2 * N + e] * g;
+                    second_map[e] = s_acc[HALF_TILE][1][2 * N + e] * fmaf(sign, g, delta_q[HALF_TILE][N / 2][(2 * N & 3) + e]);
                 }
+                ds_words[HALF_TILE][0][N / 4][N % 4] = __builtin_bit_cast(unsigned int, vec_from_f32<T, 2>(first_map));
+                ds_words[HALF_TILE][1][N / 4][N % 4] = __builtin_bit_cast(unsigned int, vec_from_f32<T, 2>(second_map));
             };
             auto beside = [&]<int K, int N>() {
                 if constexpr (N % 2 == 0) {
                     constexpr int kAhead = W == 64 ? 1 : 3;
-                    if constexpr (exponential_slot(0, N, H) - kAhead == K) read_statistics.template operator()<0, N, false>();
-                    if constexpr (exponential_slot(1, N, H) - kAhead == K) read_statistics.template operator()<1, N, false>();
-                    if constexpr (gradient_slot(0, N, H) - kAhead == K) read_statistics.template operator()<0, N, true>();
-                    if constexpr (gradient_slot(1, N, H) - kAhead == K) read_statistics.template operator()<1, N, true>();
+                    if constexpr (exponential_slot(0, N, H) - kAhead == K) read_statistics.template operator()<0, N, 0>();
+                    if constexpr (exponential_slot(1, N, H) - kAhead == K) read_statistics.template operator()<1, N, 0>();
+                    if constexpr (H - kAhead == K) read_statistics.template operator()<0, N, 1>();
+                    if constexpr (3 * H - kAhead == K) read_statistics.template operator()<1, N, 1>();
+                    if constexpr (gradient_slot(0, N, H) - kAhead == K) read_statistics.template operator()<0, N, 2>();
+                    if constexpr (gradient_slot(1, N, H) - kAhead == K) read_statistics.template operator()<1, N, 2>();
                 }
                 if constexpr (exponential_slot(0, N, H) == K) exponentials.template operator()<0, N>();
                 if constexpr (exponential_slot(1, N, H) == K) exponentials.template operator()<1, N>();
@@ -885,16 +899,16 @@ __global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(Different
             const int tile0 = head * tiles_per_head;
             const int begin = max(0, first_index - tile0), end = min(tiles_per_head, total_tiles - tile0);
             if (begin >= end) continue;
-            const float minus_lambda = -p.lambda[kvh * group + head];
+            const float sign = sign_of_second(p.lambda[kvh * group + head]);
             for (int t = begin; t < min(masked_per_head, end); ++t) {
                 const int tile = tile0 + t, q0 = q_begin + t * kStream;
                 arrive();
                 const int causal_first = p.causal ? k_row - p.offset - q0 - 4 * (lane >> 5) : -(1 << 30);
-                tile_body.template operator()<true>(tile & 1, minus_lambda, k_live ? causal_first : (1 << 30), next_tile(tile + 1));
+                tile_body.template operator()<true>(tile & 1, sign, k_live ? causal_first : (1 << 30), next_tile(tile + 1));
             }
             for (int t = max(masked_per_head, begin); t < end; ++t) {
                 arrive();
-                tile_body.template operator()<false>((tile0 + t) & 1, minus_lambda, 0, next_tile(tile0 + t + 1));
+                tile_body.template operator()<false>((tile0 + t) & 1, sign, 0, next_tile(tile0 + t + 1));
             }
         }
         __syncthreads();  // the next key block's first loads overwrite stage 0
