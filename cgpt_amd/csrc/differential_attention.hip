@@ -150,6 +150,8 @@ __global__ __launch_bounds__(kThreads) void differential_dq_scalar_kernel(Params
 // see the key in ascending order.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void differential_dkv_scalar_kernel(Params p) {
+    __shared__ double stage[kScalarWaves];
+    add_lambda_parts<kThreads>(p, stage);
     const long row = static_cast<long>(blockIdx.x) * kScalarWaves + threadIdx.x / kWave;
     if (row >= static_cast<long>(p.batch) * p.ks * p.hkv) return;
     const long rows = static_cast<long>(p.batch) * p.qs * p.hq;
@@ -181,21 +183,6 @@ __global__ __launch_bounds__(kThreads) void differential_dkv_scalar_kernel(Param
     dk.b *= p.scale;
     dk.store(static_cast<T*>(p.dk) + row * p.d, p.d, p.accumulate != 0);
     dv.store(static_cast<T*>(p.dv) + row * p.d, p.d, p.accumulate != 0);
-}
-
-// dlambda of a head per workgroup, from its `parts` parts in an order that they alone fix.
-constexpr int kLambdaThreads = 1024;
-__global__ __launch_bounds__(kLambdaThreads) void differential_dlambda_kernel(float* dlambda, const float* __restrict__ partial,
-                                                                              long parts, int accumulate) {
-    __shared__ double stage[kLambdaThreads];
-    const float* from = partial + blockIdx.x * parts;
-    double sum = 0.0;
-    for (long i = threadIdx.x; i < parts; i += kLambdaThreads) sum += from[i];
-    stage[threadIdx.x] = sum;
-    __syncthreads();
-    if (threadIdx.x >= kWave) return;
-    sum = tree_sum_1024(stage);
-    if (threadIdx.x == 0) dlambda[blockIdx.x] = static_cast<float>(accumulate ? sum + dlambda[blockIdx.x] : sum);
 }
 
 // ------------------------------------------------------------------------------------------------ lambda
@@ -333,6 +320,7 @@ int differential_backward_scratch(DifferentialArgs& a, int statistics, long lamb
     const std::size_t first = rounded(static_cast<std::size_t>(statistics) * a.batch * a.qs * a.hq * sizeof(float));
     const std::size_t fixed = first + rounded(static_cast<std::size_t>(lambda_parts) * a.hq * sizeof(float));
     const std::size_t part = 2 * static_cast<std::size_t>(a.batch) * a.ks * a.hkv * a.d * sizeof(float);
+    a.lambda_parts = lambda_parts;
     a.splits = splits;
     auto wanted = [&] { return fixed + (a.splits > 1 ? a.splits * part : 0); };
     void* memory = nullptr;
@@ -343,13 +331,6 @@ int differential_backward_scratch(DifferentialArgs& a, int statistics, long lamb
     a.delta = static_cast<float*>(memory);
     a.lambda_partial = reinterpret_cast<float*>(static_cast<char*>(memory) + first);
     a.partial = reinterpret_cast<float*>(static_cast<char*>(memory) + fixed);
-    return CGPTX_OK;
-}
-
-int differential_dlambda(const DifferentialArgs& a, long parts, hipStream_t stream) {
-    hipLaunchKernelGGL(differential_dlambda_kernel, dim3(static_cast<unsigned int>(a.hq)), dim3(kLambdaThreads), 0, stream, a.dlambda,
-                       a.lambda_partial, parts, a.accumulate);
-    CGPTX_LAUNCH_CHECK();
     return CGPTX_OK;
 }
 
@@ -464,6 +445,6 @@ extern "C" int cgptx_differential_attention_backward(void* grad_query, void* gra
         hipLaunchKernelGGL((differential_dkv_scalar_kernel<T>), dim3(scalar_blocks(batch * kv_sequence * kv_heads)), dim3(kThreads), 0,
                            stream, p);
         CGPTX_LAUNCH_CHECK();
-        return differential_dlambda(p, lambda_parts, stream);
+        return CGPTX_OK;
     });
 }

@@ -13,7 +13,8 @@ struct DifferentialArgs {
     const void *q, *k, *v, *dout, *o, *o2;
     const float *lambda, *lse;
     float* delta;           // scalar kernels [2][batch, qs, hq]: delta1, delta2; matrix kernels [4]: those behind both LSE·log2 e
-    float* lambda_partial;  // [hq][parts]: what a head's dlambda is the sum of
+    float* lambda_partial;  // [hq][lambda_parts]: what a head's dlambda is the sum of
+    long lambda_parts;
     int batch, qs, ks, hq, hkv, d;
     float scale;
     int causal, offset, accumulate;
@@ -41,7 +42,25 @@ KeyWalk key_walk(const DifferentialArgs& args);
 // Takes a backward pass's scratch, [`statistics` floats per (batch, query, head) | dlambda's parts | parts of shared key blocks], and
 // sets args' pointers and splits: at most `splits`, as many as an arena that cannot grow has room for.
 int differential_backward_scratch(DifferentialArgs& args, int statistics, long lambda_parts, int splits, hipStream_t stream);
-// dlambda from its parts.
-int differential_dlambda(const DifferentialArgs& args, long parts, hipStream_t stream);
+// dlambda from the parts that the dQ pass left, by the workgroups of the dK/dV pass that follows it, which has THREADS threads in each and
+// none but this to add: a launch of its own took 3 to 5 us. From the last workgroup on, as the first ones have most to do. A
+// head's sum has an order of its own, whatever the grid: every THREADS-th part in a thread, then a tree.
+template <int THREADS>
+__device__ __forceinline__ void add_lambda_parts(const DifferentialArgs& p, double* stage /* [THREADS / 64] */) {
+    const unsigned int blocks = gridDim.x * gridDim.y * gridDim.z;
+    const unsigned int linear = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z);
+    for (unsigned int h = blocks - 1 - linear; h < static_cast<unsigned int>(p.hq); h += blocks) {
+        const float* from = p.lambda_partial + h * p.lambda_parts;
+        double sum = 0.0;
+        for (long i = threadIdx.x; i < p.lambda_parts; i += THREADS) sum += from[i];
+        sum = tree_sum_64(sum);
+        __syncthreads();
+        if (threadIdx.x % kWave == 0) stage[threadIdx.x / kWave] = sum;
+        __syncthreads();
+        if (threadIdx.x != 0) continue;
+        for (int w = 1; w < THREADS / kWave; ++w) sum += stage[w];
+        p.dlambda[h] = static_cast<float>(p.accumulate ? sum + p.dlambda[h] : sum);
+    }
+}
 
 }  // namespace cgptx

@@ -407,7 +407,7 @@ __global__ __launch_bounds__(kF32Threads) void differential_f32_dq_kernel(Differ
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) sum += wave_rest[w][lane];
         sum = wave_sum<kTile>(sum);
-        if (lane == 0) p.lambda_partial[(static_cast<long>(h) * p.batch + b) * gridDim.x + q0 / kTile] = -sum;
+        if (lane == 0) p.lambda_partial[h * p.lambda_parts + static_cast<long>(b) * gridDim.x + q0 / kTile] = -sum;
     }
     const Share<D> share;
     quad sum = share.collect(lds);
@@ -522,6 +522,8 @@ __global__ __launch_bounds__(kF32Threads) void differential_f32_dkv_kernel(Diffe
     deposit<D, false>(lds, wave, dv, 1.0f);
     __syncthreads();
     store(static_cast<float*>(p.dv), p.partial + (2 * part + 1) * count, share.collect(lds), source<D, false>(share.at, p.d));
+    __syncthreads();
+    add_lambda_parts<kF32Threads>(p, reinterpret_cast<double*>(lds));
 }
 
 template <auto Kernel, int SMEM>
@@ -550,8 +552,7 @@ int differential_f32_backward(DifferentialArgs a, hipStream_t stream) {
     walk.block_rows = walk.stream_rows = kTile;
     walk.waves = kWaves;
     walk.tile_us = 10.0;
-    const long lambda_parts = row_tiles(a.qs) * a.batch;
-    if (int st = differential_backward_scratch(a, 2, lambda_parts, key_block_parts(walk), stream)) return st;
+    if (int st = differential_backward_scratch(a, 2, row_tiles(a.qs) * a.batch, key_block_parts(walk), stream)) return st;
     if (int st = a.d <= 64 ? launch<differential_f32_dq_kernel<64>, kSmemBytes<64>>(row_tiles(a.qs), a.hq, a, stream)
                            : launch<differential_f32_dq_kernel<128>, kSmemBytes<128>>(row_tiles(a.qs), a.hq, a, stream))
         return st;
@@ -562,7 +563,7 @@ int differential_f32_backward(DifferentialArgs a, hipStream_t stream) {
         const long count = static_cast<long>(a.batch) * a.ks * a.hkv * a.d;
         if (int st = launch_dkv_reduce<float>(count, a.dk, a.dv, a.partial, a.splits, a.accumulate, stream)) return st;
     }
-    return differential_dlambda(a, lambda_parts, stream);
+    return CGPTX_OK;
 }
 
 }  // namespace cgptx

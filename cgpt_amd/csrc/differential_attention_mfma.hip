@@ -640,9 +640,8 @@ __global__ __launch_bounds__(kThreads, 2) void differential_dq_kernel(Differenti
         // -(delta2 + rest) of the wavefront's rows.
         const float mine = at.live ? rest + (lane < 32 ? delta2 : 0.0f) : 0.0f;
         const float sum = wave_sum(mine);
-        constexpr int kRowWaves = 4 / PARTS;
-        const long blocks = gridDim.x, part = (static_cast<long>(at.b) * blocks + at.q_block / (kBlockRows / PARTS)) * kRowWaves + at.row_wave;
-        if (lane == 0) p.lambda_partial[at.h * (blocks * p.batch * kRowWaves) + part] = -sum;
+        const long part = (static_cast<long>(at.b) * gridDim.x + at.q_block / (kBlockRows / PARTS)) * (4 / PARTS) + at.row_wave;
+        if (lane == 0) p.lambda_partial[at.h * p.lambda_parts + part] = -sum;
     }
     if (!at.live) return;
     const float factor[2] = {p.scale, -lambda * p.scale};
@@ -923,6 +922,7 @@ __global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(Different
             store_columns<T, W, false>(static_cast<T*>(p.dv) + k_offset, p.d, p.accumulate != 0, [&](int t, int e) { return dv[t][e]; });
         }
     }
+    add_lambda_parts<kThreads>(p, reinterpret_cast<double*>(wide_smem));
 }
 
 template <typename Fn>
@@ -1001,14 +1001,12 @@ int differential_mfma_backward(DifferentialArgs a, hipStream_t stream) {
     walk.waves = 1;
     walk.tile_us = a.d <= 64 ? 1.2 : 2.0;
     if (int st = differential_backward_scratch(a, 4, lambda_parts(a), key_block_parts(walk), stream)) return st;
-    if (int st = dispatch(a, [&]<typename T, int W>() -> int {
-            if (int s = two_parts(a) ? launch_rows<differential_dq_kernel<T, W, 2>, W, 2>(a, stream)
-                                     : launch_rows<differential_dq_kernel<T, W, 1>, W, 1>(a, stream))
-                return s;
-            return launch_dkv<T, W>(a, stream);
-        }))
-        return st;
-    return differential_dlambda(a, lambda_parts(a), stream);
+    return dispatch(a, [&]<typename T, int W>() -> int {
+        if (int st = two_parts(a) ? launch_rows<differential_dq_kernel<T, W, 2>, W, 2>(a, stream)
+                                  : launch_rows<differential_dq_kernel<T, W, 1>, W, 1>(a, stream))
+            return st;
+        return launch_dkv<T, W>(a, stream);
+    });
 }
 
 }  // namespace cgptx
