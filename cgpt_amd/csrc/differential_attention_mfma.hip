@@ -467,7 +467,7 @@ __global__ __launch_bounds__(kThreads, 2) void differential_forward_kernel(Diffe
 __device__ __forceinline__ float sign_of_second(float lambda) { return lambda > 0.0f ? -1.0f : 1.0f; }
 
 template <typename T, int W, int PARTS>
-__global__ __launch_bounds__(kThreads, 2) void differential_dq_kernel(DifferentialArgs p) {
+__global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void differential_dq_kernel(DifferentialArgs p) {
     using frag = typename Mma<T>::frag;
     constexpr int STEPS = W / 16, HALF = STEPS / 2, DT = W / 32;
     T* const lds = wide_stages<T, W, PARTS>();  // [stage][part][K | V]
