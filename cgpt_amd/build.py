@@ -125,7 +125,7 @@ def build_dispatch(force: bool = True) -> pathlib.Path:
 
 INTERFACE_TEST_SOURCES = [ROOT / "tests" / "cpp" / name
                           for name in ("ops_interface_test.cpp", "block_backward_test.cpp", "data_upload_test.cpp",
-                                       "gemm_group_test.cpp", "gemm_plan_test.cpp")]
+                                       "gemm_group_test.cpp", "gemm_plan_test.cpp", "branch_ops_test.cpp")]
 INTERFACE_TEST_BINARY = ROOT / "tests" / "cpp" / "ops_interface_test.bin"
 
 
