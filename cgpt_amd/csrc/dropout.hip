@@ -7,7 +7,9 @@
 // function of (seed, offset, element) alone, whatever the type, the alignment and the launch, and the backward pass makes it
 // again. 16 bits: the probability is a multiple of 2^-16, at half of the generator's work per element of 32.
 //
-// A thread takes the eight elements of a counter value at a time.
+// A thread takes the eight elements of a counter value. What bounds it is memory: the generator's ten rounds run while the values
+// are on their way. 33554432 bf16 values, forward onto a residual and backward (335 MB): 56 us, 6.0 TB/s. A thread to
+// every eight elements instead of a few to each takes 225 us for 134217728 of them where 16 workgroups a CU in a loop took 257.
 #include "common.hpp"
 
 namespace cgptx {
@@ -41,27 +43,27 @@ __device__ __forceinline__ vec_t<std::uint32_t, 4> philox(std::uint64_t counter,
 }
 
 // Eight elements on a 16-byte boundary.
-template <typename T>
+template <bool ONCE, typename T>
 __device__ __forceinline__ vec_t<T, kGroup> load_group(const T* p) {
     if constexpr (sizeof(T) == 2) {
-        return load_vec<T, kGroup>(p);
+        return load_vec_once<ONCE, T, kGroup>(p);
     } else {
-        const vec_t<T, 4> a = load_vec<T, 4>(p), b = load_vec<T, 4>(p + 4);
+        const vec_t<T, 4> a = load_vec_once<ONCE, T, 4>(p), b = load_vec_once<ONCE, T, 4>(p + 4);
         return {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     }
 }
-template <typename T>
+template <bool ONCE, typename T>
 __device__ __forceinline__ void store_group(T* p, vec_t<T, kGroup> v) {
     if constexpr (sizeof(T) == 2) {
-        store_vec<T, kGroup>(p, v);
+        store_vec_once<ONCE, T, kGroup>(p, v);
     } else {
-        store_vec<T, 4>(p, vec_t<T, 4>{v[0], v[1], v[2], v[3]});
-        store_vec<T, 4>(p + 4, vec_t<T, 4>{v[4], v[5], v[6], v[7]});
+        store_vec_once<ONCE, T, 4>(p, vec_t<T, 4>{v[0], v[1], v[2], v[3]});
+        store_vec_once<ONCE, T, 4>(p + 4, vec_t<T, 4>{v[4], v[5], v[6], v[7]});
     }
 }
 
 // output = dropout(input) + added, rounded once; `added` (or null) and input may be the output.
-template <typename T>
+template <typename T, bool ONCE>
 __global__ __launch_bounds__(kThreads) void dropout_kernel(T* output, const T* input, const T* added, DropoutArgs args, bool vector_ok) {
     using Values = vec_t<T, kGroup>;
     const std::uint64_t first = args.offset + (args.counter != nullptr ? *args.counter : 0);
@@ -72,8 +74,8 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(T* output, const T* i
         const bool whole = vector_ok && at + kGroup <= args.count;
         Values x, y;
         if (whole) {
-            x = load_group<T>(input + at);
-            if (added != nullptr) y = load_group<T>(added + at);
+            x = load_group<ONCE, T>(input + at);
+            if (added != nullptr) y = load_group<ONCE, T>(added + at);
         } else {
 #pragma unroll
             for (int e = 0; e < kGroup; ++e) {
@@ -92,7 +94,7 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(T* output, const T* i
             out[e] = from_f32<T>(number >= args.threshold ? fmaf(to_f32(static_cast<T>(x[e])), args.scale, beside) : beside);
         }
         if (whole) {
-            store_group<T>(output + at, out);
+            store_group<ONCE, T>(output + at, out);
         } else {
 #pragma unroll
             for (int e = 0; e < kGroup; ++e)
@@ -120,9 +122,13 @@ int launch(const char* name, void* output, const void* input, const void* added,
     args.count = count;
     return dispatch_dtype(dtype, [&]<typename T>() -> int {
         const std::size_t blocks = ((count + kGroup - 1) / kGroup + kThreads - 1) / kThreads;
-        const std::size_t cap = static_cast<std::size_t>(compute_units()) * 16;
+        const std::size_t cap = std::size_t{1} << 23;  // 2^31 threads
         const bool vector_ok = is_aligned16(output) && is_aligned16(input) && is_aligned16(added);
-        hipLaunchKernelGGL((dropout_kernel<T>), dim3(static_cast<unsigned int>(blocks < cap ? blocks : cap)), dim3(kThreads), 0,
+        // A call that moves more than half of what the memory-side cache holds leaves it to its neighbours: the pair of calls above
+        // 62.7 -> 55.9 us; of two calls that move half of it each (without the residual) 42.7 us, 46.8 if they did.
+        const bool once = count * sizeof(T) * (added != nullptr && added != output ? 3 : 2) > kMemoryCacheBytes / 2;
+        auto kernel = once ? dropout_kernel<T, true> : dropout_kernel<T, false>;
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned int>(blocks < cap ? blocks : cap)), dim3(kThreads), 0,
                            static_cast<hipStream_t>(stream), static_cast<T*>(output), static_cast<const T*>(input),
                            static_cast<const T*>(added), args, vector_ok);
         CGPTX_LAUNCH_CHECK();
