@@ -23,8 +23,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWavesPerBlock = kThreads / kWave;
+constexpr int kLongThreads = 1024;  // of the kernels for rows of any length
 
-// Sum over the workgroup, the same bits in every thread. `stage` may be used again behind the next call's first barrier.
+// Sum over kLongThreads, the same bits in every thread. `stage` may be used again behind the next call's first barrier.
 __device__ __forceinline__ float block_sum(float v, float* stage) {
     v = wave_sum(v);
     __syncthreads();
@@ -32,87 +33,10 @@ __device__ __forceinline__ float block_sum(float v, float* stage) {
     __syncthreads();
     v = 0.0f;
 #pragma unroll
-    for (int s = 0; s < kWavesPerBlock; ++s) v += stage[s];
+    for (int s = 0; s < kLongThreads / kWave; ++s) v += stage[s];
     return v;
 }
 
-template <typename T, bool Backward>
-__global__ __launch_bounds__(kThreads) void layernorm_row_kernel(T* out, float* __restrict__ statistics /* [rows][mean, r] */,
-                                                                 const T* __restrict__ dy, const T* residual, const T* x,
-                                                                 const T* __restrict__ w, const T* __restrict__ bias, int rows,
-                                                                 int hidden, float inv_hidden, float eps) {
-    __shared__ float stage[kWavesPerBlock];
-    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
-        const std::size_t base = static_cast<std::size_t>(row) * hidden;
-        float sum = 0.0f;
-        for (int c = threadIdx.x; c < hidden; c += kThreads) sum += to_f32(x[base + c]);
-        const float mean = block_sum(sum, stage) * inv_hidden;
-        float squares = 0.0f;
-        for (int c = threadIdx.x; c < hidden; c += kThreads) {
-            const float d = to_f32(x[base + c]) - mean;
-            squares = fmaf(d, d, squares);
-        }
-        const float r = 1.0f / sqrtf(block_sum(squares, stage) * inv_hidden + eps);
-        if constexpr (Backward) {
-            float g_sum = 0.0f, gx_sum = 0.0f;
-            for (int c = threadIdx.x; c < hidden; c += kThreads) {
-                const float g = to_f32(dy[base + c]) * to_f32(w[c]);
-                g_sum += g;
-                gx_sum = fmaf(g, (to_f32(x[base + c]) - mean) * r, gx_sum);
-            }
-            const float g_mean = block_sum(g_sum, stage) * inv_hidden;
-            const float gx_mean = block_sum(gx_sum, stage) * inv_hidden;
-            if (threadIdx.x == 0) {
-                statistics[2 * static_cast<std::size_t>(row)] = mean;
-                statistics[2 * static_cast<std::size_t>(row) + 1] = r;
-            }
-            for (int c = threadIdx.x; c < hidden; c += kThreads) {
-                const float xh = (to_f32(x[base + c]) - mean) * r;
-                float v = r * (to_f32(dy[base + c]) * to_f32(w[c]) - g_mean - xh * gx_mean);
-                if (residual != nullptr) v += to_f32(residual[base + c]);
-                out[base + c] = from_f32<T>(v);
-            }
-        } else {
-            for (int c = threadIdx.x; c < hidden; c += kThreads) {
-                float v = (to_f32(x[base + c]) - mean) * r * to_f32(w[c]);
-                if (bias != nullptr) v += to_f32(bias[c]);
-                out[base + c] = from_f32<T>(v);
-            }
-        }
-    }
-}
-
-// Partial sums [slices][hidden] of dw and, behind them, of db: 64 columns and a slice of the rows per workgroup.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void layernorm_column_kernel(float* __restrict__ partial, const T* __restrict__ dy,
-                                                                    const T* __restrict__ x, const float* __restrict__ statistics,
-                                                                    int rows, int hidden, int rows_per_slice) {
-    __shared__ float stage[2][kWavesPerBlock][kWave];
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int col = blockIdx.x * kWave + lane;
-    const int row_begin = blockIdx.y * rows_per_slice, row_end = min(rows, row_begin + rows_per_slice);
-    float dw = 0.0f, db = 0.0f;
-    if (col < hidden) {
-        for (int row = row_begin + wave; row < row_end; row += kWavesPerBlock) {
-            const std::size_t index = static_cast<std::size_t>(row) * hidden + col;
-            const float mean = statistics[2 * static_cast<std::size_t>(row)], r = statistics[2 * static_cast<std::size_t>(row) + 1];
-            const float g = to_f32(dy[index]);
-            dw = fmaf(g, (to_f32(x[index]) - mean) * r, dw);
-            db += g;
-        }
-    }
-    stage[0][wave][lane] = dw;
-    stage[1][wave][lane] = db;
-    __syncthreads();
-    if (wave < 2 && col < hidden) {
-        float total = 0.0f;
-#pragma unroll
-        for (int s = 0; s < kWavesPerBlock; ++s) total += stage[wave][s][lane];
-        partial[(static_cast<std::size_t>(wave) * gridDim.y + blockIdx.y) * hidden + col] = total;
-    }
-}
-
-// ------------------------------------------------------------------------------------------------ rows in registers
 // 16 bytes of a row, at any element's address: a row's start is aligned as its width allows (the vector memory instructions
 // take any address).
 template <typename T>
@@ -140,19 +64,143 @@ __device__ __forceinline__ void store_some(T* p, vec_t<T, kVec128<T>> v, int cou
         if (e < count) p[e] = v[e];
 }
 
-// Sums over the LPR lanes, or the WAVES wavefronts, of a row; the same bits in all of its lanes.
-template <int LPR, int WAVES>
-__device__ __forceinline__ float row_sum(float v, float* stage) {
-    v = wave_sum<LPR>(v);
-    if constexpr (WAVES > 1) {
-        __syncthreads();
-        if ((threadIdx.x & (kWave - 1)) == 0) stage[threadIdx.x / kWave] = v;
-        __syncthreads();
-        v = 0.0f;
+// ------------------------------------------------------------------------------------------------ rows of any length
+// A row in walks of a workgroup: use(first column, elements of it, its values as fp32).
+template <typename T, typename Use>
+__device__ __forceinline__ void walk_row(const T* row, int hidden, Use&& use) {
+    constexpr int VEC = kVec128<T>;
+    for (int col = threadIdx.x * VEC; col < hidden; col += kLongThreads * VEC)
+        use(col, hidden - col, vec_to_f32<T, VEC>(load_some<T>(row + col, hidden - col)));
+}
+
+template <typename T, bool Backward>
+__global__ __launch_bounds__(kLongThreads) void layernorm_row_kernel(T* out, float* __restrict__ statistics /* [rows][mean, r] */,
+                                                                     const T* __restrict__ dy, const T* residual, const T* x,
+                                                                     const T* __restrict__ w, const T* __restrict__ bias, int rows,
+                                                                     int hidden, float inv_hidden, float eps) {
+    constexpr int VEC = kVec128<T>;
+    using F = vec_t<float, VEC>;
+    __shared__ float stage[kLongThreads / kWave];
+    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+        const std::size_t base = static_cast<std::size_t>(row) * hidden;
+        float sum = 0.0f;
+        walk_row(x + base, hidden, [&](int, int, const F& v) {
 #pragma unroll
-        for (int s = 0; s < WAVES; ++s) v += stage[s];
+            for (int e = 0; e < VEC; ++e) sum += v[e];
+        });
+        const float mean = block_sum(sum, stage) * inv_hidden;
+        float squares = 0.0f;
+        walk_row(x + base, hidden, [&](int, int count, const F& v) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float d = e < count ? v[e] - mean : 0.0f;
+                squares = fmaf(d, d, squares);
+            }
+        });
+        const float r = 1.0f / sqrtf(block_sum(squares, stage) * inv_hidden + eps);
+        if constexpr (Backward) {
+            float g_sum = 0.0f, gx_sum = 0.0f;
+            walk_row(x + base, hidden, [&](int col, int count, const F& v) {
+                const F grad = vec_to_f32<T, VEC>(load_some<T>(dy + base + col, count)), weight = vec_to_f32<T, VEC>(load_some<T>(w + col, count));
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float g = grad[e] * weight[e];
+                    g_sum += g;
+                    gx_sum = fmaf(g, (v[e] - mean) * r, gx_sum);
+                }
+            });
+            const float g_mean = block_sum(g_sum, stage) * inv_hidden;
+            const float gx_mean = block_sum(gx_sum, stage) * inv_hidden;
+            if (threadIdx.x == 0) {
+                statistics[2 * static_cast<std::size_t>(row)] = mean;
+                statistics[2 * static_cast<std::size_t>(row) + 1] = r;
+            }
+            walk_row(x + base, hidden, [&](int col, int count, const F& v) {
+                const F grad = vec_to_f32<T, VEC>(load_some<T>(dy + base + col, count)), weight = vec_to_f32<T, VEC>(load_some<T>(w + col, count));
+                F dx;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) dx[e] = r * (grad[e] * weight[e] - g_mean - (v[e] - mean) * r * gx_mean);
+                if (residual != nullptr) dx += vec_to_f32<T, VEC>(load_some<T>(residual + base + col, count));
+                store_some<T>(out + base + col, vec_from_f32<T, VEC>(dx), count);
+            });
+        } else {
+            walk_row(x + base, hidden, [&](int col, int count, const F& v) {
+                const F weight = vec_to_f32<T, VEC>(load_some<T>(w + col, count));
+                F y = bias != nullptr ? vec_to_f32<T, VEC>(load_some<T>(bias + col, count)) : F(0.0f);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) y[e] = fmaf((v[e] - mean) * r, weight[e], y[e]);
+                store_some<T>(out + base + col, vec_from_f32<T, VEC>(y), count);
+            });
+        }
     }
-    return v;
+}
+
+// Partial sums [slices][hidden] of dw and, behind them, of db: a vector of columns per lane and a slice of the rows per workgroup.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void layernorm_column_kernel(float* __restrict__ partial, const T* __restrict__ dy,
+                                                                    const T* __restrict__ x, const float* __restrict__ statistics,
+                                                                    int rows, int hidden, int rows_per_slice) {
+    constexpr int VEC = kVec128<T>;
+    using F = vec_t<float, VEC>;
+    __shared__ F stage[2][kWavesPerBlock][kWave];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int col = (blockIdx.x * kWave + lane) * VEC, count = hidden - col;
+    const int row_begin = blockIdx.y * rows_per_slice, row_end = min(rows, row_begin + rows_per_slice);
+    F dw(0.0f), db(0.0f);
+    if (count > 0) {
+        for (int row = row_begin + wave; row < row_end; row += kWavesPerBlock) {
+            const std::size_t index = static_cast<std::size_t>(row) * hidden + col;
+            const float mean = statistics[2 * static_cast<std::size_t>(row)], r = statistics[2 * static_cast<std::size_t>(row) + 1];
+            const F g = vec_to_f32<T, VEC>(load_some<T>(dy + index, count)), v = vec_to_f32<T, VEC>(load_some<T>(x + index, count));
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                dw[e] = fmaf(g[e], (v[e] - mean) * r, dw[e]);
+                db[e] += g[e];
+            }
+        }
+    }
+    stage[0][wave][lane] = dw;
+    stage[1][wave][lane] = db;
+    __syncthreads();
+    if (wave < 2 && count > 0) {
+        F total(0.0f);
+#pragma unroll
+        for (int s = 0; s < kWavesPerBlock; ++s) total += stage[wave][s][lane];
+        float* to = partial + (static_cast<std::size_t>(wave) * gridDim.y + blockIdx.y) * hidden + col;
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4)
+            store_some<float>(to + e, vec_t<float, 4>{total[e], total[e + 1], total[e + 2], total[e + 3]}, count - e);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ rows in registers
+// Sums over the LPR lanes, or the WAVES wavefronts, of a row; the same bits in all of its lanes. `stage` is not used for another sum
+// before the workgroup has met twice more: one barrier a sum is enough.
+template <int LPR, int WAVES, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float (*stage)[WAVES]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = wave_sum<LPR>(v[n]);
+    if constexpr (WAVES > 1) {
+        if ((threadIdx.x & (kWave - 1)) == 0)
+#pragma unroll
+            for (int n = 0; n < N; ++n) stage[n][threadIdx.x / kWave] = v[n];
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            v[n] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < WAVES; ++s) v[n] += stage[n][s];
+        }
+    }
+}
+// Makes the compiler forget what it has computed from a vector, so that it is computed again and not kept in registers.
+template <bool FORGET, typename V>
+__device__ __forceinline__ void forget(V& v) {
+    if constexpr (FORGET) {
+        auto words = __builtin_bit_cast(vec_t<unsigned int, 4>, v);
+        asm volatile("" : "+v"(words));
+        v = __builtin_bit_cast(V, words);
+    }
 }
 
 // LPR lanes of a wavefront (WAVES = 1), or WAVES wavefronts, share a row; a lane holds K vectors of it.
@@ -167,20 +215,23 @@ __global__ __launch_bounds__(WAVES > 4 ? WAVES * kWave : kThreads) void layernor
     static_assert(WAVES == 1 || kRowsPerBlock == 1, "the wavefronts of a row meet at the workgroup's barriers");
     using F = vec_t<float, VEC>;
     using V = vec_t<T, VEC>;
-    __shared__ float stage[WAVES];
+    // Sixteen wavefronts of a workgroup leave 128 registers: what a row's vectors give is computed again for every use.
+    constexpr bool LEAN = WAVES > 4, AHEAD = !(Backward && LEAN && K * VEC > 8);  // AHEAD: the next row is requested before this one is used
+    __shared__ float stage[4][WAVES];  // mean | variance | both means of the gradient
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int sub = WAVES > 1 ? static_cast<int>(threadIdx.x) : lane % LPR;
     const int slot = WAVES > 1 ? 0 : wave * kRowsPerWave + lane / LPR;  // which of the workgroup's rows
 
     int count[K];  // elements of the row that a lane's vectors hold
-    F wv[K], acc_w[K], acc_b[K], bv[K];
+    V wv[K], bv[K];
+    F acc_w[K], acc_b[K];
 #pragma unroll
     for (int c = 0; c < K; ++c) {
         const int col = (c * LPR * WAVES + sub) * VEC;
         count[c] = hidden - col;
-        wv[c] = vec_to_f32<T, VEC>(load_some<T>(w + col, count[c]));
+        wv[c] = load_some<T>(w + col, count[c]);
         acc_w[c] = acc_b[c] = F(0.0f);
-        if constexpr (!Backward) bv[c] = bias != nullptr ? vec_to_f32<T, VEC>(load_some<T>(bias + col, count[c])) : F(0.0f);
+        if constexpr (!Backward) bv[c] = bias != nullptr ? load_some<T>(bias + col, count[c]) : V(static_cast<T>(0.0f));
     }
     struct Row {
         V x[K], dy[K], residual[K];
@@ -202,61 +253,79 @@ __global__ __launch_bounds__(WAVES > 4 ? WAVES * kWave : kThreads) void layernor
     fetch(static_cast<long>(blockIdx.x) * kRowsPerBlock + slot, now);
     for (long first = static_cast<long>(blockIdx.x) * kRowsPerBlock; first < rows; first += stride) {
         const long row = first + slot;
-        if (first + stride < rows) fetch(row + stride, next);
+        if (AHEAD && first + stride < rows) fetch(row + stride, next);
         const std::size_t base = static_cast<std::size_t>(row) * hidden;
-        F xc[K], g[K];
-        float sum = 0.0f;
+        float sum[1] = {0.0f}, squares[1] = {0.0f};
 #pragma unroll
         for (int c = 0; c < K; ++c) {
-            xc[c] = vec_to_f32<T, VEC>(now.x[c]);
+            const F xv = vec_to_f32<T, VEC>(now.x[c]);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) sum += xc[c][e];
+            for (int e = 0; e < VEC; ++e) sum[0] += xv[e];
+            forget<LEAN>(now.x[c]);
         }
-        const float mean = row_sum<LPR, WAVES>(sum, stage) * inv_hidden;
-        float squares = 0.0f;
+        row_sums<LPR, WAVES>(sum, stage);
+        const float mean = sum[0] * inv_hidden;
+        auto centred = [&](int c) __attribute__((always_inline)) {
+            F xc = vec_to_f32<T, VEC>(now.x[c]);
 #pragma unroll
-        for (int c = 0; c < K; ++c)
+            for (int e = 0; e < VEC; ++e) xc[e] = e < count[c] ? xc[e] - mean : 0.0f;
+            return xc;
+        };
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                xc[c][e] = e < count[c] ? xc[c][e] - mean : 0.0f;
-                squares = fmaf(xc[c][e], xc[c][e], squares);
-            }
-        const float r = 1.0f / sqrtf(row_sum<LPR, WAVES>(squares, stage) * inv_hidden + eps);
+        for (int c = 0; c < K; ++c) {
+            const F xc = centred(c);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) squares[0] = fmaf(xc[e], xc[e], squares[0]);
+            forget<LEAN>(now.x[c]);
+        }
+        row_sums<LPR, WAVES>(squares, stage + 1);
+        const float r = 1.0f / sqrtf(squares[0] * inv_hidden + eps);
         if constexpr (Backward) {
-            float g_sum = 0.0f, gx_sum = 0.0f;
+            auto scaled = [&](int c) __attribute__((always_inline)) {
+                F g = vec_to_f32<T, VEC>(now.dy[c]);
+                const F weight = vec_to_f32<T, VEC>(wv[c]);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) g[e] *= weight[e];
+                return g;
+            };
+            float g_sums[2] = {0.0f, 0.0f};  // of g and of g xh
 #pragma unroll
             for (int c = 0; c < K; ++c) {
-                g[c] = vec_to_f32<T, VEC>(now.dy[c]);
+                const F xc = centred(c), g = scaled(c), grad = vec_to_f32<T, VEC>(now.dy[c]);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    xc[c][e] *= r;
-                    acc_w[c][e] = fmaf(g[c][e], xc[c][e], acc_w[c][e]);
-                    acc_b[c][e] += g[c][e];
-                    g[c][e] *= wv[c][e];
-                    g_sum += g[c][e];
-                    gx_sum = fmaf(g[c][e], xc[c][e], gx_sum);
+                    const float xh = xc[e] * r;
+                    acc_w[c][e] = fmaf(grad[e], xh, acc_w[c][e]);
+                    acc_b[c][e] += grad[e];
+                    g_sums[0] += g[e];
+                    g_sums[1] = fmaf(g[e], xh, g_sums[1]);
                 }
+                forget<LEAN>(now.x[c]);
+                forget<LEAN>(now.dy[c]);
             }
-            const float g_mean = row_sum<LPR, WAVES>(g_sum, stage) * inv_hidden;
-            const float gx_mean = row_sum<LPR, WAVES>(gx_sum, stage) * inv_hidden;
+            row_sums<LPR, WAVES>(g_sums, stage + 2);
+            const float g_mean = g_sums[0] * inv_hidden, gx_mean = g_sums[1] * inv_hidden;
 #pragma unroll
             for (int c = 0; c < K; ++c) {
+                const F xc = centred(c), g = scaled(c);
                 F v;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v[e] = r * (g[c][e] - g_mean - xc[c][e] * gx_mean);
+                for (int e = 0; e < VEC; ++e) v[e] = r * (g[e] - g_mean - xc[e] * r * gx_mean);
                 if (residual != nullptr) v += vec_to_f32<T, VEC>(now.residual[c]);
                 if (row < rows) store_some<T>(out + base + (c * LPR * WAVES + sub) * VEC, vec_from_f32<T, VEC>(v), count[c]);
             }
         } else {
 #pragma unroll
             for (int c = 0; c < K; ++c) {
+                const F xc = centred(c), weight = vec_to_f32<T, VEC>(wv[c]), shift = vec_to_f32<T, VEC>(bv[c]);
                 F v;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v[e] = fmaf(xc[c][e] * r, wv[c][e], bv[c][e]);
+                for (int e = 0; e < VEC; ++e) v[e] = fmaf(xc[e] * r, weight[e], shift[e]);
                 if (row < rows) store_some<T>(out + base + (c * LPR * WAVES + sub) * VEC, vec_from_f32<T, VEC>(v), count[c]);
             }
         }
-        now = next;
+        if constexpr (AHEAD) now = next;
+        else if (first + stride < rows) fetch(row + stride, now);
     }
     if constexpr (Backward) {
         float* const mine[2] = {partial + static_cast<std::size_t>(blockIdx.x) * hidden,
@@ -266,11 +335,10 @@ __global__ __launch_bounds__(WAVES > 4 ? WAVES * kWave : kThreads) void layernor
             for (int c = 0; c < K; ++c) {
                 const int col = (c * LPR * WAVES + sub) * VEC;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e)
-                    if (e < count[c]) {
-                        mine[0][col + e] = acc_w[c][e];
-                        mine[1][col + e] = acc_b[c][e];
-                    }
+                for (int e = 0; e < VEC; e += 4) {
+                    store_some<float>(mine[0] + col + e, vec_t<float, 4>{acc_w[c][e], acc_w[c][e + 1], acc_w[c][e + 2], acc_w[c][e + 3]}, count[c] - e);
+                    store_some<float>(mine[1] + col + e, vec_t<float, 4>{acc_b[c][e], acc_b[c][e + 1], acc_b[c][e + 2], acc_b[c][e + 3]}, count[c] - e);
+                }
             }
         } else {
             // The row slots of a wavefront, then the workgroup's wavefronts.
@@ -350,7 +418,7 @@ int validate(const char* name, std::size_t rows, std::size_t hidden, float eps, 
     return CGPTX_OK;
 }
 
-int row_blocks(int rows) { return rows < compute_units() * 8 ? rows : compute_units() * 8; }
+int row_blocks(int rows) { return rows < compute_units() * 2 ? rows : compute_units() * 2; }
 
 }  // namespace
 }  // namespace cgptx
@@ -371,7 +439,7 @@ extern "C" int cgptx_layernorm_forward(void* output, const void* input, const vo
             CGPTX_LAUNCH_CHECK();
             return CGPTX_OK;
         }
-        hipLaunchKernelGGL((layernorm_row_kernel<T, false>), dim3(row_blocks(r)), dim3(kThreads), 0, stream, static_cast<T*>(output),
+        hipLaunchKernelGGL((layernorm_row_kernel<T, false>), dim3(row_blocks(r)), dim3(kLongThreads), 0, stream, static_cast<T*>(output),
                            nullptr, nullptr, nullptr, static_cast<const T*>(input), static_cast<const T*>(weight),
                            static_cast<const T*>(bias), r, h, 1.0f / static_cast<float>(h), epsilon);
         CGPTX_LAUNCH_CHECK();
@@ -414,11 +482,11 @@ extern "C" int cgptx_layernorm_backward(void* grad_input, void* grad_weight, voi
         if (int s = scratch(stream, statistics_bytes + 2 * static_cast<std::size_t>(slices) * hidden * sizeof(float), &mem)) return s;
         auto* statistics = static_cast<float*>(mem);
         auto* partial = reinterpret_cast<float*>(static_cast<char*>(mem) + statistics_bytes);
-        hipLaunchKernelGGL((layernorm_row_kernel<T, true>), dim3(row_blocks(r)), dim3(kThreads), 0, stream, static_cast<T*>(grad_input),
+        hipLaunchKernelGGL((layernorm_row_kernel<T, true>), dim3(row_blocks(r)), dim3(kLongThreads), 0, stream, static_cast<T*>(grad_input),
                            statistics, dy, static_cast<const T*>(residual), x, static_cast<const T*>(weight), nullptr, r, h,
                            1.0f / static_cast<float>(h), epsilon);
         CGPTX_LAUNCH_CHECK();
-        hipLaunchKernelGGL((layernorm_column_kernel<T>), dim3((h + kWave - 1) / kWave, slices), dim3(kThreads), 0, stream, partial, dy,
+        hipLaunchKernelGGL((layernorm_column_kernel<T>), dim3((h + kWave * kVec128<T> - 1) / (kWave * kVec128<T>), slices), dim3(kThreads), 0, stream, partial, dy,
                            x, statistics, r, h, rows_per_slice);
         CGPTX_LAUNCH_CHECK();
         launch_column_partial_reduce<T>(static_cast<T*>(grad_weight), partial, slices, h, 0, stream);
