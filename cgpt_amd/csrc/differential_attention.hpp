@@ -19,17 +19,18 @@ struct DifferentialArgs {
     float scale;
     int causal, offset, accumulate;
     int dtype;
-    // dK/dV on the matrix cores, set by its launch (fp32: splits only):
+    // dK/dV on the matrix cores, set by its launch (fp32: splits only); a forward pass whose keys are shared sets splits, partial, delta:
     int paired;      // a workgroup takes key blocks (i, last - i) instead of one
     int splits;      // workgroups that share a key block's query tiles (never with paired)
     int by_block;    // splits > 1: workgroups go out block by block over all (batch, kv-head) pairs
+    int pack;        // forward pass whose keys are shared: heads of a group that have their rows in one block
     float* partial;  // splits > 1: [splits][dK | dV][key, kv head, d] sums of the parts
 };
 
 // Whether the 16-bit matrix kernels serve a call's types and sizes: halves of a head in multiples of 8 (128-bit chunks of a row), and
 // 64 rows of a tensor within 1 GiB, which their 32-bit offsets within a tile reach. Their tensors lie on 16-byte boundaries.
 bool differential_mfma_takes(const DifferentialArgs& args);
-int differential_mfma_forward(const DifferentialArgs& args, hipStream_t stream);
+int differential_mfma_forward(DifferentialArgs args, hipStream_t stream);  // takes scratch where few queries share many keys
 int differential_mfma_backward(DifferentialArgs args, hipStream_t stream);  // takes its scratch itself
 
 // The fp32 ones: halves of a head in multiples of 4, tensors on 16-byte boundaries.

@@ -96,23 +96,20 @@ struct TileOffsets {
     }
 };
 
-// The operand that stays in registers, from global memory: lane -> row row0 + lane%32 of a tensor's (batch, head), padded columns
-// 16*step + 8*(lane/32) .. + 7; rows past the end are zeros.
+// The operand that stays in registers, from global memory: lane -> its row (lane%32), padded columns 16*step + 8*(lane/32) .. + 7; zeros for
+// a row that is not live. The row lies `row_bytes` behind element `offset` of the tensor, whose part that the wavefront's rows
+// are in has `bytes` from there on.
 template <typename T, int W, bool HALVES>
-__device__ __forceinline__ void load_rows(typename Mma<T>::frag (&rows)[W / 16], const void* tensor, long offset, long row_stride, int count, int row0,
-                                          int d) {
+__device__ __forceinline__ void load_rows(typename Mma<T>::frag (&rows)[W / 16], const void* tensor, long offset, long bytes, int row_bytes,
+                                          bool live, int d) {
     using frag = typename Mma<T>::frag;
-    const int lane = threadIdx.x & 63;
-    RowStream s;
-    s.base = static_cast<const char*>(tensor) + offset * static_cast<long>(sizeof(T));
-    s.row_bytes = static_cast<int>(row_stride * sizeof(T));
-    s.bytes = ((count - 1) * row_stride + d) * static_cast<long>(sizeof(T));
-    const __amdgpu_buffer_rsrc_t rsrc = s.at(min(row0, count - 1));
-    const int row = row0 < count ? (lane & 31) * s.row_bytes : 1 << 30;
+    const int half = (threadIdx.x & 63) >> 5;
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(static_cast<const T*>(tensor) + offset), 0,
+                                                                          static_cast<int>(min(bytes, 1l << 30)), 0x00020000);
 #pragma unroll
     for (int i = 0; i < W / 16; ++i) {
-        const int column = source_column<W, HALVES>(i * 16 + (lane >> 5) * 8, d);
-        rows[i] = __builtin_bit_cast(frag, load_words(rsrc, column >= 0 ? row + column * static_cast<int>(sizeof(T)) : 1 << 30));
+        const int column = source_column<W, HALVES>(i * 16 + half * 8, d);
+        rows[i] = __builtin_bit_cast(frag, load_words(rsrc, live && column >= 0 ? row_bytes + column * static_cast<int>(sizeof(T)) : 1 << 30));
     }
 }
 
@@ -230,42 +227,68 @@ __device__ __forceinline__ int register_column(int index, int d) {
 }
 
 struct RowTiles {
-    int b, h, kvh, q_block, row_wave, part, q_row;
-    bool live;
-    template <int PARTS>
+    int b, h, kvh, row, row_wave, part;  // row: of the workgroup's first, of a head's queries
+    int first_q, last_q;                 // tokens of the wavefront's first and last row
+    int q;                               // token of this lane's row
+    int beside;                          // heads from h to this lane's row's
+    bool live, wave_live;
+    template <int PARTS, bool SPLIT = false>
     __device__ __forceinline__ static RowTiles of(const DifferentialArgs& p, int wave) {
         constexpr int kRows = kBlockRows / PARTS;
-        const BlockCoordinates where = block_coordinates<kRows>(p.hkv);
         RowTiles r;
-        r.b = where.b;
-        r.h = where.h;
-        r.kvh = where.h / (p.hq / p.hkv);
-        r.q_block = where.q_block;
+        const int pack = SPLIT ? p.pack : 1;
+        if constexpr (SPLIT) {  // workgroups that share a query block next to each other
+            r.b = blockIdx.z;
+            r.h = blockIdx.y * pack;
+            r.row = static_cast<int>(blockIdx.x) / p.splits * kRows;
+        } else {
+            const BlockCoordinates where = block_coordinates<kRows>(p.hkv);
+            r.b = where.b;
+            r.h = where.h;
+            r.row = where.q_block;
+        }
+        r.kvh = r.h / (p.hq / p.hkv);
         r.row_wave = wave % (4 / PARTS);
         r.part = wave / (4 / PARTS);
-        r.q_row = r.q_block + r.row_wave * 32 + static_cast<int>(threadIdx.x & 31);
-        r.live = r.q_row < p.qs;
+        const int first = r.row + r.row_wave * 32, mine = first + static_cast<int>(threadIdx.x & 31);
+        r.first_q = first / pack;
+        r.last_q = min((first + 31) / pack, p.qs - 1);
+        r.q = mine / pack;
+        r.beside = mine - r.q * pack;
+        r.live = r.q < p.qs;
+        r.wave_live = r.first_q < p.qs;
         return r;
+    }
+    // Elements from the start of a tensor like q to this lane's row.
+    __device__ __forceinline__ long offset(const DifferentialArgs& p) const {
+        return ((static_cast<long>(b) * p.qs + q) * p.hq + h + beside) * p.d;
     }
 };
 
-template <typename T, int W, int PARTS>
+// SPLIT: p.splits workgroups share a query block's keys, and a block has the rows of p.pack heads of a group, which read the same keys;
+// each workgroup leaves its sums, and the maxima that they stand to, in p.partial, and
+// differential_combine_kernel brings them together.
+template <typename T, int W, int PARTS, bool SPLIT>
 __global__ __launch_bounds__(kThreads, 2) void differential_forward_kernel(DifferentialArgs p) {
     using frag = typename Mma<T>::frag;
     constexpr int STEPS = W / 16, HALF = STEPS / 2, DT = W / 32;
     T* const lds = wide_stages<T, W, PARTS>();  // [stage][part][K | V]
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const RowTiles at = RowTiles::of<PARTS>(p, wave);
+    const RowTiles at = RowTiles::of<PARTS, SPLIT>(p, wave);
     const long q_stride = static_cast<long>(p.hq) * p.d, kv_stride = static_cast<long>(p.hkv) * p.d;
-    const long q_offset = (static_cast<long>(at.b) * p.qs + at.q_row) * q_stride + at.h * p.d;
+    const long q_offset = at.offset(p), first_row = at.wave_live ? ((static_cast<long>(at.b) * p.qs + at.first_q) * p.hq + at.h) * p.d : 0;
+    const int row_bytes = ((at.q - at.first_q) * p.hq + at.beside) * p.d * static_cast<int>(sizeof(T));
+    const long wave_bytes = at.wave_live ? ((at.last_q - at.first_q + 1) * q_stride - at.h * p.d) * static_cast<long>(sizeof(T)) : 0;
     const long kv_offset = static_cast<long>(at.b) * p.ks * kv_stride + at.kvh * p.d;
     const RowStream k_src = make_stream<T, W, true>(p.k, kv_offset, kv_stride, p.ks, p.d, wave, p.d);
     const RowStream v_src = make_stream<T, W, false>(p.v, kv_offset, kv_stride, p.ks, p.d, wave, p.d);
 
-    const int last_q_block = min(at.q_block + kBlockRows / PARTS, p.qs) - 1;
+    const int last_q_block = min((at.row + kBlockRows / PARTS - 1) / (SPLIT ? p.pack : 1), p.qs - 1);
     const int k_end = p.causal ? min(p.ks, p.offset + last_q_block + 1) : p.ks;
-    const int tiles = (k_end + kStream - 1) / kStream;
+    const int all_tiles = (k_end + kStream - 1) / kStream, split = SPLIT ? static_cast<int>(blockIdx.x) % p.splits : 0;
+    const int begin = SPLIT ? static_cast<int>(static_cast<long>(split) * all_tiles / p.splits) : 0;
+    const int tiles = SPLIT ? static_cast<int>(static_cast<long>(split + 1) * all_tiles / p.splits) : all_tiles;  // end of this workgroup's
     auto request = [&](int j, T* stage) __attribute__((always_inline)) {
 #pragma unroll
         for (int g = 0; g < PARTS; ++g) {
@@ -274,11 +297,10 @@ __global__ __launch_bounds__(kThreads, 2) void differential_forward_kernel(Diffe
             stream_rows<T, W>(v_src, (j + g) * kStream, stage + (2 * g + 1) * kWideTile<W>, wave);
         }
     };
-    request(0, lds);
+    request(begin, lds);
 
     frag qf[STEPS];
-    const long head = static_cast<long>(at.b) * p.qs * q_stride + at.h * p.d;
-    load_rows<T, W, true>(qf, p.q, head, q_stride, p.qs, at.q_block + at.row_wave * 32, p.d);
+    load_rows<T, W, true>(qf, p.q, first_row, wave_bytes, row_bytes, at.live, p.d);
     const TileOffsets<W> offsets(lane);
 
     // Both maps' sums, and their running maxima m of the raw scores (the scale is positive) as in attention.hip: mb = m * scale2, 0 while
@@ -294,15 +316,14 @@ __global__ __launch_bounds__(kThreads, 2) void differential_forward_kernel(Diffe
         l[i] = 0.0f;
     }
     const float scale2 = p.scale * kLog2e;
-    const int wave_first_q = at.q_block + at.row_wave * 32;
-    const int wave_last_q = min(wave_first_q + 31, p.qs - 1);
-    const bool wave_live = wave_first_q < p.qs;
-    const int q_limit = p.causal ? p.offset + at.q_row : p.ks;  // largest visible key of this lane's query
+    const int wave_first_q = at.first_q, wave_last_q = at.last_q;
+    const bool wave_live = at.wave_live;
+    const int q_limit = p.causal ? p.offset + at.q : p.ks;  // largest visible key of this lane's query
     const int clear_limit = p.causal ? min(p.ks - 1, p.offset + wave_first_q) : p.ks - 1;  // tiles up to here need no mask
 
     LeftOut left(p, wave_first_q);
-    for (int first = 0; first < tiles; first += PARTS) {
-        const int j = first + at.part, k0 = j * kStream, stage = (first / PARTS) & 1;
+    for (int first = begin; first < tiles; first += PARTS) {
+        const int j = first + at.part, k0 = j * kStream, stage = ((first - begin) / PARTS) & 1;
         const int tile = (stage * PARTS + at.part) * 2 * kWideTile<W>;  // K's; V's is the next
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's part of the tiles is in LDS
         __syncthreads();                     // ... and everybody else's; the other stage is free
@@ -450,6 +471,19 @@ __global__ __launch_bounds__(kThreads, 2) void differential_forward_kernel(Diffe
 #pragma unroll
     for (int i = 0; i < 2; ++i) l[i] += other_half(l[i]);
     if (!at.live) return;
+    if constexpr (SPLIT) {
+        const long rows = static_cast<long>(p.batch) * p.qs * p.hq, row = (static_cast<long>(at.b) * p.qs + at.q) * p.hq + at.h + at.beside;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const long to = (static_cast<long>(split) * 2 + i) * rows + row;
+            store_columns<float, W, false>(p.partial + to * p.d, p.d, false, [&](int t, int e) { return o[i][t][e]; });
+            if (lane < 32) {
+                p.delta[2 * to] = l[i] > 0.0f || l[i] != l[i] ? mb[i] : -INFINITY;  // no key that the row sees: no part of it
+                p.delta[2 * to + 1] = l[i];
+            }
+        }
+        return;
+    }
     const float lambda = p.lambda[at.h];
     const float inverse1 = 1.0f / l[0], inverse2 = 1.0f / l[1];
     store_columns<T, W, false>(static_cast<T*>(p.out) + q_offset, p.d, false,
@@ -457,10 +491,48 @@ __global__ __launch_bounds__(kThreads, 2) void differential_forward_kernel(Diffe
     if (p.second != nullptr)
         store_columns<T, W, false>(static_cast<T*>(p.second) + q_offset, p.d, false, [&](int t, int e) { return o[1][t][e] * inverse2; });
     if (p.lse_out != nullptr) {  // one map from either half of the wavefront
-        const long rows = static_cast<long>(p.batch) * p.qs * p.hq, row = (static_cast<long>(at.b) * p.qs + at.q_row) * p.hq + at.h;
+        const long rows = static_cast<long>(p.batch) * p.qs * p.hq, row = (static_cast<long>(at.b) * p.qs + at.q) * p.hq + at.h + at.beside;
         const bool second = lane >= 32;
         p.lse_out[(second ? rows : 0) + row] = ((second ? mb[1] : mb[0]) + log2f(second ? l[1] : l[0])) * kLn2;
     }
+}
+
+// A row of a forward pass whose keys were shared, from what the workgroups left: both maps' sums brought to their common maxima. What
+// bounds it is the way to memory, where the other XCDs' workgroups have left their parts: a workgroup has a row, a wavefront a map's even or odd
+// parts, and all of its loads are on their way before the first is used (one after the other, a wavefront to a row: 17 us for 32
+// parts).
+constexpr int kMostSplits = 64;
+template <typename T, int MOST>
+__global__ __launch_bounds__(kThreads) void differential_combine_kernel(DifferentialArgs p) {
+    __shared__ vec_t<float, 2> stage[4][kWave];
+    const long rows = static_cast<long>(p.batch) * p.qs * p.hq, row = blockIdx.x;
+    const int lane = threadIdx.x & (kWave - 1), at = 2 * lane, wave = threadIdx.x / kWave, map = wave & 1, odd = wave >> 1;
+    vec_t<float, 2> part[MOST / 2];
+#pragma unroll
+    for (int u = 0; u < MOST / 2; ++u)
+        if (2 * u + odd < p.splits) part[u] = load_vec<float, 2>(p.partial + ((2l * (2 * u + odd) + map) * rows + row) * p.d + min(at, p.d - 2));
+    // A part per lane: all their maxima and sums at once.
+    const long mine = 2 * ((2l * min(lane, p.splits - 1) + map) * rows + row);
+    const float part_top = lane < p.splits ? p.delta[mine] : -INFINITY, part_sum = lane < p.splits ? p.delta[mine + 1] : 0.0f;
+    const float top = wave_max(part_top), weight = part_top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(part_top - top);
+    const float sum = wave_sum(part_sum * weight);
+    vec_t<float, 2> o(0.0f);
+#pragma unroll
+    for (int u = 0; u < MOST / 2; ++u) {
+        if (2 * u + odd >= p.splits) break;
+        const float factor = __shfl(weight, 2 * u + odd, kWave);
+        o[0] = fmaf(part[u][0], factor, o[0]);
+        o[1] = fmaf(part[u][1], factor, o[1]);
+    }
+    stage[wave][lane] = o * (1.0f / sum);
+    if (p.lse_out != nullptr && odd == 0 && lane == 0) p.lse_out[map * rows + row] = (top + log2f(sum)) * kLn2;
+    __syncthreads();
+    if (wave != 0 || at >= p.d) return;
+    const float lambda = p.lambda[row % p.hq];
+    const vec_t<float, 2> first = stage[0][lane] + stage[2][lane], second = stage[1][lane] + stage[3][lane];
+    const vec_t<float, 2> out{fmaf(-lambda, second[0], first[0]), fmaf(-lambda, second[1], first[1])};
+    store_vec<T, 2>(static_cast<T*>(p.out) + row * p.d + at, vec_from_f32<T, 2>(out));
+    if (p.second != nullptr) store_vec<T, 2>(static_cast<T*>(p.second) + row * p.d + at, vec_from_f32<T, 2>(second));
 }
 
 // The sign of -lambda.
@@ -475,12 +547,14 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void differential_dq_ker
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const RowTiles at = RowTiles::of<PARTS>(p, wave);
     const long q_stride = static_cast<long>(p.hq) * p.d, kv_stride = static_cast<long>(p.hkv) * p.d;
-    const long q_offset = (static_cast<long>(at.b) * p.qs + at.q_row) * q_stride + at.h * p.d;
+    const long q_offset = at.offset(p), first_row = at.wave_live ? ((static_cast<long>(at.b) * p.qs + at.first_q) * p.hq + at.h) * p.d : 0;
+    const int row_bytes = ((at.q - at.first_q) * p.hq + at.beside) * p.d * static_cast<int>(sizeof(T));
+    const long wave_bytes = at.wave_live ? ((at.last_q - at.first_q + 1) * q_stride - at.h * p.d) * static_cast<long>(sizeof(T)) : 0;
     const long kv_offset = static_cast<long>(at.b) * p.ks * kv_stride + at.kvh * p.d;
     const RowStream k_src = make_stream<T, W, true>(p.k, kv_offset, kv_stride, p.ks, p.d, wave, p.d);
     const RowStream v_src = make_stream<T, W, false>(p.v, kv_offset, kv_stride, p.ks, p.d, wave, p.d);
 
-    const int last_q_block = min(at.q_block + kBlockRows / PARTS, p.qs) - 1;
+    const int last_q_block = min(at.row + kBlockRows / PARTS, p.qs) - 1;
     const int k_end = p.causal ? min(p.ks, p.offset + last_q_block + 1) : p.ks;
     const int tiles = (k_end + kStream - 1) / kStream;
     auto request = [&](int j, T* stage) __attribute__((always_inline)) {
@@ -494,16 +568,15 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void differential_dq_ker
     request(0, lds);
 
     frag qf[STEPS], dof[STEPS];
-    const long head = static_cast<long>(at.b) * p.qs * q_stride + at.h * p.d;
-    load_rows<T, W, true>(qf, p.q, head, q_stride, p.qs, at.q_block + at.row_wave * 32, p.d);
-    load_rows<T, W, false>(dof, p.dout, head, q_stride, p.qs, at.q_block + at.row_wave * 32, p.d);
+    load_rows<T, W, true>(qf, p.q, first_row, wave_bytes, row_bytes, at.live, p.d);
+    load_rows<T, W, false>(dof, p.dout, first_row, wave_bytes, row_bytes, at.live, p.d);
     const float lambda = p.lambda[at.h];
-    const long rows = static_cast<long>(p.batch) * p.qs * p.hq, row = (static_cast<long>(at.b) * p.qs + at.q_row) * p.hq + at.h;
+    const long rows = static_cast<long>(p.batch) * p.qs * p.hq, row = (static_cast<long>(at.b) * p.qs + at.q) * p.hq + at.h;
     float delta1, delta2;
     {
         frag of[STEPS], o2f[STEPS];
-        load_rows<T, W, false>(of, p.o, head, q_stride, p.qs, at.q_block + at.row_wave * 32, p.d);
-        load_rows<T, W, false>(o2f, p.o2, head, q_stride, p.qs, at.q_block + at.row_wave * 32, p.d);
+        load_rows<T, W, false>(of, p.o, first_row, wave_bytes, row_bytes, at.live, p.d);
+        load_rows<T, W, false>(o2f, p.o2, first_row, wave_bytes, row_bytes, at.live, p.d);
         delta2 = row_delta<T, STEPS>(dof, o2f);
         delta1 = fmaf(lambda, delta2, row_delta<T, STEPS>(dof, of));
     }
@@ -530,10 +603,9 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void differential_dq_ker
     for (int t = 0; t < DT; ++t) dq[t] = acc_t(0.0f);
     float rest = 0.0f;  // rowsum(P2 (G - delta2)): what the rounding of O2 left in delta2
     const float scale2 = p.scale * kLog2e;
-    const int wave_first_q = at.q_block + at.row_wave * 32;
-    const int wave_last_q = min(wave_first_q + 31, p.qs - 1);
-    const bool wave_live = wave_first_q < p.qs;
-    const int q_limit = p.causal ? p.offset + at.q_row : p.ks;
+    const int wave_first_q = at.first_q, wave_last_q = at.last_q;
+    const bool wave_live = at.wave_live;
+    const int q_limit = p.causal ? p.offset + at.q : p.ks;
     const int clear_limit = p.causal ? min(p.ks - 1, p.offset + wave_first_q) : p.ks - 1;
 
     LeftOut left(p, wave_first_q);
@@ -640,7 +712,7 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void differential_dq_ker
         // -(delta2 + rest) of the wavefront's rows.
         const float mine = at.live ? rest + (lane < 32 ? delta2 : 0.0f) : 0.0f;
         const float sum = wave_sum(mine);
-        const long part = (static_cast<long>(at.b) * gridDim.x + at.q_block / (kBlockRows / PARTS)) * (4 / PARTS) + at.row_wave;
+        const long part = (static_cast<long>(at.b) * gridDim.x + at.row / (kBlockRows / PARTS)) * (4 / PARTS) + at.row_wave;
         if (lane == 0) p.lambda_partial[at.h * p.lambda_parts + part] = -sum;
     }
     if (!at.live) return;
@@ -731,8 +803,11 @@ __global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(Different
         const bool k_live = k_row < p.ks;
         const long k_head = static_cast<long>(b) * p.ks * kv_stride + kvh * p.d, k_offset = k_head + k_row * kv_stride;
         frag kf[STEPS], vf[STEPS];
-        load_rows<T, W, true>(kf, p.k, k_head, kv_stride, p.ks, k_block + wave * 32, p.d);
-        load_rows<T, W, false>(vf, p.v, k_head, kv_stride, p.ks, k_block + wave * 32, p.d);
+        const int first_key = k_block + wave * 32, key_bytes = (lane & 31) * static_cast<int>(kv_stride * sizeof(T));
+        const long wave_bytes = first_key < p.ks ? ((min(p.ks - first_key, 32) - 1) * kv_stride + p.d) * static_cast<long>(sizeof(T)) : 0;
+        const long first_row = first_key < p.ks ? k_head + first_key * kv_stride : 0;
+        load_rows<T, W, true>(kf, p.k, first_row, wave_bytes, key_bytes, k_live, p.d);
+        load_rows<T, W, false>(vf, p.v, first_row, wave_bytes, key_bytes, k_live, p.d);
         acc_t dk[DT], dv[DT];
 #pragma unroll
         for (int t = 0; t < DT; ++t) dk[t] = dv[t] = acc_t(0.0f);
@@ -938,7 +1013,7 @@ bool two_parts(const DifferentialArgs& a) {
     const long blocks = (static_cast<long>(a.qs) + kBlockRows / 2 - 1) / (kBlockRows / 2) * a.hq * a.batch;
     return a.ks > kStream && blocks <= static_cast<long>(compute_units()) * (a.d <= 64 ? 2 : 1);
 }
-template <auto Kernel, int W, int PARTS>
+template <auto Kernel, int W, int PARTS, bool SPLIT = false>
 int launch_rows(const DifferentialArgs& a, hipStream_t stream) {
     constexpr int smem = PARTS == 1 ? 0 : 8 * kWideTile<W> * 2;  // [stage][part][K | V] of 16-bit elements
     if constexpr (PARTS > 1) {
@@ -946,8 +1021,9 @@ int launch_rows(const DifferentialArgs& a, hipStream_t stream) {
             hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
         CGPTX_HIP(status);
     }
-    const dim3 grid(static_cast<unsigned int>((a.qs + kBlockRows / PARTS - 1) / (kBlockRows / PARTS)), static_cast<unsigned int>(a.hq),
-                    static_cast<unsigned int>(a.batch));
+    const long rows = static_cast<long>(a.qs) * (SPLIT ? a.pack : 1);
+    const dim3 grid(static_cast<unsigned int>((rows + kBlockRows / PARTS - 1) / (kBlockRows / PARTS) * (SPLIT ? a.splits : 1)),
+                    static_cast<unsigned int>(a.hq / (SPLIT ? a.pack : 1)), static_cast<unsigned int>(a.batch));
     hipLaunchKernelGGL(Kernel, grid, dim3(kThreads), smem, stream, a);
     CGPTX_LAUNCH_CHECK();
     return CGPTX_OK;
@@ -987,10 +1063,52 @@ bool differential_mfma_takes(const DifferentialArgs& a) {
     return a.dtype != CGPTX_F32 && a.d % 16 == 0 && kStream * row <= (std::size_t{1} << 30);
 }
 
-int differential_mfma_forward(const DifferentialArgs& a, hipStream_t stream) {
+// Workgroups that share a query block's keys in the forward pass: as many as find a place on the chip beside each other, of four tiles
+// or more, if that is predicted to take less time: sharing costs a launch and the sums' way to memory and back. Few queries of many keys
+// (a token at a time against a long sequence) leave most of the chip idle otherwise: one query of 8:2 heads of 128, bf16, on 8192 keys
+// 164 -> 16 us, on 131072 2694 -> 54.
+int forward_splits(const DifferentialArgs& a) {
+    if (!two_parts(a)) return 1;
+    const long blocks = (static_cast<long>(a.qs) * a.pack + kBlockRows / 2 - 1) / (kBlockRows / 2) * (a.hq / a.pack) * a.batch;
+    const long keys = a.causal ? std::min<long>(a.ks, static_cast<long>(a.offset) + a.qs) : a.ks, tiles = (keys + kStream - 1) / kStream;
+    const long most = std::min<long>({static_cast<long>(compute_units()) * (a.d <= 64 ? 2 : 1) / blocks, tiles / 4, kMostSplits});
+    const double pair_us = a.d <= 64 ? 1.4 : 2.2;  // two tiles, one in either part of a workgroup
+    const double megabytes = static_cast<double>(a.batch) * a.qs * a.hq * a.d * 16e-6;  // both maps' sums of a part, there and back
+    long best = 1;
+    double best_us = 0.0;
+    for (long splits = 1; splits <= most; ++splits) {
+        const double us = static_cast<double>((tiles + 2 * splits - 1) / (2 * splits)) * pair_us + (splits > 1 ? 5.0 + 0.4 * megabytes * splits : 0.0);
+        if (splits == 1 || us < best_us) {
+            best = splits;
+            best_us = us;
+        }
+    }
+    return static_cast<int>(best);
+}
+
+int differential_mfma_forward(DifferentialArgs a, hipStream_t stream) {
+    const std::size_t rows = static_cast<std::size_t>(a.batch) * a.qs * a.hq, part = 2 * rows * (a.d + 2) * sizeof(float);
+    const int group = a.hq / a.hkv;
+    a.pack = static_cast<long>(a.qs) * group <= kBlockRows / 2 ? group : 1;  // one block has a whole group's rows
+    a.splits = forward_splits(a);
+    if (a.splits > 1) {  // an arena that cannot grow has room for fewer
+        void* memory = nullptr;
+        std::size_t held = 0;
+        if (int st = scratch_up_to(stream, a.splits * part, &memory, &held)) return st;
+        a.splits = static_cast<int>(std::min<std::size_t>(a.splits, held / part));
+        a.partial = static_cast<float*>(memory);
+        a.delta = a.partial + 2 * rows * a.d * static_cast<std::size_t>(std::max(a.splits, 0));
+    }
     return dispatch(a, [&]<typename T, int W>() -> int {
-        return two_parts(a) ? launch_rows<differential_forward_kernel<T, W, 2>, W, 2>(a, stream)
-                            : launch_rows<differential_forward_kernel<T, W, 1>, W, 1>(a, stream);
+        if (a.splits > 1) {
+            if (int st = launch_rows<differential_forward_kernel<T, W, 2, true>, W, 2, true>(a, stream)) return st;
+            auto combine = a.splits <= 8 ? differential_combine_kernel<T, 8> : differential_combine_kernel<T, kMostSplits>;
+            hipLaunchKernelGGL(combine, dim3(static_cast<unsigned int>(rows)), dim3(kThreads), 0, stream, a);
+            CGPTX_LAUNCH_CHECK();
+            return CGPTX_OK;
+        }
+        return two_parts(a) ? launch_rows<differential_forward_kernel<T, W, 2, false>, W, 2>(a, stream)
+                            : launch_rows<differential_forward_kernel<T, W, 1, false>, W, 1>(a, stream);
     });
 }
 

@@ -4,13 +4,18 @@ Tolerances, for every element. u = eps/2 of the storage type; the kernels round 
 once before a product (relative to the value), and each result once. The backward pass is given the forward pass's rounded
 outputs: delta2 = dO.O2 is then off by u sum|dO O2|, delta1 = dO.O + lambda delta2 by u sum|dO|(|O| + 2 lambda |O2|). What fp32
 does to scores and exponentials is within C = 2^-24 (64 products + 32) (1 + max|score|) relative to a probability, and a sum of
-n terms in fp32 within 2^-24 n of their magnitudes; 16-bit storage has both far below u."""
+n terms in fp32 within 2^-24 n of their magnitudes; 16-bit storage has both far below u.
+
+Half precision rounds what is below 2^-14 by up to 2^-25 whatever its size, and the probabilities of a row of thousands of keys (5000
+keys: 2e-4 on average, their difference less) and their score gradients get there. A factor that is off by 2^-25 adds 2^-25 of the
+other factor: hence terms of 2^-25 sum|dO| for dv and 2^-25 s sum|k|, sum|q| for dq and dk. In the forward pass the factors
+stand to the row's largest one, which is P's maximum times as much when all is done."""
 import math
 
 import pytest
 import torch
 
-from cgpt_amd import ops
+from cgpt_amd import capi, ops
 from tests.util import DTYPE_IDS, DTYPES, launches, randn
 
 pytestmark = pytest.mark.gpu
@@ -58,6 +63,7 @@ def reference(c, q, k, v, lambdas, dout=None, dtype=None):
     u, f = torch.finfo(dtype).eps / 2, 2.0 ** -24
     if dtype == torch.float32:
         u = 0.0  # nothing is rounded on the way; the bounds' own terms stay
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
     half, group = c["d"] // 2, c["hq"] // c["hkv"]
     scale = c["scale"] or 1 / math.sqrt(half)
     qh, kh, vh = heads_first(q), heads_first(k, group), heads_first(v, group)
@@ -83,8 +89,11 @@ def reference(c, q, k, v, lambdas, dout=None, dtype=None):
 
     av1, av2 = product(p1, vh.abs()), product(p2, vh.abs())
     r = {"out": back(out), "second": back(o2), "lse": torch.stack([l.permute(0, 2, 1) for l in lses])}
-    r["out_err"] = back((u + 2 * soft + n * f) * (av1 + lam.abs() * av2))
-    r["second_err"] = back((u + 2 * soft + n * f) * av2)
+    seen = torch.ones_like(p1) if hidden is None else (~hidden).double().expand_as(p1)
+    small = tiny * product(seen, vh.abs())
+    small1, small2 = (small * p.amax(-1, keepdim=True) for p in (p1, p2))
+    r["out_err"] = back((u + 2 * soft + n * f) * (av1 + lam.abs() * av2) + small1 + lam.abs() * small2)
+    r["second_err"] = back((u + 2 * soft + n * f) * av2 + small2)
     r["lse_err"] = 2 * soft + n * f + 4 * f * r["lse"].abs()
     if dout is None:
         return r
@@ -101,14 +110,14 @@ def reference(c, q, k, v, lambdas, dout=None, dtype=None):
     d1_err = (do.abs() * o_err).sum(-1, keepdim=True) + lam.abs() * d2_err + 2 * f * (c["d"] + 8) * (do * out).abs().sum(-1, keepdim=True)
     ds1, ds2 = p1 * (g - d1), -lam * p2 * (g - d2)
     spread1, spread2 = p1 * (g.abs() + d1.abs()), lam.abs() * p2 * (g.abs() + d2.abs())
-    e1 = u * ds1.abs() + p1 * (d1_err + g_err) * (1 + u) + (2 * soft + 4 * f) * spread1
-    e2 = u * ds2.abs() + lam.abs() * p2 * (d2_err + g_err) * (1 + u) + (2 * soft + 4 * f) * spread2
+    e1 = tiny * seen + u * ds1.abs() + p1 * (d1_err + g_err) * (1 + u) + (2 * soft + 4 * f) * spread1
+    e2 = tiny * seen * torch.clamp(lam.abs(), min=1.0) + u * ds2.abs() + lam.abs() * p2 * (d2_err + g_err) * (1 + u) + (2 * soft + 4 * f) * spread2
     k1, k2, q1, q2 = kh[..., :half], kh[..., half:], qh[..., :half], qh[..., half:]
     dq = torch.cat([product(ds1, k1), product(ds2, k2)], -1) * scale
     dq_err = torch.cat([product(e1 + n * f * spread1, k1.abs()), product(e2 + n * f * spread2, k2.abs())], -1) * scale
     m = c["qs"] * group + 24
     pd = p1 - lam * p2
-    pd_err = u * pd.abs() + (2 * soft + (m + 4) * f) * (p1 + lam.abs() * p2)
+    pd_err = tiny * seen + u * pd.abs() + (2 * soft + (m + 4) * f) * (p1 + lam.abs() * p2)
 
     def grouped(t):
         return t.view(c["b"], c["hkv"], group, *t.shape[2:]).sum(2)
@@ -160,6 +169,53 @@ def test_forward_and_backward(device, c, dtype):
         check(got, want[name], want[name + "_err"], name)
     for got, name in zip(backward(c, q, k, v, dout, lambdas, saved), GRADS):
         check(got, want[name], want[name + "_err"], name)
+
+
+# A token or a few against many keys: the keys of a block of queries are shared by several workgroups, a group's heads share a block.
+LONG = [case(1, 1, 3000, 8, 2, 128), case(2, 1, 700, 4, 1, 64), case(1, 1, 5000, 2, 2, 32), case(1, 7, 2000, 6, 2, 96), case(3, 21, 1100, 3, 1, 112),
+        case(1, 22, 1100, 3, 1, 128), case(1, 30, 1500, 4, 4, 64, causal=False), case(1, 64, 2100, 2, 1, 128), case(1, 200, 2500, 1, 1, 128),
+        case(1, 1000, 1000, 1, 1, 64), case(1, 3, 1300, 16, 1, 80, causal=False), case(1, 5, 900, 4, 2, 64, off=400)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=DTYPE_IDS)
+@pytest.mark.parametrize("c", LONG, ids=["-".join(str(v) for v in c.values()) for c in LONG])
+def test_few_queries_of_many_keys(device, c, dtype):
+    q, k, v, dout, lambdas = inputs(c, dtype, device)
+    saved = forward(c, q, k, v, lambdas)
+    want = reference(c, q, k, v, lambdas, dout)
+    for got, name in zip(saved, ("out", "second", "lse")):
+        check(got, want[name], want[name + "_err"], name)
+    for got, name in zip(backward(c, q, k, v, dout, lambdas, saved), GRADS):
+        check(got, want[name], want[name + "_err"], name)
+    again = forward(c, q, k, v, lambdas)
+    assert all(torch.equal(a, b) for a, b in zip(saved, again))
+    alone = torch.full_like(q, 7.0)
+    ops.differential_attention_forward(alone, None, None, q, k, v, lambdas, None, options(c))
+    assert torch.equal(alone, saved[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=DTYPE_IDS)
+def test_recorded_without_a_call_before(device, dtype):
+    """A forward call asks for scratch only where it is faster with it: recorded first, it does without. A backward call says that it
+    cannot."""
+    c = case(1, 3, 2000, 4, 2, 64)
+    q, k, v, dout, lambdas = inputs(c, dtype, device)
+    want = reference(c, q, k, v, lambdas)
+    out, second, lse = torch.zeros_like(q), torch.zeros_like(q), torch.zeros((2, *q.shape[:3]), device=device)
+    grads = [torch.zeros_like(t) for t in (q, k, v, lambdas)]
+    torch.cuda.synchronize()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+        ops.differential_attention_forward(out, second, lse, q, k, v, lambdas, None, options(c))
+        with pytest.raises(capi.CgptxCaptureError):
+            ops.differential_attention_backward(*grads, dout, out, second, lse, q, k, v, lambdas, None, options(c))
+    for _ in range(3):
+        out.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, name in zip((out, second, lse), ("out", "second", "lse")):
+            check(got, want[name], want[name + "_err"], name)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=DTYPE_IDS)
@@ -247,6 +303,23 @@ def test_what_stands_behind_the_mask_does_not_matter(device, dtype, d):
         for got, name in ((out, "out"), (second, "second"), (dq, "dq")):
             check(got[:, :live], want[name][:, :live], want[name + "_err"][:, :live], name)
         check(lse[:, :, :live], want["lse"][:, :, :live], want["lse_err"][:, :, :live], "lse")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=DTYPE_IDS)
+def test_what_stands_behind_the_mask_of_few_queries(device, dtype):
+    c = case(2, 20, 1500, 6, 2, 128, off=900)
+    q, k, v, dout, lambdas = inputs(c, dtype, device)
+    want = reference(c, q, k, v, lambdas)
+    k[:, 920:] = float("nan")
+    v[:, 920:] = float("inf")
+    for got, name in zip(forward(c, q, k, v, lambdas), ("out", "second", "lse")):
+        check(got, want[name], want[name + "_err"], name)
+    k[:, 910:] = float("nan")
+    v[:, 910:] = float("nan")
+    out, second, lse = forward(c, q, k, v, lambdas)
+    for got, name in ((out, "out"), (second, "second")):
+        check(got[:, :10], want[name][:, :10], want[name + "_err"][:, :10], name)
+        assert torch.isnan(got[:, 10:]).all()
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=DTYPE_IDS)
