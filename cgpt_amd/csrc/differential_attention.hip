@@ -136,8 +136,8 @@ __global__ __launch_bounds__(kThreads) void differential_dq_scalar_kernel(Params
         dq.a = fmaf(ds.a, kr.a, dq.a);
         dq.b = fmaf(ds.b, kr.b, dq.b);
     }
-    dq.a *= p.scale;
-    dq.b *= p.scale;
+    dq.a *= p.gradient_scale;
+    dq.b *= p.gradient_scale;
     dq.store(static_cast<T*>(p.dq) + row * p.d, p.d, p.accumulate != 0);
     if ((threadIdx.x & (kWave - 1)) == 0) {
         p.delta[row] = delta1;
@@ -179,8 +179,8 @@ __global__ __launch_bounds__(kThreads) void differential_dkv_scalar_kernel(Param
             dk.b = fmaf(ds.b, q.b, dk.b);
         }
     }
-    dk.a *= p.scale;
-    dk.b *= p.scale;
+    dk.a *= p.gradient_scale;
+    dk.b *= p.gradient_scale;
     dk.store(static_cast<T*>(p.dk) + row * p.d, p.d, p.accumulate != 0);
     dv.store(static_cast<T*>(p.dv) + row * p.d, p.d, p.accumulate != 0);
 }
@@ -276,6 +276,7 @@ Params make_params(const Shape& s, const void* q, const void* k, const void* v, 
     p.hkv = static_cast<int>(s.hkv);
     p.d = static_cast<int>(s.d);
     p.scale = s.scale > 0.0f ? s.scale : 1.0f / std::sqrt(static_cast<float>(s.d / 2));
+    p.gradient_scale = s.ks > 1 ? p.scale : 0.0f;
     p.causal = s.causal ? 1 : 0;
     p.offset = s.causal ? static_cast<int>(s.offset) : 0;
     p.dtype = s.dtype;

@@ -12,11 +12,15 @@ struct DifferentialArgs {
     float* dlambda;
     const void *q, *k, *v, *dout, *o, *o2;
     const float *lambda, *lse;
-    float* delta;           // scalar kernels [2][batch, qs, hq]: delta1, delta2; matrix kernels [4]: those behind both LSE·log2 e
+    // Statistics of the rows, [n][batch, qs, hq]. Backward: delta1, delta2 of the scalar and fp32 kernels; of the 16-bit ones, four in
+    // the form that their dK/dV takes (lse1·log2 e, lse2·log2 e - log2|lambda|, -delta1, sign(-lambda)(delta1 - delta2)). Forward
+    // with shared keys: [splits][2][batch, qs, hq] pairs of a map's largest score and the sum that stands to it.
+    float* delta;
     float* lambda_partial;  // [hq][lambda_parts]: what a head's dlambda is the sum of
     long lambda_parts;
     int batch, qs, ks, hq, hkv, d;
-    float scale;
+    float scale;           // of the scores
+    float gradient_scale;  // of their gradients: the same, and 0 where there is one key, whose share is 1 whatever the score
     int causal, offset, accumulate;
     int dtype;
     // dK/dV on the matrix cores, set by its launch (fp32: splits only); a forward pass whose keys are shared sets splits, partial, delta:

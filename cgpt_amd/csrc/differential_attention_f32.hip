@@ -400,7 +400,7 @@ __global__ __launch_bounds__(kF32Threads) void differential_f32_dq_kernel(Differ
     }
     rest = group_sum(rest);
     if (lane < kTile) wave_rest[wave][lane] = live ? (wave == 0 ? rest + delta2 : rest) : 0.0f;
-    deposit<D, true>(lds, wave, dq, p.scale);
+    deposit<D, true>(lds, wave, dq, p.gradient_scale);
     __syncthreads();
     if (threadIdx.x < kTile) {
         float sum = wave_rest[0][lane];
@@ -515,7 +515,7 @@ __global__ __launch_bounds__(kF32Threads) void differential_f32_dkv_kernel(Diffe
         if (p.accumulate && p.splits == 1) sum += load_vec<float, 4>(to);
         store_vec<float, 4>(to, sum);
     };
-    deposit<D, true>(lds, wave, dk, p.scale);
+    deposit<D, true>(lds, wave, dk, p.gradient_scale);
     __syncthreads();
     store(static_cast<float*>(p.dk), p.partial + 2 * part * count, share.collect(lds), source<D, true>(share.at, p.d));
     __syncthreads();

@@ -57,8 +57,9 @@ def product(a, b):
     return torch.matmul(a.contiguous(), b.contiguous())
 
 
-def reference(c, q, k, v, lambdas, dout=None, dtype=None):
-    """Results in 64 bits, [batch, sequence, heads, width], and their bounds."""
+def reference(c, q, k, v, lambdas, dout=None, dtype=None, summed=False):
+    """Results in 64 bits, [batch, sequence, heads, width], and their bounds; `summed`: for deltas that are rowsum(P G) in fp32, whatever
+    the outputs were rounded to."""
     dtype = dtype or q.dtype
     u, f = torch.finfo(dtype).eps / 2, 2.0 ** -24
     if dtype == torch.float32:
@@ -108,6 +109,11 @@ def reference(c, q, k, v, lambdas, dout=None, dtype=None):
     o_err = heads_first(r["out_err"]) + step * out.abs()
     d2_err = (do.abs() * o2_err).sum(-1, keepdim=True) + f * (c["d"] + 8) * (do * o2).abs().sum(-1, keepdim=True)
     d1_err = (do.abs() * o_err).sum(-1, keepdim=True) + lam.abs() * d2_err + 2 * f * (c["d"] + 8) * (do * out).abs().sum(-1, keepdim=True)
+    # rowsum(P G) in fp32: the rounded delta comes back in with the sum of P's row, which is one to n f + 2 C.
+    d1_sum, d2_sum = ((p * (g_err + (2 * soft + (n + 8) * f) * g.abs())).sum(-1, keepdim=True) + (2 * soft + (n + 8) * f) * (d.abs() + d_err) * 2
+                      for p, d, d_err in ((p1, d1, d1_err), (p2, d2, d2_err)))
+    if summed:
+        d1_err, d2_err = d1_sum, d2_sum
     ds1, ds2 = p1 * (g - d1), -lam * p2 * (g - d2)
     spread1, spread2 = p1 * (g.abs() + d1.abs()), lam.abs() * p2 * (g.abs() + d2.abs())
     e1 = tiny * seen + u * ds1.abs() + p1 * (d1_err + g_err) * (1 + u) + (2 * soft + 4 * f) * spread1
@@ -129,9 +135,7 @@ def reference(c, q, k, v, lambdas, dout=None, dtype=None):
     for name, value in (("dq", dq), ("dq_err", dq_err), ("dk", dk), ("dk_err", dk_err), ("dv", dv), ("dv_err", dv_err)):
         r[name] = back(value)
     r["dlam"] = -d2.sum((0, 2, 3))
-    # rowsum(P2 G) in fp32, whatever O2 was rounded to: the rounded delta2 comes back in with the sum of P2's row, which is one to n f + 2 C.
-    per_row = (p2 * (g_err + (2 * soft + (n + 8) * f) * g.abs())).sum(-1, keepdim=True) + (2 * soft + (n + 8) * f) * (d2.abs() + d2_err) * 2
-    r["dlam_err"] = per_row.sum((0, 2, 3)) + f * 64 * d2.abs().sum((0, 2, 3))
+    r["dlam_err"] = d2_sum.sum((0, 2, 3)) + f * 64 * d2.abs().sum((0, 2, 3))
     return r
 
 
@@ -169,6 +173,31 @@ def test_forward_and_backward(device, c, dtype):
         check(got, want[name], want[name + "_err"], name)
     for got, name in zip(backward(c, q, k, v, dout, lambdas, saved), GRADS):
         check(got, want[name], want[name + "_err"], name)
+
+
+# Sequences of few tokens: a row's score gradients are differences of what its keys give, near nothing for the first rows.
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("c", [case(3, 2, 2, 4, 2, 64), case(7, 4, 4, 4, 2, 128), case(1, 13, 13, 2, 1, 80), case(2, 64, 64, 2, 2, 32),
+                               case(2, 100, 5, 2, 1, 128, causal=False), case(1, 300, 40, 2, 2, 64, causal=False)],
+                         ids=["2", "4", "13", "64", "5-keys", "40-keys"])
+def test_few_keys(device, c, dtype):
+    q, k, v, dout, lambdas = inputs(c, dtype, device)
+    want = reference(c, q, k, v, lambdas, dout, summed=True)
+    for got, name in zip(backward(c, q, k, v, dout, lambdas, forward(c, q, k, v, lambdas)), GRADS):
+        check(got, want[name], want[name + "_err"], name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=DTYPE_IDS)
+@pytest.mark.parametrize("c", [case(2, 1, 1, 4, 2, 128), case(1, 150, 1, 4, 1, 64, causal=False), case(3, 7, 1, 2, 2, 36, causal=False)],
+                         ids=["token", "queries", "narrow"])
+def test_one_key_has_no_score_gradient(device, c, dtype):
+    q, k, v, dout, lambdas = inputs(c, dtype, device)
+    saved = forward(c, q, k, v, lambdas)
+    dq, dk, _, _ = backward(c, q, k, v, dout, lambdas, saved)
+    assert not dq.any() and not dk.any()
+    base = [randn(t.shape, t.dtype, 50 + i).to(device) for i, t in enumerate((q, k, v, lambdas))]
+    dq, dk, _, _ = backward(c, q, k, v, dout, lambdas, saved, base)
+    assert torch.equal(dq, base[0]) and torch.equal(dk, base[1])
 
 
 # A token or a few against many keys: the keys of a block of queries are shared by several workgroups, a group's heads share a block.
