@@ -881,7 +881,19 @@ __global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(Different
         // MASKED: some (query, key) pairs of this wavefront are hidden (causal mask, keys past the end); first = first visible register
         // coordinate for this lane's key. Queries past the end need nothing: their dO rows, delta and lse are zeros.
         auto tile_body = [&]<bool MASKED>(int stage, float sign, int first, const NextTile& next) {
-            constexpr int H = W / 16, kSlots = 8 * H, kLookAhead = W == 64 ? 2 : 4;
+            constexpr int H = W / 16, kSlots = 8 * H, kLookAhead = W == 64 ? 2 : 6;
+            if constexpr (W == 128) {
+                using words = vec_t<unsigned int, 4>;
+                // K and V are operands only: in the accumulation registers, where the matrix instructions read them as they are. Left to
+                // the compiler they were copied out in every tile, some 60 of its 860 instructions.
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    auto k_words = __builtin_bit_cast(words, kf[i]), v_words = __builtin_bit_cast(words, vf[i]);
+                    asm volatile("" : "+a"(k_words), "+a"(v_words));
+                    kf[i] = __builtin_bit_cast(frag, k_words);
+                    vf[i] = __builtin_bit_cast(frag, v_words);
+                }
+            }
             const TileOffsets<W> here = offsets.at(stage * 2 * kWideTile<W>);
             const float* stat = stats + stage * 4 * kStream + 4 * (lane >> 5);
             acc_t s_acc[2][2], g_acc[2];                              // [half][map]
