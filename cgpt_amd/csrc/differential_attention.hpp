@@ -37,7 +37,7 @@ bool differential_mfma_takes(const DifferentialArgs& args);
 int differential_mfma_forward(DifferentialArgs args, hipStream_t stream);  // takes scratch where few queries share many keys
 int differential_mfma_backward(DifferentialArgs args, hipStream_t stream);  // takes its scratch itself
 
-// The fp32 ones: halves of a head in multiples of 4, tensors on 16-byte boundaries.
+// The fp32 ones: halves of a head in multiples of 4, 16 rows of a tensor within 1 GiB, tensors on 16-byte boundaries.
 bool differential_f32_takes(const DifferentialArgs& args);
 int differential_f32_forward(const DifferentialArgs& args, hipStream_t stream);
 int differential_f32_backward(DifferentialArgs args, hipStream_t stream);

@@ -16,6 +16,7 @@ constexpr int kF32Threads = kWaves * kWave;
 constexpr int kTile = 16;  // stationary rows of a workgroup, streamed rows of a step
 
 using quad = vec_t<float, 4>;
+using pair = vec_t<float, 2>;
 
 __device__ __forceinline__ quad mfma(float a, float b, quad c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
@@ -30,18 +31,37 @@ __device__ __forceinline__ int source(int c, int d) {
     }
 }
 
-// A row as an operand that is contracted over the head dimension: lane l holds row l % 16's padded columns 16 c + 4 (l / 16) .. + 3 of
-// chunk c. Rows that do not exist are zeros.
+// Rows row0 .. row0 + 15 of a head, of which those below `limit` exist, as a buffer: what lies outside it, like kNowhere, is read as
+// zero, without a branch around each load. The arguments are the same in all lanes.
+struct TileRows {
+    __amdgpu_buffer_rsrc_t rsrc;
+    int row_bytes;
+    static constexpr int kNowhere = 1 << 30;  // differential_f32_takes has a tile end before it
+    __device__ __forceinline__ TileRows(const float* head, long row_stride, int row0, int limit, int d) {
+        const int rows = min(limit - row0, kTile);
+        const float* first = head + (rows > 0 ? row0 * row_stride : 0);
+        row_bytes = static_cast<int>(row_stride) * 4;
+        rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(first), 0, rows > 0 ? (rows - 1) * row_bytes + d * 4 : 0, 0x00020000);
+    }
+    __device__ __forceinline__ quad four(int row, int column) const {
+        const int at = column >= 0 ? row * row_bytes + column * 4 : kNowhere;
+        return __builtin_bit_cast(quad, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0));
+    }
+    __device__ __forceinline__ pair two(int row, int column) const {
+        const int at = column >= 0 ? row * row_bytes + column * 4 : kNowhere;
+        return __builtin_bit_cast(pair, __builtin_amdgcn_raw_buffer_load_b64(rsrc, at, 0, 0));
+    }
+};
+
+// A tile as an operand that is contracted over the head dimension: lane l holds row l % 16's padded columns 16 c + 4 (l / 16) .. + 3
+// of chunk c. Rows that do not exist are zeros.
 template <int D, bool HALVES>
 struct RowOperand {
     quad chunk[D / 16];
-    __device__ __forceinline__ void load(const float* row, bool live, int d) {
-        const int at = ((threadIdx.x & (kWave - 1)) >> 4) * 4;
+    __device__ __forceinline__ void load(const TileRows& tile, int d) {
+        const int lane = threadIdx.x & (kWave - 1);
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-            const int column = source<D, HALVES>(16 * c + at, d);
-            chunk[c] = live && column >= 0 ? load_vec<float, 4>(row + column) : quad(0.0f);
-        }
+        for (int c = 0; c < D / 16; ++c) chunk[c] = tile.four(lane & 15, source<D, HALVES>(16 * c + (lane >> 4) * 4, d));
     }
 };
 template <int FROM, int TO, int D, bool HALVES>
@@ -70,27 +90,20 @@ __device__ __forceinline__ constexpr int map_of(int b, int e) {
 template <int D, bool HALVES>
 struct ColumnOperand {
     quad part[4][D / 64];
-    __device__ __forceinline__ void load(const float* base, long row_stride, int row0, int limit, int d) {
+    __device__ __forceinline__ void load(const TileRows& tile, int d) {
         const int lane = threadIdx.x & (kWave - 1), m = lane & 15;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = row0 + 4 * (lane >> 4) + r;
-            const float* from = base + row * row_stride;
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int b = 0; b < D / 64; ++b) {
-                const int first = source<D, HALVES>(padded_column<D, HALVES>(b, 0, m), d);
-                part[r][b] = quad(0.0f);
-                if (row >= limit) continue;
+                const int row = 4 * (lane >> 4) + r, first = source<D, HALVES>(padded_column<D, HALVES>(b, 0, m), d);
                 if constexpr (HALVES && D == 64) {
-                    const int second = source<D, HALVES>(padded_column<D, HALVES>(b, 2, m), d);
-                    if (first < 0) continue;  // the halves are equally wide
-                    const vec_t<float, 2> x = load_vec<float, 2>(from + first), y = load_vec<float, 2>(from + second);
+                    const pair x = tile.two(row, first), y = tile.two(row, source<D, HALVES>(padded_column<D, HALVES>(b, 2, m), d));
                     part[r][b] = quad{x[0], x[1], y[0], y[1]};
-                } else if (first >= 0) {
-                    part[r][b] = load_vec<float, 4>(from + first);
+                } else {
+                    part[r][b] = tile.four(row, first);
                 }
             }
-        }
     }
 };
 template <int D>
@@ -132,13 +145,15 @@ __device__ __forceinline__ void accumulate_visible(Result<D>& result, const floa
                                 __shfl(r == 0 ? second[0] : r == 1 ? second[1] : r == 2 ? second[2] : second[3], from, kWave)};
         if (row0 + i >= limit || !visible(i)) continue;
         const float* row = base + (row0 + i) * row_stride;
+        int group = lane >> 4;
+        asm volatile("" : "+v"(group));  // the columns are worked out here, not kept in registers through the walk
 #pragma unroll
         for (int b = 0; b < D / 64; ++b)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const int column = source<D, HALVES>(padded_column<D, HALVES>(b, e, 4 * (lane >> 4) + c), d);
+                    const int column = source<D, HALVES>(padded_column<D, HALVES>(b, e, 4 * group + c), d);
                     if (column >= 0) result[b][e][c] = fmaf(row[column], value[HALVES ? map_of<D>(b, e) : 0], result[b][e][c]);
                 }
     }
@@ -193,18 +208,18 @@ __device__ __forceinline__ void clear(Result<D>& result) {
 }
 
 template <int D>
-__global__ __launch_bounds__(kF32Threads) void differential_f32_forward_kernel(DifferentialArgs p) {
+__global__ __launch_bounds__(kF32Threads, D == 64 ? 4 : 2) void differential_f32_forward_kernel(DifferentialArgs p) {
     extern __shared__ __align__(16) float lds[];
     __shared__ float wave_max[2][kWaves][kTile], wave_total[2][kWaves][kTile];
     constexpr int HALF = D / 32;
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, g = lane >> 4;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), g = lane >> 4;
     const int q0 = (gridDim.x - 1 - blockIdx.x) * kTile, h = blockIdx.y, b = blockIdx.z, kvh = h / (p.hq / p.hkv);  // longest first
     const int query = q0 + (lane & 15);
     const long q_stride = static_cast<long>(p.hq) * p.d, kv_stride = static_cast<long>(p.hkv) * p.d;
     const float* k_base = static_cast<const float*>(p.k) + static_cast<long>(b) * p.ks * kv_stride + static_cast<long>(kvh) * p.d;
     const float* v_base = static_cast<const float*>(p.v) + static_cast<long>(b) * p.ks * kv_stride + static_cast<long>(kvh) * p.d;
     RowOperand<D, true> q;
-    q.load(static_cast<const float*>(p.q) + (static_cast<long>(b) * p.qs + query) * q_stride + static_cast<long>(h) * p.d, query < p.qs, p.d);
+    q.load(TileRows(static_cast<const float*>(p.q) + static_cast<long>(b) * p.qs * q_stride + static_cast<long>(h) * p.d, q_stride, q0, p.qs, p.d), p.d);
     const int last_key = p.causal ? min(p.ks - 1, p.offset + min(q0 + kTile, p.qs) - 1) : p.ks - 1;
     const int tiles = last_key / kTile + 1;
     const int my_last = p.causal ? min(p.ks - 1, p.offset + query) : p.ks - 1;
@@ -215,15 +230,14 @@ __global__ __launch_bounds__(kF32Threads) void differential_f32_forward_kernel(D
     clear<D>(o[0]);
     clear<D>(o[1]);
     auto key_rows = [&](RowOperand<D, true>& k, int t) {
-        const int key = t * kTile + (lane & 15);
-        k.load(k_base + key * kv_stride, key < p.ks && t < tiles, p.d);
+        k.load(TileRows(k_base, kv_stride, t * kTile, t < tiles ? p.ks : 0, p.d), p.d);
     };
     bool left_out = false;
     RowOperand<D, true> k, ahead;
     key_rows(k, wave);
     for (int t = wave; t < tiles; t += kWaves) {
         ColumnOperand<D, false> v;
-        v.load(v_base, kv_stride, t * kTile, p.ks, p.d);
+        v.load(TileRows(v_base, kv_stride, t * kTile, p.ks, p.d), p.d);
         key_rows(ahead, t + kWaves);
         quad s[2] = {product<0, HALF>(k, q), product<HALF, 2 * HALF>(k, q)};  // lane: query l % 16, keys 4 g + r
 #pragma unroll
@@ -261,7 +275,7 @@ __global__ __launch_bounds__(kF32Threads) void differential_f32_forward_kernel(D
     if (left_out) {
         for (int t = wave; t < tiles; t += kWaves) {
             ColumnOperand<D, false> v;
-            v.load(v_base, kv_stride, t * kTile, p.ks, p.d);
+            v.load(TileRows(v_base, kv_stride, t * kTile, p.ks, p.d), p.d);
             if (t < first_masked || !non_finite(v)) continue;
             key_rows(k, t);
             quad s[2] = {product<0, HALF>(k, q), product<HALF, 2 * HALF>(k, q)};
@@ -316,9 +330,9 @@ __global__ __launch_bounds__(kF32Threads) void differential_f32_forward_kernel(D
 }
 
 template <int D>
-__device__ __forceinline__ float row_delta(const RowOperand<D, false>& dout, const float* row, bool live, int d) {
+__device__ __forceinline__ float row_delta(const RowOperand<D, false>& dout, const TileRows& rows, int d) {
     RowOperand<D, false> o;
-    o.load(row, live, d);
+    o.load(rows, d);
     float sum = 0.0f;
 #pragma unroll
     for (int c = 0; c < D / 16; ++c)
@@ -328,26 +342,27 @@ __device__ __forceinline__ float row_delta(const RowOperand<D, false>& dout, con
 }
 
 template <int D>
-__global__ __launch_bounds__(kF32Threads) void differential_f32_dq_kernel(DifferentialArgs p) {
+__global__ __launch_bounds__(kF32Threads, D == 64 ? 4 : 2) void differential_f32_dq_kernel(DifferentialArgs p) {
     extern __shared__ __align__(16) float lds[];
     __shared__ float wave_rest[kWaves][kTile];
     constexpr int HALF = D / 32;
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, g = lane >> 4;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), g = lane >> 4;
     const int q0 = (gridDim.x - 1 - blockIdx.x) * kTile, h = blockIdx.y, b = blockIdx.z, kvh = h / (p.hq / p.hkv);
     const int query = q0 + (lane & 15);
     const bool live = query < p.qs;
     const long q_stride = static_cast<long>(p.hq) * p.d, kv_stride = static_cast<long>(p.hkv) * p.d;
     const float* k_base = static_cast<const float*>(p.k) + static_cast<long>(b) * p.ks * kv_stride + static_cast<long>(kvh) * p.d;
     const float* v_base = static_cast<const float*>(p.v) + static_cast<long>(b) * p.ks * kv_stride + static_cast<long>(kvh) * p.d;
-    const long q_row = (static_cast<long>(b) * p.qs + query) * q_stride + static_cast<long>(h) * p.d;
+    const long q_head = static_cast<long>(b) * p.qs * q_stride + static_cast<long>(h) * p.d;
+    auto rows_of = [&](const void* tensor) { return TileRows(static_cast<const float*>(tensor) + q_head, q_stride, q0, p.qs, p.d); };
     const long rows = static_cast<long>(p.batch) * p.qs * p.hq, stat = (static_cast<long>(b) * p.qs + query) * p.hq + h;
     const float lambda = p.lambda[h];
     RowOperand<D, true> q;
     RowOperand<D, false> dout;
-    q.load(static_cast<const float*>(p.q) + q_row, live, p.d);
-    dout.load(static_cast<const float*>(p.dout) + q_row, live, p.d);
-    const float delta2 = row_delta<D>(dout, static_cast<const float*>(p.o2) + q_row, live, p.d);
-    const float delta1 = fmaf(lambda, delta2, row_delta<D>(dout, static_cast<const float*>(p.o) + q_row, live, p.d));
+    q.load(rows_of(p.q), p.d);
+    dout.load(rows_of(p.dout), p.d);
+    const float delta2 = row_delta<D>(dout, rows_of(p.o2), p.d);
+    const float delta1 = fmaf(lambda, delta2, row_delta<D>(dout, rows_of(p.o), p.d));
     if (wave == 0 && lane < kTile && live) {
         p.delta[stat] = delta1;
         p.delta[rows + stat] = delta2;
@@ -365,11 +380,10 @@ __global__ __launch_bounds__(kF32Threads) void differential_f32_dq_kernel(Differ
         quad first, second;
     };
     auto score_gradients = [&](int t) {  // lane: query l % 16, keys 4 g + r
-        const int key = t * kTile + (lane & 15);
         RowOperand<D, true> k;
         RowOperand<D, false> v;
-        k.load(k_base + key * kv_stride, key < p.ks, p.d);
-        v.load(v_base + key * kv_stride, key < p.ks, p.d);
+        k.load(TileRows(k_base, kv_stride, t * kTile, p.ks, p.d), p.d);
+        v.load(TileRows(v_base, kv_stride, t * kTile, p.ks, p.d), p.d);
         const quad s1 = product<0, HALF>(k, q), s2 = product<HALF, 2 * HALF>(k, q), grad = product<0, 2 * HALF>(v, dout);
         Gradients ds;
 #pragma unroll
@@ -382,7 +396,7 @@ __global__ __launch_bounds__(kF32Threads) void differential_f32_dq_kernel(Differ
     };
     for (int t = wave; t <= last_key / kTile; t += kWaves) {
         ColumnOperand<D, true> columns;
-        columns.load(k_base, kv_stride, t * kTile, p.ks, p.d);
+        columns.load(TileRows(k_base, kv_stride, t * kTile, p.ks, p.d), p.d);
         Gradients ds = score_gradients(t);
         rest += (ds.second[0] + ds.second[1]) + (ds.second[2] + ds.second[3]);
         if (t >= first_masked && non_finite(columns)) left_out = true;
@@ -391,7 +405,7 @@ __global__ __launch_bounds__(kF32Threads) void differential_f32_dq_kernel(Differ
     if (left_out) {
         for (int t = wave; t <= last_key / kTile; t += kWaves) {
             ColumnOperand<D, true> columns;
-            columns.load(k_base, kv_stride, t * kTile, p.ks, p.d);
+            columns.load(TileRows(k_base, kv_stride, t * kTile, p.ks, p.d), p.d);
             if (t < first_masked || !non_finite(columns)) continue;
             const Gradients ds = score_gradients(t);
             accumulate_visible<D, true>(dq, k_base, kv_stride, t * kTile, p.ks, p.d, ds.first, ds.second * -lambda,
@@ -419,20 +433,20 @@ __global__ __launch_bounds__(kF32Threads) void differential_f32_dq_kernel(Differ
 }
 
 template <int D>
-__global__ __launch_bounds__(kF32Threads) void differential_f32_dkv_kernel(DifferentialArgs p) {
+__global__ __launch_bounds__(kF32Threads, D == 64 ? 4 : 2) void differential_f32_dkv_kernel(DifferentialArgs p) {
     extern __shared__ __align__(16) float lds[];
     constexpr int HALF = D / 32;
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, g = lane >> 4;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), g = lane >> 4;
     const int part = blockIdx.x % p.splits, k0 = blockIdx.x / p.splits * kTile;  // the first keys have most queries
     const int kvh = blockIdx.y, b = blockIdx.z, group = p.hq / p.hkv;
     const int key = k0 + (lane & 15);
     const long q_stride = static_cast<long>(p.hq) * p.d, kv_stride = static_cast<long>(p.hkv) * p.d;
-    const long kv_row = (static_cast<long>(b) * p.ks + key) * kv_stride + static_cast<long>(kvh) * p.d;
+    const long kv_head = static_cast<long>(b) * p.ks * kv_stride + static_cast<long>(kvh) * p.d;
     const long rows = static_cast<long>(p.batch) * p.qs * p.hq;
     RowOperand<D, true> k;
     RowOperand<D, false> v;
-    k.load(static_cast<const float*>(p.k) + kv_row, key < p.ks, p.d);
-    v.load(static_cast<const float*>(p.v) + kv_row, key < p.ks, p.d);
+    k.load(TileRows(static_cast<const float*>(p.k) + kv_head, kv_stride, k0, p.ks, p.d), p.d);
+    v.load(TileRows(static_cast<const float*>(p.v) + kv_head, kv_stride, k0, p.ks, p.d), p.d);
     const int first_query = p.causal ? max(0, key - p.offset) : 0;  // that sees this lane's key
     const int first_tile = p.causal ? max(0, k0 - p.offset) / kTile : 0;
     const int tiles = max(0, (p.qs + kTile - 1) / kTile - first_tile);
@@ -450,14 +464,13 @@ __global__ __launch_bounds__(kF32Threads) void differential_f32_dkv_kernel(Diffe
             const int head = i / tiles, row0 = (first_tile + i - head * tiles) * kTile, h = kvh * group + head;
             const float* q_base = static_cast<const float*>(p.q) + static_cast<long>(b) * p.qs * q_stride + static_cast<long>(h) * p.d;
             const float* do_base = static_cast<const float*>(p.dout) + static_cast<long>(b) * p.qs * q_stride + static_cast<long>(h) * p.d;
-            const int query = row0 + (lane & 15);
             const float lambda = p.lambda[h];
             quad s1, s2, grad;
             {
                 RowOperand<D, true> q;
                 RowOperand<D, false> dout;
-                q.load(q_base + query * q_stride, query < p.qs, p.d);
-                dout.load(do_base + query * q_stride, query < p.qs, p.d);
+                q.load(TileRows(q_base, q_stride, row0, p.qs, p.d), p.d);
+                dout.load(TileRows(do_base, q_stride, row0, p.qs, p.d), p.d);
                 s1 = product<0, HALF>(q, k);  // lane: key l % 16, queries 4 g + r
                 s2 = product<HALF, 2 * HALF>(q, k);
                 grad = product<0, 2 * HALF>(dout, v);
@@ -482,12 +495,12 @@ __global__ __launch_bounds__(kF32Threads) void differential_f32_dkv_kernel(Diffe
              __attribute__((always_inline)) {
         {
             ColumnOperand<D, false> columns;
-            columns.load(do_base, q_stride, row0, p.qs, p.d);
+            columns.load(TileRows(do_base, q_stride, row0, p.qs, p.d), p.d);
             if (masked(row0) && non_finite(columns)) left_out = true;
             else accumulate<D, false>(dv, columns, map, map);
         }
         ColumnOperand<D, true> columns;
-        columns.load(q_base, q_stride, row0, p.qs, p.d);
+        columns.load(TileRows(q_base, q_stride, row0, p.qs, p.d), p.d);
         if (masked(row0) && non_finite(columns)) left_out = true;
         else accumulate<D, true>(dk, columns, ds1, ds2);
     });
@@ -498,11 +511,11 @@ __global__ __launch_bounds__(kF32Threads) void differential_f32_dkv_kernel(Diffe
             auto visible = [&](int i) { return row0 + i >= first_query; };
             {
                 ColumnOperand<D, false> columns;
-                columns.load(do_base, q_stride, row0, p.qs, p.d);
+                columns.load(TileRows(do_base, q_stride, row0, p.qs, p.d), p.d);
                 if (non_finite(columns)) accumulate_visible<D, false>(dv, do_base, q_stride, row0, p.qs, p.d, map, map, visible);
             }
             ColumnOperand<D, true> columns;
-            columns.load(q_base, q_stride, row0, p.qs, p.d);
+            columns.load(TileRows(q_base, q_stride, row0, p.qs, p.d), p.d);
             if (non_finite(columns)) accumulate_visible<D, true>(dk, q_base, q_stride, row0, p.qs, p.d, ds1, ds2, visible);
         });
     }
@@ -540,7 +553,9 @@ long row_tiles(int rows) { return (static_cast<long>(rows) + kTile - 1) / kTile;
 
 }  // namespace
 
-bool differential_f32_takes(const DifferentialArgs& a) { return a.dtype == CGPTX_F32 && a.d % 8 == 0; }
+bool differential_f32_takes(const DifferentialArgs& a) {
+    return a.dtype == CGPTX_F32 && a.d % 8 == 0 && static_cast<long>(a.hq) * a.d * 4 * kTile <= TileRows::kNowhere;
+}
 
 int differential_f32_forward(const DifferentialArgs& a, hipStream_t stream) {
     return a.d <= 64 ? launch<differential_f32_forward_kernel<64>, kSmemBytes<64>>(row_tiles(a.qs), a.hq, a, stream)
