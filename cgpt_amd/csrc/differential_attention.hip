@@ -13,8 +13,10 @@
 // rowsum(dS2), which is what that rounding left (the rows of P2 sum to one).
 //
 // This file holds the entries and the kernels that take every call: head widths that are not multiples of 16 (fp32: of 8), tensors off
-// 16-byte boundaries (differential_attention_mfma.hip and differential_attention_f32.hip have the others). One wavefront per output row, fp32 arithmetic, lane l holding elements l and l + 64 of the head. No atomics: every row has one
-// owner that adds its terms in a fixed order.
+// 16-byte boundaries (differential_attention_mfma.hip and differential_attention_f32.hip have the others). One wavefront per output
+// row, fp32 arithmetic, lane l holding elements l and l + 64 of the head. No atomics: every row has one owner that adds its terms in
+// a fixed order. What bounds them is the reduction over the lanes for every score: 32 x 1024 tokens of 8:2 heads of 128, bf16, take
+// 21 ms forward and 46 backward where the matrix kernels take 0.16 and 0.36.
 #include "differential_attention.hpp"
 
 #include <algorithm>

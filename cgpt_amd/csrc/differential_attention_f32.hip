@@ -2,6 +2,10 @@
 // that of attention_f32.hip: 16 stationary rows per workgroup, the streamed tiles of 16 split between its eight wavefronts, score
 // registers that are the second product's operand as they are, partial results that meet in LDS in wavefront order).
 //
+// 4 x 512 tokens of 8:2 heads of 128: forward 102 us (3.2 GFLOP, 32 TFLOP/s of 154), backward 232. A tile comes from the caches once
+// for 16 stationary rows, and that it is waited for bounds it; read with a branch around each load, and with the columns of the rows behind the
+// walk held in registers through it, the same took 112 and 317.
+//
 // Rows of q and k are kept as two halves of D/2 columns, padded with zeros from d/2, so that a map's scores are the product over its
 // chunks, and a result block of dq or dk belongs to one map. V, dO and their products are shared by the maps. A row touches no row
 // that the causal mask hides from it: see left_out.
