@@ -31,13 +31,14 @@ struct DifferentialArgs {
     float* partial;  // splits > 1: [splits][dK | dV][key, kv head, d] sums of the parts
 };
 
-// Whether the 16-bit matrix kernels serve a call's types and sizes: halves of a head in multiples of 8 (128-bit chunks of a row), and
-// 64 rows of a tensor within 1 GiB, which their 32-bit offsets within a tile reach. Their tensors lie on 16-byte boundaries.
+// Whether the 16-bit matrix kernels serve a call's types and sizes: halves of a head in multiples of 8 (128-bit chunks of a row). 64
+// rows of at most 65535 heads of 128 are less than 1 GiB, which their 32-bit offsets within a tile reach. Their tensors lie on 16-byte
+// boundaries.
 bool differential_mfma_takes(const DifferentialArgs& args);
 int differential_mfma_forward(DifferentialArgs args, hipStream_t stream);  // takes scratch where few queries share many keys
 int differential_mfma_backward(DifferentialArgs args, hipStream_t stream);  // takes its scratch itself
 
-// The fp32 ones: halves of a head in multiples of 4, 16 rows of a tensor within 1 GiB, tensors on 16-byte boundaries.
+// The fp32 ones: halves of a head in multiples of 4, tensors on 16-byte boundaries.
 bool differential_f32_takes(const DifferentialArgs& args);
 int differential_f32_forward(const DifferentialArgs& args, hipStream_t stream);
 int differential_f32_backward(DifferentialArgs args, hipStream_t stream);

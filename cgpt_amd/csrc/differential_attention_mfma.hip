@@ -1100,10 +1100,7 @@ long lambda_parts(const DifferentialArgs& a) {
 
 }  // namespace
 
-bool differential_mfma_takes(const DifferentialArgs& a) {
-    const std::size_t row = static_cast<std::size_t>(std::max(a.hq, a.hkv)) * a.d * 2;
-    return a.dtype != CGPTX_F32 && a.d % 16 == 0 && kStream * row <= (std::size_t{1} << 30);
-}
+bool differential_mfma_takes(const DifferentialArgs& a) { return a.dtype != CGPTX_F32 && a.d % 16 == 0; }
 
 // Workgroups that share a query block's keys in the forward pass: as many as find a place on the chip beside each other, of four tiles
 // or more, if that is predicted to take less time: sharing costs a launch and the sums' way to memory and back. Few queries of many keys

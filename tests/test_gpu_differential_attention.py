@@ -175,6 +175,34 @@ def test_forward_and_backward(device, c, dtype):
         check(got, want[name], want[name + "_err"], name)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_a_long_cache(device, dtype):
+    """More than 2^31 elements of keys and values. The last key has scores of more than 32, the others 0: they share 2^21 e^-32 < 2^-25 of
+    either map."""
+    c = case(1, 1, (1 << 21) + 77, 8, 8, 128)
+    q, _, _, dout, lambdas = inputs(dict(c, ks=1), dtype, device)
+    k, v, dk, dv = (torch.zeros((1, c["ks"], 8, 128), dtype=dtype, device=device) for _ in range(4))
+    v[:, :-1] = 1.0
+    k[:, -1:], v[:, -1:] = q * 8.0, randn((1, 1, 8, 128), dtype, 40).to(device)
+    scores = q.view(8, 2, 64).double().square().sum(-1)  # 8 times that / sqrt(64)
+    assert scores.min() > 32
+    lam, last, u = lambdas.double().view(1, 1, 8, 1), v[:, -1:].double(), torch.finfo(dtype).eps / 2
+    # C of either map and what the other keys share, of values that are 1 or the last key's.
+    rest = 2 * 2.0 ** -24 * (64 + 32) * (1 + scores.max().item()) + 2.0 ** -24
+    out, second, lse = forward(c, q, k, v, lambdas)
+    for got, want in ((second, last), (out, (1 - lam) * last)):
+        assert ((got.double() - want).abs() <= want.abs() * u * 1.01 + 2 * rest * (1 + last.abs())).all()
+    dq, dlambdas = torch.full_like(q, 7.0), torch.full_like(lambdas, 7.0)
+    ops.differential_attention_backward(dq, dk, dv, dlambdas, dout, out, second, lse, q, k, v, lambdas, None, options(c))
+    want = (1 - lam) * dout.double()  # the maps' difference is rounded to storage once, the result once more
+    assert ((dv[:, -1:].double() - want).abs() <= want.abs() * 2.01 * u + 2 * rest * dout.double().abs()).all()
+    assert dv[:, :-1].abs().max().item() <= 2 * rest * dout.abs().max().item()
+    assert torch.isfinite(dq).all() and torch.isfinite(dk[:, -1:]).all()
+    terms = dout.double() * last
+    bound = (rest + 2.0 ** -24 * (128 + 8)) * (terms.abs() + dout.double().abs()).sum(-1).flatten()
+    assert ((dlambdas.double() + terms.sum(-1).flatten()).abs() <= bound).all()
+
+
 # Sequences of few tokens: a row's score gradients are differences of what its keys give, near nothing for the first rows.
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
 @pytest.mark.parametrize("c", [case(3, 2, 2, 4, 2, 64), case(7, 4, 4, 4, 2, 128), case(1, 13, 13, 2, 1, 80), case(2, 64, 64, 2, 2, 32),

@@ -188,6 +188,28 @@ def test_residual_in_place_and_twice_the_same(device, hidden):
         assert torch.equal(a, c) and torch.equal(a, d)
 
 
+@pytest.mark.parametrize("rows,hidden", [((1 << 21) + 5, 1024), ((1 << 16) + 3, 32771)], ids=["rows", "long"])
+def test_a_large_tensor(device, rows, hidden):
+    """The last rows lie behind 2^31 elements: they come out as in a call of their own, whose columns' sums the whole call's contain."""
+    dtype, last = torch.bfloat16, 3
+    x, dy = (torch.zeros((rows, hidden), dtype=dtype, device=device) for _ in range(2))
+    x[-last:], dy[-last:] = randn((last, hidden), dtype, 1).to(device), randn((last, hidden), dtype, 2).to(device)
+    w, b = randn((hidden,), dtype, 3).to(device), randn((hidden,), dtype, 4).to(device)
+    out, alone = torch.full_like(x, 7.0), torch.full_like(x[-last:], 7.0)
+    ops.layernorm_forward(out, x, w, b, 1e-5)
+    ops.layernorm_forward(alone, x[-last:], w, b, 1e-5)
+    assert torch.equal(out[-last:], alone)
+    assert torch.equal(out[:-last].amin(0), b) and torch.equal(out[:-last].amax(0), b)
+    dw, db, dw_alone, db_alone = (torch.full_like(w, 7.0) for _ in range(4))
+    ops.layernorm_backward(out, dw, db, dy, x, w, 1e-5)
+    ops.layernorm_backward(alone, dw_alone, db_alone, dy[-last:], x[-last:], w, 1e-5)
+    assert torch.equal(out[-last:], alone) and not out[:-last].any()
+    # The other rows add zeros; three summands in another order, rounded to storage: a step of the sum and what fp32 loses of the terms.
+    terms = dy[-last:].double().abs().sum(0)
+    for got, want, size in ((db, db_alone, terms), (dw, dw_alone, terms * hidden ** 0.5)):
+        assert ((got.double() - want.double()).abs() <= want.double().abs() * torch.finfo(dtype).eps + 2.0 ** -21 * size).all()
+
+
 def test_gradient_against_differences(device):
     """Along a direction in x, w and b: central differences of the formula in 64 bits. Their error is h^2/6 of the third derivative
     (below 1e3 here, h = 1e-4) and 2^-53/h of the loss's terms."""
