@@ -1050,10 +1050,14 @@ int dispatch(const DifferentialArgs& a, Fn&& fn) {
 }
 
 // Whether forward and dQ run in two parts: blocks of 64 rows that all find a place on the chip at once (two per CU with heads of 64),
-// and more than one key tile.
+// and more than one key tile. Where the longest block of 128 rows walks many tiles while others are done early (a causal mask), or
+// blocks of 64 rows find places beside each other, twice as many: 2 x 2048 tokens of 8 heads of 128, causal, forward 80 -> 61 us, backward 134
+// -> 123; 1 x 4096 of 12 heads of 64 88 -> 71 and 197 -> 177. Blocks of equal length on 128-wide heads lose by it (78 -> 100), as do walks of up
+// to 16 tiles (8 x 512 tokens of 12 heads of 64 19 -> 21) and, nearly always, more blocks (4 x 2048 of 8 heads of 128 84 -> 116).
 bool two_parts(const DifferentialArgs& a) {
     const long blocks = (static_cast<long>(a.qs) + kBlockRows / 2 - 1) / (kBlockRows / 2) * a.hq * a.batch;
-    return a.ks > kStream && blocks <= static_cast<long>(compute_units()) * (a.d <= 64 ? 2 : 1);
+    const bool narrow = a.d <= 64, uneven = a.causal && a.offset <= a.qs, long_walk = a.ks >= 24 * kStream;
+    return a.ks > kStream && blocks <= static_cast<long>(compute_units()) * (narrow ? 2 : 1) * (long_walk && (uneven || narrow) ? 2 : 1);
 }
 template <auto Kernel, int W, int PARTS, bool SPLIT = false>
 int launch_rows(const DifferentialArgs& a, hipStream_t stream) {

@@ -231,7 +231,8 @@ def test_one_key_has_no_score_gradient(device, c, dtype):
 # A token or a few against many keys: the keys of a block of queries are shared by several workgroups, a group's heads share a block.
 LONG = [case(1, 1, 3000, 8, 2, 128), case(2, 1, 700, 4, 1, 64), case(1, 1, 5000, 2, 2, 32), case(1, 7, 2000, 6, 2, 96), case(3, 21, 1100, 3, 1, 112),
         case(1, 22, 1100, 3, 1, 128), case(1, 30, 1500, 4, 4, 64, causal=False), case(1, 64, 2100, 2, 1, 128), case(1, 200, 2500, 1, 1, 128),
-        case(1, 1000, 1000, 1, 1, 64), case(1, 3, 1300, 16, 1, 80, causal=False), case(1, 5, 900, 4, 2, 64, off=400)]
+        case(1, 1000, 1000, 1, 1, 64), case(1, 2048, 2048, 10, 2, 128), case(2, 1600, 1700, 5, 5, 112, off=100), case(1, 1990, 1600, 20, 4, 64, causal=False),
+        case(1, 3, 1300, 16, 1, 80, causal=False), case(1, 5, 900, 4, 2, 64, off=400)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=DTYPE_IDS)
