@@ -479,6 +479,30 @@ def test_on_another_stream(device):
     assert all(torch.equal(a, b) for a, b in zip((*saved, *grads), (*saved2, *grads2)))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=DTYPE_IDS)
+def test_two_streams_at_once(device, dtype):
+    """Calls on two streams have working memory of their own: the same bits as one after the other."""
+    cases = [case(1, 1, 3000, 8, 2, 128), case(2, 300, 300, 4, 2, 128)]
+    given = [inputs(c, dtype, device, seed=3 + i) for i, c in enumerate(cases)]
+
+    def both(c, t, stream):
+        saved = forward(c, *t[:3], t[4], stream)
+        return [*saved, *backward(c, *t, saved, stream=stream)]
+
+    want = [both(c, t, None) for c, t in zip(cases, given)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(both(cases[i], given[i], stream))
+    torch.cuda.synchronize()
+    for expected, runs in zip(want, got):
+        for run in runs:
+            assert all(torch.equal(a, b) for a, b in zip(expected, run))
+
+
 def test_launches(device):
     c = case(2, 300, 300, 4, 2, 128)
     q, k, v, _, lambdas = inputs(c, torch.bfloat16, device)
