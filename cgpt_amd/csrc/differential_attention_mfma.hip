@@ -830,14 +830,16 @@ __global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(Different
         if (turn == 1 && block_index <= block) break;
         const int k_block = block_index * kBlockRows;
         const int k_row = k_block + wave * 32 + (lane & 31);
-        const bool k_live = k_row < p.ks;
+        // A key that no query sees is zeros here, whatever its rows hold: its hidden probabilities are factors of G, and the zeros of
+        // queries past the end factors of both.
+        const bool k_live = k_row < p.ks, k_seen = k_live && (!p.causal || k_row - p.offset < p.qs);
         const long k_head = static_cast<long>(b) * p.ks * kv_stride + kvh * p.d, k_offset = k_head + k_row * kv_stride;
         frag kf[STEPS], vf[STEPS];
         const int first_key = k_block + wave * 32, key_bytes = (lane & 31) * static_cast<int>(kv_stride * sizeof(T));
         const long wave_bytes = first_key < p.ks ? ((min(p.ks - first_key, 32) - 1) * kv_stride + p.d) * static_cast<long>(sizeof(T)) : 0;
         const long first_row = first_key < p.ks ? k_head + first_key * kv_stride : 0;
-        load_rows<T, W, true>(kf, p.k, first_row, wave_bytes, key_bytes, k_live, p.d);
-        load_rows<T, W, false>(vf, p.v, first_row, wave_bytes, key_bytes, k_live, p.d);
+        load_rows<T, W, true>(kf, p.k, first_row, wave_bytes, key_bytes, k_seen, p.d);
+        load_rows<T, W, false>(vf, p.v, first_row, wave_bytes, key_bytes, k_seen, p.d);
         acc_t dk[DT], dv[DT];
 #pragma unroll
         for (int t = 0; t < DT; ++t) dk[t] = dv[t] = acc_t(0.0f);
