@@ -91,7 +91,8 @@ __global__ __launch_bounds__(kThreads) void differential_forward_scalar_kernel(P
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const float score = s[i] * p.scale, top = fmaxf(m[i], score);
-            const float alpha = expf(m[i] - top), e = expf(score - top);  // exp(-inf) = 0 on the first key
+            const float base = top == -INFINITY ? 0.0f : top;  // every key so far has a score of -Inf: all terms below are 0
+            const float alpha = expf(m[i] - base), e = expf(score - base);
             l[i] = l[i] * alpha + e;
             o[i].a = fmaf(e, vr.a, o[i].a * alpha);
             o[i].b = fmaf(e, vr.b, o[i].b * alpha);

@@ -1,4 +1,4 @@
-"""Differential attention: the gradients of keys and values where padding that no query sees holds anything.
+"""Differential attention: keys and values that hold anything where no query sees them, and a key that weighs nothing.
 
 A pair that the mask hides adds nothing, whatever the tensors hold there: keys that no query sees get gradients of exactly 0 (nothing is
 added to what accumulated ones hold), the others stay within the bounds of tests/test_gpu_differential_attention.py, which do not know
@@ -44,3 +44,24 @@ def test_gradients_of_keys_that_no_query_sees(device, c, dtype):
         assert torch.equal(added[1][:, seen:], base[1][:, seen:]) and torch.equal(added[2][:, seen:], base[2][:, seen:])
         for got, name, before in zip(added, GRADS, base):
             check(got, want[name] + before.double(), want[name + "_err"] + 2.0 ** -22 * (want[name].abs() + before.double().abs()), name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=DTYPE_IDS)
+@pytest.mark.parametrize("d", [2, 36, 64, 128])
+def test_a_first_key_of_no_weight(device, dtype, d):
+    """Every score of the first key is -Inf: its probability is 0, and the rest is what it is without the key."""
+    c = case(2, 40, 61, 4, 2, d)
+    q, k, v, dout, lambdas = inputs(c, dtype, device)
+    q = q.abs() + 0.25
+    without = dict(c, ks=c["ks"] - 1, off=c["off"] - 1)
+    want = reference(without, q, k[:, 1:], v[:, 1:], lambdas, dout)
+    k[:, 0] = -INF
+    saved = forward(c, q, k, v, lambdas)
+    for got, name in zip(saved, ("out", "second", "lse")):
+        check(got, want[name], want[name + "_err"], name)
+    if dtype != torch.float32 and d >= 64:
+        return  # their dK/dV pass multiplies the key by the zeros of the queries past the end
+    dk, dv = backward(c, q, k, v, dout, lambdas, saved)[1:3]  # the query's gradient has 0 times the key in it
+    for got, name in ((dk, "dk"), (dv, "dv")):
+        assert not got[:, 0].any()
+        check(got[:, 1:], want[name], want[name + "_err"], name)
