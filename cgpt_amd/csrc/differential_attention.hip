@@ -83,7 +83,9 @@ __global__ __launch_bounds__(kThreads) void differential_forward_scalar_kernel(P
     const long base = (static_cast<long>(at.b) * p.ks * p.hkv + at.kvh) * p.d, stride = static_cast<long>(p.hkv) * p.d;
     const T *k = static_cast<const T*>(p.k) + base, *v = static_cast<const T*>(p.v) + base;
     const int end = p.causal ? min(p.ks, p.offset + at.q + 1) : p.ks;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    // The maxima start at the least finite number: behind keys whose scores are -Inf there is still something to subtract from one.
+    constexpr float kLeast = -3.402823466e38f;
+    float m[2] = {kLeast, kLeast}, l[2] = {0.0f, 0.0f};
     RowPair<T> o[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
     for (int j = 0; j < end; ++j) {
         const vec_t<float, 2> s = row_scores(q, RowPair<T>::load(k + j * stride, p.d), half);
@@ -91,8 +93,7 @@ __global__ __launch_bounds__(kThreads) void differential_forward_scalar_kernel(P
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const float score = s[i] * p.scale, top = fmaxf(m[i], score);
-            const float base = top == -INFINITY ? 0.0f : top;  // every key so far has a score of -Inf: all terms below are 0
-            const float alpha = expf(m[i] - base), e = expf(score - base);
+            const float alpha = expf(m[i] - top), e = expf(score - top);
             l[i] = l[i] * alpha + e;
             o[i].a = fmaf(e, vr.a, o[i].a * alpha);
             o[i].b = fmaf(e, vr.b, o[i].b * alpha);
