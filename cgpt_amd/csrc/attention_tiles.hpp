@@ -300,30 +300,33 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void attention_dkv_reduce_kernel(T* __restrict__ dk, T* __restrict__ dv,
                                                                        const float* __restrict__ partial, long count,
                                                                        int splits, int accumulate) {
-    const long quad = static_cast<long>(blockIdx.x) * kThreads + threadIdx.x;
-    if (quad >= count / 2) return;  // count elements of dK, then of dV
-    const bool second = quad >= count / 4;
-    const long at = (second ? quad - count / 4 : quad) * 4;
-    const float* source = partial + (second ? count : 0) + at;
-    vec_t<float, 4> sum = load_vec<float, 4>(source);
-    int s = 1;
-    for (; s + 3 < splits; s += 4) {
-        vec_t<float, 4> v[4];
+    const long stride = static_cast<long>(gridDim.x) * kThreads;
+#pragma unroll 1
+    for (long quad = static_cast<long>(blockIdx.x) * kThreads + threadIdx.x; quad < count / 2; quad += stride) {  // count elements of dK, then of dV
+        const bool second = quad >= count / 4;
+        const long at = (second ? quad - count / 4 : quad) * 4;
+        const float* source = partial + (second ? count : 0) + at;
+        vec_t<float, 4> sum = load_vec<float, 4>(source);
+        int s = 1;
+        for (; s + 3 < splits; s += 4) {
+            vec_t<float, 4> v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = load_vec<float, 4>(source + 2 * (s + i) * count);
+            for (int i = 0; i < 4; ++i) v[i] = load_vec<float, 4>(source + 2 * (s + i) * count);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += v[i];
+            for (int i = 0; i < 4; ++i) sum += v[i];
+        }
+        for (; s < splits; ++s) sum += load_vec<float, 4>(source + 2 * s * count);
+        T* out = (second ? dv : dk) + at;
+        if (accumulate) sum += vec_to_f32<T, 4>(load_vec<T, 4>(out));
+        store_vec<T, 4>(out, vec_from_f32<T, 4>(sum));
     }
-    for (; s < splits; ++s) sum += load_vec<float, 4>(source + 2 * s * count);
-    T* out = (second ? dv : dk) + at;
-    if (accumulate) sum += vec_to_f32<T, 4>(load_vec<T, 4>(out));
-    store_vec<T, 4>(out, vec_from_f32<T, 4>(sum));
 }
 
 template <typename T>
 int launch_dkv_reduce(long count, void* dk, void* dv, const float* partial, int splits, int accumulate, hipStream_t stream) {
-    hipLaunchKernelGGL((attention_dkv_reduce_kernel<T>), dim3(static_cast<unsigned int>((count / 2 + kThreads - 1) / kThreads)),
-                       dim3(kThreads), 0, stream, static_cast<T*>(dk), static_cast<T*>(dv), partial, count, splits, accumulate);
+    const long blocks = std::min<long>((count / 2 + kThreads - 1) / kThreads, kLaunchThreads / kThreads);
+    hipLaunchKernelGGL((attention_dkv_reduce_kernel<T>), dim3(static_cast<unsigned int>(blocks)), dim3(kThreads), 0, stream,
+                       static_cast<T*>(dk), static_cast<T*>(dv), partial, count, splits, accumulate);
     CGPTX_LAUNCH_CHECK();
     return CGPTX_OK;
 }

@@ -147,6 +147,8 @@ void clear_error();
     } while (0)
 
 #define CGPTX_LAUNCH_CHECK() CGPTX_HIP(hipGetLastError())
+// Threads along an axis of a grid, at most. A launch of 2^32 or more has run a part of its grid only, without an error.
+constexpr std::size_t kLaunchThreads = std::size_t{1} << 31;
 
 inline bool valid_dtype(int dtype) { return dtype == CGPTX_F16 || dtype == CGPTX_BF16 || dtype == CGPTX_F32; }
 inline std::size_t dtype_size(int dtype) { return dtype == CGPTX_F32 ? 4 : 2; }

@@ -62,6 +62,11 @@ __device__ __forceinline__ RowPair<T> of_maps(float first, float second, int hal
     return {lane < half ? first : second, lane + kWave < half ? first : second};
 }
 
+// A wavefront's row. The workgroups fill a second axis of the grid where there are more than a launch has along one.
+__device__ __forceinline__ long scalar_row() {
+    return (blockIdx.x + static_cast<long>(gridDim.x) * blockIdx.y) * kScalarWaves + threadIdx.x / kWave;
+}
+
 struct QueryRow {
     int b, q, h, kvh;
     __device__ __forceinline__ QueryRow(long row, const Params& p) {
@@ -74,7 +79,7 @@ struct QueryRow {
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void differential_forward_scalar_kernel(Params p) {
-    const long row = static_cast<long>(blockIdx.x) * kScalarWaves + threadIdx.x / kWave;
+    const long row = scalar_row();
     const long rows = static_cast<long>(p.batch) * p.qs * p.hq;
     if (row >= rows) return;
     const QueryRow at(row, p);
@@ -114,7 +119,7 @@ __global__ __launch_bounds__(kThreads) void differential_forward_scalar_kernel(P
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void differential_dq_scalar_kernel(Params p) {
-    const long row = static_cast<long>(blockIdx.x) * kScalarWaves + threadIdx.x / kWave;
+    const long row = scalar_row();
     const long rows = static_cast<long>(p.batch) * p.qs * p.hq;
     if (row >= rows) return;
     const QueryRow at(row, p);
@@ -156,7 +161,7 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void differential_dkv_scalar_kernel(Params p) {
     __shared__ double stage[kScalarWaves];
     add_lambda_parts<kThreads>(p, stage);
-    const long row = static_cast<long>(blockIdx.x) * kScalarWaves + threadIdx.x / kWave;
+    const long row = scalar_row();
     if (row >= static_cast<long>(p.batch) * p.ks * p.hkv) return;
     const long rows = static_cast<long>(p.batch) * p.qs * p.hq;
     const int kvh = static_cast<int>(row % p.hkv), j = static_cast<int>((row / p.hkv) % p.ks);
@@ -263,7 +268,7 @@ int validate(const char* name, const Shape& s) {
     if (s.batch > 65535 || s.qs > limit || s.ks > limit || s.hq > 65535 || (s.causal && s.offset > limit) || s.hq * s.d > limit)
         return fail(CGPTX_OVERFLOW, n + ": dimension exceeds the supported range");
     const std::size_t rows = std::max(s.batch * s.qs * s.hq, s.batch * s.ks * s.hkv);
-    if (rows / kScalarWaves >= (std::size_t{1} << 31)) return fail(CGPTX_OVERFLOW, n + ": grid too large");
+    if (rows / kScalarWaves >= (std::size_t{1} << 31)) return fail(CGPTX_OVERFLOW, n + ": too many rows");
     return CGPTX_OK;
 }
 
@@ -287,7 +292,10 @@ Params make_params(const Shape& s, const void* q, const void* k, const void* v, 
     return p;
 }
 
-unsigned int scalar_blocks(std::size_t rows) { return static_cast<unsigned int>((rows + kScalarWaves - 1) / kScalarWaves); }
+dim3 scalar_grid(std::size_t rows) {
+    const std::size_t blocks = (rows + kScalarWaves - 1) / kScalarWaves, axis = std::min(blocks, kLaunchThreads / kThreads);
+    return dim3(static_cast<unsigned int>(axis), static_cast<unsigned int>((blocks + axis - 1) / axis));
+}
 
 bool aligned(std::initializer_list<const void*> tensors) {
     for (const void* t : tensors)
@@ -318,6 +326,11 @@ KeyWalk key_walk(const DifferentialArgs& a) {
     walk.causal = a.causal;
     walk.offset = a.offset;
     return walk;
+}
+
+int launchable_parts(const KeyWalk& walk, int threads) {
+    const long key_blocks = (walk.ks + walk.block_rows - 1) / walk.block_rows;
+    return static_cast<int>(std::min<long>(key_block_parts(walk), std::max<long>(static_cast<long>(kLaunchThreads) / threads / key_blocks, 1)));
 }
 
 int differential_backward_scratch(DifferentialArgs& a, int statistics, long lambda_parts, int splits, hipStream_t stream) {
@@ -403,8 +416,8 @@ extern "C" int cgptx_differential_attention_forward(void* output, void* second, 
         if (differential_f32_takes(p)) return differential_f32_forward(p, static_cast<hipStream_t>(stream));
     }
     return dispatch_dtype(dtype, [&]<typename T>() -> int {
-        hipLaunchKernelGGL((differential_forward_scalar_kernel<T>), dim3(scalar_blocks(batch * query_sequence * query_heads)),
-                           dim3(kThreads), 0, static_cast<hipStream_t>(stream), p);
+        hipLaunchKernelGGL((differential_forward_scalar_kernel<T>), scalar_grid(batch * query_sequence * query_heads), dim3(kThreads), 0,
+                           static_cast<hipStream_t>(stream), p);
         CGPTX_LAUNCH_CHECK();
         return CGPTX_OK;
     });
@@ -445,9 +458,9 @@ extern "C" int cgptx_differential_attention_backward(void* grad_query, void* gra
     const long lambda_parts = static_cast<long>(batch * query_sequence);
     if (int st = differential_backward_scratch(p, 2, lambda_parts, 1, stream)) return st;
     return dispatch_dtype(dtype, [&]<typename T>() -> int {
-        hipLaunchKernelGGL((differential_dq_scalar_kernel<T>), dim3(scalar_blocks(rows)), dim3(kThreads), 0, stream, p);
+        hipLaunchKernelGGL((differential_dq_scalar_kernel<T>), scalar_grid(rows), dim3(kThreads), 0, stream, p);
         CGPTX_LAUNCH_CHECK();
-        hipLaunchKernelGGL((differential_dkv_scalar_kernel<T>), dim3(scalar_blocks(batch * kv_sequence * kv_heads)), dim3(kThreads), 0,
+        hipLaunchKernelGGL((differential_dkv_scalar_kernel<T>), scalar_grid(batch * kv_sequence * kv_heads), dim3(kThreads), 0,
                            stream, p);
         CGPTX_LAUNCH_CHECK();
         return CGPTX_OK;

@@ -38,13 +38,14 @@ bool differential_mfma_takes(const DifferentialArgs& args);
 int differential_mfma_forward(DifferentialArgs args, hipStream_t stream);  // takes scratch where few queries share many keys
 int differential_mfma_backward(DifferentialArgs args, hipStream_t stream);  // takes its scratch itself
 
-// The fp32 ones: halves of a head in multiples of 4, tensors on 16-byte boundaries.
+// The fp32 ones: halves of a head in multiples of 4, tensors on 16-byte boundaries, no more tiles of 16 rows than a launch has workgroups.
 bool differential_f32_takes(const DifferentialArgs& args);
 int differential_f32_forward(const DifferentialArgs& args, hipStream_t stream);
 int differential_f32_backward(DifferentialArgs args, hipStream_t stream);
 
-// A call's part of what key_block_parts goes by.
+// A call's part of what key_block_parts goes by, and the parts for workgroups of `threads` each that one launch has room for.
 KeyWalk key_walk(const DifferentialArgs& args);
+int launchable_parts(const KeyWalk& walk, int threads);
 // Takes a backward pass's scratch, [`statistics` floats per (batch, query, head) | dlambda's parts | parts of shared key blocks], and
 // sets args' pointers and splits: at most `splits`, as many as an arena that cannot grow has room for.
 int differential_backward_scratch(DifferentialArgs& args, int statistics, long lambda_parts, int splits, hipStream_t stream);

@@ -12,6 +12,8 @@
 #include "attention_tiles.hpp"
 #include "differential_attention.hpp"
 
+#include <algorithm>
+
 namespace cgptx {
 namespace {
 
@@ -557,7 +559,9 @@ long row_tiles(int rows) { return (static_cast<long>(rows) + kTile - 1) / kTile;
 
 }  // namespace
 
-bool differential_f32_takes(const DifferentialArgs& a) { return a.dtype == CGPTX_F32 && a.d % 8 == 0; }
+bool differential_f32_takes(const DifferentialArgs& a) {
+    return a.dtype == CGPTX_F32 && a.d % 8 == 0 && row_tiles(std::max(a.qs, a.ks)) <= static_cast<long>(kLaunchThreads / kF32Threads);
+}
 
 int differential_f32_forward(const DifferentialArgs& a, hipStream_t stream) {
     return a.d <= 64 ? launch<differential_f32_forward_kernel<64>, kSmemBytes<64>>(row_tiles(a.qs), a.hq, a, stream)
@@ -569,7 +573,7 @@ int differential_f32_backward(DifferentialArgs a, hipStream_t stream) {
     walk.block_rows = walk.stream_rows = kTile;
     walk.waves = kWaves;
     walk.tile_us = 10.0;
-    if (int st = differential_backward_scratch(a, 2, row_tiles(a.qs) * a.batch, key_block_parts(walk), stream)) return st;
+    if (int st = differential_backward_scratch(a, 2, row_tiles(a.qs) * a.batch, launchable_parts(walk, kF32Threads), stream)) return st;
     if (int st = a.d <= 64 ? launch<differential_f32_dq_kernel<64>, kSmemBytes<64>>(row_tiles(a.qs), a.hq, a, stream)
                            : launch<differential_f32_dq_kernel<128>, kSmemBytes<128>>(row_tiles(a.qs), a.hq, a, stream))
         return st;

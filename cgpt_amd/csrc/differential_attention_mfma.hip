@@ -1163,7 +1163,7 @@ int differential_mfma_backward(DifferentialArgs a, hipStream_t stream) {
     walk.stream_rows = kStream;
     walk.waves = 1;
     walk.tile_us = a.d <= 64 ? 1.2 : 2.0;
-    if (int st = differential_backward_scratch(a, 4, lambda_parts(a), key_block_parts(walk), stream)) return st;
+    if (int st = differential_backward_scratch(a, 4, lambda_parts(a), launchable_parts(walk, kThreads), stream)) return st;
     return dispatch(a, [&]<typename T, int W>() -> int {
         if (int st = two_parts(a) ? launch_rows<differential_dq_kernel<T, W, 2>, W, 2>(a, stream)
                                   : launch_rows<differential_dq_kernel<T, W, 1>, W, 1>(a, stream))

@@ -122,7 +122,7 @@ int launch(const char* name, void* output, const void* input, const void* added,
     args.count = count;
     return dispatch_dtype(dtype, [&]<typename T>() -> int {
         const std::size_t blocks = ((count + kGroup - 1) / kGroup + kThreads - 1) / kThreads;
-        const std::size_t cap = std::size_t{1} << 23;  // 2^31 threads
+        const std::size_t cap = kLaunchThreads / kThreads;
         const bool vector_ok = is_aligned16(output) && is_aligned16(input) && is_aligned16(added);
         // A call that moves more than half of what the memory-side cache holds leaves it to its neighbours: the pair of calls above
         // 62.7 -> 55.9 us; of two calls that move half of it each (without the residual) 42.7 us, 46.8 if they did.

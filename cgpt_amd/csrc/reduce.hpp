@@ -112,14 +112,17 @@ template <typename T, int COLUMNS>
 __global__ __launch_bounds__(kFinishThreads) void column_partial_reduce_kernel(
     T* __restrict__ out, const float* __restrict__ partial, int parts, int hidden, int accumulate, int units) {
     __shared__ float folded[kFolded], stage[4 * COLUMNS];
-    column_partial_reduce_body<T, COLUMNS>(out, partial, parts, hidden, accumulate, static_cast<int>(blockIdx.x), units, folded, stage);
+    const int group = static_cast<int>(blockIdx.x + gridDim.x * blockIdx.y);
+    column_partial_reduce_body<T, COLUMNS>(out, partial, parts, hidden, accumulate, group, units, folded, stage);
 }
 template <typename T>
 void launch_column_partial_reduce(T* out, const float* partial, int parts, int hidden, int accumulate, hipStream_t stream) {
     const int columns = finish_columns(hidden);
     auto kernel = columns == 16 ? column_partial_reduce_kernel<T, 16> : column_partial_reduce_kernel<T, 32>;
-    hipLaunchKernelGGL(kernel, dim3((hidden + columns - 1) / columns), dim3(kFinishThreads), 0, stream, out, partial, parts, hidden,
-                       accumulate, compute_units());
+    constexpr unsigned int most = kLaunchThreads / kFinishThreads;
+    const unsigned int groups = static_cast<unsigned int>(hidden + columns - 1) / static_cast<unsigned int>(columns), axis = groups < most ? groups : most;
+    hipLaunchKernelGGL(kernel, dim3(axis, (groups + axis - 1) / axis), dim3(kFinishThreads), 0, stream, out, partial, parts, hidden, accumulate,
+                       compute_units());
 }
 
 // The same over a table of reductions (blockIdx.y picks the entry): the same additions in the same order for every entry,
