@@ -336,7 +336,7 @@ int launchable_parts(const KeyWalk& walk, int threads) {
 int differential_backward_scratch(DifferentialArgs& a, int statistics, long lambda_parts, int splits, hipStream_t stream) {
     auto rounded = [](std::size_t bytes) { return (bytes + 255) & ~std::size_t{255}; };
     const std::size_t first = rounded(static_cast<std::size_t>(statistics) * a.batch * a.qs * a.hq * sizeof(float));
-    const std::size_t fixed = first + rounded(static_cast<std::size_t>(lambda_parts) * a.hq * sizeof(float));
+    const std::size_t by_row_block = rounded(static_cast<std::size_t>(lambda_parts) * a.hq * sizeof(float)), fixed = first + 2 * by_row_block;
     const std::size_t part = 2 * static_cast<std::size_t>(a.batch) * a.ks * a.hkv * a.d * sizeof(float);
     a.lambda_parts = lambda_parts;
     a.splits = splits;
@@ -348,6 +348,7 @@ int differential_backward_scratch(DifferentialArgs& a, int statistics, long lamb
     if (int st = scratch(stream, wanted(), &memory)) return st;
     a.delta = static_cast<float*>(memory);
     a.lambda_partial = reinterpret_cast<float*>(static_cast<char*>(memory) + first);
+    a.largest = reinterpret_cast<float*>(static_cast<char*>(memory) + first + by_row_block);
     a.partial = reinterpret_cast<float*>(static_cast<char*>(memory) + fixed);
     return CGPTX_OK;
 }

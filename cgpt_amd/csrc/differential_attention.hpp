@@ -17,6 +17,7 @@ struct DifferentialArgs {
     // with shared keys: [splits][2][batch, qs, hq] pairs of a map's largest score and the sum that stands to it.
     float* delta;
     float* lambda_partial;  // [hq][lambda_parts]: what a head's dlambda is the sum of
+    float* largest;         // [hq][lambda_parts], half precision on the matrix cores: the largest |dO| of the same rows
     long lambda_parts;
     int batch, qs, ks, hq, hkv, d;
     float scale;           // of the scores
@@ -46,8 +47,8 @@ int differential_f32_backward(DifferentialArgs args, hipStream_t stream);
 // A call's part of what key_block_parts goes by, and the parts for workgroups of `threads` each that one launch has room for.
 KeyWalk key_walk(const DifferentialArgs& args);
 int launchable_parts(const KeyWalk& walk, int threads);
-// Takes a backward pass's scratch, [`statistics` floats per (batch, query, head) | dlambda's parts | parts of shared key blocks], and
-// sets args' pointers and splits: at most `splits`, as many as an arena that cannot grow has room for.
+// Takes a backward pass's scratch, [`statistics` floats per (batch, query, head) | dlambda's parts and the largest |dO| | parts of shared
+// key blocks], and sets args' pointers and splits: at most `splits`, as many as an arena that cannot grow has room for.
 int differential_backward_scratch(DifferentialArgs& args, int statistics, long lambda_parts, int splits, hipStream_t stream);
 // dlambda from the parts that the dQ pass left, by the workgroups of the dK/dV pass that follows it, which has THREADS threads in each and
 // none but this to add: a launch of its own took 3 to 5 us. From the last workgroup on, as the first ones have most to do. A

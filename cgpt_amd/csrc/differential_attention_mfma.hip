@@ -540,8 +540,105 @@ __global__ __launch_bounds__(kThreads) void differential_combine_kernel(Differen
     if (p.second != nullptr) store_vec<T, 2>(static_cast<T*>(p.second) + row * p.d + at, vec_from_f32<T, 2>(second));
 }
 
+// Half precision's smallest normal number is 2^-14. Score gradients P (G - delta) are rounded to storage before their products, and where
+// output gradients are small (P is some 1/n beside a dO of any size) they are below it and lose their digits. So they are enlarged by a power of
+// two, which costs nothing inside P's exponent, and the sums are made smaller by it: by what brings the largest |dO| (of the row for
+// dq, of the (batch entry, kv head) for dk) to between 1 and 2. Sums that are not finite then, beside large values of v, are taken again in
+// fp32 (dq_of_row, dk_of_row).
+template <typename T>
+constexpr bool kEnlarged = __is_same(T, f16_t);
+// The power that brings `largest` to between 1 and 2: 0 from 1 on and for what is no number, at most `most`.
+__device__ __forceinline__ int power_to_one(float largest, int most) {
+    return max(min(127 - static_cast<int>(__float_as_uint(largest) >> 23), most), 0);
+}
+// The largest of the absolute values of a row in half precision, in all lanes of the row.
+template <int STEPS>
+__device__ __forceinline__ float largest_of_row(const Mma<f16_t>::frag (&row)[STEPS]) {
+    using words = vec_t<unsigned int, 4>;
+    using pair = vec_t<unsigned short, 2>;
+    pair top(static_cast<unsigned short>(0));
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = __builtin_elementwise_max(top, __builtin_bit_cast(pair, __builtin_bit_cast(words, row[s])[w] & 0x7FFF7FFFu));
+    const unsigned short mine = top[0] > top[1] ? top[0] : top[1];
+    const float value = to_f32(__builtin_bit_cast(f16_t, mine));
+    return __uint_as_float(max(__float_as_uint(value), __float_as_uint(other_half(value))));  // as bits: a NaN is the largest
+}
+// Whether any of the sums is not finite.
+template <int DT>
+__device__ __forceinline__ bool any_not_finite(const acc_t (&sums)[DT]) {
+    float zero = 0.0f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) zero = fmaf(sums[t][e], 0.0f, zero);
+    return !(zero == 0.0f);
+}
 // The sign of -lambda.
 __device__ __forceinline__ float sign_of_second(float lambda) { return lambda > 0.0f ? -1.0f : 1.0f; }
+
+// A row of d elements in a wavefront, lane l with elements l and l + 64, those of the second map apart from those of the first.
+struct WaveRow {
+    float x[2];
+    template <typename T>
+    __device__ __forceinline__ static WaveRow load(const T* row, int d) {
+        const int lane = threadIdx.x & 63;
+        return {{lane < d ? to_f32(row[lane]) : 0.0f, lane + kWave < d ? to_f32(row[lane + kWave]) : 0.0f}};
+    }
+    __device__ __forceinline__ float dot(const WaveRow& y) const { return wave_sum(fmaf(x[0], y.x[0], x[1] * y.x[1])); }
+    __device__ __forceinline__ bool finite() const { return !__any(!(fmaf(x[0], 0.0f, x[1] * 0.0f) == 0.0f)); }
+    // The product's elements of the first map or the second.
+    __device__ __forceinline__ float dot(const WaveRow& y, bool second, int d) const {
+        const int lane = threadIdx.x & 63;
+        const float a = (lane >= d / 2) == second ? x[0] * y.x[0] : 0.0f, b = (lane + kWave >= d / 2) == second ? x[1] * y.x[1] : 0.0f;
+        return wave_sum(a + b);
+    }
+    __device__ __forceinline__ void add(const WaveRow& y, float first, float second, int d) {
+        const int lane = threadIdx.x & 63;
+        x[0] = fmaf(lane < d / 2 ? first : second, y.x[0], x[0]);
+        x[1] = fmaf(lane + kWave < d / 2 ? first : second, y.x[1], x[1]);
+    }
+    template <typename T>
+    __device__ __forceinline__ void store(T* row, int d, float factor, bool accumulate) const {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            T* to = row + lane + i * kWave;
+            if (lane + i * kWave < d) *to = from_f32<T>(fmaf(x[i], factor, accumulate ? to_f32(*to) : 0.0f));
+        }
+    }
+};
+// A row of dq by a wavefront, its products in fp32: of `keys` keys from k and v on, its probabilities exp(score * scale - lse).
+template <typename T>
+__device__ __noinline__ WaveRow dq_of_row(const T* q, const T* d_o, const T* k, const T* v, long kv_stride, int keys, int d, float scale, float lse1,
+                                          float lse2, float delta1, float delta2, float lambda) {
+    const WaveRow query = WaveRow::load(q, d), dout = WaveRow::load(d_o, d);
+    WaveRow sum{};
+    for (int j = 0; j < keys; ++j) {
+        const WaveRow key = WaveRow::load(k + j * kv_stride, d);
+        const float g = dout.dot(WaveRow::load(v + j * kv_stride, d));
+        const float ds1 = expf(query.dot(key, false, d) * scale - lse1) * (g - delta1), ds2 = expf(query.dot(key, true, d) * scale - lse2) * (g - delta2);
+        sum.add(key, ds1, -lambda * ds2, d);
+    }
+    return sum;
+}
+// Adds to a row of dk by a wavefront, its products in fp32, what `queries` queries give, `stride` heads apart from q and d_o on, with their four
+// statistics `rows` apart.
+template <typename T>
+__device__ __noinline__ WaveRow dk_of_row(WaveRow sum, WaveRow k, WaveRow v, const T* q, const T* d_o, const float* statistics, long rows, int queries,
+                                          int stride, int d, float scale2, float sign) {
+    for (int i = 0; i < queries; ++i) {
+        const long head = static_cast<long>(i) * stride;
+        const float* of_row = statistics + head;
+        const WaveRow query = WaveRow::load(q + head * d, d);
+        const float g = WaveRow::load(d_o + head * d, d).dot(v) + of_row[2 * rows];  // G - delta1
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(query.dot(k, false, d), scale2, -of_row[0]));
+        const float p2 = __builtin_amdgcn_exp2f(fmaf(query.dot(k, true, d), scale2, -of_row[rows]));
+        sum.add(query, p1 * g, p2 * fmaf(sign, g, of_row[3 * rows]), d);
+    }
+    return sum;
+}
 
 template <typename T, int W, int PARTS>
 __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void differential_dq_kernel(DifferentialArgs p) {
@@ -585,7 +682,7 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void differential_dq_ker
         delta2 = row_delta<T, STEPS>(dof, o2f);
         delta1 = fmaf(lambda, delta2, row_delta<T, STEPS>(dof, of));
     }
-    const float lse1 = at.live ? p.lse[row] * kLog2e : 0.0f, lse2 = at.live ? p.lse[rows + row] * kLog2e : 0.0f;
+    float lse1 = at.live ? p.lse[row] * kLog2e : 0.0f, lse2 = at.live ? p.lse[rows + row] * kLog2e : 0.0f;
     int k_off[STEPS], kt_off[DT][2];
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) k_off[s] = wide_direct_offset<W>(lane, s);
@@ -599,6 +696,7 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void differential_dq_ker
 #pragma unroll
     for (int t = 0; t < DT; ++t) dq[t] = acc_t(0.0f);
     float rest = 0.0f;  // rowsum(P2 (G - delta2)): what the rounding of O2 left in delta2
+    const long row_part = (static_cast<long>(at.b) * gridDim.x + at.row / (kBlockRows / PARTS)) * (4 / PARTS) + at.row_wave;
     const float scale2 = p.scale * kLog2e;
     const int wave_first_q = at.first_q, wave_last_q = at.last_q;
     const bool wave_live = at.wave_live;
@@ -637,6 +735,12 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void differential_dq_ker
         p.delta[rows + row] = lse2 - log2f(fabsf(lambda));
         p.delta[2 * rows + row] = -delta1;
         p.delta[3 * rows + row] = sign_of_second(lambda) * (delta1 - delta2);
+    }
+    if constexpr (kEnlarged<T>) {
+        const float largest = largest_of_row<STEPS>(dof), power = static_cast<float>(power_to_one(largest, 24)), of_wave = wave_max(largest);
+        lse1 -= power;
+        lse2 -= power;
+        if (lane == 0 && at.part == 0) p.largest[at.h * p.lambda_parts + row_part] = of_wave;
     }
     LeftOut left(p, wave_first_q);
     for (int first = 0; first < tiles; first += PARTS) {
@@ -738,15 +842,40 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void differential_dq_ker
         add_sums<DT>(meet, dq, 1.0f, 1.0f);
         rest += meet[4 * DT * kWave][0];
     }
+    float smaller = 1.0f;
+    bool stored = false;
+    if constexpr (kEnlarged<T>) {
+        using words = vec_t<unsigned int, 4>;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {  // the power again: it takes no register through the walk
+            auto w = __builtin_bit_cast(words, dof[s]);
+            asm volatile("" : "+v"(w));
+            dof[s] = __builtin_bit_cast(frag, w);
+        }
+        const int power = power_to_one(largest_of_row<STEPS>(dof), 24);
+        smaller = ldexpf(1.0f, -power);
+        rest *= smaller;
+        const bool finite = (delta1 + delta2 + lse1 + lse2) * 0.0f == 0.0f;
+        const unsigned long long half = __ballot(at.live && power > 0 && finite && any_not_finite(dq));
+        for (unsigned int lost = static_cast<unsigned int>(half | half >> 32); lost != 0; lost &= lost - 1) {
+            const int from = __builtin_ctz(lost), q = __shfl(at.q, from);
+            const long of_row = (static_cast<long>(at.b) * p.qs + q) * p.hq + at.h;
+            const WaveRow exact = dq_of_row<T>(static_cast<const T*>(p.q) + of_row * p.d, static_cast<const T*>(p.dout) + of_row * p.d,
+                                               static_cast<const T*>(p.k) + kv_offset, static_cast<const T*>(p.v) + kv_offset, kv_stride,
+                                               p.causal ? min(p.ks, p.offset + q + 1) : p.ks, p.d, p.scale, p.lse[of_row], p.lse[rows + of_row],
+                                               __shfl(delta1, from), __shfl(delta2, from), lambda);
+            exact.store(static_cast<T*>(p.dq) + of_row * p.d, p.d, p.gradient_scale, p.accumulate != 0);
+            stored = stored || (lane & 31) == from;
+        }
+    }
     {
         // -(delta2 + rest) of the wavefront's rows.
         const float mine = at.live ? rest + (lane < 32 ? delta2 : 0.0f) : 0.0f;
         const float sum = wave_sum(mine);
-        const long part = (static_cast<long>(at.b) * gridDim.x + at.row / (kBlockRows / PARTS)) * (4 / PARTS) + at.row_wave;
-        if (lane == 0) p.lambda_partial[at.h * p.lambda_parts + part] = -sum;
+        if (lane == 0) p.lambda_partial[at.h * p.lambda_parts + row_part] = -sum;
     }
-    if (!at.live) return;
-    const float factor[2] = {p.gradient_scale, -lambda * p.gradient_scale};
+    if (!at.live || stored) return;
+    const float factor[2] = {p.gradient_scale * smaller, -lambda * p.gradient_scale * smaller};
     store_columns<T, W, true>(static_cast<T*>(p.dq) + q_offset, p.d, p.accumulate != 0,
                               [&](int t, int e) { return dq[t][e] * factor[t / (DT / 2)]; });
 }
@@ -788,6 +917,22 @@ constexpr Slot dkv_slot(int k, int h) {
 constexpr int exponential_slot(int half, int n, int h) { return (half == 0 ? h + 2 : 3 * h + 2) + n * (2 * h - 2) / 8; }
 constexpr int gradient_slot(int half, int n, int h) { return (half == 0 ? 4 * h + h / 2 : 6 * h - h / 4) + n * (half == 0 ? 3 * h / 2 : 5 * h / 4) / 8; }
 
+// The power for dk of a (batch entry, kv head): by the largest |dO| that the dQ pass found, and so that P1 + |lambda| P2 stays in range.
+// Every wavefront works it out by itself.
+__device__ __forceinline__ int enlargement(const DifferentialArgs& p, int b, int kvh, float scale2) {
+    const int lane = threadIdx.x & 63, group = p.hq / p.hkv, per_head = static_cast<int>(p.lambda_parts / p.batch);
+    const float* from = p.largest + static_cast<long>(kvh) * group * p.lambda_parts + static_cast<long>(b) * per_head;
+    float largest = 0.0f, weight = 0.0f;
+    for (int i = lane; i < group * per_head; i += kWave) {
+        const int head = i / per_head;
+        largest = fmaxf(largest, from[head * p.lambda_parts + (i - head * per_head)]);
+    }
+    for (int head = lane; head < group; head += kWave) weight = fmaxf(weight, fabsf(p.lambda[kvh * group + head]));
+    const int most = 14 - (static_cast<int>(__float_as_uint(1.0f + wave_max(weight)) >> 23) - 127);
+    const int power = scale2 > 0x1p-60f ? power_to_one(wave_max(largest), most) : 0;
+    return __builtin_amdgcn_readfirstlane(power);
+}
+
 template <typename T, int W>
 __global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(DifferentialArgs p) {
     using frag = typename Mma<T>::frag;
@@ -825,6 +970,10 @@ __global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(Different
     const int key_blocks = (p.ks + kBlockRows - 1) / kBlockRows;
     const int part = p.splits > 1 ? block % p.splits : 0;
     if (p.splits > 1) block /= p.splits;
+    int power = 0;  // score gradients and probabilities are 2^power as large
+    if constexpr (kEnlarged<T>) power = enlargement(p, b, kvh, scale2);
+    const float score0 = static_cast<float>(power) / scale2;  // where scores start
+    const float smaller = ldexpf(1.0f, -power), k_factor = p.gradient_scale * smaller;
     for (int turn = 0; turn < (p.paired ? 2 : 1); ++turn) {
         const int block_index = turn == 0 ? block : key_blocks - 1 - block;
         if (turn == 1 && block_index <= block) break;
@@ -917,7 +1066,7 @@ __global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(Different
                 constexpr Slot at = dkv_slot(K, H);
                 if constexpr (at.product == Product::scores) {
                     constexpr int map = at.index % 2, s = at.index / 2;
-                    s_acc[at.half][map] = Mma<T>::run(operand[K], kf[map * HALF + s], s == 0 ? acc_t(0.0f) : s_acc[at.half][map]);
+                    s_acc[at.half][map] = Mma<T>::run(operand[K], kf[map * HALF + s], s == 0 ? acc_t(kEnlarged<T> ? score0 : 0.0f) : s_acc[at.half][map]);
                 } else if constexpr (at.product == Product::grads) {
                     g_acc[at.half] = Mma<T>::run(operand[K], vf[at.index], g_acc[at.half]);  // from -delta1 on
                 } else {
@@ -1030,15 +1179,37 @@ __global__ __launch_bounds__(kThreads, 1) void differential_dkv_kernel(Different
             }
         }
         __syncthreads();  // the next key block's first loads overwrite stage 0
+        const long count = static_cast<long>(p.batch) * p.ks * kv_stride;
+        float* const part_dk = p.splits > 1 ? p.partial + 2 * part * count : nullptr;
+        bool stored = false;  // dk
+        if constexpr (kEnlarged<T>) {
+            const unsigned long long half = __ballot(k_seen && power > 0 && any_not_finite(dk));
+            for (unsigned int lost = static_cast<unsigned int>(half | half >> 32); lost != 0; lost &= lost - 1) {
+                const int from = __builtin_ctz(lost), key = k_block + wave * 32 + from;
+                const long of_key = k_head + key * kv_stride;
+                const WaveRow k = WaveRow::load(static_cast<const T*>(p.k) + of_key, p.d), v = WaveRow::load(static_cast<const T*>(p.v) + of_key, p.d);
+                if (!k.finite() || !v.finite()) continue;
+                WaveRow exact{};
+                for (int tile = first_index; tile < total_tiles; ++tile) {
+                    const int head = kvh * group + tile / tiles_per_head, q0 = q_begin + tile % tiles_per_head * kStream;
+                    const int first = p.causal ? max(q0, key - p.offset) : q0, end = min(q0 + kStream, p.qs);
+                    const long row = (static_cast<long>(b) * p.qs + first) * p.hq + head;
+                    exact = dk_of_row<T>(exact, k, v, static_cast<const T*>(p.q) + row * p.d, static_cast<const T*>(p.dout) + row * p.d, p.delta + row,
+                                         rows, end - first, p.hq, p.d, scale2, sign_of_second(p.lambda[head]));
+                }
+                if (part_dk != nullptr) exact.store(part_dk + of_key, p.d, p.gradient_scale, false);
+                else exact.store(static_cast<T*>(p.dk) + of_key, p.d, p.gradient_scale, p.accumulate != 0);
+                stored = stored || (lane & 31) == from;
+            }
+        }
         if (!k_live) continue;
         if (p.splits > 1) {
-            const long count = static_cast<long>(p.batch) * p.ks * kv_stride;
-            float* to = p.partial + 2 * part * count + k_offset;
-            store_columns<float, W, true>(to, p.d, false, [&](int t, int e) { return dk[t][e] * p.gradient_scale; });
-            store_columns<float, W, false>(to + count, p.d, false, [&](int t, int e) { return dv[t][e]; });
+            float* to = part_dk + k_offset;
+            if (!stored) store_columns<float, W, true>(to, p.d, false, [&](int t, int e) { return dk[t][e] * k_factor; });
+            store_columns<float, W, false>(to + count, p.d, false, [&](int t, int e) { return dv[t][e] * smaller; });
         } else {
-            store_columns<T, W, true>(static_cast<T*>(p.dk) + k_offset, p.d, p.accumulate != 0, [&](int t, int e) { return dk[t][e] * p.gradient_scale; });
-            store_columns<T, W, false>(static_cast<T*>(p.dv) + k_offset, p.d, p.accumulate != 0, [&](int t, int e) { return dv[t][e]; });
+            if (!stored) store_columns<T, W, true>(static_cast<T*>(p.dk) + k_offset, p.d, p.accumulate != 0, [&](int t, int e) { return dk[t][e] * k_factor; });
+            store_columns<T, W, false>(static_cast<T*>(p.dv) + k_offset, p.d, p.accumulate != 0, [&](int t, int e) { return dv[t][e] * smaller; });
         }
     }
     add_lambda_parts<kThreads>(p, reinterpret_cast<double*>(wide_smem));
