@@ -208,7 +208,11 @@ int cgptx_dropout_backward(void* grad_input, const void* grad_output, size_t cou
 
 /* Gradients of differential attention (see cgptx_differential_attention_forward, which leaves output, second and
  * logsumexp). grad_lambda: fp32 [query_heads]. accumulate_grads adds to all four. The workgroups' parts of every sum meet
- * in an order that the sizes fix: results do not depend on scheduling. */
+ * in a fixed order: results do not depend on scheduling. How many parts there are goes by the sizes and, where the scratch
+ * arena cannot grow (a call that is recorded on a stream where no eager call of its sizes ran), by what it has room for:
+ * such a call adds in another order than an eager one, and its results may differ from that one's by rounding. In 16-bit
+ * storage P1 - lambda P2 and the score gradients are rounded to it once before their products, as in plain attention; in
+ * half precision they are enlarged by a power of two first where output gradients are below 1. */
 int cgptx_differential_attention_backward(
     void* grad_query, void* grad_key, void* grad_value, float* grad_lambda,
     const void* grad_output, const void* output, const void* second,
@@ -386,7 +390,9 @@ int cgptx_dropout_forward(void* output, const void* input, const void* residual,
  *   output = softmax(s q1 k1') v - lambda[head] softmax(s q2 k2') v.
  * head_dim: even, at most 128; attention_scale <= 0 selects s = 1/sqrt(head_dim/2); lambda: fp32 [query_heads], on the
  * device. For the backward pass: second [batch, query_sequence, query_heads, head_dim] = softmax(s q2 k2') v, logsumexp
- * fp32 [2, batch, query_sequence, query_heads] of both maps; either may be NULL. */
+ * fp32 [2, batch, query_sequence, query_heads] of both maps; either may be NULL. Few queries of many keys: workgroups share
+ * the keys, as many as the scratch arena has room for; recorded where it cannot grow, the call adds in another order. In 16-bit
+ * storage a map's probabilities are rounded to it once before their product with v. */
 int cgptx_differential_attention_forward(
     void* output, void* second, float* logsumexp, const void* query,
     const void* key, const void* value, const float* lambda, size_t batch,
