@@ -168,7 +168,7 @@ class EmbeddingBackwardOptions:  # include/ops/backward/embedding_backward.h:6-1
 class DropoutOptions:
     """Which mask (cgptx_dropout_forward in include/cgptx.h): of how many elements, from which key, from which counter value on. A
     call uses up (count + 7) // 8 counter values. counter: device int64 tensor of one element, added to the offset when the call
-    runs."""
+    runs. The defaults are one mask like any other: calls that are to have masks of their own need a seed or an offset of their own."""
 
     probability: float = 0.1
     seed: int = 0

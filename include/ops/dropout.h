@@ -4,6 +4,7 @@
 #include "core/status.h"
 #include "core/tensor.h"
 
+// The defaults are one mask like any other: calls that are to have masks of their own need a seed or an offset of their own.
 struct DropoutOptions {
     float probability = 0.1F;
     std::uint64_t seed = 0;
