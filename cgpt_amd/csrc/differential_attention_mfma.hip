@@ -543,13 +543,14 @@ __global__ __launch_bounds__(kThreads) void differential_combine_kernel(Differen
 // Half precision's smallest normal number is 2^-14. Score gradients P (G - delta) are rounded to storage before their products, and where
 // output gradients are small (P is some 1/n beside a dO of any size) they are below it and lose their digits. So they are enlarged by a power of
 // two, which costs nothing inside P's exponent, and the sums are made smaller by it: by what brings the largest |dO| (of the row for
-// dq, of the (batch entry, kv head) for dk) to between 1 and 2. Sums that are not finite then, beside large values of v, are taken again in
-// fp32 (dq_of_row, dk_of_row).
+// dq, of the (batch entry, kv head) for dk and dv) to between 32 and 64. Beside values of v around 1 that leaves six bits below 65504 for the
+// product of head_dim terms and ten more below 2^-14 for P than without. Sums that are not finite then, beside larger values of v, are taken again
+// in fp32 (dq_of_row, dk_of_row).
 template <typename T>
 constexpr bool kEnlarged = __is_same(T, f16_t);
-// The power that brings `largest` to between 1 and 2: 0 from 1 on and for what is no number, at most `most`.
-__device__ __forceinline__ int power_to_one(float largest, int most) {
-    return max(min(127 - static_cast<int>(__float_as_uint(largest) >> 23), most), 0);
+// The power that brings `largest` to between 32 and 64: 0 from 32 on and for what is no number, at most `most`.
+__device__ __forceinline__ int enlarging_power(float largest, int most) {
+    return max(min(127 + 5 - static_cast<int>(__float_as_uint(largest) >> 23), most), 0);
 }
 // The largest of the absolute values of a row in half precision, in all lanes of the row.
 template <int STEPS>
@@ -737,7 +738,7 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void differential_dq_ker
         p.delta[3 * rows + row] = sign_of_second(lambda) * (delta1 - delta2);
     }
     if constexpr (kEnlarged<T>) {
-        const float largest = largest_of_row<STEPS>(dof), power = static_cast<float>(power_to_one(largest, 24)), of_wave = wave_max(largest);
+        const float largest = largest_of_row<STEPS>(dof), power = static_cast<float>(enlarging_power(largest, 24)), of_wave = wave_max(largest);
         lse1 -= power;
         lse2 -= power;
         if (lane == 0 && at.part == 0) p.largest[at.h * p.lambda_parts + row_part] = of_wave;
@@ -852,7 +853,7 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void differential_dq_ker
             asm volatile("" : "+v"(w));
             dof[s] = __builtin_bit_cast(frag, w);
         }
-        const int power = power_to_one(largest_of_row<STEPS>(dof), 24);
+        const int power = enlarging_power(largest_of_row<STEPS>(dof), 24);
         smaller = ldexpf(1.0f, -power);
         rest *= smaller;
         const bool finite = (delta1 + delta2 + lse1 + lse2) * 0.0f == 0.0f;
@@ -929,7 +930,7 @@ __device__ __forceinline__ int enlargement(const DifferentialArgs& p, int b, int
     }
     for (int head = lane; head < group; head += kWave) weight = fmaxf(weight, fabsf(p.lambda[kvh * group + head]));
     const int most = 14 - (static_cast<int>(__float_as_uint(1.0f + wave_max(weight)) >> 23) - 127);
-    const int power = scale2 > 0x1p-60f ? power_to_one(wave_max(largest), most) : 0;
+    const int power = scale2 > 0x1p-60f ? enlarging_power(wave_max(largest), most) : 0;
     return __builtin_amdgcn_readfirstlane(power);
 }
 
