@@ -704,24 +704,29 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void differential_dq_ker
     const int q_limit = p.causal ? p.offset + at.q : p.ks;
     const int clear_limit = p.causal ? min(p.ks - 1, p.offset + wave_first_q) : p.ks - 1;
 
-    if (tiles == 1) {
-        // Rows that see few keys: their score gradients are small beside the deltas that they are differences of, so that the rounding
-        // of O and O2 in these shows (4 queries of 4 keys, bf16: dQ off by 0.0037 of its norm, 0.0024 with this). All keys are in one
-        // tile: rowsum(P (G - delta)) first, which is what delta lacks, then the walk.
+    // Rows that see few keys: their score gradients are small beside the deltas that they are differences of, so that the rounding of O and
+    // O2 in these shows (4 queries of 4 keys, bf16: dQ off by 0.0037 of its norm, 0.0024 with what follows; the first 64 rows of 1001 tokens, more
+    // than a third of dQ's norm, fp16: 1.58 times as far off as the rounded exact dQ, 1.43 with it). Where all keys that a wavefront's rows see
+    // are in the first tile: rowsum(P (G - delta)) first, which is what delta lacks, then the walk.
+    auto few_keys = [&](int last_q) { return tiles == 1 || (p.causal && p.offset + last_q < kStream); };
+    if (few_keys(min(at.row + 31, p.qs - 1))) {  // of the workgroup's first wavefront
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's part of the tile is in LDS
         __syncthreads();
+    }
+    if (few_keys(wave_last_q)) {
         float lack1 = 0.0f, lack2 = 0.0f;
 #pragma unroll 1
-        for (int sub = 0; sub < 2; ++sub) {
+        for (int first_key = 0; first_key < kStream; first_key += 32) {
+            const T* k_rows = lds + first_key * W;
             acc_t st[2] = {acc_t(0.0f), acc_t(0.0f)}, g(0.0f);
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
-                st[s / HALF] = Mma<T>::run(*reinterpret_cast<const frag*>(lds + sub * 32 * W + k_off[s]), qf[s], st[s / HALF]);
-                g = Mma<T>::run(*reinterpret_cast<const frag*>(lds + kWideTile<W> + sub * 32 * W + k_off[s]), dof[s], g);
+                st[s / HALF] = Mma<T>::run(*reinterpret_cast<const frag*>(k_rows + k_off[s]), qf[s], st[s / HALF]);
+                g = Mma<T>::run(*reinterpret_cast<const frag*>(k_rows + kWideTile<W> + k_off[s]), dof[s], g);
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                if (sub * 32 + 4 * (lane >> 5) + 8 * (e >> 2) + (e & 3) > min(q_limit, p.ks - 1)) continue;
+                if (first_key + 4 * (lane >> 5) + 8 * (e >> 2) + (e & 3) > min(q_limit, p.ks - 1)) continue;
                 lack1 = fmaf(__builtin_amdgcn_exp2f(fmaf(st[0][e], scale2, -lse1)), g[e] - delta1, lack1);
                 lack2 = fmaf(__builtin_amdgcn_exp2f(fmaf(st[1][e], scale2, -lse2)), g[e] - delta2, lack2);
             }

@@ -1,6 +1,6 @@
-"""Differential attention's gradients in half precision where output gradients are small.
+"""Differential attention's gradients where 16 bits have few digits: of small output gradients in half precision, of rows that see few keys.
 
-They are linear in dO: with dO times 2^-s, a product that is exact here, the results are those of dO times 2^-s, within as much less. What is
+Gradients are linear in dO: with dO times 2^-s, a product that is exact here, the results are those of dO times 2^-s, within as much less. What is
 left beside that is half a step among the smallest numbers that the results themselves are stored in (check allows 2^-24)."""
 import pytest
 import torch
@@ -83,3 +83,24 @@ def test_output_gradients_that_are_no_numbers_stay_in_their_rows(device):
         assert not torch.isfinite(dq[:, 70]).any()
         rest = [i for i in range(200) if i != 70]
         check(dq[:, rest], want["dq"][:, rest], want["dq_err"][:, rest], "dq")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("c", [case(5, 1001, 1001, 12, 4, 64), case(16, 300, 300, 8, 2, 128), case(3, 100, 100, 4, 2, 64), case(24, 130, 140, 8, 8, 96)],
+                         ids=["64", "128", "few-blocks", "offset"])
+def test_rows_that_see_few_keys(device, c, dtype):
+    """The first rows of a longer sequence, which most of dq's norm is in: rowsum(P (G - delta)) is taken off there, whatever O was rounded to.
+
+    Bound: `reference` with deltas that are summed, for rows whose block of 32 sees one tile of 64 keys; for every row its usual bounds. In
+    the 2-norm: dq's rounding is one error of half a step at most, evenly spread, and that of the score gradients another that is as
+    large beside the result: sqrt(2) of the exact dq's rounding error, and 1.5 with what the deltas of the other rows add."""
+    q, k, v, dout, lambdas = inputs(c, dtype, device)
+    dq = backward(c, q, k, v, dout, lambdas, forward(c, q, k, v, lambdas))[0]
+    want, summed = reference(c, q, k, v, lambdas, dout), reference(c, q, k, v, lambdas, dout, summed=True)
+    few = (64 - c["off"]) // 32 * 32
+    check(dq[:, :few], want["dq"][:, :few], summed["dq_err"][:, :few], "dq of few keys")
+    check(dq, want["dq"], want["dq_err"], "dq")
+    rounding = (want["dq"].to(dtype).double() - want["dq"]).norm().item()
+    off = (dq.double() - want["dq"]).norm().item()
+    print(f"[parity] dq: {off / rounding:.3f} of the exact dq's rounding")
+    assert off <= 1.5 * rounding
