@@ -543,14 +543,14 @@ __global__ __launch_bounds__(kThreads) void differential_combine_kernel(Differen
 // Half precision's smallest normal number is 2^-14. Score gradients P (G - delta) are rounded to storage before their products, and where
 // output gradients are small (P is some 1/n beside a dO of any size) they are below it and lose their digits. So they are enlarged by a power of
 // two, which costs nothing inside P's exponent, and the sums are made smaller by it: by what brings the largest |dO| (of the row for
-// dq, of the (batch entry, kv head) for dk and dv) to between 32 and 64. Beside values of v around 1 that leaves six bits below 65504 for the
-// product of head_dim terms and ten more below 2^-14 for P than without. Sums that are not finite then, beside larger values of v, are taken again
-// in fp32 (dq_of_row, dk_of_row).
+// dq, of the (batch entry, kv head) for dk and dv) to between 4 and 8, where dO of deviation 1 has it. P v has to be some thousands there
+// before a score gradient of 128 columns passes 65504; sums that are not finite then are taken again in fp32 (dq_of_row, dk_of_row), some
+// hundred times slower.
 template <typename T>
 constexpr bool kEnlarged = __is_same(T, f16_t);
-// The power that brings `largest` to between 32 and 64: 0 from 32 on and for what is no number, at most `most`.
+// The power that brings `largest` to between 4 and 8: 0 from 4 on and for what is no number, at most `most`.
 __device__ __forceinline__ int enlarging_power(float largest, int most) {
-    return max(min(127 + 5 - static_cast<int>(__float_as_uint(largest) >> 23), most), 0);
+    return max(min(127 + 2 - static_cast<int>(__float_as_uint(largest) >> 23), most), 0);
 }
 // The largest of the absolute values of a row in half precision, in all lanes of the row.
 template <int STEPS>
