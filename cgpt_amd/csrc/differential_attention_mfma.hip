@@ -743,7 +743,9 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void differential_dq_ker
         p.delta[3 * rows + row] = sign_of_second(lambda) * (delta1 - delta2);
     }
     if constexpr (kEnlarged<T>) {
-        const float largest = largest_of_row<STEPS>(dof), power = static_cast<float>(enlarging_power(largest, 24)), of_wave = wave_max(largest);
+        const float largest = largest_of_row<STEPS>(dof), power = static_cast<float>(enlarging_power(largest, 24));
+        const bool finite = (delta1 + delta2 + lse1 + lse2) * 0.0f == 0.0f;  // if not, no sum that the row is in will be: nothing to save
+        const float of_wave = wave_max(finite ? largest : INFINITY);
         lse1 -= power;
         lse2 -= power;
         if (lane == 0 && at.part == 0) p.largest[at.h * p.lambda_parts + row_part] = of_wave;

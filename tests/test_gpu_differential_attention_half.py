@@ -104,3 +104,19 @@ def test_rows_that_see_few_keys(device, c, dtype):
     off = (dq.double() - want["dq"]).norm().item()
     print(f"[parity] dq: {off / rounding:.3f} of the exact dq's rounding")
     assert off <= 1.5 * rounding
+
+
+@pytest.mark.parametrize("what", ["q", "k", "v"])
+def test_tensors_with_an_infinity_beside_small_output_gradients(device, what):
+    """Keys and heads that the infinity does not reach are what they are without it."""
+    c = case(2, 260, 260, 4, 2, 64)
+    q, k, v, _, lambdas = inputs(c, torch.float16, device)
+    dout = few_bits(q.shape, 8, device) * 2.0 ** -6
+    want = reference(c, q, k, v, lambdas, dout)
+    {"q": q, "k": k, "v": v}[what][0, 130, :2 if what == "q" else 1] = float("inf")
+    dq, dk, dv, _ = backward(c, q, k, v, dout, lambdas, forward(c, q, k, v, lambdas))
+    for got, name in ((dq, "dq"), (dk, "dk"), (dv, "dv")):
+        heads = 2 if name == "dq" else 1
+        check(got[1], want[name][1], want[name + "_err"][1], name)
+        check(got[0, :, heads:], want[name][0, :, heads:], want[name + "_err"][0, :, heads:], name)
+    check(dq[0, :130], want["dq"][0, :130], want["dq_err"][0, :130], "dq")
