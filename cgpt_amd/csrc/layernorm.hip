@@ -14,7 +14,9 @@
 // needs by a workgroup, and columns by a kernel of their own.
 //
 // 32768 x 1024 in bf16: forward 24.5 us (5.5 TB/s), backward with the residual gradient 57 (4.7 TB/s: the row pass 45, the column
-// sums' launch 5.5). 5005 x 1001 in fp32, backward: 17.7 (13.4 and 4). 16 x 768 in fp16, forward: 3.1 on the device.
+// sums' launch 5.5). 5005 x 1001 in fp32, backward: 17.7 (13.4 and 4). 16 x 768 in fp16, forward: 3.1 on the device. Backward rows of
+// more than 8192 values in fp32 are in registers by name only: sixteen wavefronts leave 128 a lane, and 150 values are spilled (1024 x
+// 16384: 87 us, 2.3 TB/s). 16384 x 2048 in bf16, 288 registers and so one wavefront a SIMD: 40 us, 5.0 TB/s.
 #include "common.hpp"
 #include "reduce.hpp"
 

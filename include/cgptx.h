@@ -211,8 +211,9 @@ int cgptx_dropout_backward(void* grad_input, const void* grad_output, size_t cou
  * in a fixed order: results do not depend on scheduling. How many parts there are goes by the sizes and, where the scratch
  * arena cannot grow (a call that is recorded on a stream where no eager call of its sizes ran), by what it has room for:
  * such a call adds in another order than an eager one, and its results may differ from that one's by rounding. In 16-bit
- * storage P1 - lambda P2 and the score gradients are rounded to it once before their products, as in plain attention; in
- * half precision they are enlarged by a power of two first where output gradients are below 1. */
+ * storage P1 - lambda P2 and the score gradients are rounded to it once before their products, as in plain attention, and
+ * row sums come from output and second as they are stored; in half precision the former are enlarged by a power of two
+ * first where output gradients are small. Keys that no query sees get gradients of 0 whatever they hold. */
 int cgptx_differential_attention_backward(
     void* grad_query, void* grad_key, void* grad_value, float* grad_lambda,
     const void* grad_output, const void* output, const void* second,
