@@ -40,7 +40,7 @@ DEVICE_FLAGS = [
 # place). The option belongs to the compiler's backend, not to its documented interface: it is probed once and
 # left out, with a warning, when this hipcc does not know it (the kernels are correct either way, the
 # accumulators are then copied between the two register files).
-FILE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("attention.hip", "differential_attention_mfma.hip")}
+FILE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("attention.hip", "differential_attention_mfma.hip", "linear_attention.hip")}
 _probed_flags: dict[tuple[str, ...], bool] = {}
 
 

@@ -67,6 +67,8 @@ PROTOTYPES = {
     "cgptx_differential_attention_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz,
                                               _f, _i, _sz, _i, _i, _vp],
     "cgptx_differential_lambda_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _i, _vp],
+    "cgptx_linear_attention_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _f, _i, _i, _vp],
+    "cgptx_sandwich_norm_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _f, _f, _i, _vp],
     "cgptx_adamw_workspace_create": [ctypes.POINTER(_vp)],
     "cgptx_adamw_workspace_destroy": [_vp],
     "cgptx_adamw_step_many_async": [_vp, ctypes.POINTER(AdamWEntry), _sz, ctypes.POINTER(AdamWOptions), _u64, _vp],
@@ -87,6 +89,9 @@ PROTOTYPES = {
     "cgptx_dropout_forward": [_vp, _vp, _vp, _sz, _f, _u64, _u64, _vp, _i, _vp],
     "cgptx_differential_attention_forward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _f, _i, _sz, _i, _vp],
     "cgptx_differential_lambda_forward": [_vp, _vp, _vp, _vp, _vp, _f, _sz, _sz, _sz, _i, _vp],
+    "cgptx_linear_attention_forward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _f, _i, _vp],
+    "cgptx_linear_attention_step": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _f, _i, _vp],
+    "cgptx_sandwich_norm_forward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _f, _f, _i, _vp],
     "cgptx_add": [_vp, _vp, _vp, _sz, _i, _vp],
     "cgptx_model_create": [ctypes.POINTER(_vp), ctypes.POINTER(ModelConfig), _sz, _sz, _u64],
     "cgptx_model_destroy": [_vp],

@@ -648,6 +648,97 @@ PyObject* differential_lambda_backward(Call c) {  // four gradients, grad_lambda
     });
 }
 
+// A state of linear attention, or none.
+bool is_state(const at::Tensor* t, const Attention& a, size_t batch) {
+    return t == nullptr || (t->dim() == 4 && at(t, 0) == batch && at(t, 1) == a.kv_heads && at(t, 2) == a.head_dim && at(t, 3) == a.head_dim);
+}
+bool linear(const Attention& a, const at::Tensor* q, const at::Tensor* k, const at::Tensor* v, const at::Tensor* log_decay) {
+    return a.fits(q, k, v) && a.causal && a.offset == 0 && at(q, 1) == at(k, 1) && log_decay->dim() == 1 && at(log_decay, 0) == a.kv_heads;
+}
+float* values(const at::Tensor* t) { return static_cast<float*>(data(t)); }
+
+PyObject* linear_attention_forward(Call c) {  // output, final_state or None, query, key, value, log_decay, initial_state or None, options, stream
+    const at::Tensor *o = c.tensor(0), *q = c.tensor(2), *k = c.tensor(3), *v = c.tensor(4), *log_decay = c.f32(5);
+    const at::Tensor *after = c.args[1] != Py_None ? c.f32(1) : nullptr, *before = c.args[6] != Py_None ? c.f32(6) : nullptr;
+    if (!c.ok) return none();
+    const Attention a(c, c.args[7]);
+    if (!c.need(c.ok && linear(a, q, k, v, log_decay) && same(o, q) && is_state(after, a, at(q, 0)) && is_state(before, a, at(q, 0))) ||
+        !c.here({o, after, q, k, v, log_decay, before}))
+        return none();
+    const auto stream = stream_of(c, 8);
+    return finish(c, [&] {
+        return cgptx_linear_attention_forward(data(o), values(after), data(q), data(k), data(v), values(log_decay), values(before), at(q, 0),
+                                              at(q, 1), a.query_heads, a.kv_heads, a.head_dim, a.scale, c.code, stream);
+    });
+}
+
+PyObject* linear_attention_backward(Call c) {  // grad_query, grad_key, grad_value, grad_initial_state or None, grad_output, grad_final_state or None, query, key, value, log_decay, initial_state or None, options, accumulate, stream
+    const at::Tensor *dq = c.tensor(0), *dk = c.tensor(1), *dv = c.tensor(2), *d_o = c.tensor(4), *q = c.tensor(6), *k = c.tensor(7),
+                     *v = c.tensor(8), *log_decay = c.f32(9);
+    const at::Tensor *d_before = c.args[3] != Py_None ? c.f32(3) : nullptr, *d_after = c.args[5] != Py_None ? c.f32(5) : nullptr,
+                     *before = c.args[10] != Py_None ? c.f32(10) : nullptr;
+    if (!c.ok) return none();
+    const Attention a(c, c.args[11]);
+    const int accumulate = c.flag(12);
+    if (!c.need(c.ok && linear(a, q, k, v, log_decay) && same(q, d_o) && same(q, dq) && same(k, dk) && same(k, dv) &&
+                is_state(d_before, a, at(q, 0)) && is_state(d_after, a, at(q, 0)) && is_state(before, a, at(q, 0))) ||
+        !c.here({dq, dk, dv, d_before, d_o, d_after, q, k, v, log_decay, before}))
+        return none();
+    const auto stream = stream_of(c, 13);
+    return finish(c, [&] {
+        return cgptx_linear_attention_backward(data(dq), data(dk), data(dv), values(d_before), data(d_o), values(d_after), data(q), data(k), data(v),
+                                               values(log_decay), values(before), at(q, 0), at(q, 1), a.query_heads, a.kv_heads, a.head_dim, a.scale,
+                                               accumulate, c.code, stream);
+    });
+}
+
+PyObject* linear_attention_step(Call c) {  // output, next_state, state, query, key, value, log_decay, options, stream
+    const at::Tensor *o = c.tensor(0), *q = c.tensor(3), *k = c.tensor(4), *v = c.tensor(5), *next = c.f32(1), *state = c.f32(2), *log_decay = c.f32(6);
+    if (!c.ok) return none();
+    const Attention a(c, c.args[7]);
+    if (!c.need(c.ok && linear(a, q, k, v, log_decay) && at(q, 1) == 1 && same(o, q) && is_state(next, a, at(q, 0)) && is_state(state, a, at(q, 0))) ||
+        !c.here({o, next, state, q, k, v, log_decay}))
+        return none();
+    const auto stream = stream_of(c, 8);
+    return finish(c, [&] {
+        return cgptx_linear_attention_step(data(o), values(next), values(state), data(q), data(k), data(v), values(log_decay), at(q, 0), a.query_heads,
+                                           a.kv_heads, a.head_dim, a.scale, c.code, stream);
+    });
+}
+
+// Whether a gate (or none) has a row for every equal number of x's rows.
+bool gates(const at::Tensor* gate, const at::Tensor* x) {
+    return gate == nullptr || (gate->dim() == 2 && gate->size(1) == x->size(1) && gate->size(0) > 0 && x->size(0) % gate->size(0) == 0);
+}
+
+PyObject* sandwich_norm_forward(Call c) {  // stream_output, normed, stream_input, branch, branch_weight, gate or None, norm_weight, residual_scale, epsilon, stream
+    const at::Tensor *s = c.tensor(0), *y = c.tensor(1), *x = c.tensor(2), *f = c.tensor(3), *u = c.tensor(4), *gate = c.tensor(5, true), *w = c.tensor(6);
+    const float scale = c.number(c.args[7]), epsilon = c.positive(8);
+    if (!c.need(c.ok && x->dim() == 2 && same(x, s) && same(x, y) && same(x, f) && is_row(u, x) && is_row(w, x) && gates(gate, x)) ||
+        !c.here({s, y, x, f, u, gate, w}))
+        return none();
+    const auto stream = stream_of(c, 9);
+    return finish(c, [&] {
+        return cgptx_sandwich_norm_forward(data(s), data(y), data(x), data(f), data(u), data(gate), data(w), at(x, 0), at(x, 1),
+                                           gate != nullptr ? at(gate, 0) : 0, scale, epsilon, c.code, stream);
+    });
+}
+
+PyObject* sandwich_norm_backward(Call c) {  // grad_stream_input, grad_branch, grad_branch_weight, grad_gate or None, grad_norm_weight, grad_stream_output or None, grad_normed, stream_output, branch, branch_weight, gate or None, norm_weight, residual_scale, epsilon, stream
+    const at::Tensor *dx = c.tensor(0), *df = c.tensor(1), *du = c.tensor(2), *dgate = c.tensor(3, true), *dw = c.tensor(4), *ds = c.tensor(5, true),
+                     *dy = c.tensor(6), *s = c.tensor(7), *f = c.tensor(8), *u = c.tensor(9), *gate = c.tensor(10, true), *w = c.tensor(11);
+    const float scale = c.number(c.args[12]), epsilon = c.positive(13);
+    if (!c.need(c.ok && s->dim() == 2 && same(s, dx) && same(s, df) && same(s, dy) && same(s, f) && (ds == nullptr || same(s, ds)) && is_row(u, s) &&
+                is_row(w, s) && is_row(du, s) && is_row(dw, s) && gates(gate, s) && (dgate == nullptr || (gate != nullptr && same(gate, dgate)))) ||
+        !c.here({dx, df, du, dgate, dw, ds, dy, s, f, u, gate, w}))
+        return none();
+    const auto stream = stream_of(c, 14);
+    return finish(c, [&] {
+        return cgptx_sandwich_norm_backward(data(dx), data(df), data(du), data(dgate), data(dw), data(ds), data(dy), data(s), data(f), data(u), data(gate),
+                                            data(w), at(s, 0), at(s, 1), gate != nullptr ? at(gate, 0) : 0, scale, epsilon, c.code, stream);
+    });
+}
+
 // A tensor that refuses to say what it is makes the call one that is not taken.
 template <PyObject* (*Function)(Call), int COUNT>
 PyObject* operation(PyObject*, PyObject* const* args, Py_ssize_t count) {
@@ -690,6 +781,11 @@ PyMethodDef methods[] = {
     method<differential_attention_backward, 15>("differential_attention_backward"),
     method<differential_lambda_forward, 7>("differential_lambda_forward"),
     method<differential_lambda_backward, 10>("differential_lambda_backward"),
+    method<linear_attention_forward, 9>("linear_attention_forward"),
+    method<linear_attention_backward, 14>("linear_attention_backward"),
+    method<linear_attention_step, 9>("linear_attention_step"),
+    method<sandwich_norm_forward, 10>("sandwich_norm_forward"),
+    method<sandwich_norm_backward, 15>("sandwich_norm_backward"),
     {"tensors", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(call<tensors>)), METH_FASTCALL, "(dtype code, pointers) or None"},
     {"same_shape", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(call<same_shape>)), METH_FASTCALL, "whether all shapes are equal"},
     {"adamw_entries", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(call<adamw_entries>)), METH_FASTCALL, "fills an entry array"},

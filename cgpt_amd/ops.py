@@ -565,6 +565,78 @@ def differential_lambda_backward(grad_query1, grad_key1, grad_query2, grad_key2,
     capi.call("cgptx_differential_lambda_backward", g1, g2, g3, g4, grad_lambdas.data_ptr(), q1, k1, q2, k2, *sizes, code, _stream(stream))
 
 
+def _linear_check(name, q, k, v, log_decay, options, *states):
+    """Sizes of the call: (batch, sequence, query heads, kv heads, head_dim). Linear attention is causal, and what came before is in the state."""
+    batch, sequence, kv_sequence, hq, hkv, d = _attention_check(name, q, k, v, options)
+    if not options.causal or options.query_position_offset or kv_sequence != sequence:
+        raise ValueError(f"{name}: queries and keys must be of the same tokens, the mask causal and its offset 0")
+    if log_decay.dtype != torch.float32 or tuple(log_decay.shape) != (hkv,):
+        raise ValueError(f"{name}: log_decay must be a device F32 tensor with shape [kv_heads]")
+    if any(t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (batch, hkv, d, d)) for t in states):
+        raise ValueError(f"{name}: states must be F32 [batch, kv_heads, head_dim, head_dim]")
+    return batch, sequence, hq, hkv, d
+
+
+def linear_attention_backward(grad_query, grad_key, grad_value, grad_initial_state, grad_output, grad_final_state, query, key, value, log_decay,
+                              initial_state=None, stream=None, options: FlashAttentionOptions = FlashAttentionOptions(),
+                              accumulate_grads: bool = False):
+    """Gradients of linear_attention_forward. grad_final_state: the gradient that reaches the final state, or None; grad_initial_state: the one that
+    reaches the initial state, None where it is not wanted. The decays get none."""
+    status = _native.linear_attention_backward(grad_query, grad_key, grad_value, grad_initial_state, grad_output, grad_final_state, query, key,
+                                               value, log_decay, initial_state, options, accumulate_grads, stream)
+    if status == 0:
+        return
+    if status:
+        capi.check(status)
+    name = "linear_attention_backward"
+    tensors = (grad_query, grad_key, grad_value, grad_output, query, key, value)
+    states = (grad_initial_state, grad_final_state, initial_state)
+    code, dq, dk, dv, do, q, k, v = _tensors(*tensors) or _reject(name, *tensors)
+    _require_device(name, log_decay, *(t for t in states if t is not None))
+    _on_current_device(name, *tensors, log_decay, *states)
+    sizes = _linear_check(name, query, key, value, log_decay, options, *states)
+    if not _same_shape(query, grad_output, grad_query) or not _same_shape(key, grad_key, grad_value):
+        raise ValueError(f"{name}: gradient shapes must match their tensors")
+    capi.call("cgptx_linear_attention_backward", dq, dk, dv, _ptr(grad_initial_state), do, _ptr(grad_final_state), q, k, v, log_decay.data_ptr(),
+              _ptr(initial_state), *sizes, options.attention_scale, int(accumulate_grads), code, _stream(stream))
+
+
+def _sandwich_check(name, residual_scale, epsilon, gate, weights, *rows):
+    if not (math.isfinite(epsilon) and epsilon > 0 and math.isfinite(residual_scale)):
+        raise ValueError(f"{name}: epsilon must be finite and positive, the residual scale finite")
+    first = rows[0]
+    if first.dim() != 2 or any(t is not None and not _same_shape(t, first) for t in rows) or \
+            any(tuple(t.shape) != (first.shape[1],) for t in weights):
+        raise ValueError(f"{name}: incompatible shapes")
+    if gate is None:
+        return *first.shape, 0
+    if gate.dim() != 2 or gate.shape[1] != first.shape[1] or not gate.shape[0] or first.shape[0] % gate.shape[0]:
+        raise ValueError(f"{name}: the gate must have one row for every equal number of rows")
+    return *first.shape, gate.shape[0]
+
+
+def sandwich_norm_backward(grad_stream_input, grad_branch, grad_branch_weight, grad_gate, grad_norm_weight, grad_stream_output, grad_normed,
+                           stream_output, branch, branch_weight, gate, norm_weight, residual_scale, epsilon, stream=None):
+    """Gradients of sandwich_norm_forward from those of its outputs. stream_output is the forward's; grad_stream_output, the gradient that reaches
+    it past the norm, may be None, and grad_stream_input may be grad_stream_output; grad_gate may be None, and is without a gate."""
+    status = _native.sandwich_norm_backward(grad_stream_input, grad_branch, grad_branch_weight, grad_gate, grad_norm_weight, grad_stream_output,
+                                            grad_normed, stream_output, branch, branch_weight, gate, norm_weight, residual_scale, epsilon, stream)
+    if status == 0:
+        return
+    if status:
+        capi.check(status)
+    name = "sandwich_norm_backward"
+    tensors = (grad_stream_input, grad_branch, grad_branch_weight, grad_gate, grad_norm_weight, grad_stream_output, grad_normed, stream_output,
+               branch, branch_weight, gate, norm_weight)
+    code, *pointers = _tensors(*tensors) or _reject(name, *tensors)
+    _on_current_device(name, *tensors)
+    sizes = _sandwich_check(name, residual_scale, epsilon, gate, (grad_branch_weight, grad_norm_weight, branch_weight, norm_weight), stream_output,
+                            grad_stream_input, grad_branch, grad_stream_output, grad_normed, branch)
+    if grad_gate is not None and (gate is None or not _same_shape(grad_gate, gate)):
+        raise ValueError(f"{name}: the gate's gradient must match the gate")
+    capi.call("cgptx_sandwich_norm_backward", *pointers, *sizes, residual_scale, epsilon, code, _stream(stream))
+
+
 # ------------------------------------------------------------------------------ AdamW
 class AdamWState:
     """AdamWState (include/optim/adamw.h:33-46): F32 master copy and moments."""
@@ -962,3 +1034,63 @@ def differential_lambda_forward(lambdas, query1, key1, query2, key2, initial, st
     if not math.isfinite(initial):
         raise ValueError(f"{name}: the initial value must be finite")
     capi.call("cgptx_differential_lambda_forward", lambdas.data_ptr(), q1, k1, q2, k2, initial, *sizes, code, _stream(stream))
+
+
+def linear_attention_forward(output, final_state, query, key, value, log_decay, initial_state=None, stream=None,
+                             options: FlashAttentionOptions = FlashAttentionOptions()):
+    """Linear attention with a decay per kv head: S_t = exp(log_decay) S_{t-1} + k_t v_t', output_t = s S_t' q_t; the query heads of a group read their
+    kv head's S. query [batch, sequence, query heads, head_dim], key and value with kv heads, log_decay F32 [kv_heads], at most 0; states F32
+    [batch, kv_heads, head_dim, head_dim]: initial_state None: zeros, final_state None: not wanted (include/cgptx.h)."""
+    status = _native.linear_attention_forward(output, final_state, query, key, value, log_decay, initial_state, options, stream)
+    if status == 0:
+        return
+    if status:
+        capi.check(status)
+    name = "linear_attention_forward"
+    code, o, q, k, v = _tensors(output, query, key, value) or _reject(name, output, query, key, value)
+    states = (final_state, initial_state)
+    _require_device(name, log_decay, *(t for t in states if t is not None))
+    _on_current_device(name, output, query, key, value, log_decay, *states)
+    sizes = _linear_check(name, query, key, value, log_decay, options, *states)
+    if not _same_shape(output, query):
+        raise ValueError(f"{name}: output must match query")
+    capi.call("cgptx_linear_attention_forward", o, _ptr(final_state), q, k, v, log_decay.data_ptr(), _ptr(initial_state), *sizes,
+              options.attention_scale, code, _stream(stream))
+
+
+def linear_attention_step(output, next_state, state, query, key, value, log_decay, stream=None,
+                          options: FlashAttentionOptions = FlashAttentionOptions()):
+    """One token of linear attention for every sequence of [batch, 1, heads, head_dim] tensors: next_state = exp(log_decay) state + k v', output
+    from next_state, which may be state itself."""
+    status = _native.linear_attention_step(output, next_state, state, query, key, value, log_decay, options, stream)
+    if status == 0:
+        return
+    if status:
+        capi.check(status)
+    name = "linear_attention_step"
+    code, o, q, k, v = _tensors(output, query, key, value) or _reject(name, output, query, key, value)
+    _require_device(name, next_state, state, log_decay)
+    _on_current_device(name, output, next_state, state, query, key, value, log_decay)
+    batch, sequence, hq, hkv, d = _linear_check(name, query, key, value, log_decay, options, next_state, state)
+    if sequence != 1 or not _same_shape(output, query):
+        raise ValueError(f"{name}: query and output must be one token of every sequence")
+    capi.call("cgptx_linear_attention_step", o, next_state.data_ptr(), state.data_ptr(), q, k, v, log_decay.data_ptr(), batch, hq, hkv, d,
+              options.attention_scale, code, _stream(stream))
+
+
+def sandwich_norm_forward(stream_output, normed, stream_input, branch, branch_weight, gate, norm_weight, residual_scale, epsilon, stream=None):
+    """The norms between two branches: stream_output = residual_scale * stream_input + gate * rmsnorm(branch) * branch_weight, normed =
+    rmsnorm(stream_output) * norm_weight over the rows of [rows, hidden]. gate [gate rows, hidden]: one row for every rows / gate rows rows in
+    turn, or None. stream_output may be stream_input."""
+    status = _native.sandwich_norm_forward(stream_output, normed, stream_input, branch, branch_weight, gate, norm_weight, residual_scale, epsilon,
+                                           stream)
+    if status == 0:
+        return
+    if status:
+        capi.check(status)
+    name = "sandwich_norm_forward"
+    tensors = (stream_output, normed, stream_input, branch, branch_weight, gate, norm_weight)
+    code, *pointers = _tensors(*tensors) or _reject(name, *tensors)
+    _on_current_device(name, *tensors)
+    sizes = _sandwich_check(name, residual_scale, epsilon, gate, (branch_weight, norm_weight), stream_input, stream_output, normed, branch)
+    capi.call("cgptx_sandwich_norm_forward", *pointers, *sizes, residual_scale, epsilon, code, _stream(stream))

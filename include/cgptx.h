@@ -232,6 +232,31 @@ int cgptx_differential_lambda_backward(void* grad_query1, void* grad_key1,
                                        const void* key2, size_t sets, size_t heads,
                                        size_t width, int dtype, cgptx_stream stream);
 
+/* Gradients of linear attention (see cgptx_linear_attention_forward). grad_final_state: the gradient that reaches the final state, NULL
+ * for none; grad_initial_state: the one that reaches the initial state, NULL where it is not wanted, else no other tensor of the call;
+ * both fp32 like the states. accumulate_grads adds to grad_query, grad_key and grad_value; grad_initial_state is overwritten. The decays get
+ * no gradient: they are constants of a model. How sums are cut and rounded is as in the forward call. */
+int cgptx_linear_attention_backward(
+    void* grad_query, void* grad_key, void* grad_value, float* grad_initial_state,
+    const void* grad_output, const float* grad_final_state, const void* query,
+    const void* key, const void* value, const float* log_decay,
+    const float* initial_state, size_t batch, size_t sequence, size_t query_heads,
+    size_t kv_heads, size_t head_dim, float attention_scale, int accumulate_grads,
+    int dtype, cgptx_stream stream);
+
+/* Gradients of the norms between two branches (see cgptx_sandwich_norm_forward). stream_output is the forward's; grad_stream_output is the
+ * gradient that reaches it past the norm (NULL for none), grad_normed the one of normed. With G = grad_stream_output + that norm's gradient:
+ * grad_stream_input = residual_scale*G, grad_branch the branch norm's gradient of gate*G, grad_gate = sum G*rmsnorm(branch)*branch_weight
+ * over the rows of a gate. grad_gate may be NULL (and is, without a gate); grad_stream_input may be grad_stream_output. Outputs are
+ * overwritten. */
+int cgptx_sandwich_norm_backward(
+    void* grad_stream_input, void* grad_branch, void* grad_branch_weight,
+    void* grad_gate, void* grad_norm_weight, const void* grad_stream_output,
+    const void* grad_normed, const void* stream_output, const void* branch,
+    const void* branch_weight, const void* gate, const void* norm_weight,
+    size_t rows, size_t hidden, size_t gate_rows, float residual_scale,
+    float epsilon, int dtype, cgptx_stream stream);
+
 /* ------------------------------------------------------------------- AdamW */
 
 /* AdamWOptions — include/optim/adamw.h:12-27. */
@@ -408,6 +433,41 @@ int cgptx_differential_lambda_forward(float* lambda, const void* query1,
                                       const void* key2, float initial, size_t sets,
                                       size_t heads, size_t width, int dtype,
                                       cgptx_stream stream);
+
+/* Linear attention with a decay for each key/value head (no counterpart in the reference; tensors, heads and scale are
+ * flash_gqa_attention's, one sequence length for all). A kv head keeps a matrix S [head_dim, head_dim] that the query heads of its group read:
+ *   S_t = exp(log_decay) S_{t-1} + k_t v_t',  output_t = s S_t' q_t.
+ * log_decay: fp32 [kv_heads] on the device, at most 0 (larger values count as 0; -inf forgets all but the token itself). States are fp32
+ * [batch, kv_heads, head_dim (k), head_dim (v)]; initial_state NULL: zeros; final_state, the matrix behind the last token, may be
+ * NULL and must not be initial_state. Any head_dim up to 128; attention_scale <= 0 selects 1/sqrt(head_dim). The final state of 16-bit inputs is
+ * exact to 2^-16 and less; for the output, scores, states and decayed values are rounded to 16 bits once where they enter a product. A token that
+ * is not finite reaches itself and the tokens behind it. Long sequences are walked in parts side by side, as many as the scratch arena has room
+ * for: recorded where it cannot grow, the call adds in another order. */
+int cgptx_linear_attention_forward(
+    void* output, float* final_state, const void* query, const void* key,
+    const void* value, const float* log_decay, const float* initial_state,
+    size_t batch, size_t sequence, size_t query_heads, size_t kv_heads,
+    size_t head_dim, float attention_scale, int dtype, cgptx_stream stream);
+
+/* One token of linear attention for every sequence: query, output [batch, query_heads, head_dim], key, value [batch, kv_heads, head_dim];
+ * next_state = exp(log_decay) state + k v', output from next_state, which may be state itself. All sums are fp32. */
+int cgptx_linear_attention_step(
+    void* output, float* next_state, const float* state, const void* query,
+    const void* key, const void* value, const float* log_decay, size_t batch,
+    size_t query_heads, size_t kv_heads, size_t head_dim, float attention_scale,
+    int dtype, cgptx_stream stream);
+
+/* The norm behind a branch with its gate, the scale of the residual stream and the norm in front of the next branch (no counterpart in the
+ * reference):
+ *   stream_output = residual_scale*stream_input + gate*rmsnorm(branch)*branch_weight,  normed = rmsnorm(stream_output)*norm_weight,
+ * rows of `hidden` values, rmsnorm(x) = x/sqrt(mean(x^2) + eps); the second norm reads stream_output as it is stored. gate
+ * [gate_rows, hidden]: one row for all rows (a learned vector), one for each, or one for every rows/gate_rows rows in turn (a sequence's);
+ * NULL with gate_rows 0: no gate. stream_output may be stream_input. */
+int cgptx_sandwich_norm_forward(
+    void* stream_output, void* normed, const void* stream_input,
+    const void* branch, const void* branch_weight, const void* gate,
+    const void* norm_weight, size_t rows, size_t hidden, size_t gate_rows,
+    float residual_scale, float epsilon, int dtype, cgptx_stream stream);
 
 /* Residual helpers used by the block (src/core/transformer_block.cu:134-144, 242-248):
  * out = a + b, and out += b, elementwise over `count` values. */
