@@ -11,17 +11,19 @@
 //
 // A workgroup walks chunks of 64 tokens: in a chunk the pairs are a masked product of tiles, Z'P' with P = (X Y') g^|t-r|, and what came before
 // it is C' X'. The matrix stays in the accumulation registers from chunk to chunk, 32 of its columns a wavefront, and goes as an operand into its
-// product as it lies (the columns of Y are read in the order that makes it so). Long sequences are cut into segments that
-// workgroups walk side by side: one launch leaves each segment's own matrix, one adds them up along the sequence, and the third starts each
-// segment from there.
+// product as it lies (the columns of Y are read in the order that makes it so). Where there are fewer sequences than compute units, they are cut into
+// segments that workgroups walk side by side: one launch leaves each segment's own matrix, one adds them up along the sequence, and the third starts
+// each segment from there.
 //
 // 16-bit storage: P, C and the decayed Z are rounded to it once where they become operands, sums are fp32. In half precision a power of two
-// brings them into its range where they leave it. Matrices that the caller gets (fp32) come from Z in two parts, high and low.
+// brings them into its range where they leave it. The matrix in a walk is fed with the decayed Z in two parts, high and low,
+// and the matrices that are stored (fp32) with three in bfloat16.
 // An Inf or NaN reaches the tokens that see it and no others: chunks that hold one are added up token by token.
 #include "attention_tiles.hpp"
 
 #include <cmath>
 #include <string>
+#include <type_traits>
 
 namespace cgptx {
 namespace {
@@ -50,38 +52,63 @@ constexpr int kTile = kChunk * kPitch<T, W>;
 template <typename T>
 constexpr int kPairsPitch = sizeof(T) == 2 ? kChunk : kChunk + 4;
 
+// A lane's offset in a tile, one register for all of a kind of reads: the swizzle only flips bits of it (16-bit storage). `anew` keeps the
+// compiler from holding the sums with every step's constant in registers of their own.
+__device__ __forceinline__ int anew(int offset) {
+    asm volatile("" : "+v"(offset));
+    return offset;
+}
+template <typename T, int W>
+__device__ __forceinline__ int row_offset() {
+    const int lane = threadIdx.x & 63;
+    if constexpr (sizeof(T) == 2) return wide_direct_offset<W>(lane, 0);
+    else return (lane & 31) * kPitch<T, W> + 8 * (lane >> 5);
+}
 // Row block + lane%32 of a tile, columns 16 step + 8 (lane/32) .. + 7.
 template <typename T, int W>
-__device__ __forceinline__ frag_t<T> row_frag(const T* tile, int block, int step) {
-    const int lane = threadIdx.x & 63;
+__device__ __forceinline__ frag_t<T> row_frag(const T* tile, int offset, int block, int step) {
     if constexpr (sizeof(T) == 2) {
-        return *reinterpret_cast<const frag_t<T>*>(tile + block * W + wide_direct_offset<W>(lane, step));
+        return *reinterpret_cast<const frag_t<T>*>(tile + block * W + (offset ^ (16 * step)));
     } else {
-        const T* from = tile + (block + (lane & 31)) * kPitch<T, W> + 16 * step + 8 * (lane >> 5);
+        const T* from = tile + block * kPitch<T, W> + offset + 16 * step;
         const auto lo = load_vec<T, 4>(from), hi = load_vec<T, 4>(from + 4);
         return frag_t<T>{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     }
 }
-// Column 32 t + lane%32 of a tile, rows block + {0-3 | 4-7} and eight further. SWAPPED: the columns of a group of sixteen in the order 0-3, 8-11,
-// 4-7, 12-15, so that a product's registers 8 s .. 8 s + 7 hold rows 16 s + 8 (lane/32) .. + 7: those of row_frag.
-template <typename T, int W, bool SWAPPED>
+// Column 32 t + lane%32 of a tile, rows block + {0-3 | 4-7} and eight further.
+template <typename T, int W>
 __device__ __forceinline__ frag_t<T> column_frag(const T* tile, int block, int t) {
     const int lane = threadIdx.x & 63;
     if constexpr (sizeof(T) == 2) {
-        if constexpr (!SWAPPED) {
-            return wide_transposed_frag<T>(tile + block * W, wide_transposed_offset<W>(lane, t, 0), wide_transposed_offset<W>(lane, t, 1));
-        } else {
-            auto offset = [&](int second) {
-                const int row = (lane >> 5) * 4 + ((lane & 15) >> 2) + second * 8, chunk = t * 4 + ((lane >> 4) & 1) * 2 + (lane & 1);
-                return row * W + ((chunk ^ swizzle<W>(row)) * 8) + ((lane >> 1) & 1) * 4;
-            };
-            return wide_transposed_frag<T>(tile + block * W, offset(0), offset(1));
-        }
+        return wide_transposed_frag<T>(tile + block * W, wide_transposed_offset<W>(lane, t, 0), wide_transposed_offset<W>(lane, t, 1));
     } else {
-        const int m = lane & 31, column = 32 * t + (SWAPPED ? (m & 0x13) | ((m & 4) << 1) | ((m & 8) >> 1) : m);
         frag_t<T> f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = tile[(block + (e & 4) * 2 + 4 * (lane >> 5) + (e & 3)) * kPitch<T, W> + column];
+        for (int e = 0; e < 8; ++e) f[e] = tile[(block + (e & 4) * 2 + 4 * (lane >> 5) + (e & 3)) * kPitch<T, W> + 32 * t + (lane & 31)];
+        return f;
+    }
+}
+// The same with the columns of a group of sixteen in the order 0-3, 8-11, 4-7, 12-15, so that a product's registers 8 s .. 8 s + 7 hold rows
+// 16 s + 8 (lane/32) .. + 7: those of row_frag.
+template <typename T, int W>
+__device__ __forceinline__ int swapped_offset() {
+    const int lane = threadIdx.x & 63;
+    if constexpr (sizeof(T) == 2) {
+        const int row = (lane >> 5) * 4 + ((lane & 15) >> 2), chunk = ((lane >> 4) & 1) * 2 + (lane & 1);
+        return row * W + ((chunk ^ swizzle<W>(row)) * 8) + ((lane >> 1) & 1) * 4;
+    } else {
+        const int m = lane & 31;
+        return 4 * (lane >> 5) * kPitch<T, W> + ((m & 0x13) | ((m & 4) << 1) | ((m & 8) >> 1));
+    }
+}
+template <typename T, int W>
+__device__ __forceinline__ frag_t<T> swapped_frag(const T* tile, int offset, int block, int t) {
+    if constexpr (sizeof(T) == 2) {  // eight rows further bit 4 of the offset is flipped
+        return wide_transposed_frag<T>(tile + block * W, offset ^ (32 * t), (offset ^ (32 * t) ^ 16) + 8 * W);
+    } else {
+        frag_t<T> f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = tile[(block + (e & 4) * 2 + (e & 3)) * kPitch<T, W> + offset + 32 * t];
         return f;
     }
 }
@@ -113,59 +140,77 @@ struct Rows {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* from, int bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(from), 0, bytes, 0x00020000);
 }
-// 16 bytes a lane, 1 KiB in all, straight into LDS.
-__device__ __forceinline__ void load_chunks(__amdgpu_buffer_rsrc_t rsrc, void* to, int voffset, int soffset) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_ptr)(to), 16, voffset, soffset, 0, 0);
+__device__ __forceinline__ vec_t<unsigned int, 4> load_words(__amdgpu_buffer_rsrc_t rsrc, int voffset, int soffset) {
+    return __builtin_bit_cast(vec_t<unsigned int, 4>, __builtin_amdgcn_raw_buffer_load_b128(rsrc, voffset, soffset, 0));
 }
-// Rows row0 .. row0 + 63 of a head, zeros behind the last token and behind column d. DIRECT (16-bit storage, 16-byte boundaries): straight into
-// LDS; the tile is there behind s_waitcnt vmcnt(0) and a barrier.
-template <typename T, int W, bool DIRECT>
-__device__ __forceinline__ void load_tile(T* tile, const Rows<T>& rows, int row0, int tokens, int d, bool vectors) {
-    constexpr int kThreadsHere = W * 2;  // W/32 wavefronts
-    const T* first = rows.base + static_cast<long>(row0) * rows.stride;
-    const int left = min(kChunk, tokens - row0);
-    if constexpr (DIRECT) {
-        constexpr int kChunks = W / 8, kRowsPerLoad = 64 / kChunks, kWaves = W / 32;
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const int row_bytes = static_cast<int>(rows.stride) * 2;
-        const __amdgpu_buffer_rsrc_t rsrc = buffer_of(first, (left - 1) * row_bytes + d * 2);
-        const int r = wave * kRowsPerLoad + lane / kChunks, chunk = (lane % kChunks) ^ swizzle<W>(r);
-        const int voffset = chunk * 8 < d ? r * row_bytes + chunk * 16 : 1 << 30;
-#pragma unroll
-        for (int i = 0; i < kChunk / (kWaves * kRowsPerLoad); ++i)
-            load_chunks(rsrc, tile + (i * kWaves + wave) * kRowsPerLoad * W, voffset, i * kWaves * kRowsPerLoad * row_bytes);
-    } else {
-        constexpr int VEC = kVec128<T>, kPieces = W / VEC;
-        for (int n = threadIdx.x; n < kChunk * kPieces; n += kThreadsHere) {
-            const int r = n / kPieces, piece = n % kPieces, column = piece * VEC;
-            vec_t<T, VEC> v(static_cast<T>(0.0f));
-            if (r < left && column < d) {
-                const T* from = first + static_cast<long>(r) * rows.stride + column;
-                if (vectors) {
-                    v = load_vec<T, VEC>(from);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e)
-                        if (column + e < d) v[e] = from[e];
-                }
-            }
-            if constexpr (sizeof(T) == 2) store_vec<T, VEC>(tile + r * W + ((piece ^ swizzle<W>(r)) * 8), v);
-            else store_vec<T, VEC>(tile + r * kPitch<T, W> + column, v);
+__device__ __forceinline__ void store_words(vec_t<unsigned int, 4> words, __amdgpu_buffer_rsrc_t rsrc, int voffset) {
+    __builtin_amdgcn_raw_buffer_store_b128(words, rsrc, voffset, 0, 0);
+}
+// Rows row0 .. row0 + 63 of a head on their way to a tile, zeros behind the last token and behind column d. STAGED (16-bit storage on 16-byte
+// boundaries): fetch asks for them, and they wait in registers until store. (Loads straight into LDS would save the registers, but every
+// transposing read of another tile waits for them.)
+template <typename T, int W, bool STAGED>
+struct Incoming {
+    static constexpr int kThreadsHere = W * 2;  // W/32 wavefronts
+    static constexpr int kChunks = W / 8;       // of a row
+    Rows<T> rows;
+    int row0;
+    __amdgpu_buffer_rsrc_t rsrc;
+    int voffset, further;  // a lane's first piece; bytes to its next one, sixteen rows on
+    vec_t<unsigned int, 4> piece[STAGED ? 4 : 1];
+
+    __device__ __forceinline__ Incoming(long stride, int d) {
+        if constexpr (STAGED) {
+            const int row_bytes = static_cast<int>(stride) * 2, r = threadIdx.x / kChunks, chunk = threadIdx.x % kChunks;
+            voffset = chunk * 8 < d ? r * row_bytes + chunk * 16 : 1 << 30;
+            further = 16 * row_bytes;
         }
     }
-}
-// The tiles that load_tile asked for are there, for every wavefront.
-__device__ __forceinline__ void tiles_there() {
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-    __syncthreads();
-}
+    // Says which rows; the four pieces of STAGED are asked for, and stored, one by one.
+    __device__ __forceinline__ void set(const Rows<T>& from, int first, int tokens, int d) {
+        rows = from;
+        row0 = first;
+        if constexpr (STAGED)
+            rsrc = buffer_of(rows.base + static_cast<long>(row0) * rows.stride, (min(kChunk, tokens - row0) - 1) * static_cast<int>(rows.stride) * 2 + d * 2);
+    }
+    __device__ __forceinline__ void fetch(int i) {
+        if constexpr (STAGED) piece[i] = load_words(rsrc, voffset, i * further);
+    }
+    __device__ __forceinline__ void store(int i, T* tile, int tokens, int d, bool vectors) const {
+        if constexpr (STAGED) {
+            const int r = threadIdx.x / kChunks, chunk = threadIdx.x % kChunks;
+            *reinterpret_cast<vec_t<unsigned int, 4>*>(tile + (r + i * 16) * W + ((chunk ^ swizzle<W>(r)) * 8)) = piece[i];
+        } else if (i == 0) {
+            const T* first = rows.base + static_cast<long>(row0) * rows.stride;
+            const int left = min(kChunk, tokens - row0);
+            constexpr int VEC = kVec128<T>, kPieces = W / VEC;
+#pragma unroll 4
+            for (int n = threadIdx.x; n < kChunk * kPieces; n += kThreadsHere) {
+                const int r = n / kPieces, p = n % kPieces, column = p * VEC;
+                vec_t<T, VEC> v(static_cast<T>(0.0f));
+                if (r < left && column < d) {
+                    const T* from = first + static_cast<long>(r) * rows.stride + column;
+                    if (vectors) {
+                        v = load_vec<T, VEC>(from);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e)
+                            if (column + e < d) v[e] = from[e];
+                    }
+                }
+                if constexpr (sizeof(T) == 2) store_vec<T, VEC>(tile + r * W + ((p ^ swizzle<W>(r)) * 8), v);
+                else store_vec<T, VEC>(tile + r * kPitch<T, W> + column, v);
+            }
+        }
+    }
+};
 
 // log2 of the decay. No growth: what is above 1 counts as 1. A head that forgets everything (-inf) has 0^0 = 1.
 __device__ __forceinline__ float log2_decay(float log_decay) {
     const float l = log_decay * kLog2e;
     return l > 0.0f ? 0.0f : l < -1.0e4f ? -1.0e4f : l;  // a NaN stays one
 }
-__device__ __forceinline__ float power(float l, int n) { return exp2f(l * static_cast<float>(n)); }
+__device__ __forceinline__ float power(float l, int n) { return __builtin_amdgcn_exp2f(l * static_cast<float>(n)); }
 
 template <typename V>
 __device__ __forceinline__ float finite_test(const V& f, float sum) {  // stays 0 while all is finite
@@ -194,20 +239,25 @@ __device__ __forceinline__ float range_scale(float largest, int low, int high) {
 template <typename T>
 constexpr bool kNarrow = __is_same(T, f16_t);  // a range that sums leave
 
+// The work of a chunk is written in slots: a few matrix instructions, the reads of operands for a later slot, vector work for the next one. What stands
+// in a slot stays there (left to itself the compiler reads an operand right before it is used, and every read's way through the LDS
+// is waited for).
+__device__ __forceinline__ void slot_end() { __builtin_amdgcn_sched_barrier(0); }
 // Z of a wavefront's 32 columns: four operands of sixteen rows.
 template <typename T>
 struct Values {
     frag_t<T> z[4];
     template <int W>
-    __device__ __forceinline__ void load(const T* tile, int column_block) {
+    __device__ __forceinline__ void load(const T* tile, int column_block, int first = 0, int count = 4) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) z[s] = column_frag<T, W, false>(tile, 16 * s, column_block);
+        for (int s = 0; s < 4; ++s)
+            if (s >= first && s < first + count) z[s] = column_frag<T, W>(tile, 16 * s, column_block);
     }
-    __device__ __forceinline__ bool finite() const {
+    __device__ __forceinline__ float finite_sum() const {  // 0 where all is finite
         float sum = 0.0f;
 #pragma unroll
         for (int s = 0; s < 4; ++s) sum = finite_test(z[s], sum);
-        return !__any(!(sum == 0.0f));
+        return sum;
     }
     __device__ __forceinline__ float largest() const {
         float most = 0.0f;
@@ -224,66 +274,107 @@ struct Values {
 // Weights of a chunk's tokens as what follows the chunk sees them (forward in time: 1 for token `end`, else g^(end - token); backward: g^(token
 // + 1)), for the rows that a lane's operands hold.
 struct Weights {
-    float base[8];  // of the rows of sixteen
-    float l, scale;
-    bool reverse;
+    vec_t<float, 8> w[4];
     __device__ __forceinline__ static int row(int e) { return 4 * ((threadIdx.x & 63) >> 5) + (e & 3) + 2 * (e & 4); }
-    __device__ __forceinline__ Weights(float l_, float scale_, bool reverse_) : l(l_), scale(scale_), reverse(reverse_) {
+    __device__ __forceinline__ Weights(float l, float scale, bool reverse, int end) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) base[e] = scale * power(l, reverse ? row(e) + 1 : 16 - row(e));
-    }
-    // Of block s of sixteen rows; `end` is kChunk but for a sequence's last chunk.
-    __device__ __forceinline__ vec_t<float, 8> of(int s, int end) const {
-        vec_t<float, 8> w;
-        if (reverse || end == kChunk) {
-            const float f = power(l, reverse ? 16 * s : 48 - 16 * s);
+        for (int s = 0; s < 4; ++s)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = base[e] * f;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = scale * power(l, max(end - 16 * s - row(e), 0));
-        }
-        return w;
+            for (int e = 0; e < 8; ++e) w[s][e] = scale * power(l, reverse ? 16 * s + row(e) + 1 : max(end - 16 * s - row(e), 0));
     }
 };
 
-// matrix += Y' (w Z) over a chunk, the matrix decayed by `factor` first. EXACT: w Z in two parts.
-template <typename T, int W, bool EXACT>
-__device__ __forceinline__ void update_matrix(acc_t (&matrix)[W / 32], float factor, const T* y_tile, const Values<T>& values, const Weights& weights,
-                                              int end) {
-    float up = 1.0f;
-    if constexpr (kNarrow<T>) {
-        up = range_scale(values.largest(), -3, 15);
-        up = up < 1.0f ? 1.0f : up;  // only what is small loses digits
-        factor *= up;
-    }
-    if (factor != 1.0f)
+// w Z of sixteen rows as operands, made in eight steps. 16-bit storage: two parts leave 2^-16 of it in bfloat16 and 2^-22 in half precision, a
+// third one 2^-24.
+template <typename T, int PARTS>
+struct Weighted {
+    static constexpr int kParts = sizeof(T) == 4 ? 1 : kNarrow<T> ? 2 : PARTS;
+    vec_t<T, 2> part[kParts][4];
+    vec_t<float, 2> rest[4];
+    __device__ __forceinline__ void step(int i, const frag_t<T>& z, const vec_t<float, 8>& w, float up) {
+        const int j = i / 2;
+        if (i % 2 == 0) {
+            rest[j] = vec_t<float, 2>{to_f32(z[2 * j]) * w[2 * j], to_f32(z[2 * j + 1]) * w[2 * j + 1]};
+            if constexpr (kNarrow<T>) rest[j] *= up;
+            part[0][j] = vec_from_f32<T, 2>(rest[j]);
+        } else {
 #pragma unroll
-        for (int k = 0; k < W / 32; ++k)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) matrix[k][i] *= factor;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        auto w = weights.of(s, end);
-        if constexpr (kNarrow<T>) w *= up;
-        const vec_t<float, 8> product = vec_to_f32<T, 8>(values.z[s]) * w;
-        const frag_t<T> high = vec_from_f32<T, 8>(product);
-        frag_t<T> low;
-        if constexpr (EXACT && sizeof(T) == 2) low = vec_from_f32<T, 8>(product - vec_to_f32<T, 8>(high));
-#pragma unroll
-        for (int k = 0; k < W / 32; ++k) {
-            const frag_t<T> y = column_frag<T, W, true>(y_tile, 16 * s, k);
-            matrix[k] = multiply<T>(y, high, matrix[k]);
-            if constexpr (EXACT && sizeof(T) == 2) matrix[k] = multiply<T>(y, low, matrix[k]);
+            for (int n = 1; n < kParts; ++n) {
+                rest[j] -= vec_to_f32<T, 2>(part[n - 1][j]);
+                part[n][j] = vec_from_f32<T, 2>(rest[j]);
+            }
         }
     }
-    if constexpr (kNarrow<T>)
-        if (up != 1.0f) {
-            const float down = 1.0f / up;
+    __device__ __forceinline__ frag_t<T> operand(int n) const {
+        return frag_t<T>{part[n][0][0], part[n][0][1], part[n][1][0], part[n][1][1], part[n][2][0], part[n][2][1], part[n][3][0], part[n][3][1]};
+    }
+};
+template <typename T, int W>
+__device__ __forceinline__ void read_rows_of(frag_t<T> (&y)[W / 32], const T* tile, int offset, int s) {
 #pragma unroll
-            for (int k = 0; k < W / 32; ++k)
+    for (int k = 0; k < W / 32; ++k) y[k] = swapped_frag<T, W>(tile, offset, 16 * s, k);
+}
+// matrix += Y' (w Z) for sixteen rows; between(i) follows the i-th matrix instruction, of `count`.
+template <typename T, int K, int PARTS, typename Between>
+__device__ __forceinline__ void add_rows(acc_t (&matrix)[K], const frag_t<T> (&y)[K], const Weighted<T, PARTS>& z, Between&& between) {
+    constexpr int kParts = Weighted<T, PARTS>::kParts;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) matrix[k][i] *= down;
+    for (int n = 0; n < kParts; ++n) {
+        const frag_t<T> part = z.operand(n);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            matrix[k] = multiply<T>(y[k], part, matrix[k]);
+            between(n * K + k, kParts * K);
+            slot_end();
+        }
+    }
+}
+// The steps of `all` that come behind instruction i of `count`.
+template <typename Step>
+__device__ __forceinline__ void share_of(int all, int i, int count, Step&& step) {
+#pragma unroll
+    for (int n = 0; n < all; ++n)
+        if (n * count / all == i) step(n);
+}
+// Half precision: what small values are enlarged by before they are weighted, the matrix along with them until it is brought back.
+template <typename T, int K>
+__device__ __forceinline__ float enlarge(acc_t (&matrix)[K], const Values<T>& values) {
+    if constexpr (!kNarrow<T>) return 1.0f;
+    const float up = fmaxf(range_scale(values.largest(), -3, 15), 1.0f);
+    if (up != 1.0f)
+#pragma unroll
+        for (int k = 0; k < K; ++k) matrix[k] *= up;
+    return up;
+}
+template <typename T, int K>
+__device__ __forceinline__ void bring_back(acc_t (&matrix)[K], float up) {
+    if (kNarrow<T> && up != 1.0f)
+#pragma unroll
+        for (int k = 0; k < K; ++k) matrix[k] *= 1.0f / up;
+}
+
+template <int K>
+__device__ __forceinline__ float largest_of(const acc_t (&matrix)[K]) {
+    float most = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(matrix[k][i]));
+    return wave_max(most);
+}
+// The matrix that a walk starts from: `factor` times the stored one, zeros for none. A wavefront has 32 columns.
+template <int K>
+__device__ __forceinline__ void load_matrix(acc_t (&matrix)[K], const float* from, float factor, bool transposed, int d, int wave) {
+    const int column = wave * 32 + (threadIdx.x & 31), row0 = matrix_row(0);
+    const __amdgpu_buffer_rsrc_t rsrc = buffer_of(from, from != nullptr ? d * d * 4 : 0);  // reads behind its end give zeros
+    const int row_step = (transposed ? 1 : d) * 4, first = (transposed ? column * d + row0 : row0 * d + column) * 4;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int further = 32 * k + 16 * (i >> 3) + (i & 7);  // rows
+            const int at = column < d && row0 + further < d ? first + further * row_step : 1 << 30;
+            matrix[k][i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, at, 0, 0)) * factor;
         }
 }
 
@@ -295,6 +386,7 @@ struct LinearArgs {
     float *ahead, *behind;  // [batch x kv_heads][segments][d][d]: what comes before a segment, and the gradient from behind it
     int batch, tokens, hq, hkv, d;
     int segments, segment_chunks;
+    int heads_each;  // query heads that a workgroup takes one after the other, of a group
     float scale;
     int accumulate, vectors;
 };
@@ -311,28 +403,60 @@ struct Task {
     float pair_scale, matrix_scale, out_scale;  // of P, of what is added to the matrix, of the matrix's part of the output
 };
 
-// The output of one head in one segment.
-template <typename T, int W, bool REVERSE, bool DIRECT>
+// The output of one head in one segment. In a chunk: scores and what came before it | pairs there: X and Z have been read, the next chunk's
+// are on their way (Y has two buffers) | products with Z, the matrix, the output | the next chunk is there.
+template <typename T, int W, bool REVERSE, bool STAGED>
 __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>& task, int b, int head, int segment, T* lds) {
     constexpr int K = W / 32, kTables = W == 128 ? 1 : 2;
-    T *x_tile = lds, *y_tile = lds + kTile<T, W>, *z_tile = lds + 2 * kTile<T, W>, *pairs = lds + 3 * kTile<T, W>;
+    T *x_tile = lds, *z_tile = lds + kTile<T, W>, *y_tiles = lds + 2 * kTile<T, W>, *pairs = lds + 4 * kTile<T, W>;
     __shared__ float pair_scales[3];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int d = a.d, tokens = a.tokens;
-    const int heads_each = task.y_heads > task.x_heads ? task.y_heads / task.x_heads : 1;
-    const int y_first = static_cast<int>(static_cast<long>(head) * task.y_heads / task.x_heads);
-    const int kv = REVERSE ? head : y_first;
+    const int group = a.hq / a.hkv, heads_each = REVERSE ? group : a.heads_each;
+    const int kv = REVERSE ? head : head / group, y_first = REVERSE ? head * group : kv;
     const float l = log2_decay(a.log_decay[kv]);
 
     const long x_stride = static_cast<long>(task.x_heads) * d, y_stride = static_cast<long>(task.y_heads) * d;
     const Rows<T> x{task.x + static_cast<long>(b) * tokens * x_stride + static_cast<long>(head) * d, x_stride};
     const long y_offset = static_cast<long>(b) * tokens * y_stride + static_cast<long>(y_first) * d;
+    const Rows<T> y{task.y + y_offset, y_stride}, z{task.z + y_offset, y_stride};
+
+    const int chunks_in_all = (tokens + kChunk - 1) / kChunk;
+    const int first_chunk = segment * a.segment_chunks, last_chunk = min(first_chunk + a.segment_chunks, chunks_in_all) - 1;
+    const int steps = last_chunk - first_chunk + 1;
+    auto row_of = [&](int step) { return (REVERSE ? last_chunk - step : first_chunk + step) * kChunk; };
+    Incoming<T, W, STAGED> in_x(x_stride, d), in_y(y_stride, d), in_z(y_stride, d);
+    // Forward in time the heads of a group share Y and Z, backward X and the output.
+    auto turn_to = [&](int step, int each) __attribute__((always_inline)) {
+        const int row0 = row_of(step);
+        const long along = static_cast<long>(each) * d, x_along = REVERSE ? 0 : along, y_along = REVERSE ? along : 0;
+        in_x.set(Rows<T>{x.base + x_along, x.stride}, row0, tokens, d);
+        in_y.set(Rows<T>{y.base + y_along, y.stride}, row0, tokens, d);
+        in_z.set(Rows<T>{z.base + y_along, z.stride}, row0, tokens, d);
+    };
+    // Piece n of the next tiles, of four or (all) twelve.
+    auto fetch = [&](auto all, int n) __attribute__((always_inline)) {
+        if constexpr (!decltype(all)::value) in_x.fetch(n);
+        else if (n % 3 == 0) in_x.fetch(n / 3);
+        else if (n % 3 == 1) in_y.fetch(n / 3);
+        else in_z.fetch(n / 3);
+    };
+    auto store_tiles = [&](auto all, int n, int buffer) __attribute__((always_inline)) {
+        if constexpr (!decltype(all)::value) in_x.store(n, x_tile, tokens, d, a.vectors);
+        else if (n % 3 == 0) in_x.store(n / 3, x_tile, tokens, d, a.vectors);
+        else if (n % 3 == 1) in_y.store(n / 3, y_tiles + buffer * kTile<T, W>, tokens, d, a.vectors);
+        else in_z.store(n / 3, z_tile, tokens, d, a.vectors);
+    };
+    turn_to(0, 0);
+#pragma unroll
+    for (int n = 0; n < 12; ++n) fetch(std::true_type{}, n);
 
     // Which 32 x 32 tiles of pairs a wavefront makes: 0 and 1 on the diagonal, 2 the one beside it. W = 64: wavefront 0 makes 0 and 2.
     float table[kTables][16];
+    unsigned int seen[kTables][8];  // bfloat16: masks of two elements each
     auto tile_t = [](int tile) { return tile == 2 ? (REVERSE ? 0 : 1) : tile; };
     auto tile_r = [](int tile) { return tile == 2 ? (REVERSE ? 1 : 0) : tile; };
-    auto my_tile = [&](int n) { return n == 0 ? wave : 2; };
+    auto my_tile = [&](int n) { return n == 0 ? min(wave, 2) : 2; };  // (what two wavefronts make is the same)
     auto apart = [&](int tile, int i) {
         const int t = tile_t(tile) * 32 + (lane & 31), r = tile_r(tile) * 32 + acc_row(i);
         return REVERSE ? r - t : t - r;
@@ -340,159 +464,290 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
 #pragma unroll
     for (int n = 0; n < kTables; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) table[n][i] = task.pair_scale * power(l, max(apart(my_tile(n), i), 0));
-    const Weights weights(l, task.matrix_scale, REVERSE);
+        for (int i = 0; i < 16; ++i) {
+            const int far = apart(my_tile(n), i);
+            table[n][i] = far >= 0 ? task.pair_scale * power(l, far) : 0.0f;
+            if (i % 2 == 0) seen[n][i / 2] = 0;
+            if (far >= 0) seen[n][i / 2] |= i % 2 == 0 ? 0xFFFFu : 0xFFFF0000u;
+        }
+    const Weights weights(l, task.matrix_scale, REVERSE, kChunk);
 
     acc_t matrix[K];
-    const int column = wave * 32 + (lane & 31);
+    load_matrix<K>(matrix, task.carry, task.carry_factor, task.transposed, d, wave);
+    const int row_at = row_offset<T, W>(), swapped_at = swapped_offset<T, W>();
+    T* const out = task.out + static_cast<long>(b) * tokens * x_stride + static_cast<long>(head) * d;
+    auto add_what_is_there = [&](acc_t (&o)[2], const T* out, int row0, int length) {
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+        for (int t = 0; t < 2; ++t) {
+            const int place = t * 32 + (lane & 31);
+            if (place >= length) continue;
+            const T* from = out + (row0 + place) * x_stride;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int row = 32 * k + matrix_row(i);
-            matrix[k][i] = task.carry != nullptr && row < d && column < d ? task.carry[task.transposed ? column * d + row : row * d + column] * task.carry_factor : 0.0f;
-        }
-    bool empty = task.carry == nullptr;
-
-    const int chunks_in_all = (tokens + kChunk - 1) / kChunk;
-    const int first_chunk = segment * a.segment_chunks, last_chunk = min(first_chunk + a.segment_chunks, chunks_in_all) - 1;
-    const int steps = last_chunk - first_chunk + 1;
-    for (int step = 0; step < steps; ++step) {
-        const int row0 = (REVERSE ? last_chunk - step : first_chunk + step) * kChunk;
-        const int length = min(kChunk, tokens - row0);
-        acc_t o[2];
-        for (int each = 0; each < heads_each; ++each) {
-            __syncthreads();  // everybody has read the last tiles
-            const Rows<T> y{task.y + y_offset + static_cast<long>(each) * d, y_stride}, z{task.z + y_offset + static_cast<long>(each) * d, y_stride};
-            if (each == 0) load_tile<T, W, DIRECT>(x_tile, x, row0, tokens, d, a.vectors);
-            load_tile<T, W, DIRECT>(y_tile, y, row0, tokens, d, a.vectors);
-            load_tile<T, W, DIRECT>(z_tile, z, row0, tokens, d, a.vectors);
-            tiles_there();
-            // P' = (Y X') g^.., tile by tile.
-#pragma unroll
-            for (int n = 0; n < kTables; ++n) {
-                const int tile = my_tile(n);
-                if (tile > 2 || (n > 0 && wave > 0)) continue;
-                const int tt = tile_t(tile), tr = tile_r(tile);
-                acc_t p(0.0f);
-#pragma unroll
-                for (int s = 0; s < W / 16; ++s) p = multiply<T>(row_frag<T, W>(y_tile, tr * 32, s), row_frag<T, W>(x_tile, tt * 32, s), p);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) p[i] = apart(tile, i) >= 0 ? p[i] * table[n][i] : 0.0f;
-                if constexpr (kNarrow<T>) {
-                    float most = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(p[i]));
-                    const float scale = range_scale(wave_max(most), -3, 15);
-                    if (scale != 1.0f)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) p[i] *= scale;
-                    if (lane == 0) pair_scales[tile] = scale;
-                }
-#pragma unroll
-                for (int s = 0; s < 2; ++s) *reinterpret_cast<frag_t<T>*>(pairs_at<T>(pairs, tt * 32 + (lane & 31), 4 * tr + 2 * s + half)) = operand_of<T>(p, s);
+            for (int i = 0; i < 16; ++i) {
+                const int at = wave * 32 + acc_row(i);
+                if (at < d) o[t][i] += to_f32(from[at]);
             }
-            // What came before the chunk.
-            if (each == 0) {
-                o[0] = o[1] = acc_t(0.0f);
-                if (!empty) {
-                    float scale = 1.0f;
+        }
+    };
+    // A quarter of a chunk's output. Rows and columns that are not there lie behind the end of a buffer, where stores are dropped.
+    auto store_output = [&](int quarter, const acc_t (&o)[2], const acc_t (&within)[2], const float (&since)[2], T* out, int row0, int length)
+                            __attribute__((always_inline)) {
+        const int t = quarter / 2, g = quarter % 2 * 2, place = t * 32 + (lane & 31);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(o[t][4 * g + e], since[t], within[t][4 * g + e]);
+        T* first = out + row0 * x_stride;
+        if constexpr (STAGED) {
+            const __amdgpu_buffer_rsrc_t rsrc = buffer_of(first, static_cast<int>(((length - 1) * x_stride + d) * static_cast<long>(sizeof(T))));
+            // A lane has quads of its row's columns, its partner in the other half of the wavefront the quads between: swapped, each has eight in a
+            // row.
+            const int at = wave * 32 + 8 * (g + half), row = place * static_cast<int>(x_stride * sizeof(T));
+            vec_t<float, 8> all;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const auto swapped = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[e]), __float_as_uint(v[4 + e]), false, false);
+                all[e] = __uint_as_float(swapped[0]);
+                all[4 + e] = __uint_as_float(swapped[1]);
+            }
+            store_words(__builtin_bit_cast(vec_t<unsigned int, 4>, vec_from_f32<T, 8>(all)), rsrc, place < length && at < d ? row + at * 2 : 1 << 30);
+        } else {
+            if (place >= length) return;
+            T* to = first + place * x_stride;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int at = wave * 32 + 8 * (g + q) + 4 * half;
+                if (a.vectors) {
+                    if (at < d) store_vec<T, 4>(to + at, vec_from_f32<T, 4>(vec_t<float, 4>{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]}));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (at + e < d) to[at + e] = from_f32<T>(v[4 * q + e]);
+                }
+            }
+        }
+    };
+    int buffer = 0;
+#pragma unroll
+    for (int n = 0; n < 12; ++n) store_tiles(std::true_type{}, n, 0);
+    for (int step = 0; step < steps; ++step) {
+        const int row0 = row_of(step), length = min(kChunk, tokens - row0);
+        acc_t o[2], within[2];  // by what came before the chunk, and by its own tokens
+        float since[2];
+        for (int each = 0; each < heads_each; ++each) {
+            const T* y_tile = y_tiles + buffer * kTile<T, W>;
+            const bool last_each = each + 1 == heads_each;
+            T* const out_each = REVERSE ? out : out + static_cast<long>(each) * d;
+            __syncthreads();  // the tiles are there
+
+            // The next tiles are asked for (behind the last ones, those once more). P' = (Y X') g^.., tile by tile, and in a chunk's first round
+            // what came before it, C' X'.
+            turn_to(last_each ? min(step + 1, steps - 1) : step, last_each ? 0 : each + 1);
+            Values<T> values;
+            float matrix_scale = 1.0f, finite_sum;
+            if constexpr (kNarrow<T>)
+                if (!REVERSE || each == 0) matrix_scale = range_scale(largest_of(matrix), -3, 15);
+            const float passed = power(l, length);
+            // BEFORE: with what came before; DECAY: the matrix decays once it has been read; ALL: of the next tiles, not X alone.
+            auto scores = [&](auto before, auto decay, auto all) __attribute__((always_inline)) {
+                constexpr bool FIRST = decltype(before)::value, DECAY = decltype(decay)::value;
+                constexpr int STEPS = W / 16, AHEAD = 2;
+                const int at = anew(row_at);
+                frag_t<T> xs[AHEAD + 1][2], ys[AHEAD + 1][kTables], m[2];
+                acc_t p[kTables];
+                auto read = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) xs[s % (AHEAD + 1)][t] = row_frag<T, W>(x_tile, at, 32 * t, s);
+#pragma unroll
+                    for (int n = 0; n < kTables; ++n) ys[s % (AHEAD + 1)][n] = row_frag<T, W>(y_tile, at, tile_r(my_tile(n)) * 32, s);
+                };
+                auto operand = [&](int s) __attribute__((always_inline)) {
+                    if constexpr (FIRST) {
+                        acc_t from = matrix[s / 2];
+                        if constexpr (kNarrow<T>) from *= matrix_scale;
+                        m[s % 2] = operand_of<T>(from, s % 2);
+                    }
+                };
+                auto forget = [&](int s) __attribute__((always_inline)) {  // of what operand(s) has read
+                    if constexpr (DECAY)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) matrix[s / 2][8 * (s % 2) + e] *= passed;
+                };
+                auto load = [&](int s, int n) __attribute__((always_inline)) {
+                    constexpr int each = kTables + (FIRST ? 2 : 0);
+                    share_of(decltype(all)::value ? 12 : 4, s * each + n, STEPS * each, [&](int i) __attribute__((always_inline)) { fetch(all, i); });
+                };
+#pragma unroll
+                for (int s = 0; s < AHEAD; ++s) read(s);
+                operand(0);
+#pragma unroll
+                for (int n = 0; n < kTables; ++n) p[n] = acc_t(0.0f);
+                if constexpr (FIRST) o[0] = o[1] = acc_t(0.0f);
+                slot_end();
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) {
+                    if (s + AHEAD < STEPS) read(s + AHEAD);
+                    else values.template load<W>(z_tile, wave, 2 * (s + AHEAD - STEPS), 2);
+#pragma unroll
+                    for (int n = 0; n < kTables; ++n) {
+                        p[n] = multiply<T>(ys[s % (AHEAD + 1)][n], tile_t(my_tile(n)) == 0 ? xs[s % (AHEAD + 1)][0] : xs[s % (AHEAD + 1)][1], p[n]);
+                        load(s, n);
+                        slot_end();
+                    }
+                    if constexpr (FIRST) {
+                        o[0] = multiply<T>(m[s % 2], xs[s % (AHEAD + 1)][0], o[0]);
+                        if (s + 1 < STEPS) operand(s + 1);
+                        load(s, kTables);
+                        slot_end();
+                        o[1] = multiply<T>(m[s % 2], xs[s % (AHEAD + 1)][1], o[1]);
+                        forget(s);
+                        load(s, kTables + 1);
+                        slot_end();
+                    }
+                }
+                finite_sum = values.finite_sum();
+                // What the mask hides is 0 whatever the scores are.
+#pragma unroll
+                for (int n = 0; n < kTables; ++n) {
+                    const int tile = my_tile(n), tt = tile_t(tile), tr = tile_r(tile);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        if constexpr (__is_same(T, bf16_t)) {
+                            p[n][i] *= table[n][i];
+                        } else {
+                            float& weight = table[n][i];
+                            asm volatile("" : "+v"(weight));  // compared anew: no registers for sixteen masks
+                            p[n][i] = weight != 0.0f ? p[n][i] * weight : 0.0f;
+                        }
+                    }
                     if constexpr (kNarrow<T>) {
                         float most = 0.0f;
 #pragma unroll
-                        for (int k = 0; k < K; ++k)
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(matrix[k][i]));
-                        scale = range_scale(wave_max(most), -3, 15);
+                        for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(p[n][i]));
+                        const float scale = range_scale(wave_max(most), -3, 15);
+                        p[n] *= scale;
+                        pair_scales[tile] = scale;
                     }
 #pragma unroll
-                    for (int k = 0; k < K; ++k)
+                    for (int s = 0; s < 2; ++s) {
+                        frag_t<T> part = operand_of<T>(p[n], s);
+                        if constexpr (__is_same(T, bf16_t)) {
+                            auto words = __builtin_bit_cast(vec_t<unsigned int, 4>, part);
 #pragma unroll
-                        for (int s = 0; s < 2; ++s) {
-                            frag_t<T> m;
-                            if constexpr (kNarrow<T>) {
-                                acc_t scaled = matrix[k];
-                                if (scale != 1.0f) scaled *= scale;
-                                m = operand_of<T>(scaled, s);
-                            } else {
-                                m = operand_of<T>(matrix[k], s);
-                            }
-#pragma unroll
-                            for (int t = 0; t < 2; ++t) o[t] = multiply<T>(m, row_frag<T, W>(x_tile, 32 * t, 2 * k + s), o[t]);
+                            for (int w = 0; w < 4; ++w) words[w] &= seen[n][4 * s + w];
+                            part = __builtin_bit_cast(frag_t<T>, words);
                         }
-                    const float factor = task.out_scale / scale;
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const int place = t * 32 + (lane & 31);
-                        const float f = factor * power(l, max(REVERSE ? length - 1 - place : place, 0));
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[t][i] *= f;
+                        *reinterpret_cast<frag_t<T>*>(pairs_at<T>(pairs, tt * 32 + (lane & 31), 4 * tr + 2 * s + half)) = part;
                     }
                 }
+            };
+            constexpr std::true_type yes;
+            constexpr std::false_type no;
+            if constexpr (REVERSE) {
+                if (each == 0) scores(yes, yes, yes);
+                else scores(no, no, yes);
+            } else {
+                if (last_each) scores(yes, yes, yes);
+                else scores(yes, no, no);
             }
-            __syncthreads();  // all pairs are there
-            Values<T> values;
-            values.template load<W>(z_tile, wave);
-            if (values.finite()) {
+            if (!REVERSE || each == 0) {
+                const float factor = task.out_scale / matrix_scale;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int place = t * 32 + (lane & 31);
+                    since[t] = factor * power(l, max(REVERSE ? length - 1 - place : place, 0));
+                    within[t] = acc_t(0.0f);
+                }
+                if (a.accumulate) add_what_is_there(within, out_each, row0, length);
+            }
+            const bool finite = !__any(!(finite_sum == 0.0f));
+            const bool update = REVERSE || last_each;
+            const float up = update ? enlarge<T, K>(matrix, values) : 1.0f;
+            __syncthreads();  // all pairs are there, X and Z have been read
+            auto pair_frag = [&](int t, int r, int s) { return *reinterpret_cast<const frag_t<T>*>(pairs_at<T>(pairs, t * 32 + (lane & 31), 4 * r + 2 * s + half)); };
+            Values<T> shown = values;
+            if (!finite) {
+                // A pair that the mask hides is 0, but 0 x Inf is NaN in a product of tiles: token by token, for those that see it.
+#pragma unroll 1
+                for (int r = 0; r < kChunk; ++r)
+#pragma unroll
+                    for (int tile = 0; tile < 3; ++tile) {
+                        const int tt = tile_t(tile), tr = tile_r(tile);
+                        if ((r >> 5) != tr) continue;
+                        float scale = 1.0f;
+                        if constexpr (kNarrow<T>) scale = 1.0f / pair_scales[tile];
+                        const int place = tt * 32 + (lane & 31);
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) {
+                            if (((r >> 4) & 1) != s) continue;
+                            frag_t<T> one = values.z[2 * tr + s];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (Weights::row(e) != (r & 15)) one[e] = static_cast<T>(0.0f);
+                            const acc_t term = multiply<T>(one, pair_frag(tt, tr, s), acc_t(0.0f));
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) within[tt][i] = (REVERSE ? r >= place : r <= place) ? fmaf(term[i], scale, within[tt][i]) : within[tt][i];
+                        }
+                    }
+#pragma unroll
+                for (int s = 0; s < 4; ++s) shown.z[s] = frag_t<T>(static_cast<T>(0.0f));
+            }
+            frag_t<T> seen_pairs[3][2];
+#pragma unroll
+            for (int tile = 0; tile < 3; ++tile)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) seen_pairs[tile][s] = pair_frag(tile_t(tile), tile_r(tile), s);
+            auto add_pairs = [&](auto&& between) __attribute__((always_inline)) {
 #pragma unroll
                 for (int tile = 0; tile < 3; ++tile) {
                     const int tt = tile_t(tile), tr = tile_r(tile);
                     float scale = 1.0f;
                     if constexpr (kNarrow<T>) {
                         scale = pair_scales[tile];
-                        if (scale != 1.0f) o[tt] *= scale;
+                        if (scale != 1.0f) within[tt] *= scale;
                     }
 #pragma unroll
-                    for (int s = 0; s < 2; ++s)
-                        o[tt] = multiply<T>(values.z[2 * tr + s], *reinterpret_cast<const frag_t<T>*>(pairs_at<T>(pairs, tt * 32 + (lane & 31), 4 * tr + 2 * s + half)), o[tt]);
+                    for (int s = 0; s < 2; ++s) {
+                        within[tt] = multiply<T>(shown.z[2 * tr + s], seen_pairs[tile][s], within[tt]);
+                        between(2 * tile + s);
+                        slot_end();
+                    }
                     if constexpr (kNarrow<T>)
-                        if (scale != 1.0f) o[tt] *= 1.0f / scale;
+                        if (scale != 1.0f) within[tt] *= 1.0f / scale;
                 }
-            } else {
-                // A pair that the mask hides is 0, but 0 x Inf is NaN in a product of tiles.
-                for (int r = 0; r < kChunk; ++r)
+            };
+            if (!update) {
+                add_pairs([&](int i) __attribute__((always_inline)) { share_of(4, i, 6, [&](int n) __attribute__((always_inline)) { store_tiles(no, n, buffer); }); });
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const int place = t * 32 + (lane & 31), in_block = r & 15;
-                        const bool seen = REVERSE ? r >= place : r <= place;
-                        if (!seen) continue;
-                        const int c = 2 * (r >> 4) + ((in_block >> 2) & 1), e = (in_block & 3) + 4 * (in_block >> 3);
-                        float p = to_f32(pairs_at<T>(pairs, place, c)[e]);
-                        if constexpr (kNarrow<T>) p *= 1.0f / pair_scales[(r >> 5) == t ? t : 2];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int at = wave * 32 + acc_row(i);
-                            T value;
-                            if constexpr (sizeof(T) == 2) value = z_tile[r * W + (((at >> 3) ^ swizzle<W>(r)) * 8) + (at & 7)];
-                            else value = z_tile[r * kPitch<T, W> + at];
-                            o[t][i] = fmaf(p, to_f32(value), o[t][i]);
-                        }
-                    }
+                for (int g = 0; g < 4; ++g) store_output(g, o, within, since, out_each, row0, length);
+                continue;
             }
-            if (step + 1 < steps) update_matrix<T, W, false>(matrix, each == 0 ? power(l, length) : 1.0f, y_tile, values, weights, kChunk);
-        }
-        empty = false;
+            Weighted<T, 2> weighted[2];
+            frag_t<T> rows[2][K];
+            const int swapped = anew(swapped_at);
+            read_rows_of<T, W>(rows[0], y_tile, swapped, 0);
+            slot_end();
+            add_pairs([&](int i) __attribute__((always_inline)) {
+                share_of(8, i, 6, [&](int n) __attribute__((always_inline)) { weighted[0].step(n, values.z[0], weights.w[0], up); });
+            });
+            buffer ^= 1;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int place = t * 32 + (lane & 31);
-            if (place >= length) continue;
-            T* to = task.out + static_cast<long>(b) * tokens * x_stride + static_cast<long>(row0 + place) * x_stride + static_cast<long>(head) * d;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int at = wave * 32 + 8 * g + 4 * half;
-                vec_t<float, 4> v{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]};
-                if (a.vectors) {
-                    if (at < d) {
-                        if (a.accumulate) v += vec_to_f32<T, 4>(load_vec<T, 4>(to + at));
-                        store_vec<T, 4>(to + at, vec_from_f32<T, 4>(v));
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (at + e < d) to[at + e] = from_f32<T>(a.accumulate ? v[e] + to_f32(to[at + e]) : v[e]);
-                }
+            for (int s = 0; s < 4; ++s) {
+                if (s < 3) read_rows_of<T, W>(rows[(s + 1) % 2], y_tile, swapped, s + 1);
+                add_rows<T, K, 2>(matrix, rows[s % 2], weighted[s % 2], [&](int i, int count) __attribute__((always_inline)) {
+                    if (s < 3)
+                        share_of(8, i, count, [&](int n) __attribute__((always_inline)) { weighted[(s + 1) % 2].step(n, values.z[s + 1], weights.w[s + 1], up); });
+                    if (s >= 1)
+                        share_of(12, (s - 1) * count + i, 3 * count, [&](int n) __attribute__((always_inline)) { store_tiles(yes, n, buffer); });
+                    if constexpr (!REVERSE)
+                        if (s == 3)
+                            share_of(4, i, count, [&](int n) __attribute__((always_inline)) { store_output(n, o, within, since, out_each, row0, length); });
+                });
             }
+            bring_back<T, K>(matrix, up);
         }
+        if constexpr (REVERSE)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) store_output(g, o, within, since, out, row0, length);
     }
 }
 
@@ -526,10 +781,110 @@ __device__ __forceinline__ const float* carry_of(const float* stored, const floa
     return given != nullptr ? given + pair * matrix : nullptr;
 }
 
-template <typename T, int W, bool DIRECT>
-__global__ __launch_bounds__(W * 2, 2) void linear_forward_kernel(LinearArgs a) {
-    const int group = a.hq / a.hkv;
-    const Unit u = unit_of(blockIdx.x, group, gridDim.x / group, a.segments);
+// A segment's own matrix: what its tokens leave to those behind it (k v') or, reverse, before it (q dO' of the group's heads). The last one's goes
+// to `after` as its last token sees it, the first one's to d_before, each where the caller asked for it; a sequence's only one with what is passed
+// on through it.
+template <typename T, int W, bool STAGED>
+__device__ __forceinline__ void sum_segment(const LinearArgs& a, bool reverse, int pair, int segment, T* lds) {
+    constexpr int K = W / 32;
+    const int b = pair / a.hkv, kv = pair % a.hkv, d = a.d, tokens = a.tokens;
+    const bool outermost = segment == (reverse ? 0 : a.segments - 1);
+    const long matrix_size = static_cast<long>(d) * d;
+    float* to = reverse ? a.behind : a.ahead;
+    if (outermost) {
+        to = reverse ? a.d_before : a.after;
+        if (to == nullptr) return;
+        to += pair * matrix_size;
+    } else {
+        to += (static_cast<long>(pair) * a.segments + segment) * matrix_size;
+    }
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const float l = log2_decay(a.log_decay[kv]);
+    Weights weights(l, reverse ? a.scale : 1.0f, reverse, kChunk);
+    const int heads = reverse ? a.hq : a.hkv, heads_each = reverse ? a.hq / a.hkv : 1;
+    const long stride = static_cast<long>(heads) * d;
+    const T* y_base = static_cast<const T*>(reverse ? a.q : a.k) + static_cast<long>(b) * tokens * stride + static_cast<long>(kv) * heads_each * d;
+    const T* z_base = static_cast<const T*>(reverse ? a.dout : a.v) + static_cast<long>(b) * tokens * stride + static_cast<long>(kv) * heads_each * d;
+
+    acc_t matrix[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) matrix[k] = acc_t(0.0f);
+    const int first_chunk = segment * a.segment_chunks, last_chunk = min(first_chunk + a.segment_chunks, (tokens + kChunk - 1) / kChunk) - 1;
+    const int steps = (last_chunk - first_chunk + 1) * heads_each;  // a chunk's heads one after the other
+    auto row_of = [&](int step) { return (reverse ? last_chunk - step / heads_each : first_chunk + step / heads_each) * kChunk; };
+    Incoming<T, W, STAGED> in_y(stride, d), in_z(stride, d);
+    auto turn_to = [&](int step) __attribute__((always_inline)) {
+        const long along = static_cast<long>(step % heads_each) * d;
+        in_y.set(Rows<T>{y_base + along, stride}, row_of(step), tokens, d);
+        in_z.set(Rows<T>{z_base + along, stride}, row_of(step), tokens, d);
+    };
+    auto fetch = [&](int i) __attribute__((always_inline)) {
+        in_y.fetch(i);
+        in_z.fetch(i);
+    };
+    auto store_tiles = [&](int i, int step) __attribute__((always_inline)) {
+        T* tiles = lds + (step & 1) * 2 * kTile<T, W>;
+        in_y.store(i, tiles, tokens, d, a.vectors);
+        in_z.store(i, tiles + kTile<T, W>, tokens, d, a.vectors);
+    };
+    const int swapped_at = swapped_offset<T, W>();
+    turn_to(0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) fetch(i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) store_tiles(i, 0);
+    for (int step = 0; step < steps; ++step) {
+        const T* tiles = lds + (step & 1) * 2 * kTile<T, W>;
+        const int row0 = row_of(step), length = min(kChunk, tokens - row0);
+        const int end = outermost && !reverse && row0 + kChunk >= tokens ? length - 1 : length;  // the token that sees weight 1
+        __syncthreads();  // the tiles are there
+        turn_to(min(step + 1, steps - 1));  // (behind the last ones, those once more)
+        Values<T> values;
+        frag_t<T> rows[2][K];
+        Weighted<T, 3> weighted[2];
+        const int swapped = anew(swapped_at);
+        values.template load<W>(tiles + kTile<T, W>, wave);
+        read_rows_of<T, W>(rows[0], tiles, swapped, 0);
+        if (step % heads_each == 0) {
+            const float passed = power(l, end);
+#pragma unroll
+            for (int k = 0; k < K; ++k) matrix[k] *= passed;
+        }
+        if (!reverse && end != kChunk) weights = Weights(l, 1.0f, false, end);
+        const float up = enlarge<T, K>(matrix, values);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) weighted[0].step(i, values.z[0], weights.w[0], up);
+        slot_end();
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            if (s < 3) read_rows_of<T, W>(rows[(s + 1) % 2], tiles, swapped, s + 1);
+            add_rows<T, K, 3>(matrix, rows[s % 2], weighted[s % 2], [&](int i, int count) __attribute__((always_inline)) {
+                if (s == 0) share_of(4, i, count, fetch);
+                if (s < 3) share_of(8, i, count, [&](int n) __attribute__((always_inline)) { weighted[(s + 1) % 2].step(n, values.z[s + 1], weights.w[s + 1], up); });
+                if (s == 3) share_of(4, i, count, [&](int n) __attribute__((always_inline)) { store_tiles(n, step + 1); });
+            });
+        }
+        bring_back<T, K>(matrix, up);
+    }
+    const int column = wave * 32 + (lane & 31);
+    const float* given = a.segments > 1 ? nullptr : reverse ? a.d_after : a.before;
+    if (given != nullptr) given += pair * matrix_size;
+    const float passed = power(l, tokens);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int row = 32 * k + matrix_row(i);
+            if (row < d && column < d) to[row * d + column] = given != nullptr ? fmaf(given[row * d + column], passed, matrix[k][i]) : matrix[k][i];
+        }
+}
+
+// The outputs; behind them, where a sequence is one segment, the last states.
+template <typename T, int W, bool STAGED>
+__global__ __launch_bounds__(W * 2, 1) void linear_forward_kernel(LinearArgs a) {
+    const unsigned int group = a.hq / a.hkv, members = group / a.heads_each, units = a.batch * a.hkv * a.segments;
+    if (blockIdx.x >= units * members) return sum_segment<T, W, STAGED>(a, false, static_cast<int>(blockIdx.x - units * members), 0, shared_memory<T>());
+    const Unit u = unit_of(blockIdx.x, members, units, a.segments);
     const int b = u.pair / a.hkv, kv = u.pair % a.hkv;
     Task<T> task;
     task.x = static_cast<const T*>(a.q);
@@ -544,13 +899,15 @@ __global__ __launch_bounds__(W * 2, 2) void linear_forward_kernel(LinearArgs a) 
     task.pair_scale = a.scale;
     task.matrix_scale = 1.0f;
     task.out_scale = a.scale;
-    walk_segment<T, W, false, DIRECT>(a, task, b, kv * group + u.member, u.segment, shared_memory<T>());
+    walk_segment<T, W, false, STAGED>(a, task, b, kv * static_cast<int>(group) + u.member * a.heads_each, u.segment, shared_memory<T>());
 }
 
-// dk and dv of all units first, whose walks are as many times longer as a group has heads, then dq.
-template <typename T, int W, bool DIRECT>
-__global__ __launch_bounds__(W * 2, 2) void linear_backward_kernel(LinearArgs a) {
-    const unsigned int group = a.hq / a.hkv, units = gridDim.x / (group + 2);
+// dk and dv of all units first, whose walks are as many times longer as a group has heads, then dq; behind them, where a sequence is one segment, the
+// gradients of the first states.
+template <typename T, int W, bool STAGED>
+__global__ __launch_bounds__(W * 2, 1) void linear_backward_kernel(LinearArgs a) {
+    const unsigned int group = a.hq / a.hkv, members = group / a.heads_each, units = a.batch * a.hkv * a.segments;
+    if (blockIdx.x >= units * (members + 2)) return sum_segment<T, W, STAGED>(a, true, static_cast<int>(blockIdx.x - units * (members + 2)), 0, shared_memory<T>());
     Task<T> task;
     const T *q = static_cast<const T*>(a.q), *k = static_cast<const T*>(a.k), *v = static_cast<const T*>(a.v), *dout = static_cast<const T*>(a.dout);
     if (blockIdx.x < 2 * units) {
@@ -567,9 +924,9 @@ __global__ __launch_bounds__(W * 2, 2) void linear_backward_kernel(LinearArgs a)
         task.transposed = dk;
         task.pair_scale = task.matrix_scale = a.scale;
         task.out_scale = 1.0f;
-        walk_segment<T, W, true, DIRECT>(a, task, u.pair / a.hkv, u.pair % a.hkv, u.segment, shared_memory<T>());
+        walk_segment<T, W, true, STAGED>(a, task, u.pair / a.hkv, u.pair % a.hkv, u.segment, shared_memory<T>());
     } else {
-        const Unit u = unit_of(blockIdx.x - 2 * units, group, units, a.segments);
+        const Unit u = unit_of(blockIdx.x - 2 * units, members, units, a.segments);
         const int kv = u.pair % a.hkv;
         task.x = dout;
         task.y = v;
@@ -583,70 +940,20 @@ __global__ __launch_bounds__(W * 2, 2) void linear_backward_kernel(LinearArgs a)
         task.pair_scale = a.scale;
         task.matrix_scale = 1.0f;
         task.out_scale = a.scale;
-        walk_segment<T, W, false, DIRECT>(a, task, u.pair / a.hkv, kv * static_cast<int>(group) + u.member, u.segment, shared_memory<T>());
+        walk_segment<T, W, false, STAGED>(a, task, u.pair / a.hkv, kv * static_cast<int>(group) + u.member * a.heads_each, u.segment, shared_memory<T>());
     }
 }
 
-// Every segment's own matrix: what its tokens leave to those behind it (blockIdx.y = 0: k v') or before it (1: q dO' of the group's heads). The
-// last one's goes to `after` as its last token sees it, the first one's to d_before; each where the caller asked for it.
-template <typename T, int W, bool DIRECT>
-__global__ __launch_bounds__(W * 2, 2) void linear_segments_kernel(LinearArgs a, int first_part) {
-    constexpr int K = W / 32;
-    T* lds = shared_memory<T>();
-    T *y_tile = lds, *z_tile = lds + kTile<T, W>;
-    const bool reverse = first_part + blockIdx.y == 1;
-    const int pair = static_cast<int>(blockIdx.x / a.segments), segment = static_cast<int>(blockIdx.x % a.segments);
-    const int b = pair / a.hkv, kv = pair % a.hkv, d = a.d, tokens = a.tokens;
-    const bool outermost = segment == (reverse ? 0 : a.segments - 1);
-    const long matrix_size = static_cast<long>(d) * d;
-    float* to = reverse ? a.behind : a.ahead;
-    if (outermost) {
-        to = reverse ? a.d_before : a.after;
-        if (to == nullptr) return;
-        to += pair * matrix_size;
-    } else {
-        to += (static_cast<long>(pair) * a.segments + segment) * matrix_size;
-    }
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const float l = log2_decay(a.log_decay[kv]);
-    const Weights weights(l, reverse ? a.scale : 1.0f, reverse);
-    const int heads = reverse ? a.hq : a.hkv, heads_each = reverse ? a.hq / a.hkv : 1;
-    const long stride = static_cast<long>(heads) * d;
-    const T* y_base = static_cast<const T*>(reverse ? a.q : a.k) + static_cast<long>(b) * tokens * stride + static_cast<long>(kv) * heads_each * d;
-    const T* z_base = static_cast<const T*>(reverse ? a.dout : a.v) + static_cast<long>(b) * tokens * stride + static_cast<long>(kv) * heads_each * d;
-
-    acc_t matrix[K];
-#pragma unroll
-    for (int k = 0; k < K; ++k) matrix[k] = acc_t(0.0f);
-    const int first_chunk = segment * a.segment_chunks, last_chunk = min(first_chunk + a.segment_chunks, (tokens + kChunk - 1) / kChunk) - 1;
-    for (int step = 0; step <= last_chunk - first_chunk; ++step) {
-        const int row0 = (reverse ? last_chunk - step : first_chunk + step) * kChunk;
-        const int length = min(kChunk, tokens - row0);
-        const int end = outermost && !reverse && row0 + kChunk >= tokens ? length - 1 : length;  // the token that sees weight 1
-        for (int each = 0; each < heads_each; ++each) {
-            __syncthreads();
-            load_tile<T, W, DIRECT>(y_tile, Rows<T>{y_base + static_cast<long>(each) * d, stride}, row0, tokens, d, a.vectors);
-            load_tile<T, W, DIRECT>(z_tile, Rows<T>{z_base + static_cast<long>(each) * d, stride}, row0, tokens, d, a.vectors);
-            tiles_there();
-            Values<T> values;
-            values.template load<W>(z_tile, wave);
-            update_matrix<T, W, true>(matrix, each == 0 ? power(l, end) : 1.0f, y_tile, values, weights, end);
-        }
-    }
-    const int column = wave * 32 + (lane & 31);
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int row = 32 * k + matrix_row(i);
-            if (row < d && column < d) to[row * d + column] = matrix[k][i];
-        }
+// Every segment's own matrix; blockIdx.y = 1: reverse.
+template <typename T, int W, bool STAGED>
+__global__ __launch_bounds__(W * 2, 2) void linear_segments_kernel(LinearArgs a) {
+    sum_segment<T, W, STAGED>(a, blockIdx.y == 1, static_cast<int>(blockIdx.x / a.segments), static_cast<int>(blockIdx.x % a.segments), shared_memory<T>());
 }
 
 // The segments' matrices become what comes before each (blockIdx.y = 0) or behind it (1), in order along the sequence, a thread an element.
 constexpr int kAhead = 8;  // loads in flight
-__global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a, int first_part) {
-    const bool reverse = first_part + blockIdx.y == 1;
+__global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a) {
+    const bool reverse = blockIdx.y == 1;
     const long matrix = static_cast<long>(a.d) * a.d, at = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;
     if (at >= matrix * a.batch * a.hkv) return;
     const long pair = at / matrix, element = at - pair * matrix;
@@ -655,26 +962,24 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a, int firs
     float* result = reverse ? a.d_before : a.after;
     float running = given != nullptr ? given[at] * (reverse ? 1.0f : power(l, 1)) : 0.0f;
     const int n = a.segments, whole = a.segment_chunks * kChunk, last = a.tokens - (n - 1) * whole;  // tokens of the last segment
-    if (n > 1) {
-        float* slots = (reverse ? a.behind : a.ahead) + pair * n * matrix + element;
-        for (int j0 = 0; j0 < n; j0 += kAhead) {
-            float own[kAhead];
+    float* slots = (reverse ? a.behind : a.ahead) + pair * n * matrix + element;
+    for (int j0 = 0; j0 < n; j0 += kAhead) {
+        float own[kAhead];
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                const int place = j0 + j;
-                own[j] = place < n - 1 ? slots[static_cast<long>(reverse ? n - 1 - place : place) * matrix] : 0.0f;
-            }
+        for (int j = 0; j < kAhead; ++j) {
+            const int place = j0 + j;
+            own[j] = place < n - 1 ? slots[static_cast<long>(reverse ? n - 1 - place : place) * matrix] : 0.0f;
+        }
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                const int place = j0 + j;
-                if (place >= n) break;
-                const int segment = reverse ? n - 1 - place : place;
-                slots[static_cast<long>(segment) * matrix] = running;
-                if (place < n - 1) running = fmaf(running, power(l, segment == n - 1 ? last : whole), own[j]);
-            }
+        for (int j = 0; j < kAhead; ++j) {
+            const int place = j0 + j;
+            if (place >= n) break;
+            const int segment = reverse ? n - 1 - place : place;
+            slots[static_cast<long>(segment) * matrix] = running;
+            if (place < n - 1) running = fmaf(running, power(l, segment == n - 1 ? last : whole), own[j]);
         }
     }
-    if (result != nullptr) result[at] = fmaf(running, power(l, reverse ? (n == 1 ? last : whole) : last - 1), result[at]);
+    if (result != nullptr) result[at] = fmaf(running, power(l, reverse ? whole : last - 1), result[at]);
 }
 
 // ------------------------------------------------------------------------------------------------ one token
@@ -799,19 +1104,30 @@ LinearArgs make_args(const Shape& s, const void* q, const void* k, const void* v
     return a;
 }
 
-// Segments for `walks` workgroups in each, of whole chunks: as many as keep every compute unit busy twice over.
-void cut(LinearArgs& a, long walks, int most) {
-    const int chunks = (a.tokens + kChunk - 1) / kChunk;
-    const long wanted = std::max<long>(1, (2L * compute_units() + walks - 1) / walks);
-    const int segments = static_cast<int>(std::min<long>({wanted, static_cast<long>((chunks + 3) / 4), static_cast<long>(most)}));
+// Cuts the sequences into at most `most` segments of whole chunks, and says how many of a group's query heads a workgroup takes one after the other.
+// Walks that give three compute units of four work are not cut: two segments each would need their matrices first (32 sequences of 1024 tokens,
+// 8 query and 2 kv heads of 128: 58 us forward and 168 backward, cut in two 93 and 223). Then every query head has a workgroup of its own;
+// where sequences have to be cut, a group's heads share what is done for k and v (58 and 168 us against 70 and 198 for that batch in four segments), unless
+// that leaves units without work. Segments are two chunks or longer (2 sequences of 333 fp32 tokens, 4 heads of 40: 52 us, four chunks or longer 69), two
+// a unit where the tokens allow it (32768 tokens, 12 and 4 heads of 64: 71 and 142 us, one a unit 76 and 151).
+void cut(LinearArgs& a, int most) {
+    const int chunks = (a.tokens + kChunk - 1) / kChunk, group = a.hq / a.hkv;
+    const long pairs = static_cast<long>(a.batch) * a.hkv, units = compute_units();
+    auto fills = [&](long walks) { return walks * 4 >= units * 3; };
+    auto segments_for = [&](long walks) {
+        if (fills(walks)) return 1;
+        return static_cast<int>(std::min<long>({(2 * units + walks - 1) / walks, static_cast<long>((chunks + 1) / 2), static_cast<long>(most)}));
+    };
+    a.heads_each = !fills(pairs * group) && fills(pairs * segments_for(pairs)) ? group : 1;
+    const int segments = segments_for(pairs * (group / a.heads_each));
     a.segment_chunks = (chunks + segments - 1) / segments;
     a.segments = (chunks + a.segment_chunks - 1) / a.segment_chunks;
 }
 
 template <typename T, int W>
-constexpr int kWalkBytes = (3 * kTile<T, W> + kChunk * kPairsPitch<T>) * static_cast<int>(sizeof(T));
+constexpr int kWalkBytes = (4 * kTile<T, W> + kChunk * kPairsPitch<T>) * static_cast<int>(sizeof(T));
 template <typename T, int W>
-constexpr int kSegmentBytes = 2 * kTile<T, W> * static_cast<int>(sizeof(T));
+constexpr int kSegmentBytes = 4 * kTile<T, W> * static_cast<int>(sizeof(T));
 
 template <auto Kernel>
 int allow_shared(int bytes) {
@@ -820,38 +1136,37 @@ int allow_shared(int bytes) {
     return check_hip(once, "hipFuncSetAttribute");
 }
 
-template <typename T, int W, bool DIRECT>
+template <typename T, int W, bool STAGED>
 int run(LinearArgs& a, bool backward, hipStream_t stream) {
     const long pairs = static_cast<long>(a.batch) * a.hkv;
-    const int group = a.hq / a.hkv, parts = backward ? 2 : 1;
+    const int parts = backward ? 2 : 1;
     const std::size_t slots = static_cast<std::size_t>(pairs) * a.d * a.d;
-    cut(a, pairs * group, 1 << 20);
+    cut(a, 1 << 20);
     // Segments need scratch; a call that cannot have it all takes fewer, one sequence a walk with none.
     if (a.segments > 1) {
         void* memory = nullptr;
         std::size_t held = 0;
         auto wanted = [&] { return static_cast<std::size_t>(parts) * a.segments * slots * sizeof(float); };
         if (int st = scratch_up_to(stream, wanted(), &memory, &held)) return st;
-        while (a.segments > 1 && held < wanted()) cut(a, pairs * group, a.segments - 1);
+        while (a.segments > 1 && held < wanted()) cut(a, a.segments - 1);
         a.ahead = static_cast<float*>(memory);
         a.behind = a.ahead + a.segments * slots;
     }
-    const bool first = a.segments > 1 || a.after != nullptr, second = backward && (a.segments > 1 || a.d_before != nullptr);
-    const int first_part = first ? 0 : 1, count = (first ? 1 : 0) + (second ? 1 : 0);
-    if (count > 0) {
-        if (int st = allow_shared<linear_segments_kernel<T, W, DIRECT>>(kSegmentBytes<T, W>)) return st;
-        hipLaunchKernelGGL((linear_segments_kernel<T, W, DIRECT>), dim3(static_cast<unsigned int>(pairs * a.segments), count), dim3(W * 2), (kSegmentBytes<T, W>), stream, a, first_part);
+    if (a.segments > 1) {
+        if (int st = allow_shared<linear_segments_kernel<T, W, STAGED>>(kSegmentBytes<T, W>)) return st;
+        hipLaunchKernelGGL((linear_segments_kernel<T, W, STAGED>), dim3(static_cast<unsigned int>(pairs * a.segments), parts), dim3(W * 2), (kSegmentBytes<T, W>), stream, a);
         CGPTX_LAUNCH_CHECK();
-        hipLaunchKernelGGL(linear_join_kernel, dim3(static_cast<unsigned int>((slots + 255) / 256), count), dim3(256), 0, stream, a, first_part);
+        hipLaunchKernelGGL(linear_join_kernel, dim3(static_cast<unsigned int>((slots + 255) / 256), parts), dim3(256), 0, stream, a);
         CGPTX_LAUNCH_CHECK();
     }
-    const long units = pairs * a.segments;
+    const bool state_too = a.segments == 1 && (backward ? a.d_before : a.after) != nullptr;
+    const long units = pairs * a.segments, members = a.hq / a.hkv / a.heads_each, states = state_too ? pairs : 0;
     if (backward) {
-        if (int st = allow_shared<linear_backward_kernel<T, W, DIRECT>>(kWalkBytes<T, W>)) return st;
-        hipLaunchKernelGGL((linear_backward_kernel<T, W, DIRECT>), dim3(static_cast<unsigned int>(units * (group + 2))), dim3(W * 2), (kWalkBytes<T, W>), stream, a);
+        if (int st = allow_shared<linear_backward_kernel<T, W, STAGED>>(kWalkBytes<T, W>)) return st;
+        hipLaunchKernelGGL((linear_backward_kernel<T, W, STAGED>), dim3(static_cast<unsigned int>(units * (members + 2) + states)), dim3(W * 2), (kWalkBytes<T, W>), stream, a);
     } else {
-        if (int st = allow_shared<linear_forward_kernel<T, W, DIRECT>>(kWalkBytes<T, W>)) return st;
-        hipLaunchKernelGGL((linear_forward_kernel<T, W, DIRECT>), dim3(static_cast<unsigned int>(units * group)), dim3(W * 2), (kWalkBytes<T, W>), stream, a);
+        if (int st = allow_shared<linear_forward_kernel<T, W, STAGED>>(kWalkBytes<T, W>)) return st;
+        hipLaunchKernelGGL((linear_forward_kernel<T, W, STAGED>), dim3(static_cast<unsigned int>(units * members + states)), dim3(W * 2), (kWalkBytes<T, W>), stream, a);
     }
     CGPTX_LAUNCH_CHECK();
     return CGPTX_OK;
@@ -859,12 +1174,10 @@ int run(LinearArgs& a, bool backward, hipStream_t stream) {
 
 int run_any(LinearArgs& a, bool backward, bool on_boundaries, int dtype, hipStream_t stream) {
     return dispatch_dtype(dtype, [&]<typename T>() -> int {
-        a.vectors = on_boundaries && a.d % kVec128<T> == 0;
-        if constexpr (sizeof(T) == 2) {
-            // 32 bits hold every offset in a chunk.
-            if (a.vectors && static_cast<long>(a.hq) * a.d * kChunk * 2 < (1L << 30))
-                return a.d <= 64 ? run<T, 64, true>(a, backward, stream) : run<T, 128, true>(a, backward, stream);
-        }
+        // 32 bits hold every offset in a chunk.
+        a.vectors = on_boundaries && a.d % kVec128<T> == 0 && static_cast<std::size_t>(a.hq) * a.d * kChunk * sizeof(T) < (std::size_t{1} << 30);
+        if constexpr (sizeof(T) == 2)
+            if (a.vectors) return a.d <= 64 ? run<T, 64, true>(a, backward, stream) : run<T, 128, true>(a, backward, stream);
         return a.d <= 64 ? run<T, 64, false>(a, backward, stream) : run<T, 128, false>(a, backward, stream);
     });
 }
