@@ -12,6 +12,7 @@
 // u and gate are constant over the rows of a gate, so one sum of G f rf stands for both their gradients. Workgroups have rows of one gate as
 // a rule (BY_BLOCK); where there are so many gates that most would have few rows, a row's lanes take whole gates one after the other
 // (BY_SLOT), and write the gate's gradient themselves. Per-workgroup partial sums go to scratch and a second launch adds them in a fixed order.
+// 32768 bfloat16 rows of 1024: forward 268 MB in 49 us (5.5 TB/s), backward with 32 gates 403 MB in 84 (4.8 TB/s), of which the second launch 5.
 #include "common.hpp"
 #include "reduce.hpp"
 #include "row_vectors.hpp"
@@ -22,6 +23,14 @@
 
 namespace cgptx {
 namespace {
+
+// Rows are stored past the caches, which keep what other workgroups are about to read (bfloat16, 2048 rows of 4096: backward 30 -> 25 us; fp32, 5005
+// rows of 1001: forward 21 -> 16, backward 43 -> 41).
+template <typename T>
+__device__ __forceinline__ void store_past(T* p, vec_t<T, kVec128<T>> v, int count) {
+    if (count >= kVec128<T>) __builtin_nontemporal_store(v, reinterpret_cast<typename Unaligned<T>::type*>(p));
+    else store_some<T>(p, v, count);
+}
 
 struct Sizes {
     int rows, hidden;
@@ -144,7 +153,7 @@ __global__ __launch_bounds__(kThreadsOf<WAVES>) void sandwich_forward_kernel(T* 
             const F stored = vec_to_f32<T, VEC>(out[c]);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) stream_squares[0] = fmaf(stored[e], stored[e], stream_squares[0]);
-            if (live) store_some<T>(stream + base + at.column(c), out[c], count[c]);
+            if (live) store_past<T>(stream + base + at.column(c), out[c], count[c]);
         }
         row_sums<LPR, WAVES>(stream_squares, stage + 1);
         const float rs = 1.0f / sqrtf(stream_squares[0] * s.inv_hidden + s.eps);
@@ -154,7 +163,7 @@ __global__ __launch_bounds__(kThreadsOf<WAVES>) void sandwich_forward_kernel(T* 
             F v;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[e] = stored[e] * rs * w[e];
-            if (live) store_some<T>(normed + base + at.column(c), vec_from_f32<T, VEC>(v), count[c]);
+            if (live) store_past<T>(normed + base + at.column(c), vec_from_f32<T, VEC>(v), count[c]);
         }
         walk = following;
         if constexpr (AHEAD) now = next;
@@ -261,8 +270,8 @@ __global__ __launch_bounds__(kThreadsOf<WAVES>) void sandwich_backward_kernel(Ou
                 of_f[e] = rf * fmaf(-fv[e] * rf, branch_mean, by[e] * u[e] * g[c][e]);
             }
             if (live) {
-                store_some<T>(dx + base + at.column(c), vec_from_f32<T, VEC>(of_x), count[c]);
-                store_some<T>(df + base + at.column(c), vec_from_f32<T, VEC>(of_f), count[c]);
+                store_past<T>(dx + base + at.column(c), vec_from_f32<T, VEC>(of_x), count[c]);
+                store_past<T>(df + base + at.column(c), vec_from_f32<T, VEC>(of_f), count[c]);
             }
         }
         if constexpr (BY_SLOT) {
