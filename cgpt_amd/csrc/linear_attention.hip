@@ -212,22 +212,29 @@ __device__ __forceinline__ float log2_decay(float log_decay) {
 }
 __device__ __forceinline__ float power(float l, int n) { return __builtin_amdgcn_exp2f(l * static_cast<float>(n)); }
 
-template <typename V>
-__device__ __forceinline__ float finite_test(const V& f, float sum) {  // stays 0 while all is finite
-    if constexpr (sizeof(f[0]) == 2) {
-        using T = std::remove_cv_t<std::remove_reference_t<decltype(f[0])>>;
-        const auto words = __builtin_bit_cast(vec_t<unsigned int, 4>, f);
+// The largest magnitude's bits of what passed, two halves of a word each for 16-bit storage: whether all is finite. (A dot product with zeros is one
+// instruction a word, but does not turn every NaN or Inf into a NaN.)
+template <typename T>
+struct Largest {
+    unsigned int bits = 0;
+    __device__ __forceinline__ void take(const frag_t<T>& f) {
+        constexpr int kWords = 8 * sizeof(T) / 4;
+        const auto words = __builtin_bit_cast(vec_t<unsigned int, kWords>, f);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            if constexpr (__is_same(T, f16_t)) sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(vec_t<f16_t, 2>, words[w]), vec_t<f16_t, 2>(static_cast<f16_t>(0.0f)), sum, false);
-            else sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(vec_t<bf16_t, 2>, words[w]), vec_t<bf16_t, 2>(static_cast<bf16_t>(0.0f)), sum, false);
+        for (int w = 0; w < kWords; ++w) {
+            if constexpr (sizeof(T) == 4) {
+                bits = max(bits, words[w] & 0x7FFFFFFFu);
+            } else {
+                using Halves = vec_t<unsigned short, 2>;
+                bits = __builtin_bit_cast(unsigned int, __builtin_elementwise_max(__builtin_bit_cast(Halves, bits), __builtin_bit_cast(Halves, words[w] & 0x7FFF7FFFu)));
+            }
         }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(f[e], 0.0f, sum);
     }
-    return sum;
-}
+    __device__ __forceinline__ bool finite() const {
+        constexpr unsigned int kInf = __is_same(T, float) ? 0x7F800000u : __is_same(T, f16_t) ? 0x7C00u : 0x7F80u;
+        return sizeof(T) == 4 ? bits < kInf : (bits & 0xFFFFu) < kInf && (bits >> 16) < kInf;
+    }
+};
 
 // Half precision: the power of two that brings a largest magnitude into 2^low .. 2^high, 1 where it is there already (or zero, or not finite).
 __device__ __forceinline__ float range_scale(float largest, int low, int high) {
@@ -235,6 +242,11 @@ __device__ __forceinline__ float range_scale(float largest, int low, int high) {
     if (e >= 128 || e <= -127 || (e >= low && e < high)) return 1.0f;
     const int target = e < low ? low : high - 1;
     return __uint_as_float(static_cast<unsigned int>(min(max(target - e, -126), 126) + 127) << 23);
+}
+// The larger magnitude of the two; what is not finite counts as none.
+__device__ __forceinline__ float larger(float most, float value) {
+    const float size = fabsf(value);
+    return size < __builtin_inff() ? fmaxf(most, size) : most;
 }
 template <typename T>
 constexpr bool kNarrow = __is_same(T, f16_t);  // a range that sums leave
@@ -253,11 +265,11 @@ struct Values {
         for (int s = 0; s < 4; ++s)
             if (s >= first && s < first + count) z[s] = column_frag<T, W>(tile, 16 * s, column_block);
     }
-    __device__ __forceinline__ float finite_sum() const {  // 0 where all is finite
-        float sum = 0.0f;
+    __device__ __forceinline__ bool finite() const {
+        Largest<T> most;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) sum = finite_test(z[s], sum);
-        return sum;
+        for (int s = 0; s < 4; ++s) most.take(z[s]);
+        return most.finite();
     }
     __device__ __forceinline__ float largest() const {
         float most = 0.0f;
@@ -265,7 +277,7 @@ struct Values {
         for (int s = 0; s < 4; ++s) {
             const auto f = vec_to_f32<T, 8>(z[s]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[e]));
+            for (int e = 0; e < 8; ++e) most = larger(most, f[e]);
         }
         return wave_max(most);
     }
@@ -336,11 +348,12 @@ __device__ __forceinline__ void share_of(int all, int i, int count, Step&& step)
     for (int n = 0; n < all; ++n)
         if (n * count / all == i) step(n);
 }
-// Half precision: what small values are enlarged by before they are weighted, the matrix along with them until it is brought back.
+// Half precision: values are weighted at the upper end of its range (the two parts of one that is 2^-17 of the largest still leave 2^-22 of it), the
+// matrix along with them until it is brought back; not by more than 2^30, which fp32 has room for.
 template <typename T, int K>
-__device__ __forceinline__ float enlarge(acc_t (&matrix)[K], const Values<T>& values) {
+__device__ __forceinline__ float enlarge(acc_t (&matrix)[K], const Values<T>& values, float largest_weight) {
     if constexpr (!kNarrow<T>) return 1.0f;
-    const float up = fmaxf(range_scale(values.largest(), -3, 15), 1.0f);
+    const float up = fminf(range_scale(values.largest() * largest_weight, 14, 15), 0x1p30f);
     if (up != 1.0f)
 #pragma unroll
         for (int k = 0; k < K; ++k) matrix[k] *= up;
@@ -359,7 +372,7 @@ __device__ __forceinline__ float largest_of(const acc_t (&matrix)[K]) {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(matrix[k][i]));
+        for (int i = 0; i < 16; ++i) most = larger(most, matrix[k][i]);
     return wave_max(most);
 }
 // The matrix that a walk starts from: `factor` times the stored one, zeros for none. A wavefront has 32 columns.
@@ -471,6 +484,7 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
             if (far >= 0) seen[n][i / 2] |= i % 2 == 0 ? 0xFFFFu : 0xFFFF0000u;
         }
     const Weights weights(l, task.matrix_scale, REVERSE, kChunk);
+    const float largest_weight = REVERSE ? task.matrix_scale * power(l, 1) : 1.0f;
 
     acc_t matrix[K];
     load_matrix<K>(matrix, task.carry, task.carry_factor, task.transposed, d, wave);
@@ -543,7 +557,8 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
             // what came before it, C' X'.
             turn_to(last_each ? min(step + 1, steps - 1) : step, last_each ? 0 : each + 1);
             Values<T> values;
-            float matrix_scale = 1.0f, finite_sum;
+            float matrix_scale = 1.0f;
+            bool finite;
             if constexpr (kNarrow<T>)
                 if (!REVERSE || each == 0) matrix_scale = range_scale(largest_of(matrix), -3, 15);
             const float passed = power(l, length);
@@ -604,7 +619,7 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
                         slot_end();
                     }
                 }
-                finite_sum = values.finite_sum();
+                finite = !__any(!values.finite());
                 // What the mask hides is 0 whatever the scores are.
 #pragma unroll
                 for (int n = 0; n < kTables; ++n) {
@@ -622,7 +637,7 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
                     if constexpr (kNarrow<T>) {
                         float most = 0.0f;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(p[n][i]));
+                        for (int i = 0; i < 16; ++i) most = larger(most, p[n][i]);
                         const float scale = range_scale(wave_max(most), -3, 15);
                         p[n] *= scale;
                         pair_scales[tile] = scale;
@@ -659,9 +674,8 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
                 }
                 if (a.accumulate) add_what_is_there(within, out_each, row0, length);
             }
-            const bool finite = !__any(!(finite_sum == 0.0f));
             const bool update = REVERSE || last_each;
-            const float up = update ? enlarge<T, K>(matrix, values) : 1.0f;
+            const float up = update ? enlarge<T, K>(matrix, values, largest_weight) : 1.0f;
             __syncthreads();  // all pairs are there, X and Z have been read
             auto pair_frag = [&](int t, int r, int s) { return *reinterpret_cast<const frag_t<T>*>(pairs_at<T>(pairs, t * 32 + (lane & 31), 4 * r + 2 * s + half)); };
             Values<T> shown = values;
@@ -801,6 +815,7 @@ __device__ __forceinline__ void sum_segment(const LinearArgs& a, bool reverse, i
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const float l = log2_decay(a.log_decay[kv]);
     Weights weights(l, reverse ? a.scale : 1.0f, reverse, kChunk);
+    const float largest_weight = reverse ? a.scale * power(l, 1) : 1.0f;
     const int heads = reverse ? a.hq : a.hkv, heads_each = reverse ? a.hq / a.hkv : 1;
     const long stride = static_cast<long>(heads) * d;
     const T* y_base = static_cast<const T*>(reverse ? a.q : a.k) + static_cast<long>(b) * tokens * stride + static_cast<long>(kv) * heads_each * d;
@@ -851,7 +866,7 @@ __device__ __forceinline__ void sum_segment(const LinearArgs& a, bool reverse, i
             for (int k = 0; k < K; ++k) matrix[k] *= passed;
         }
         if (!reverse && end != kChunk) weights = Weights(l, 1.0f, false, end);
-        const float up = enlarge<T, K>(matrix, values);
+        const float up = enlarge<T, K>(matrix, values, largest_weight);
 #pragma unroll
         for (int i = 0; i < 8; ++i) weighted[0].step(i, values.z[0], weights.w[0], up);
         slot_end();
