@@ -212,30 +212,6 @@ __device__ __forceinline__ float log2_decay(float log_decay) {
 }
 __device__ __forceinline__ float power(float l, int n) { return __builtin_amdgcn_exp2f(l * static_cast<float>(n)); }
 
-// The largest magnitude's bits of what passed, two halves of a word each for 16-bit storage: whether all is finite. (A dot product with zeros is one
-// instruction a word, but does not turn every NaN or Inf into a NaN.)
-template <typename T>
-struct Largest {
-    unsigned int bits = 0;
-    __device__ __forceinline__ void take(const frag_t<T>& f) {
-        constexpr int kWords = 8 * sizeof(T) / 4;
-        const auto words = __builtin_bit_cast(vec_t<unsigned int, kWords>, f);
-#pragma unroll
-        for (int w = 0; w < kWords; ++w) {
-            if constexpr (sizeof(T) == 4) {
-                bits = max(bits, words[w] & 0x7FFFFFFFu);
-            } else {
-                using Halves = vec_t<unsigned short, 2>;
-                bits = __builtin_bit_cast(unsigned int, __builtin_elementwise_max(__builtin_bit_cast(Halves, bits), __builtin_bit_cast(Halves, words[w] & 0x7FFF7FFFu)));
-            }
-        }
-    }
-    __device__ __forceinline__ bool finite() const {
-        constexpr unsigned int kInf = __is_same(T, float) ? 0x7F800000u : __is_same(T, f16_t) ? 0x7C00u : 0x7F80u;
-        return sizeof(T) == 4 ? bits < kInf : (bits & 0xFFFFu) < kInf && (bits >> 16) < kInf;
-    }
-};
-
 // Half precision: the power of two that brings a largest magnitude into 2^low .. 2^high, 1 where it is there already (or zero, or not finite).
 __device__ __forceinline__ float range_scale(float largest, int low, int high) {
     const int e = static_cast<int>((__float_as_uint(largest) >> 23) & 0xFF) - 127;
@@ -243,10 +219,18 @@ __device__ __forceinline__ float range_scale(float largest, int low, int high) {
     const int target = e < low ? low : high - 1;
     return __uint_as_float(static_cast<unsigned int>(min(max(target - e, -126), 126) + 127) << 23);
 }
-// The larger magnitude of the two; what is not finite counts as none.
-__device__ __forceinline__ float larger(float most, float value) {
-    const float size = fabsf(value);
-    return size < __builtin_inff() ? fmaxf(most, size) : most;
+// The largest finite magnitude that walk(use) hands out in a wavefront.
+template <typename Walk>
+__device__ __forceinline__ float largest_finite(Walk&& walk) {
+    float most = 0.0f;
+    walk([&](float value) __attribute__((always_inline)) { most = fmaxf(most, fabsf(value)); });
+    most = wave_max(most);
+    if (most == __builtin_inff()) {
+        most = 0.0f;
+        walk([&](float value) __attribute__((always_inline)) { most = fabsf(value) < __builtin_inff() ? fmaxf(most, fabsf(value)) : most; });
+        most = wave_max(most);
+    }
+    return most;
 }
 template <typename T>
 constexpr bool kNarrow = __is_same(T, f16_t);  // a range that sums leave
@@ -265,21 +249,45 @@ struct Values {
         for (int s = 0; s < 4; ++s)
             if (s >= first && s < first + count) z[s] = column_frag<T, W>(tile, 16 * s, column_block);
     }
-    __device__ __forceinline__ bool finite() const {
-        Largest<T> most;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) most.take(z[s]);
-        return most.finite();
-    }
-    __device__ __forceinline__ float largest() const {
-        float most = 0.0f;
+    // 16-bit storage: the largest magnitude's bits in each half of a word. (Dot products with constants are one instruction for two instead of two, but
+    // let Infs and NaNs get lost here.)
+    __device__ __forceinline__ unsigned int largest_bits() const {
+        using Halves = vec_t<unsigned short, 2>;
+        Halves most(static_cast<unsigned short>(0));
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            const auto f = vec_to_f32<T, 8>(z[s]);
+            const auto words = __builtin_bit_cast(vec_t<unsigned int, 2 * sizeof(T)>, z[s]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) most = larger(most, f[e]);
+            for (int w = 0; w < 4; ++w) most = __builtin_elementwise_max(most, __builtin_bit_cast(Halves, words[w] & 0x7FFF7FFFu));
         }
-        return wave_max(most);
+        return __builtin_bit_cast(unsigned int, most);
+    }
+    __device__ __forceinline__ bool finite() const {
+        if constexpr (sizeof(T) == 4) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum = fmaf(z[s][e], 0.0f, sum);
+            return sum == 0.0f;
+        } else {
+            constexpr unsigned int kInf = kNarrow<T> ? 0x7C00u : 0x7F80u;
+            const unsigned int most = largest_bits();
+            return (most & 0xFFFFu) < kInf && (most >> 16) < kInf;
+        }
+    }
+    // Half precision: the largest finite magnitude in the wavefront.
+    __device__ __forceinline__ float largest() const {
+        unsigned int bits = largest_bits();
+        bits = max(bits & 0xFFFFu, bits >> 16);
+        if (__any(bits >= 0x7C00u))
+            return largest_finite([&](auto&& use) __attribute__((always_inline)) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) use(to_f32(z[s][e]));
+            });
+        return wave_max(to_f32(__builtin_bit_cast(f16_t, static_cast<unsigned short>(bits))));
     }
 };
 
@@ -368,12 +376,12 @@ __device__ __forceinline__ void bring_back(acc_t (&matrix)[K], float up) {
 
 template <int K>
 __device__ __forceinline__ float largest_of(const acc_t (&matrix)[K]) {
-    float most = 0.0f;
+    return largest_finite([&](auto&& use) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) most = larger(most, matrix[k][i]);
-    return wave_max(most);
+            for (int i = 0; i < 16; ++i) use(matrix[k][i]);
+    });
 }
 // The matrix that a walk starts from: `factor` times the stored one, zeros for none. A wavefront has 32 columns.
 template <int K>
@@ -635,10 +643,11 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
                         }
                     }
                     if constexpr (kNarrow<T>) {
-                        float most = 0.0f;
+                        const float scale = range_scale(largest_finite([&](auto&& use) __attribute__((always_inline)) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) most = larger(most, p[n][i]);
-                        const float scale = range_scale(wave_max(most), -3, 15);
+                                                            for (int i = 0; i < 16; ++i) use(p[n][i]);
+                                                        }),
+                                                        -3, 15);
                         p[n] *= scale;
                         pair_scales[tile] = scale;
                     }
@@ -966,10 +975,12 @@ __global__ __launch_bounds__(W * 2, 2) void linear_segments_kernel(LinearArgs a)
 }
 
 // The segments' matrices become what comes before each (blockIdx.y = 0) or behind it (1), in order along the sequence, a thread an element.
-constexpr int kAhead = 8;  // loads in flight
-__global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a) {
+// What it waits for is the loads: 32 at a time in workgroups of one wavefront (128 segments of 4 matrices of 64 x 64: the call takes 66 us, with
+// 8 at a time in workgroups of four 71, with 64 at a time 118).
+constexpr int kAhead = 32, kJoinThreads = 64;
+__global__ __launch_bounds__(kJoinThreads) void linear_join_kernel(LinearArgs a) {
     const bool reverse = blockIdx.y == 1;
-    const long matrix = static_cast<long>(a.d) * a.d, at = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;
+    const long matrix = static_cast<long>(a.d) * a.d, at = static_cast<long>(blockIdx.x) * kJoinThreads + threadIdx.x;
     if (at >= matrix * a.batch * a.hkv) return;
     const long pair = at / matrix, element = at - pair * matrix;
     const float l = log2_decay(a.log_decay[pair % a.hkv]);
@@ -1137,18 +1148,20 @@ LinearArgs make_args(const Shape& s, const void* q, const void* k, const void* v
 // Cuts the sequences into at most `most` segments of whole chunks, and says how many of a group's query heads a workgroup takes one after the other.
 // Walks that give three compute units of four work are not cut: two segments each would need their matrices first (32 sequences of 1024 tokens,
 // 8 query and 2 kv heads of 128: 58 us forward and 168 backward, cut in two 93 and 223). Then every query head has a workgroup of its own;
-// where sequences have to be cut, a group's heads share what is done for k and v (58 and 168 us against 70 and 198 for that batch in four segments), unless
-// that leaves units without work. Segments are two chunks or longer (2 sequences of 333 fp32 tokens, 4 heads of 40: 52 us, four chunks or longer 69), two
-// a unit where the tokens allow it (32768 tokens, 12 and 4 heads of 64: 71 and 142 us, one a unit 76 and 151).
-void cut(LinearArgs& a, int most) {
+// where sequences have to be cut, a group's heads share what is done for k and v, unless that leaves units without work (backward has three
+// walks a segment then: 5 sequences of 1001 half precision tokens, 12 and 4 heads of 64: 48 us, heads apart 58). Segments are two chunks or
+// longer in 16-bit storage; in fp32, whose products take longer than what a segment costs, one (2 sequences of 333 tokens, 4 heads of 40: 36 us
+// forward, two chunks or longer 53). Two a unit where the tokens allow it (32768 tokens, 12 and 4 heads of 64: 66 and 145 us, one a unit
+// 72 and 148).
+void cut(LinearArgs& a, int most, bool backward, bool fp32) {
     const int chunks = (a.tokens + kChunk - 1) / kChunk, group = a.hq / a.hkv;
     const long pairs = static_cast<long>(a.batch) * a.hkv, units = compute_units();
     auto fills = [&](long walks) { return walks * 4 >= units * 3; };
     auto segments_for = [&](long walks) {
         if (fills(walks)) return 1;
-        return static_cast<int>(std::min<long>({(2 * units + walks - 1) / walks, static_cast<long>((chunks + 1) / 2), static_cast<long>(most)}));
+        return static_cast<int>(std::min<long>({(2 * units + walks - 1) / walks, static_cast<long>(fp32 ? chunks : (chunks + 1) / 2), static_cast<long>(most)}));
     };
-    a.heads_each = !fills(pairs * group) && fills(pairs * segments_for(pairs)) ? group : 1;
+    a.heads_each = !fills(pairs * group) && fills(pairs * segments_for(pairs) * (backward ? 3 : 1)) ? group : 1;
     const int segments = segments_for(pairs * (group / a.heads_each));
     a.segment_chunks = (chunks + segments - 1) / segments;
     a.segments = (chunks + a.segment_chunks - 1) / a.segment_chunks;
@@ -1171,14 +1184,14 @@ int run(LinearArgs& a, bool backward, hipStream_t stream) {
     const long pairs = static_cast<long>(a.batch) * a.hkv;
     const int parts = backward ? 2 : 1;
     const std::size_t slots = static_cast<std::size_t>(pairs) * a.d * a.d;
-    cut(a, 1 << 20);
+    cut(a, 1 << 20, backward, sizeof(T) == 4);
     // Segments need scratch; a call that cannot have it all takes fewer, one sequence a walk with none.
     if (a.segments > 1) {
         void* memory = nullptr;
         std::size_t held = 0;
         auto wanted = [&] { return static_cast<std::size_t>(parts) * a.segments * slots * sizeof(float); };
         if (int st = scratch_up_to(stream, wanted(), &memory, &held)) return st;
-        while (a.segments > 1 && held < wanted()) cut(a, a.segments - 1);
+        while (a.segments > 1 && held < wanted()) cut(a, a.segments - 1, backward, sizeof(T) == 4);
         a.ahead = static_cast<float*>(memory);
         a.behind = a.ahead + a.segments * slots;
     }
@@ -1186,7 +1199,7 @@ int run(LinearArgs& a, bool backward, hipStream_t stream) {
         if (int st = allow_shared<linear_segments_kernel<T, W, STAGED>>(kSegmentBytes<T, W>)) return st;
         hipLaunchKernelGGL((linear_segments_kernel<T, W, STAGED>), dim3(static_cast<unsigned int>(pairs * a.segments), parts), dim3(W * 2), (kSegmentBytes<T, W>), stream, a);
         CGPTX_LAUNCH_CHECK();
-        hipLaunchKernelGGL(linear_join_kernel, dim3(static_cast<unsigned int>((slots + 255) / 256), parts), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(linear_join_kernel, dim3(static_cast<unsigned int>((slots + kJoinThreads - 1) / kJoinThreads), parts), dim3(kJoinThreads), 0, stream, a);
         CGPTX_LAUNCH_CHECK();
     }
     const bool state_too = a.segments == 1 && (backward ? a.d_before : a.after) != nullptr;
