@@ -149,24 +149,24 @@ __device__ __forceinline__ void store_words(vec_t<unsigned int, 4> words, __amdg
 // Rows row0 .. row0 + 63 of a head on their way to a tile, zeros behind the last token and behind column d. STAGED (16-bit storage on 16-byte
 // boundaries): fetch asks for them, and they wait in registers until store. (Loads straight into LDS would save the registers, but every
 // transposing read of another tile waits for them.)
-template <typename T, int W, bool STAGED>
+template <typename T, int W, bool STAGED, int THREADS>
 struct Incoming {
-    static constexpr int kThreadsHere = W * 2;  // W/32 wavefronts
-    static constexpr int kChunks = W / 8;       // of a row
+    static constexpr int kChunks = W / 8;  // of a row
+    static constexpr int kRows = THREADS / kChunks, kPieces = kChunk / kRows;
     Rows<T> rows;
     int row0;
     __amdgpu_buffer_rsrc_t rsrc;
-    int voffset, further;  // a lane's first piece; bytes to its next one, sixteen rows on
-    vec_t<unsigned int, 4> piece[STAGED ? 4 : 1];
+    int voffset, further;  // a lane's first piece; bytes to its next one, kRows on
+    vec_t<unsigned int, 4> piece[STAGED ? kPieces : 1];
 
     __device__ __forceinline__ Incoming(long stride, int d) {
         if constexpr (STAGED) {
             const int row_bytes = static_cast<int>(stride) * 2, r = threadIdx.x / kChunks, chunk = threadIdx.x % kChunks;
             voffset = chunk * 8 < d ? r * row_bytes + chunk * 16 : 1 << 30;
-            further = 16 * row_bytes;
+            further = kRows * row_bytes;
         }
     }
-    // Says which rows; the four pieces of STAGED are asked for, and stored, one by one.
+    // Says which rows; the pieces of STAGED are asked for, and stored, one by one.
     __device__ __forceinline__ void set(const Rows<T>& from, int first, int tokens, int d) {
         rows = from;
         row0 = first;
@@ -179,14 +179,14 @@ struct Incoming {
     __device__ __forceinline__ void store(int i, T* tile, int tokens, int d, bool vectors) const {
         if constexpr (STAGED) {
             const int r = threadIdx.x / kChunks, chunk = threadIdx.x % kChunks;
-            *reinterpret_cast<vec_t<unsigned int, 4>*>(tile + (r + i * 16) * W + ((chunk ^ swizzle<W>(r)) * 8)) = piece[i];
+            *reinterpret_cast<vec_t<unsigned int, 4>*>(tile + (r + i * kRows) * W + ((chunk ^ swizzle<W>(r)) * 8)) = piece[i];
         } else if (i == 0) {
             const T* first = rows.base + static_cast<long>(row0) * rows.stride;
             const int left = min(kChunk, tokens - row0);
-            constexpr int VEC = kVec128<T>, kPieces = W / VEC;
+            constexpr int VEC = kVec128<T>, kVectors = W / VEC;
 #pragma unroll 4
-            for (int n = threadIdx.x; n < kChunk * kPieces; n += kThreadsHere) {
-                const int r = n / kPieces, p = n % kPieces, column = p * VEC;
+            for (int n = threadIdx.x; n < kChunk * kVectors; n += THREADS) {
+                const int r = n / kVectors, p = n % kVectors, column = p * VEC;
                 vec_t<T, VEC> v(static_cast<T>(0.0f));
                 if (r < left && column < d) {
                     const T* from = first + static_cast<long>(r) * rows.stride + column;
@@ -235,10 +235,6 @@ __device__ __forceinline__ float largest_finite(Walk&& walk) {
 template <typename T>
 constexpr bool kNarrow = __is_same(T, f16_t);  // a range that sums leave
 
-// The work of a chunk is written in slots: a few matrix instructions, the reads of operands for a later slot, vector work for the next one. What stands
-// in a slot stays there (left to itself the compiler reads an operand right before it is used, and every read's way through the LDS
-// is waited for).
-__device__ __forceinline__ void slot_end() { __builtin_amdgcn_sched_barrier(0); }
 // Z of a wavefront's 32 columns: four operands of sixteen rows.
 template <typename T>
 struct Values {
@@ -292,15 +288,19 @@ struct Values {
 };
 
 // Weights of a chunk's tokens as what follows the chunk sees them (forward in time: 1 for token `end`, else g^(end - token); backward: g^(token
-// + 1)), for the rows that a lane's operands hold.
+// + 1)), for the rows that a lane's operands hold in COUNT steps of sixteen from `first` on.
+template <int COUNT>
 struct Weights {
-    vec_t<float, 8> w[4];
+    vec_t<float, 8> w[COUNT];
     __device__ __forceinline__ static int row(int e) { return 4 * ((threadIdx.x & 63) >> 5) + (e & 3) + 2 * (e & 4); }
-    __device__ __forceinline__ Weights(float l, float scale, bool reverse, int end) {
+    __device__ __forceinline__ Weights(float l, float scale, bool reverse, int end, int first = 0) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
+        for (int s = 0; s < COUNT; ++s)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[s][e] = scale * power(l, reverse ? 16 * s + row(e) + 1 : max(end - 16 * s - row(e), 0));
+            for (int e = 0; e < 8; ++e) {
+                const int at = 16 * (first + s) + row(e);
+                w[s][e] = scale * power(l, reverse ? at + 1 : max(end - at, 0));
+            }
     }
 };
 
@@ -329,23 +329,22 @@ struct Weighted {
         return frag_t<T>{part[n][0][0], part[n][0][1], part[n][1][0], part[n][1][1], part[n][2][0], part[n][2][1], part[n][3][0], part[n][3][1]};
     }
 };
-template <typename T, int W>
-__device__ __forceinline__ void read_rows_of(frag_t<T> (&y)[W / 32], const T* tile, int offset, int s) {
+template <typename T, int W, int K>
+__device__ __forceinline__ void read_rows_of(frag_t<T> (&y)[K], const T* tile, int offset, int s) {
 #pragma unroll
-    for (int k = 0; k < W / 32; ++k) y[k] = swapped_frag<T, W>(tile, offset, 16 * s, k);
+    for (int k = 0; k < K; ++k) y[k] = swapped_frag<T, W>(tile, offset, 16 * s, k);
 }
-// matrix += Y' (w Z) for sixteen rows; between(i) follows the i-th matrix instruction, of `count`.
-template <typename T, int K, int PARTS, typename Between>
-__device__ __forceinline__ void add_rows(acc_t (&matrix)[K], const frag_t<T> (&y)[K], const Weighted<T, PARTS>& z, Between&& between) {
+// matrix += Y' (w Z) for sixteen rows, operand(n) one of kParts parts of w Z; between(i, count) follows the i-th matrix instruction of `count`.
+template <typename T, int K, int PARTS, typename Operand, typename Between>
+__device__ __forceinline__ void add_rows(acc_t (&matrix)[K], const frag_t<T> (&y)[K], Operand&& operand, Between&& between) {
     constexpr int kParts = Weighted<T, PARTS>::kParts;
 #pragma unroll
     for (int n = 0; n < kParts; ++n) {
-        const frag_t<T> part = z.operand(n);
+        const frag_t<T> part = operand(n);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             matrix[k] = multiply<T>(y[k], part, matrix[k]);
             between(n * K + k, kParts * K);
-            slot_end();
         }
     }
 }
@@ -383,10 +382,11 @@ __device__ __forceinline__ float largest_of(const acc_t (&matrix)[K]) {
             for (int i = 0; i < 16; ++i) use(matrix[k][i]);
     });
 }
-// The matrix that a walk starts from: `factor` times the stored one, zeros for none. A wavefront has 32 columns.
+// The matrix that a walk starts from: `factor` times the stored one, zeros for none. A wavefront has 32 columns and rows
+// from first_row on.
 template <int K>
-__device__ __forceinline__ void load_matrix(acc_t (&matrix)[K], const float* from, float factor, bool transposed, int d, int wave) {
-    const int column = wave * 32 + (threadIdx.x & 31), row0 = matrix_row(0);
+__device__ __forceinline__ void load_matrix(acc_t (&matrix)[K], const float* from, float factor, bool transposed, int d, int column_block, int first_row) {
+    const int column = column_block * 32 + (threadIdx.x & 31), row0 = first_row + matrix_row(0);
     const __amdgpu_buffer_rsrc_t rsrc = buffer_of(from, from != nullptr ? d * d * 4 : 0);  // reads behind its end give zeros
     const int row_step = (transposed ? 1 : d) * 4, first = (transposed ? column * d + row0 : row0 * d + column) * 4;
 #pragma unroll
@@ -424,14 +424,40 @@ struct Task {
     float pair_scale, matrix_scale, out_scale;  // of P, of what is added to the matrix, of the matrix's part of the output
 };
 
-// The output of one head in one segment. In a chunk: scores and what came before it | pairs there: X and Z have been read, the next chunk's
-// are on their way (Y has two buffers) | products with Z, the matrix, the output | the next chunk is there.
+template <int W>
+__device__ __forceinline__ int column_block_of() {
+    return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % (W / 32);
+}
+// A lane's offset further by `columns`, a power of two that no read adds by itself.
+template <typename T>
+__device__ __forceinline__ int along(int offset, int columns) {
+    return sizeof(T) == 2 ? offset ^ columns : offset + columns;
+}
+
+// The output of one head in one segment. Two wavefronts have the same 32 columns of Z, the matrix and the output, each half of the matrix's rows and half
+// of a chunk's tokens: W/2 x 32 and 32 x 32 in registers. In a chunk: scores of the pairs, by three wavefronts, and what came before it, where
+// each has half of both sums and leaves the other's to it | all is there, X and Z have been read, the next chunk's are on their way (Y has two
+// buffers in 16-bit storage) | products with Z, the matrix, the output | the next chunk is there. What bounds it is how long these steps wait for each
+// other: with a wavefront for both halves a chunk has half the instructions in all and takes as long where 16 chunks follow each other (32
+// sequences of 1024 tokens, heads of 128: 59 us forward, 162 backward; with two 58 and 167), and longer where there are few (77 tokens of
+// half precision: 11 us, with two 9; fp32, 2 x 333 tokens, backward: 37, with two 30).
+template <typename T, int W>
+constexpr int kWalkThreads = W * 4;
+template <typename T>
+constexpr int kYTiles = sizeof(T) == 2 ? 2 : 1;
+template <typename T>
+constexpr bool kShares = sizeof(T) == 2;  // the weighted Z of the wavefronts of a column block: two steps of sixteen rows each, by the LDS
 template <typename T, int W, bool REVERSE, bool STAGED>
 __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>& task, int b, int head, int segment, T* lds) {
-    constexpr int K = W / 32, kTables = W == 128 ? 1 : 2;
-    T *x_tile = lds, *z_tile = lds + kTile<T, W>, *y_tiles = lds + 2 * kTile<T, W>, *pairs = lds + 4 * kTile<T, W>;
+    constexpr int kBlocks = W / 32, K = kBlocks / 2, kSeesBoth = REVERSE ? 0 : 1;  // the half of the tokens that sees both
+    using In = Incoming<T, W, STAGED, kWalkThreads<T, W>>;
+    constexpr int kPieces = In::kPieces;
+    T *x_tile = lds, *z_tile = lds + kTile<T, W>, *y_tiles = lds + 2 * kTile<T, W>, *pairs = y_tiles + kYTiles<T> * kTile<T, W>;
+    float* halves = reinterpret_cast<float*>(pairs + kChunk * kPairsPitch<T>);
+    T* weighted_z = reinterpret_cast<T*>(halves + kWalkThreads<T, W> * 16) + column_block_of<W>() * 8 * 512;
     __shared__ float pair_scales[3];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int column_block = column_block_of<W>(), mine = wave / kBlocks, place = mine * 32 + (lane & 31);
     const int d = a.d, tokens = a.tokens;
     const int group = a.hq / a.hkv, heads_each = REVERSE ? group : a.heads_each;
     const int kv = REVERSE ? head : head / group, y_first = REVERSE ? head * group : kv;
@@ -446,84 +472,56 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
     const int first_chunk = segment * a.segment_chunks, last_chunk = min(first_chunk + a.segment_chunks, chunks_in_all) - 1;
     const int steps = last_chunk - first_chunk + 1;
     auto row_of = [&](int step) { return (REVERSE ? last_chunk - step : first_chunk + step) * kChunk; };
-    Incoming<T, W, STAGED> in_x(x_stride, d), in_y(y_stride, d), in_z(y_stride, d);
+    In in_x(x_stride, d), in_y(y_stride, d), in_z(y_stride, d);
     // Forward in time the heads of a group share Y and Z, backward X and the output.
     auto turn_to = [&](int step, int each) __attribute__((always_inline)) {
         const int row0 = row_of(step);
-        const long along = static_cast<long>(each) * d, x_along = REVERSE ? 0 : along, y_along = REVERSE ? along : 0;
-        in_x.set(Rows<T>{x.base + x_along, x.stride}, row0, tokens, d);
-        in_y.set(Rows<T>{y.base + y_along, y.stride}, row0, tokens, d);
-        in_z.set(Rows<T>{z.base + y_along, z.stride}, row0, tokens, d);
+        const long further = static_cast<long>(each) * d, x_further = REVERSE ? 0 : further, y_further = REVERSE ? further : 0;
+        in_x.set(Rows<T>{x.base + x_further, x.stride}, row0, tokens, d);
+        in_y.set(Rows<T>{y.base + y_further, y.stride}, row0, tokens, d);
+        in_z.set(Rows<T>{z.base + y_further, z.stride}, row0, tokens, d);
     };
-    // Piece n of the next tiles, of four or (all) twelve.
-    auto fetch = [&](auto all, int n) __attribute__((always_inline)) {
-        if constexpr (!decltype(all)::value) in_x.fetch(n);
-        else if (n % 3 == 0) in_x.fetch(n / 3);
-        else if (n % 3 == 1) in_y.fetch(n / 3);
-        else in_z.fetch(n / 3);
-    };
-    auto store_tiles = [&](auto all, int n, int buffer) __attribute__((always_inline)) {
-        if constexpr (!decltype(all)::value) in_x.store(n, x_tile, tokens, d, a.vectors);
-        else if (n % 3 == 0) in_x.store(n / 3, x_tile, tokens, d, a.vectors);
-        else if (n % 3 == 1) in_y.store(n / 3, y_tiles + buffer * kTile<T, W>, tokens, d, a.vectors);
-        else in_z.store(n / 3, z_tile, tokens, d, a.vectors);
-    };
+    int buffer = 0;
     turn_to(0, 0);
 #pragma unroll
-    for (int n = 0; n < 12; ++n) fetch(std::true_type{}, n);
+    for (int n = 0; n < kPieces; ++n) {
+        in_x.fetch(n);
+        in_y.fetch(n);
+        in_z.fetch(n);
+    }
 
-    // Which 32 x 32 tiles of pairs a wavefront makes: 0 and 1 on the diagonal, 2 the one beside it. W = 64: wavefront 0 makes 0 and 2.
-    float table[kTables][16];
-    unsigned int seen[kTables][8];  // bfloat16: masks of two elements each
-    auto tile_t = [](int tile) { return tile == 2 ? (REVERSE ? 0 : 1) : tile; };
-    auto tile_r = [](int tile) { return tile == 2 ? (REVERSE ? 1 : 0) : tile; };
-    auto my_tile = [&](int n) { return n == 0 ? min(wave, 2) : 2; };  // (what two wavefronts make is the same)
-    auto apart = [&](int tile, int i) {
-        const int t = tile_t(tile) * 32 + (lane & 31), r = tile_r(tile) * 32 + acc_row(i);
-        return REVERSE ? r - t : t - r;
-    };
+    // The 32 x 32 tile of pairs that a wavefront makes: 0 and 1 on the diagonal, 2 the one beside it.
+    const bool makes_pairs = wave < 3;
+    const int tile = min(wave, 2), tile_t = tile == 2 ? kSeesBoth : tile, tile_r = tile == 2 ? 1 - kSeesBoth : tile;
+    acc_t table;
+    unsigned int seen[8];  // bfloat16: masks of two elements each
 #pragma unroll
-    for (int n = 0; n < kTables; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int far = apart(my_tile(n), i);
-            table[n][i] = far >= 0 ? task.pair_scale * power(l, far) : 0.0f;
-            if (i % 2 == 0) seen[n][i / 2] = 0;
-            if (far >= 0) seen[n][i / 2] |= i % 2 == 0 ? 0xFFFFu : 0xFFFF0000u;
-        }
-    const Weights weights(l, task.matrix_scale, REVERSE, kChunk);
+    for (int i = 0; i < 16; ++i) {
+        const int t = tile_t * 32 + (lane & 31), r = tile_r * 32 + acc_row(i), far = REVERSE ? r - t : t - r;
+        table[i] = far >= 0 ? task.pair_scale * power(l, far) : 0.0f;
+        if (i % 2 == 0) seen[i / 2] = 0;
+        if (far >= 0) seen[i / 2] |= i % 2 == 0 ? 0xFFFFu : 0xFFFF0000u;
+    }
+    const Weights<kShares<T> ? 2 : 4> weights(l, task.matrix_scale, REVERSE, kChunk, kShares<T> ? 2 * mine : 0);
     const float largest_weight = REVERSE ? task.matrix_scale * power(l, 1) : 1.0f;
 
     acc_t matrix[K];
-    load_matrix<K>(matrix, task.carry, task.carry_factor, task.transposed, d, wave);
-    const int row_at = row_offset<T, W>(), swapped_at = swapped_offset<T, W>();
+    load_matrix<K>(matrix, task.carry, task.carry_factor, task.transposed, d, column_block, mine * 32 * K);
+    const int row_at = row_offset<T, W>(), swapped_at = along<T>(swapped_offset<T, W>(), mine * 32 * K);
     T* const out = task.out + static_cast<long>(b) * tokens * x_stride + static_cast<long>(head) * d;
-    auto add_what_is_there = [&](acc_t (&o)[2], const T* out, int row0, int length) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int place = t * 32 + (lane & 31);
-            if (place >= length) continue;
-            const T* from = out + (row0 + place) * x_stride;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int at = wave * 32 + acc_row(i);
-                if (at < d) o[t][i] += to_f32(from[at]);
-            }
-        }
-    };
-    // A quarter of a chunk's output. Rows and columns that are not there lie behind the end of a buffer, where stores are dropped.
-    auto store_output = [&](int quarter, const acc_t (&o)[2], const acc_t (&within)[2], const float (&since)[2], T* out, int row0, int length)
-                            __attribute__((always_inline)) {
-        const int t = quarter / 2, g = quarter % 2 * 2, place = t * 32 + (lane & 31);
+    // Eight columns of four of a chunk's output, twice (quarter 0, 1). Rows and columns that are not there lie behind the end of a buffer, where
+    // stores are dropped.
+    auto store_output = [&](int quarter, const acc_t& o, const acc_t& within, float since, T* out, int row0, int length) __attribute__((always_inline)) {
+        const int g = quarter * 2;
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fmaf(o[t][4 * g + e], since[t], within[t][4 * g + e]);
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(o[4 * g + e], since, within[4 * g + e]);
         T* first = out + row0 * x_stride;
         if constexpr (STAGED) {
             const __amdgpu_buffer_rsrc_t rsrc = buffer_of(first, static_cast<int>(((length - 1) * x_stride + d) * static_cast<long>(sizeof(T))));
             // A lane has quads of its row's columns, its partner in the other half of the wavefront the quads between: swapped, each has eight in a
             // row.
-            const int at = wave * 32 + 8 * (g + half), row = place * static_cast<int>(x_stride * sizeof(T));
+            const int at = column_block * 32 + 8 * (g + half), row = place * static_cast<int>(x_stride * sizeof(T));
             vec_t<float, 8> all;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -537,7 +535,7 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
             T* to = first + place * x_stride;
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                const int at = wave * 32 + 8 * (g + q) + 4 * half;
+                const int at = column_block * 32 + 8 * (g + q) + 4 * half;
                 if (a.vectors) {
                     if (at < d) store_vec<T, 4>(to + at, vec_from_f32<T, 4>(vec_t<float, 4>{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]}));
                 } else {
@@ -548,229 +546,274 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
             }
         }
     };
-    int buffer = 0;
+    auto store_x = [&](int n) __attribute__((always_inline)) { in_x.store(n, x_tile, tokens, d, a.vectors); };
+    auto store_y = [&](int n) __attribute__((always_inline)) { in_y.store(n, y_tiles + buffer * kTile<T, W>, tokens, d, a.vectors); };
+    auto store_z = [&](int n) __attribute__((always_inline)) { in_z.store(n, z_tile, tokens, d, a.vectors); };
 #pragma unroll
-    for (int n = 0; n < 12; ++n) store_tiles(std::true_type{}, n, 0);
+    for (int n = 0; n < kPieces; ++n) {
+        store_x(n);
+        store_y(n);
+        store_z(n);
+    }
     for (int step = 0; step < steps; ++step) {
         const int row0 = row_of(step), length = min(kChunk, tokens - row0);
-        acc_t o[2], within[2];  // by what came before the chunk, and by its own tokens
-        float since[2];
+        acc_t o, within;  // by what came before the chunk, and by its own tokens
+        float since;
         for (int each = 0; each < heads_each; ++each) {
             const T* y_tile = y_tiles + buffer * kTile<T, W>;
-            const bool last_each = each + 1 == heads_each;
+            const bool last_each = each + 1 == heads_each, update = REVERSE || last_each, before = !REVERSE || each == 0;
             T* const out_each = REVERSE ? out : out + static_cast<long>(each) * d;
             __syncthreads();  // the tiles are there
 
-            // The next tiles are asked for (behind the last ones, those once more). P' = (Y X') g^.., tile by tile, and in a chunk's first round
-            // what came before it, C' X'.
+            // The next tiles are asked for (behind the last ones, those once more), X alone where the next head shares Y and Z.
             turn_to(last_each ? min(step + 1, steps - 1) : step, last_each ? 0 : each + 1);
-            Values<T> values;
-            float matrix_scale = 1.0f;
-            bool finite;
-            if constexpr (kNarrow<T>)
-                if (!REVERSE || each == 0) matrix_scale = range_scale(largest_of(matrix), -3, 15);
-            const float passed = power(l, length);
-            // BEFORE: with what came before; DECAY: the matrix decays once it has been read; ALL: of the next tiles, not X alone.
-            auto scores = [&](auto before, auto decay, auto all) __attribute__((always_inline)) {
-                constexpr bool FIRST = decltype(before)::value, DECAY = decltype(decay)::value;
-                constexpr int STEPS = W / 16, AHEAD = 2;
-                const int at = anew(row_at);
-                frag_t<T> xs[AHEAD + 1][2], ys[AHEAD + 1][kTables], m[2];
-                acc_t p[kTables];
+            auto fetch = [&](int n) __attribute__((always_inline)) {
+                if (n < kPieces) in_x.fetch(n);
+                else if (n < 2 * kPieces) in_y.fetch(n - kPieces);
+                else in_z.fetch(n - 2 * kPieces);
+            };
+            constexpr int AHEAD = 2;
+            const int at = anew(row_at);
+            // P' = (Y X') g^..
+            if (makes_pairs) {
+                constexpr int STEPS = W / 16;
+                frag_t<T> xs[AHEAD + 1], ys[AHEAD + 1];
                 auto read = [&](int s) __attribute__((always_inline)) {
+                    xs[s % (AHEAD + 1)] = row_frag<T, W>(x_tile, at, 32 * tile_t, s);
+                    ys[s % (AHEAD + 1)] = row_frag<T, W>(y_tile, at, 32 * tile_r, s);
+                };
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) xs[s % (AHEAD + 1)][t] = row_frag<T, W>(x_tile, at, 32 * t, s);
+                for (int s = 0; s < AHEAD; ++s) read(s);
+                acc_t p(0.0f);
 #pragma unroll
-                    for (int n = 0; n < kTables; ++n) ys[s % (AHEAD + 1)][n] = row_frag<T, W>(y_tile, at, tile_r(my_tile(n)) * 32, s);
+                for (int s = 0; s < STEPS; ++s) {
+                    if (s + AHEAD < STEPS) read(s + AHEAD);
+                    p = multiply<T>(ys[s % (AHEAD + 1)], xs[s % (AHEAD + 1)], p);
+                }
+                // What the mask hides is 0 whatever the scores are.
+                if constexpr (__is_same(T, bf16_t)) {
+                    p *= table;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float weight = table[i];
+                        asm volatile("" : "+v"(weight));  // compared anew: no registers for sixteen masks
+                        p[i] = weight != 0.0f ? p[i] * weight : 0.0f;
+                    }
+                }
+                if constexpr (kNarrow<T>) {
+                    const float scale = range_scale(largest_finite([&](auto&& use) __attribute__((always_inline)) {
+#pragma unroll
+                                                        for (int i = 0; i < 16; ++i) use(p[i]);
+                                                    }),
+                                                    -3, 15);
+                    p *= scale;
+                    pair_scales[tile] = scale;
+                }
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    frag_t<T> part = operand_of<T>(p, s);
+                    if constexpr (__is_same(T, bf16_t)) {
+                        auto words = __builtin_bit_cast(vec_t<unsigned int, 4>, part);
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) words[w] &= seen[4 * s + w];
+                        part = __builtin_bit_cast(frag_t<T>, words);
+                    }
+                    *reinterpret_cast<frag_t<T>*>(pairs_at<T>(pairs, tile_t * 32 + (lane & 31), 4 * tile_r + 2 * s + half)) = part;
+                }
+            }
+            // C' X' of the wavefront's rows of C, for its own tokens and for the other half's. Once the matrix has been read it decays.
+            Values<T> values;
+            if (before) {
+                constexpr int STEPS = W / 32;
+                const int rows_at = along<T>(at, mine * 16 * STEPS);
+                float matrix_scale = 1.0f;
+                if constexpr (kNarrow<T>) matrix_scale = range_scale(largest_of(matrix), -3, 15);
+                const float passed = update ? power(l, length) : 1.0f;
+                frag_t<T> xs[AHEAD + 1][2], m[2];
+                auto fetch_some = [&](int i, int count) __attribute__((always_inline)) {
+                    share_of(kPieces, i, count, fetch);
+                    if (update) share_of(2 * kPieces, i, count, [&](int n) __attribute__((always_inline)) { fetch(kPieces + n); });
+                };
+                auto read = [&](int s) __attribute__((always_inline)) {
+                    xs[s % (AHEAD + 1)][0] = row_frag<T, W>(x_tile, rows_at, 32 * mine, s);
+                    xs[s % (AHEAD + 1)][1] = row_frag<T, W>(x_tile, rows_at, 32 - 32 * mine, s);
                 };
                 auto operand = [&](int s) __attribute__((always_inline)) {
-                    if constexpr (FIRST) {
-                        acc_t from = matrix[s / 2];
-                        if constexpr (kNarrow<T>) from *= matrix_scale;
-                        m[s % 2] = operand_of<T>(from, s % 2);
-                    }
-                };
-                auto forget = [&](int s) __attribute__((always_inline)) {  // of what operand(s) has read
-                    if constexpr (DECAY)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) matrix[s / 2][8 * (s % 2) + e] *= passed;
-                };
-                auto load = [&](int s, int n) __attribute__((always_inline)) {
-                    constexpr int each = kTables + (FIRST ? 2 : 0);
-                    share_of(decltype(all)::value ? 12 : 4, s * each + n, STEPS * each, [&](int i) __attribute__((always_inline)) { fetch(all, i); });
+                    acc_t from = matrix[s / 2];
+                    if constexpr (kNarrow<T>) from *= matrix_scale;
+                    m[s % 2] = operand_of<T>(from, s % 2);
                 };
 #pragma unroll
                 for (int s = 0; s < AHEAD; ++s) read(s);
                 operand(0);
-#pragma unroll
-                for (int n = 0; n < kTables; ++n) p[n] = acc_t(0.0f);
-                if constexpr (FIRST) o[0] = o[1] = acc_t(0.0f);
-                slot_end();
+                acc_t other(0.0f);
+                o = acc_t(0.0f);
 #pragma unroll
                 for (int s = 0; s < STEPS; ++s) {
                     if (s + AHEAD < STEPS) read(s + AHEAD);
-                    else values.template load<W>(z_tile, wave, 2 * (s + AHEAD - STEPS), 2);
+                    else values.template load<W>(z_tile, column_block, 2 * (s + AHEAD - STEPS), 2);
+                    other = multiply<T>(m[s % 2], xs[s % (AHEAD + 1)][1], other);
+                    if (s + 1 < STEPS) operand(s + 1);
+                    fetch_some(2 * s, 2 * STEPS);
+                    o = multiply<T>(m[s % 2], xs[s % (AHEAD + 1)][0], o);
 #pragma unroll
-                    for (int n = 0; n < kTables; ++n) {
-                        p[n] = multiply<T>(ys[s % (AHEAD + 1)][n], tile_t(my_tile(n)) == 0 ? xs[s % (AHEAD + 1)][0] : xs[s % (AHEAD + 1)][1], p[n]);
-                        load(s, n);
-                        slot_end();
-                    }
-                    if constexpr (FIRST) {
-                        o[0] = multiply<T>(m[s % 2], xs[s % (AHEAD + 1)][0], o[0]);
-                        if (s + 1 < STEPS) operand(s + 1);
-                        load(s, kTables);
-                        slot_end();
-                        o[1] = multiply<T>(m[s % 2], xs[s % (AHEAD + 1)][1], o[1]);
-                        forget(s);
-                        load(s, kTables + 1);
-                        slot_end();
-                    }
+                    for (int e = 0; e < 8; ++e) matrix[s / 2][8 * (s % 2) + e] *= passed;
+                    fetch_some(2 * s + 1, 2 * STEPS);
                 }
-                finite = !__any(!values.finite());
-                // What the mask hides is 0 whatever the scores are.
+                if constexpr (kNarrow<T>) {
+                    o *= 1.0f / matrix_scale;
+                    other *= 1.0f / matrix_scale;
+                }
 #pragma unroll
-                for (int n = 0; n < kTables; ++n) {
-                    const int tile = my_tile(n), tt = tile_t(tile), tr = tile_r(tile);
+                for (int n = 0; n < 4; ++n)
+                    store_vec<float, 4>(halves + ((wave * 4 + n) * 64 + lane) * 4, vec_t<float, 4>{other[4 * n], other[4 * n + 1], other[4 * n + 2], other[4 * n + 3]});
+                since = task.out_scale * power(l, max(REVERSE ? length - 1 - place : place, 0));
+                within = acc_t(0.0f);
+                if (a.accumulate && place < length) {
+                    const T* from = out_each + (row0 + place) * x_stride;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        if constexpr (__is_same(T, bf16_t)) {
-                            p[n][i] *= table[n][i];
-                        } else {
-                            float& weight = table[n][i];
-                            asm volatile("" : "+v"(weight));  // compared anew: no registers for sixteen masks
-                            p[n][i] = weight != 0.0f ? p[n][i] * weight : 0.0f;
-                        }
-                    }
-                    if constexpr (kNarrow<T>) {
-                        const float scale = range_scale(largest_finite([&](auto&& use) __attribute__((always_inline)) {
-#pragma unroll
-                                                            for (int i = 0; i < 16; ++i) use(p[n][i]);
-                                                        }),
-                                                        -3, 15);
-                        p[n] *= scale;
-                        pair_scales[tile] = scale;
-                    }
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        frag_t<T> part = operand_of<T>(p[n], s);
-                        if constexpr (__is_same(T, bf16_t)) {
-                            auto words = __builtin_bit_cast(vec_t<unsigned int, 4>, part);
-#pragma unroll
-                            for (int w = 0; w < 4; ++w) words[w] &= seen[n][4 * s + w];
-                            part = __builtin_bit_cast(frag_t<T>, words);
-                        }
-                        *reinterpret_cast<frag_t<T>*>(pairs_at<T>(pairs, tt * 32 + (lane & 31), 4 * tr + 2 * s + half)) = part;
+                        const int column = column_block * 32 + acc_row(i);
+                        if (column < d) within[i] += to_f32(from[column]);
                     }
                 }
-            };
-            constexpr std::true_type yes;
-            constexpr std::false_type no;
-            if constexpr (REVERSE) {
-                if (each == 0) scores(yes, yes, yes);
-                else scores(no, no, yes);
             } else {
-                if (last_each) scores(yes, yes, yes);
-                else scores(yes, no, no);
-            }
-            if (!REVERSE || each == 0) {
-                const float factor = task.out_scale / matrix_scale;
+                values.template load<W>(z_tile, column_block);
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const int place = t * 32 + (lane & 31);
-                    since[t] = factor * power(l, max(REVERSE ? length - 1 - place : place, 0));
-                    within[t] = acc_t(0.0f);
-                }
-                if (a.accumulate) add_what_is_there(within, out_each, row0, length);
+                for (int n = 0; n < 3 * kPieces; ++n) fetch(n);
             }
-            const bool update = REVERSE || last_each;
+            const bool finite = !__any(!values.finite());
             const float up = update ? enlarge<T, K>(matrix, values, largest_weight) : 1.0f;
-            __syncthreads();  // all pairs are there, X and Z have been read
-            auto pair_frag = [&](int t, int r, int s) { return *reinterpret_cast<const frag_t<T>*>(pairs_at<T>(pairs, t * 32 + (lane & 31), 4 * r + 2 * s + half)); };
+            if (kShares<T> && update)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    Weighted<T, 2> weighted;
+                    const frag_t<T> z = mine != 0 ? values.z[2 + s] : values.z[s];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) weighted.step(i, z, weights.w[s], up);
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) *reinterpret_cast<frag_t<T>*>(weighted_z + ((4 * mine + 2 * s + n) * 64 + lane) * 8) = weighted.operand(n);
+                }
+            __syncthreads();  // all pairs, halves and weighted Z are there, X and Z have been read
+            if (before)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const auto v = load_vec<float, 4>(halves + (((wave ^ kBlocks) * 4 + n) * 64 + lane) * 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[4 * n + e] += v[e];
+                }
+            auto pair_frag = [&](int r, int s) { return *reinterpret_cast<const frag_t<T>*>(pairs_at<T>(pairs, place, 4 * r + 2 * s + half)); };
             Values<T> shown = values;
             if (!finite) {
                 // A pair that the mask hides is 0, but 0 x Inf is NaN in a product of tiles: token by token, for those that see it.
 #pragma unroll 1
-                for (int r = 0; r < kChunk; ++r)
+                for (int r = 0; r < kChunk; ++r) {
+                    const int tr = r >> 5;
+                    if (tr != mine && mine != kSeesBoth) continue;
+                    float scale = 1.0f;
+                    if constexpr (kNarrow<T>) scale = 1.0f / pair_scales[tr == mine ? tr : 2];
 #pragma unroll
-                    for (int tile = 0; tile < 3; ++tile) {
-                        const int tt = tile_t(tile), tr = tile_r(tile);
-                        if ((r >> 5) != tr) continue;
-                        float scale = 1.0f;
-                        if constexpr (kNarrow<T>) scale = 1.0f / pair_scales[tile];
-                        const int place = tt * 32 + (lane & 31);
+                    for (int n = 0; n < 4; ++n) {
+                        if ((r >> 4) != n) continue;
+                        frag_t<T> one = values.z[n];
 #pragma unroll
-                        for (int s = 0; s < 2; ++s) {
-                            if (((r >> 4) & 1) != s) continue;
-                            frag_t<T> one = values.z[2 * tr + s];
+                        for (int e = 0; e < 8; ++e)
+                            if (Weights<1>::row(e) != (r & 15)) one[e] = static_cast<T>(0.0f);
+                        const acc_t term = multiply<T>(one, pair_frag(n / 2, n % 2), acc_t(0.0f));
 #pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                if (Weights::row(e) != (r & 15)) one[e] = static_cast<T>(0.0f);
-                            const acc_t term = multiply<T>(one, pair_frag(tt, tr, s), acc_t(0.0f));
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) within[tt][i] = (REVERSE ? r >= place : r <= place) ? fmaf(term[i], scale, within[tt][i]) : within[tt][i];
-                        }
+                        for (int i = 0; i < 16; ++i) within[i] = (REVERSE ? r >= place : r <= place) ? fmaf(term[i], scale, within[i]) : within[i];
                     }
+                }
 #pragma unroll
                 for (int s = 0; s < 4; ++s) shown.z[s] = frag_t<T>(static_cast<T>(0.0f));
             }
-            frag_t<T> seen_pairs[3][2];
+            frag_t<T> seen_pairs[2][2], own[2];
 #pragma unroll
-            for (int tile = 0; tile < 3; ++tile)
-#pragma unroll
-                for (int s = 0; s < 2; ++s) seen_pairs[tile][s] = pair_frag(tile_t(tile), tile_r(tile), s);
+            for (int s = 0; s < 2; ++s) {
+                own[s] = mine != 0 ? shown.z[2 + s] : shown.z[s];
+                seen_pairs[0][s] = pair_frag(mine, s);
+                seen_pairs[1][s] = pair_frag(1 - kSeesBoth, s);
+            }
+            // between(i) follows the i-th of two products.
             auto add_pairs = [&](auto&& between) __attribute__((always_inline)) {
-#pragma unroll
-                for (int tile = 0; tile < 3; ++tile) {
-                    const int tt = tile_t(tile), tr = tile_r(tile);
+                auto scaled = [&](int tile, auto&& add) __attribute__((always_inline)) {
                     float scale = 1.0f;
                     if constexpr (kNarrow<T>) {
                         scale = pair_scales[tile];
-                        if (scale != 1.0f) within[tt] *= scale;
+                        if (scale != 1.0f) within *= scale;
                     }
+                    add();
+                    if constexpr (kNarrow<T>)
+                        if (scale != 1.0f) within *= 1.0f / scale;
+                };
+                scaled(mine, [&]() __attribute__((always_inline)) {
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
-                        within[tt] = multiply<T>(shown.z[2 * tr + s], seen_pairs[tile][s], within[tt]);
-                        between(2 * tile + s);
-                        slot_end();
+                        within = multiply<T>(own[s], seen_pairs[0][s], within);
+                        between(s);
                     }
-                    if constexpr (kNarrow<T>)
-                        if (scale != 1.0f) within[tt] *= 1.0f / scale;
-                }
+                });
+                if (mine == kSeesBoth)
+                    scaled(2, [&]() __attribute__((always_inline)) {
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) within = multiply<T>(shown.z[2 * (1 - kSeesBoth) + s], seen_pairs[1][s], within);
+                    });
             };
             if (!update) {
-                add_pairs([&](int i) __attribute__((always_inline)) { share_of(4, i, 6, [&](int n) __attribute__((always_inline)) { store_tiles(no, n, buffer); }); });
+                add_pairs([&](int i) __attribute__((always_inline)) { share_of(kPieces, i, 2, store_x); });
 #pragma unroll
-                for (int g = 0; g < 4; ++g) store_output(g, o, within, since, out_each, row0, length);
+                for (int g = 0; g < 2; ++g) store_output(g, o, within, since, out_each, row0, length);
                 continue;
             }
-            Weighted<T, 2> weighted[2];
-            frag_t<T> rows[2][K];
+            Weighted<T, 2> weighted[kShares<T> ? 1 : 2];
+            frag_t<T> rows[2][K], shared[2][2];
             const int swapped = anew(swapped_at);
-            read_rows_of<T, W>(rows[0], y_tile, swapped, 0);
-            slot_end();
+            // Step s of what the matrix gets: Y's columns and, where it is shared, the weighted Z.
+            auto read = [&](int s) __attribute__((always_inline)) {
+                read_rows_of<T, W>(rows[s % 2], y_tile, swapped, s);
+                if constexpr (kShares<T>)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) shared[s % 2][n] = *reinterpret_cast<const frag_t<T>*>(weighted_z + ((2 * s + n) * 64 + lane) * 8);
+            };
+            read(0);
             add_pairs([&](int i) __attribute__((always_inline)) {
-                share_of(8, i, 6, [&](int n) __attribute__((always_inline)) { weighted[0].step(n, values.z[0], weights.w[0], up); });
+                if constexpr (!kShares<T>)
+                    share_of(8, i, 2, [&](int n) __attribute__((always_inline)) { weighted[0].step(n, values.z[0], weights.w[0], up); });
             });
-            buffer ^= 1;
+            if constexpr (kYTiles<T> == 2) buffer ^= 1;
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                if (s < 3) read_rows_of<T, W>(rows[(s + 1) % 2], y_tile, swapped, s + 1);
-                add_rows<T, K, 2>(matrix, rows[s % 2], weighted[s % 2], [&](int i, int count) __attribute__((always_inline)) {
-                    if (s < 3)
-                        share_of(8, i, count, [&](int n) __attribute__((always_inline)) { weighted[(s + 1) % 2].step(n, values.z[s + 1], weights.w[s + 1], up); });
+                if (s < 3) read(s + 1);
+                auto operand = [&](int n) __attribute__((always_inline)) {
+                    if constexpr (kShares<T>) return shared[s % 2][n];
+                    else return weighted[s % 2].operand(n);
+                };
+                add_rows<T, K, 2>(matrix, rows[s % 2], operand, [&](int i, int count) __attribute__((always_inline)) {
+                    if constexpr (!kShares<T>)
+                        if (s < 3)
+                            share_of(8, i, count, [&](int n) __attribute__((always_inline)) { weighted[(s + 1) % 2].step(n, values.z[s + 1], weights.w[s + 1], up); });
                     if (s >= 1)
-                        share_of(12, (s - 1) * count + i, 3 * count, [&](int n) __attribute__((always_inline)) { store_tiles(yes, n, buffer); });
+                        share_of(kPieces, (s - 1) * count + i, 3 * count, [&](int n) __attribute__((always_inline)) {
+                            store_x(n);
+                            store_z(n);
+                            if constexpr (kYTiles<T> == 2) store_y(n);
+                        });
                     if constexpr (!REVERSE)
                         if (s == 3)
-                            share_of(4, i, count, [&](int n) __attribute__((always_inline)) { store_output(n, o, within, since, out_each, row0, length); });
+                            share_of(2, i, count, [&](int n) __attribute__((always_inline)) { store_output(n, o, within, since, out_each, row0, length); });
                 });
             }
             bring_back<T, K>(matrix, up);
+            if constexpr (kYTiles<T> == 1) {
+                __syncthreads();  // Y has been read
+#pragma unroll
+                for (int n = 0; n < kPieces; ++n) store_y(n);
+            }
         }
         if constexpr (REVERSE)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) store_output(g, o, within, since, out, row0, length);
+            for (int g = 0; g < 2; ++g) store_output(g, o, within, since, out, row0, length);
     }
 }
 
@@ -807,9 +850,11 @@ __device__ __forceinline__ const float* carry_of(const float* stored, const floa
 // A segment's own matrix: what its tokens leave to those behind it (k v') or, reverse, before it (q dO' of the group's heads). The last one's goes
 // to `after` as its last token sees it, the first one's to d_before, each where the caller asked for it; a sequence's only one with what is passed
 // on through it.
-template <typename T, int W, bool STAGED>
+template <typename T, int W, bool STAGED, int HALVES>
 __device__ __forceinline__ void sum_segment(const LinearArgs& a, bool reverse, int pair, int segment, T* lds) {
-    constexpr int K = W / 32;
+    constexpr int kBlocks = W / 32, K = kBlocks / HALVES;
+    using In = Incoming<T, W, STAGED, W * 2 * HALVES>;
+    constexpr int kPieces = In::kPieces;
     const int b = pair / a.hkv, kv = pair % a.hkv, d = a.d, tokens = a.tokens;
     const bool outermost = segment == (reverse ? 0 : a.segments - 1);
     const long matrix_size = static_cast<long>(d) * d;
@@ -821,9 +866,9 @@ __device__ __forceinline__ void sum_segment(const LinearArgs& a, bool reverse, i
     } else {
         to += (static_cast<long>(pair) * a.segments + segment) * matrix_size;
     }
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), column_block = wave % kBlocks, first_row = wave / kBlocks * 32 * K;
     const float l = log2_decay(a.log_decay[kv]);
-    Weights weights(l, reverse ? a.scale : 1.0f, reverse, kChunk);
+    Weights<4> weights(l, reverse ? a.scale : 1.0f, reverse, kChunk);
     const float largest_weight = reverse ? a.scale * power(l, 1) : 1.0f;
     const int heads = reverse ? a.hq : a.hkv, heads_each = reverse ? a.hq / a.hkv : 1;
     const long stride = static_cast<long>(heads) * d;
@@ -836,11 +881,11 @@ __device__ __forceinline__ void sum_segment(const LinearArgs& a, bool reverse, i
     const int first_chunk = segment * a.segment_chunks, last_chunk = min(first_chunk + a.segment_chunks, (tokens + kChunk - 1) / kChunk) - 1;
     const int steps = (last_chunk - first_chunk + 1) * heads_each;  // a chunk's heads one after the other
     auto row_of = [&](int step) { return (reverse ? last_chunk - step / heads_each : first_chunk + step / heads_each) * kChunk; };
-    Incoming<T, W, STAGED> in_y(stride, d), in_z(stride, d);
+    In in_y(stride, d), in_z(stride, d);
     auto turn_to = [&](int step) __attribute__((always_inline)) {
-        const long along = static_cast<long>(step % heads_each) * d;
-        in_y.set(Rows<T>{y_base + along, stride}, row_of(step), tokens, d);
-        in_z.set(Rows<T>{z_base + along, stride}, row_of(step), tokens, d);
+        const long further = static_cast<long>(step % heads_each) * d;
+        in_y.set(Rows<T>{y_base + further, stride}, row_of(step), tokens, d);
+        in_z.set(Rows<T>{z_base + further, stride}, row_of(step), tokens, d);
     };
     auto fetch = [&](int i) __attribute__((always_inline)) {
         in_y.fetch(i);
@@ -851,12 +896,12 @@ __device__ __forceinline__ void sum_segment(const LinearArgs& a, bool reverse, i
         in_y.store(i, tiles, tokens, d, a.vectors);
         in_z.store(i, tiles + kTile<T, W>, tokens, d, a.vectors);
     };
-    const int swapped_at = swapped_offset<T, W>();
+    const int swapped_at = along<T>(swapped_offset<T, W>(), first_row);
     turn_to(0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) fetch(i);
+    for (int i = 0; i < kPieces; ++i) fetch(i);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) store_tiles(i, 0);
+    for (int i = 0; i < kPieces; ++i) store_tiles(i, 0);
     for (int step = 0; step < steps; ++step) {
         const T* tiles = lds + (step & 1) * 2 * kTile<T, W>;
         const int row0 = row_of(step), length = min(kChunk, tokens - row0);
@@ -867,30 +912,29 @@ __device__ __forceinline__ void sum_segment(const LinearArgs& a, bool reverse, i
         frag_t<T> rows[2][K];
         Weighted<T, 3> weighted[2];
         const int swapped = anew(swapped_at);
-        values.template load<W>(tiles + kTile<T, W>, wave);
+        values.template load<W>(tiles + kTile<T, W>, column_block);
         read_rows_of<T, W>(rows[0], tiles, swapped, 0);
         if (step % heads_each == 0) {
             const float passed = power(l, end);
 #pragma unroll
             for (int k = 0; k < K; ++k) matrix[k] *= passed;
         }
-        if (!reverse && end != kChunk) weights = Weights(l, 1.0f, false, end);
+        if (!reverse && end != kChunk) weights = Weights<4>(l, 1.0f, false, end);
         const float up = enlarge<T, K>(matrix, values, largest_weight);
 #pragma unroll
         for (int i = 0; i < 8; ++i) weighted[0].step(i, values.z[0], weights.w[0], up);
-        slot_end();
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             if (s < 3) read_rows_of<T, W>(rows[(s + 1) % 2], tiles, swapped, s + 1);
-            add_rows<T, K, 3>(matrix, rows[s % 2], weighted[s % 2], [&](int i, int count) __attribute__((always_inline)) {
-                if (s == 0) share_of(4, i, count, fetch);
+            add_rows<T, K, 3>(matrix, rows[s % 2], [&](int n) { return weighted[s % 2].operand(n); }, [&](int i, int count) __attribute__((always_inline)) {
+                if (s == 0) share_of(kPieces, i, count, fetch);
                 if (s < 3) share_of(8, i, count, [&](int n) __attribute__((always_inline)) { weighted[(s + 1) % 2].step(n, values.z[s + 1], weights.w[s + 1], up); });
-                if (s == 3) share_of(4, i, count, [&](int n) __attribute__((always_inline)) { store_tiles(n, step + 1); });
+                if (s == 3) share_of(kPieces, i, count, [&](int n) __attribute__((always_inline)) { store_tiles(n, step + 1); });
             });
         }
         bring_back<T, K>(matrix, up);
     }
-    const int column = wave * 32 + (lane & 31);
+    const int column = column_block * 32 + (lane & 31);
     const float* given = a.segments > 1 ? nullptr : reverse ? a.d_after : a.before;
     if (given != nullptr) given += pair * matrix_size;
     const float passed = power(l, tokens);
@@ -898,16 +942,16 @@ __device__ __forceinline__ void sum_segment(const LinearArgs& a, bool reverse, i
     for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const int row = 32 * k + matrix_row(i);
+            const int row = first_row + 32 * k + matrix_row(i);
             if (row < d && column < d) to[row * d + column] = given != nullptr ? fmaf(given[row * d + column], passed, matrix[k][i]) : matrix[k][i];
         }
 }
 
 // The outputs; behind them, where a sequence is one segment, the last states.
 template <typename T, int W, bool STAGED>
-__global__ __launch_bounds__(W * 2, 1) void linear_forward_kernel(LinearArgs a) {
+__global__ __launch_bounds__((kWalkThreads<T, W>), (W == 64 ? 2 : 1)) void linear_forward_kernel(LinearArgs a) {
     const unsigned int group = a.hq / a.hkv, members = group / a.heads_each, units = a.batch * a.hkv * a.segments;
-    if (blockIdx.x >= units * members) return sum_segment<T, W, STAGED>(a, false, static_cast<int>(blockIdx.x - units * members), 0, shared_memory<T>());
+    if (blockIdx.x >= units * members) return sum_segment<T, W, STAGED, 2>(a, false, static_cast<int>(blockIdx.x - units * members), 0, shared_memory<T>());
     const Unit u = unit_of(blockIdx.x, members, units, a.segments);
     const int b = u.pair / a.hkv, kv = u.pair % a.hkv;
     Task<T> task;
@@ -929,9 +973,9 @@ __global__ __launch_bounds__(W * 2, 1) void linear_forward_kernel(LinearArgs a) 
 // dk and dv of all units first, whose walks are as many times longer as a group has heads, then dq; behind them, where a sequence is one segment, the
 // gradients of the first states.
 template <typename T, int W, bool STAGED>
-__global__ __launch_bounds__(W * 2, 1) void linear_backward_kernel(LinearArgs a) {
+__global__ __launch_bounds__((kWalkThreads<T, W>), (W == 64 ? 2 : 1)) void linear_backward_kernel(LinearArgs a) {
     const unsigned int group = a.hq / a.hkv, members = group / a.heads_each, units = a.batch * a.hkv * a.segments;
-    if (blockIdx.x >= units * (members + 2)) return sum_segment<T, W, STAGED>(a, true, static_cast<int>(blockIdx.x - units * (members + 2)), 0, shared_memory<T>());
+    if (blockIdx.x >= units * (members + 2)) return sum_segment<T, W, STAGED, 2>(a, true, static_cast<int>(blockIdx.x - units * (members + 2)), 0, shared_memory<T>());
     Task<T> task;
     const T *q = static_cast<const T*>(a.q), *k = static_cast<const T*>(a.k), *v = static_cast<const T*>(a.v), *dout = static_cast<const T*>(a.dout);
     if (blockIdx.x < 2 * units) {
@@ -971,7 +1015,7 @@ __global__ __launch_bounds__(W * 2, 1) void linear_backward_kernel(LinearArgs a)
 // Every segment's own matrix; blockIdx.y = 1: reverse.
 template <typename T, int W, bool STAGED>
 __global__ __launch_bounds__(W * 2, 2) void linear_segments_kernel(LinearArgs a) {
-    sum_segment<T, W, STAGED>(a, blockIdx.y == 1, static_cast<int>(blockIdx.x / a.segments), static_cast<int>(blockIdx.x % a.segments), shared_memory<T>());
+    sum_segment<T, W, STAGED, 1>(a, blockIdx.y == 1, static_cast<int>(blockIdx.x / a.segments), static_cast<int>(blockIdx.x % a.segments), shared_memory<T>());
 }
 
 // The segments' matrices become what comes before each (blockIdx.y = 0) or behind it (1), in order along the sequence, a thread an element.
@@ -1168,7 +1212,7 @@ void cut(LinearArgs& a, int most, bool backward, bool fp32) {
 }
 
 template <typename T, int W>
-constexpr int kWalkBytes = (4 * kTile<T, W> + kChunk * kPairsPitch<T>) * static_cast<int>(sizeof(T));
+constexpr int kWalkBytes = ((2 + kYTiles<T>) * kTile<T, W> + kChunk * kPairsPitch<T>) * static_cast<int>(sizeof(T)) + kWalkThreads<T, W> * 16 * 4 + (kShares<T> ? W / 32 * 8192 : 0);
 template <typename T, int W>
 constexpr int kSegmentBytes = 4 * kTile<T, W> * static_cast<int>(sizeof(T));
 
@@ -1206,10 +1250,10 @@ int run(LinearArgs& a, bool backward, hipStream_t stream) {
     const long units = pairs * a.segments, members = a.hq / a.hkv / a.heads_each, states = state_too ? pairs : 0;
     if (backward) {
         if (int st = allow_shared<linear_backward_kernel<T, W, STAGED>>(kWalkBytes<T, W>)) return st;
-        hipLaunchKernelGGL((linear_backward_kernel<T, W, STAGED>), dim3(static_cast<unsigned int>(units * (members + 2) + states)), dim3(W * 2), (kWalkBytes<T, W>), stream, a);
+        hipLaunchKernelGGL((linear_backward_kernel<T, W, STAGED>), dim3(static_cast<unsigned int>(units * (members + 2) + states)), dim3((kWalkThreads<T, W>)), (kWalkBytes<T, W>), stream, a);
     } else {
         if (int st = allow_shared<linear_forward_kernel<T, W, STAGED>>(kWalkBytes<T, W>)) return st;
-        hipLaunchKernelGGL((linear_forward_kernel<T, W, STAGED>), dim3(static_cast<unsigned int>(units * members + states)), dim3(W * 2), (kWalkBytes<T, W>), stream, a);
+        hipLaunchKernelGGL((linear_forward_kernel<T, W, STAGED>), dim3(static_cast<unsigned int>(units * members + states)), dim3((kWalkThreads<T, W>)), (kWalkBytes<T, W>), stream, a);
     }
     CGPTX_LAUNCH_CHECK();
     return CGPTX_OK;
