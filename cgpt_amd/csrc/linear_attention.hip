@@ -245,8 +245,7 @@ struct Values {
         for (int s = 0; s < 4; ++s)
             if (s >= first && s < first + count) z[s] = column_frag<T, W>(tile, 16 * s, column_block);
     }
-    // 16-bit storage: the largest magnitude's bits in each half of a word. (Dot products with constants are one instruction for two instead of two, but
-    // let Infs and NaNs get lost here.)
+    // 16-bit storage: the largest magnitude's bits in each half of a word.
     __device__ __forceinline__ unsigned int largest_bits() const {
         using Halves = vec_t<unsigned short, 2>;
         Halves most(static_cast<unsigned short>(0));
@@ -1019,8 +1018,8 @@ __global__ __launch_bounds__(W * 2, 2) void linear_segments_kernel(LinearArgs a)
 }
 
 // The segments' matrices become what comes before each (blockIdx.y = 0) or behind it (1), in order along the sequence, a thread an element.
-// What it waits for is the loads: 32 at a time in workgroups of one wavefront (128 segments of 4 matrices of 64 x 64: the call takes 66 us, with
-// 8 at a time in workgroups of four 71, with 64 at a time 118).
+// What it waits for is the loads: 32 at a time in workgroups of one wavefront (128 segments of 4 matrices of 64 x 64: the call takes 68 us, with
+// 8 at a time in workgroups of four 74, with 64 at a time 120).
 constexpr int kAhead = 32, kJoinThreads = 64;
 __global__ __launch_bounds__(kJoinThreads) void linear_join_kernel(LinearArgs a) {
     const bool reverse = blockIdx.y == 1;
@@ -1191,12 +1190,12 @@ LinearArgs make_args(const Shape& s, const void* q, const void* k, const void* v
 
 // Cuts the sequences into at most `most` segments of whole chunks, and says how many of a group's query heads a workgroup takes one after the other.
 // Walks that give three compute units of four work are not cut: two segments each would need their matrices first (32 sequences of 1024 tokens,
-// 8 query and 2 kv heads of 128: 58 us forward and 168 backward, cut in two 93 and 223). Then every query head has a workgroup of its own;
+// 8 query and 2 kv heads of 128: 57 us forward and 173 backward, cut in two 96 and 235). Then every query head has a workgroup of its own;
 // where sequences have to be cut, a group's heads share what is done for k and v, unless that leaves units without work (backward has three
-// walks a segment then: 5 sequences of 1001 half precision tokens, 12 and 4 heads of 64: 48 us, heads apart 58). Segments are two chunks or
-// longer in 16-bit storage; in fp32, whose products take longer than what a segment costs, one (2 sequences of 333 tokens, 4 heads of 40: 36 us
-// forward, two chunks or longer 53). Two a unit where the tokens allow it (32768 tokens, 12 and 4 heads of 64: 66 and 145 us, one a unit
-// 72 and 148).
+// walks a segment then: 5 sequences of 1001 half precision tokens, 12 and 4 heads of 64: 46 us, heads apart 52). Segments are two chunks or
+// longer in 16-bit storage (of one chunk: 77 tokens 15 us instead of 9); in fp32, whose products take longer than what a segment costs, one
+// (2 sequences of 333 tokens, 4 heads of 40: 29 us forward, two chunks or longer 41). Two a unit where the tokens allow it (32768 tokens, 12 and 4
+// heads of 64, forward: 68 us, one a unit 72).
 void cut(LinearArgs& a, int most, bool backward, bool fp32) {
     const int chunks = (a.tokens + kChunk - 1) / kChunk, group = a.hq / a.hkv;
     const long pairs = static_cast<long>(a.batch) * a.hkv, units = compute_units();
