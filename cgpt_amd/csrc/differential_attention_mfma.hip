@@ -177,7 +177,8 @@ __device__ __forceinline__ bool not_finite(const T* tile, int from) {
             const auto words = *reinterpret_cast<const vec_t<unsigned int, 4>*>(tile + ((half * (W / 16) + i) * kWave + (threadIdx.x & 63)) * 8);
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const pair x = __builtin_bit_cast(pair, words[w]), zeros(static_cast<T>(0.0f));
+                const unsigned int word = words[w];  // (a bit cast of words[w] itself is compiled as one of words[0])
+                const pair x = __builtin_bit_cast(pair, word), zeros(static_cast<T>(0.0f));
                 if constexpr (__is_same(T, f16_t)) sum = __builtin_amdgcn_fdot2(x, zeros, sum, false);
                 else sum = __builtin_amdgcn_fdot2_f32_bf16(x, zeros, sum, false);
             }
