@@ -593,8 +593,8 @@ int validate(const char* name, std::size_t rows, std::size_t hidden, std::size_t
     if (rows == 0 || hidden == 0) return fail(CGPTX_INVALID_ARGUMENT, n + ": empty shape");
     if ((gate == nullptr) != (gate_rows == 0) || (gate_rows != 0 && rows % gate_rows != 0))
         return fail(CGPTX_INVALID_ARGUMENT, n + ": the gate must have one row for every equal number of rows, or none");
-    constexpr std::size_t limit = std::size_t{1} << 30;
-    if (rows > limit || hidden > limit) return fail(CGPTX_INVALID_ARGUMENT, n + ": dimensions exceed supported range");
+    // The second launch has 1024 threads for sixteen columns: 2^31 along an axis, which may have fewer than 2^32.
+    if (rows > std::size_t{1} << 30 || hidden > std::size_t{1} << 25) return fail(CGPTX_INVALID_ARGUMENT, n + ": dimensions exceed supported range");
     return CGPTX_OK;
 }
 

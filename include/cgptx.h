@@ -463,7 +463,7 @@ int cgptx_linear_attention_step(
  *   stream_output = residual_scale*stream_input + gate*rmsnorm(branch)*branch_weight,  normed = rmsnorm(stream_output)*norm_weight,
  * rows of `hidden` values, rmsnorm(x) = x/sqrt(mean(x^2) + eps); the second norm reads stream_output as it is stored. gate
  * [gate_rows, hidden]: one row for all rows (a learned vector), one for each, or one for every rows/gate_rows rows in turn (a sequence's);
- * NULL with gate_rows 0: no gate. stream_output may be stream_input. */
+ * NULL with gate_rows 0: no gate. stream_output may be stream_input. At most 2^30 rows and 2^25 columns. */
 int cgptx_sandwich_norm_forward(
     void* stream_output, void* normed, const void* stream_input,
     const void* branch, const void* branch_weight, const void* gate,

@@ -63,11 +63,11 @@ BAD_SIZES = [dict(batch=0), dict(hq=0), dict(hkv=0), dict(hq=3, hkv=2), dict(d=0
     ("cgptx_sandwich_norm_forward", norm(gates=0)),
     ("cgptx_sandwich_norm_forward", norm(gates=3)),
     *[("cgptx_sandwich_norm_forward", norm(**s)) for s in (dict(rows=0), dict(hidden=0), dict(scale=NAN), dict(scale=-INF), dict(eps=0.0), dict(eps=-1.0),
-                                                         dict(eps=NAN), dict(eps=INF), dict(dtype=9), dict(rows=2**31), dict(hidden=2**31))],
+                                                         dict(eps=NAN), dict(eps=INF), dict(dtype=9), dict(rows=2**31), dict(hidden=2**25 + 1))],
     *[("cgptx_sandwich_norm_backward", norm_backward(i)) for i in (0, 1, 2, 4, 6, 7, 8, 9, 10, 11)],
     ("cgptx_sandwich_norm_backward", norm_backward(10, gates=0)),                # a gate's gradient without a gate
     ("cgptx_sandwich_norm_backward", norm_backward(gates=3)),
-    *[("cgptx_sandwich_norm_backward", norm_backward(**s)) for s in (dict(rows=0), dict(hidden=0), dict(scale=NAN), dict(eps=0.0), dict(dtype=9))],
+    *[("cgptx_sandwich_norm_backward", norm_backward(**s)) for s in (dict(rows=0), dict(hidden=0), dict(scale=NAN), dict(eps=0.0), dict(dtype=9), dict(hidden=2**25 + 1))],
 ])
 def test_invalid_arguments(name, args):
     with pytest.raises((ValueError, OverflowError)):
