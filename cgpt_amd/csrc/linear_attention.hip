@@ -734,29 +734,31 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
                 seen_pairs[0][s] = pair_frag(mine, s);
                 seen_pairs[1][s] = pair_frag(1 - kSeesBoth, s);
             }
-            // between(i) follows the i-th of two products.
+            // between(i) follows the i-th of two products. Half precision: a tile's products, whose scale may be anything up to 2^123 where all its pairs
+            // have decayed, are added up apart; `within` itself keeps its range.
             auto add_pairs = [&](auto&& between) __attribute__((always_inline)) {
                 auto scaled = [&](int tile, auto&& add) __attribute__((always_inline)) {
-                    float scale = 1.0f;
                     if constexpr (kNarrow<T>) {
-                        scale = pair_scales[tile];
-                        if (scale != 1.0f) within *= scale;
+                        acc_t sum(0.0f);
+                        add(sum);
+                        const float back = 1.0f / pair_scales[tile];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) within[i] = fmaf(sum[i], back, within[i]);
+                    } else {
+                        add(within);
                     }
-                    add();
-                    if constexpr (kNarrow<T>)
-                        if (scale != 1.0f) within *= 1.0f / scale;
                 };
-                scaled(mine, [&]() __attribute__((always_inline)) {
+                scaled(mine, [&](acc_t& sum) __attribute__((always_inline)) {
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
-                        within = multiply<T>(own[s], seen_pairs[0][s], within);
+                        sum = multiply<T>(own[s], seen_pairs[0][s], sum);
                         between(s);
                     }
                 });
                 if (mine == kSeesBoth)
-                    scaled(2, [&]() __attribute__((always_inline)) {
+                    scaled(2, [&](acc_t& sum) __attribute__((always_inline)) {
 #pragma unroll
-                        for (int s = 0; s < 2; ++s) within = multiply<T>(shown.z[2 * (1 - kSeesBoth) + s], seen_pairs[1][s], within);
+                        for (int s = 0; s < 2; ++s) sum = multiply<T>(shown.z[2 * (1 - kSeesBoth) + s], seen_pairs[1][s], sum);
                     });
             };
             if (!update) {

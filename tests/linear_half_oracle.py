@@ -1,0 +1,94 @@
+"""Bounds of linear attention in half precision that follow the decays, head by head and chunk by chunk of 64 tokens. linear_oracle.py bounds scores and
+matrices by the largest there are, undecayed, which is loose over long sequences and strong decays.
+
+What half precision leaves of an operand, beside its half step u that linear_oracle.py counts: a tile's scores and a wavefront's part of the matrix C are
+brought to 2^-3 or more by their largest, so 2^-25 absolute is 2^-22 of that,
+  2^-22 max|P| sum |z_r| over the chunk's tokens that are seen,  2^-22 max|C| sum |x_t| since;
+the weighted z are brought to 2^14 or more by the chunk's largest z times its largest weight, in two parts, by at most 2^30: 2^-39 of that
+largest, or 2^-55, times sum |y_r|, decaying with the matrix. All of it twice rounded: times 1 + 2^-6."""
+import math
+
+import torch
+
+from tests import linear_oracle
+from tests.linear_oracle import Sum, half_step, heads_first, pairs_sum, product, rows_of
+
+CHUNK = 64
+
+
+def decays(log_decay, n):
+    return torch.exp(torch.clamp(log_decay.double(), max=0.0, min=-1e4).view(-1, 1) * n.double())
+
+
+def half_slack(x, y, z, carry, log_decay, scale, reverse):
+    """[batch, query heads, tokens, width of z]; magnitudes in, log_decay of every query head."""
+    tokens, device = x.shape[2], x.device
+    one = torch.ones(1, device=device)
+    g = decays(log_decay, one).view(1, -1, 1)
+    out_scale, matrix_scale = (1.0, scale) if reverse else (scale, 1.0)
+    matrix = torch.zeros((*x.shape[:2], y.shape[3], z.shape[3]), dtype=torch.float64, device=device)
+    if carry is not None:
+        matrix = matrix + carry * (1.0 if reverse else g[..., None])
+    lost = torch.zeros(matrix.shape[:3], dtype=torch.float64, device=device)
+    slack = torch.zeros((*x.shape[:3], z.shape[3]), dtype=torch.float64, device=device)
+    starts = range(0, tokens, CHUNK)
+    for first in reversed(starts) if reverse else starts:
+        rows = slice(first, min(first + CHUNK, tokens))
+        xs, ys, zs = x[:, :, rows], y[:, :, rows], z[:, :, rows]
+        n = xs.shape[2]
+        at = torch.arange(n, device=device)
+        since = decays(log_decay, n - 1 - at if reverse else at)[None]
+        largest = matrix.amax((2, 3))[..., None]
+        of_matrix = out_scale * since * (2.0 ** -22 * largest * xs.sum(-1) + (xs * lost[:, :, None]).sum(-1))
+        apart = at.view(1, -1) - at.view(-1, 1) if reverse else at.view(-1, 1) - at.view(1, -1)
+        seen = (apart >= 0).double()
+        w = seen * decays(log_decay, apart.clamp(min=0).reshape(-1)).view(-1, n, n)
+        scores = (scale * w * product(xs, ys.transpose(2, 3))).amax((2, 3))[..., None, None]
+        slack[:, :, rows] = 2.0 ** -22 * scores * product(seen.expand(*xs.shape[:2], n, n), zs) + of_matrix[..., None]
+        weights = matrix_scale * decays(log_decay, at + 1 if reverse else CHUNK - at)[None, ..., None]
+        passed = decays(log_decay, one * n).view(1, -1, 1)
+        left = 2.0 ** -39 * zs.amax((2, 3))[..., None] * (matrix_scale * g if reverse else 1.0) + 2.0 ** -55
+        lost = passed * lost + left * ys.sum(2)
+        matrix = passed[..., None] * matrix + product(ys.transpose(2, 3), weights * zs)
+    return slack * (1 + 2.0 ** -6)
+
+
+def half_sum(x, y, z, carry, log_decay, group, scale, carry_scale, reverse, grouped):
+    more = (log_decay, group, scale, carry_scale, reverse, torch.float32, grouped)
+    size = (x.abs(), y.abs(), z.abs(), None if carry is None else carry.abs())
+    sums, a, u = pairs_sum(x, y, z, carry, *more), pairs_sum(*size, *more).value, half_step(torch.float16)
+    slack = half_slack(*size, log_decay.repeat_interleave(group), scale, reverse)
+    if grouped:
+        slack = slack.view(x.shape[0], -1, group, *slack.shape[2:]).sum(2)
+    return Sum(sums.value, sums.error + (u * (1 + 2.0 ** -6) + 2.0 ** -22) * a + u * sums.value.abs() + 2.0 ** -25 + slack)
+
+
+def linear_forward(q, k, v, log_decay, before, scale):
+    want = linear_oracle.linear_forward(q, k, v, log_decay, before, scale)
+    if q.dtype == torch.float16:
+        group = q.shape[2] // k.shape[2]
+        scale = scale if scale > 0 else 1 / math.sqrt(q.shape[3])
+        each = None if before is None else before.double().repeat_interleave(group, dim=1)
+        want["out"] = rows_of(half_sum(heads_first(q), heads_first(k, group), heads_first(v, group), each, log_decay, group, scale, scale, False, False))
+    return want
+
+
+def linear_backward(q, k, v, log_decay, before, dout, d_after, scale):
+    want = linear_oracle.linear_backward(q, k, v, log_decay, before, dout, d_after, scale)
+    if q.dtype != torch.float16:
+        return want
+    group = q.shape[2] // k.shape[2]
+    scale = scale if scale > 0 else 1 / math.sqrt(q.shape[3])
+    qh, kh, vh, do = heads_first(q), heads_first(k, group), heads_first(v, group), heads_first(dout)
+
+    def each(t, parts=1, transposed=False):
+        if t is None:
+            return None
+        t = t.double().repeat_interleave(group, dim=1) / parts
+        return t.transpose(2, 3) if transposed else t
+
+    more = (log_decay, group, scale)
+    want["dq"] = rows_of(half_sum(do, vh, kh, each(before, transposed=True), *more, scale, False, False))
+    want["dv"] = rows_of(half_sum(kh, qh, do, each(d_after, group), *more, 1.0, True, True))
+    want["dk"] = rows_of(half_sum(vh, do, qh, each(d_after, group, True), *more, 1.0, True, True))
+    return want

@@ -1,0 +1,41 @@
+"""Linear attention where numbers come to the ends of their ranges: decays that leave next to nothing, large values beside small ones, and what is not
+finite behind them (linear_half_oracle.py has half precision's bounds)."""
+import pytest
+import torch
+
+from tests.linear_half_oracle import linear_backward, linear_forward
+from tests.linear_oracle import check
+from tests.test_gpu_linear_attention import GRADS, backward, case, forward, inputs
+from tests.util import DTYPE_IDS, DTYPES, randn
+
+pytestmark = pytest.mark.gpu
+STRONG = [-40.0, -70.0, -75.0, -78.0, -80.0, -82.0, -83.0, -84.0, -85.0, -86.0, -87.0]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=DTYPE_IDS)
+@pytest.mark.parametrize("decay", STRONG, ids=str)
+def test_scores_that_have_all_but_decayed(device, decay, dtype):
+    """Tokens 32 to 63 of a chunk see those before them with a weight of 2^-58 to 2^-126, beside values and gradients of thousands."""
+    c = case(2, 130, 4, 2, 64, decay=[decay])
+    q, k, v, dout, log_decay, before, d_after = inputs(c, dtype, device)
+    v, dout = v * 1000, dout * 100
+    want = {**linear_forward(q, k, v, log_decay, before, 0.0), **linear_backward(q, k, v, log_decay, before, dout, d_after, 0.0)}
+    check(forward(c, q, k, v, log_decay, before)[0], want["out"], "out")
+    for name, got in zip(GRADS[:3], backward(c, q, k, v, dout, log_decay, before, d_after)):
+        check(got, want[name], name)
+    there = tuple((randn(t.shape, dtype, 50 + i) * 1000).to(device) for i, t in enumerate((q, k, v)))
+    grads = backward(c, q, k, v, dout, log_decay, before, d_after, tuple(t.clone() for t in there) + (torch.zeros_like(before),), True)
+    step = max(torch.finfo(dtype).eps / 2, 2.0 ** -24)
+    for name, got, was in zip(GRADS[:3], grads, there):
+        want[name].value += was.double()
+        want[name].error += step * (was.double().abs() + want[name].value.abs())
+        check(got, want[name], name)
+
+
+@pytest.mark.parametrize("decay", [-60.0, -80.0, -82.0, -84.0, -86.0])
+def test_equal_values_under_strong_decays(device, decay):
+    """Keys and queries of ones, values of 512 in half precision: every output is 8 x 512, to a half step of the score, the values' parts and the result."""
+    c = case(1, 200, 2, 1, 64, decay=[decay])
+    q, k, v = (torch.full((1, 200, heads, 64), value, dtype=torch.float16, device=device) for heads, value in ((2, 1.0), (1, 1.0), (1, 512.0)))
+    out, after = forward(c, q, k, v, torch.tensor([decay], device=device), None)
+    assert (out == 4096).all() and (after == 512).all()
