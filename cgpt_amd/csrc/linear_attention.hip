@@ -355,14 +355,36 @@ __device__ __forceinline__ void share_of(int all, int i, int count, Step&& step)
         if (n * count / all == i) step(n);
 }
 // Half precision: values are weighted at the upper end of its range (the two parts of one that is 2^-17 of the largest still leave 2^-22 of it), the
-// matrix along with them until it is brought back; not by more than 2^30, which fp32 has room for.
+// matrix along with them until it is brought back.
 template <typename T, int K>
-__device__ __forceinline__ float enlarge(acc_t (&matrix)[K], const Values<T>& values, float largest_weight) {
-    if constexpr (!kNarrow<T>) return 1.0f;
-    const float up = fminf(range_scale(values.largest() * largest_weight, 14, 15), 0x1p30f);
-    if (up != 1.0f)
+__device__ __forceinline__ void enlarge(acc_t (&matrix)[K], float up) {
+    if (kNarrow<T> && up != 1.0f)
 #pragma unroll
         for (int k = 0; k < K; ++k) matrix[k] *= up;
+}
+// For outputs in half precision: by the largest value times the largest weight, and not by more than 2^30, which fp32 has room for.
+template <typename T, int K>
+__device__ __forceinline__ float enlarge_by_values(acc_t (&matrix)[K], const Values<T>& values, float largest_weight) {
+    if constexpr (!kNarrow<T>) return 1.0f;
+    const float up = fminf(range_scale(values.largest() * largest_weight, 14, 15), 0x1p30f);
+    enlarge<T, K>(matrix, up);
+    return up;
+}
+// For matrices that are stored: by the largest weighted value, however small (a chunk whose last values are zeros, weights that begin below 2^-30).
+// `size`, what the matrix cannot exceed, leaves it room: 64 values of less than 2^16 each add 2^22 times the largest weighted one at most.
+template <typename T, int K>
+__device__ __forceinline__ float enlarge_by_products(acc_t (&matrix)[K], float& size, const Values<T>& values, const Weights<4>& weights) {
+    if constexpr (!kNarrow<T>) return 1.0f;
+    const float largest = largest_finite([&](auto&& use) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) use(to_f32(values.z[s][e]) * weights.w[s][e]);
+    });
+    const float room = __uint_as_float(__float_as_uint(0x1p120f / size) & 0x7F800000u);  // a power of two, 2^-6 or more
+    const float up = fminf(range_scale(largest, 14, 15), room);
+    size = fminf(fmaf(largest, 0x1p22f, size), 0x1p126f);
+    enlarge<T, K>(matrix, up);
     return up;
 }
 template <typename T, int K>
@@ -683,7 +705,7 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
                 for (int n = 0; n < 3 * kPieces; ++n) fetch(n);
             }
             const bool finite = !__any(!values.finite());
-            const float up = update ? enlarge<T, K>(matrix, values, largest_weight) : 1.0f;
+            const float up = update ? enlarge_by_values<T, K>(matrix, values, largest_weight) : 1.0f;
             if (kShares<T> && update)
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
@@ -870,7 +892,7 @@ __device__ __forceinline__ void sum_segment(const LinearArgs& a, bool reverse, i
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), column_block = wave % kBlocks, first_row = wave / kBlocks * 32 * K;
     const float l = log2_decay(a.log_decay[kv]);
     Weights<4> weights(l, reverse ? a.scale : 1.0f, reverse, kChunk);
-    const float largest_weight = reverse ? a.scale * power(l, 1) : 1.0f;
+    float size = 0.0f;
     const int heads = reverse ? a.hq : a.hkv, heads_each = reverse ? a.hq / a.hkv : 1;
     const long stride = static_cast<long>(heads) * d;
     const T* y_base = static_cast<const T*>(reverse ? a.q : a.k) + static_cast<long>(b) * tokens * stride + static_cast<long>(kv) * heads_each * d;
@@ -917,11 +939,12 @@ __device__ __forceinline__ void sum_segment(const LinearArgs& a, bool reverse, i
         read_rows_of<T, W>(rows[0], tiles, swapped, 0);
         if (step % heads_each == 0) {
             const float passed = power(l, end);
+            size *= passed;
 #pragma unroll
             for (int k = 0; k < K; ++k) matrix[k] *= passed;
         }
         if (!reverse && end != kChunk) weights = Weights<4>(l, 1.0f, false, end);
-        const float up = enlarge<T, K>(matrix, values, largest_weight);
+        const float up = enlarge_by_products<T, K>(matrix, size, values, weights);
 #pragma unroll
         for (int i = 0; i < 8; ++i) weighted[0].step(i, values.z[0], weights.w[0], up);
 #pragma unroll

@@ -39,3 +39,36 @@ def test_equal_values_under_strong_decays(device, decay):
     q, k, v = (torch.full((1, 200, heads, 64), value, dtype=torch.float16, device=device) for heads, value in ((2, 1.0), (1, 1.0), (1, 512.0)))
     out, after = forward(c, q, k, v, torch.tensor([decay], device=device), None)
     assert (out == 4096).all() and (after == 512).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=DTYPE_IDS)
+@pytest.mark.parametrize("b,t", [(2, 60), (1, 700)], ids=str)
+@pytest.mark.parametrize("decay", [-15.0, -30.0, -50.0], ids=str)
+def test_stored_matrices_of_small_weights(device, decay, b, t, dtype):
+    """The first state's gradient, of which g to the first power is the largest weight."""
+    c = case(b, t, 4, 2, 64, decay=[decay])
+    q, k, v, dout, log_decay, before, _ = inputs(c, dtype, device)
+    check(backward(c, q, k, v, dout, log_decay, before, None)[3], linear_backward(q, k, v, log_decay, before, dout, None, 0.0)["d_before"], "d_before")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=DTYPE_IDS)
+@pytest.mark.parametrize("b,t", [(2, 60), (1, 700)], ids=str)
+@pytest.mark.parametrize("decay", [-0.5, -1.0], ids=str)
+def test_stored_matrices_behind_zeros(device, decay, b, t, dtype):
+    """A sequence whose last values are zeros, as a padded one's are: what its tokens leave has decayed over all of them."""
+    c = case(b, t, 4, 2, 64, states=False, decay=[decay])
+    q, k, v, _, log_decay, _, _ = inputs(c, dtype, device)
+    v[:, -50:] = 0
+    check(forward(c, q, k, v, log_decay, None)[1], linear_forward(q, k, v, log_decay, None, 0.0)["after"], "after")
+
+
+@pytest.mark.parametrize("t", [60, 700])
+def test_stored_matrices_of_uneven_heads(device, t):
+    """Heads of a group whose largest weighted gradients lie 2^130 apart: the larger ones keep their range where the small ones are enlarged."""
+    c = case(1, t, 2, 1, 64, states=False, scale=64.0, decay=[-1.1])
+    q, k, v, dout, log_decay, _, _ = inputs(c, torch.float16, device)
+    q, dout = q * 4000, dout * 4000
+    dout[:, :, 1] = 0
+    dout[:, 58:60, 1] = 2.0 ** -24
+    before = torch.zeros((1, 1, 64, 64), device=device)
+    check(backward(c, q, k, v, dout, log_decay, before, None)[3], linear_backward(q, k, v, log_decay, before, dout, None, 64.0)["d_before"], "d_before")
