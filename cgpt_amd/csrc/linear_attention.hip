@@ -516,10 +516,11 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
     const int tile = min(wave, 2), tile_t = tile == 2 ? kSeesBoth : tile, tile_r = tile == 2 ? 1 - kSeesBoth : tile;
     acc_t table;
     unsigned int seen[8];  // bfloat16: masks of two elements each
+    constexpr float kHidden = __is_same(T, bf16_t) ? 0.0f : -1.0f;  // a weight that is seen may round to 0, but is never below it
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int t = tile_t * 32 + (lane & 31), r = tile_r * 32 + acc_row(i), far = REVERSE ? r - t : t - r;
-        table[i] = far >= 0 ? task.pair_scale * power(l, far) : 0.0f;
+        table[i] = far >= 0 ? task.pair_scale * power(l, far) : kHidden;
         if (i % 2 == 0) seen[i / 2] = 0;
         if (far >= 0) seen[i / 2] |= i % 2 == 0 ? 0xFFFFu : 0xFFFF0000u;
     }
@@ -611,7 +612,7 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
                     if (s + AHEAD < STEPS) read(s + AHEAD);
                     p = multiply<T>(ys[s % (AHEAD + 1)], xs[s % (AHEAD + 1)], p);
                 }
-                // What the mask hides is 0 whatever the scores are.
+                // What the mask hides is 0 whatever the scores are; what has decayed to 0 is not where they are not finite.
                 if constexpr (__is_same(T, bf16_t)) {
                     p *= table;
                 } else {
@@ -619,7 +620,7 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
                     for (int i = 0; i < 16; ++i) {
                         float weight = table[i];
                         asm volatile("" : "+v"(weight));  // compared anew: no registers for sixteen masks
-                        p[i] = weight != 0.0f ? p[i] * weight : 0.0f;
+                        p[i] = weight < 0.0f ? 0.0f : p[i] * weight;
                     }
                 }
                 if constexpr (kNarrow<T>) {

@@ -72,3 +72,43 @@ def test_stored_matrices_of_uneven_heads(device, t):
     dout[:, 58:60, 1] = 2.0 ** -24
     before = torch.zeros((1, 1, 64, 64), device=device)
     check(backward(c, q, k, v, dout, log_decay, before, None)[3], linear_backward(q, k, v, log_decay, before, dout, None, 64.0)["d_before"], "d_before")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=DTYPE_IDS)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")], ids=str)
+@pytest.mark.parametrize("decay", [-3.0, -30.0, -87.5, -float("inf")], ids=str)
+@pytest.mark.parametrize("t", [150, 700])
+def test_what_is_not_finite_and_has_decayed(device, t, decay, bad, dtype):
+    """It reaches every token behind it (backward: in front of it) and the state, also those whose weight for it rounds to nothing, and no other token."""
+    c = case(1, t, 2, 1, 64, decay=[decay])
+    q, k, v, dout, log_decay, before, d_after = inputs(c, dtype, device)
+    want = {**linear_forward(q, k, v, log_decay, before, 0.0), **linear_backward(q, k, v, log_decay, before, dout, d_after, 0.0)}
+
+    def spoilt(got, name, at):
+        m = torch.zeros_like(got, dtype=torch.bool)
+        m[at] = True
+        assert not torch.isfinite(got[m]).any(), name
+        assert bool(((got.double() - want[name].value).abs() <= want[name].error)[~m].all()), name
+
+    for t0 in (3, 40, 70):
+        for at, of_out, of_state in (((0, t0, 0, 5), (0, slice(t0, None)), (0, 0, 5)), ((0, t0, 0, 5), (0, slice(t0, None), slice(None), 5), (0, 0, slice(None), 5))):
+            key = of_state == (0, 0, 5)
+            broken = (k if key else v).clone()
+            broken[at] = bad
+            out, after = forward(c, q, broken if key else k, v if key else broken, log_decay, before)
+            spoilt(out, "out", of_out)
+            spoilt(after, "after", of_state)
+        broken = q.clone()
+        broken[0, t0, 1, 5] = bad
+        dq, dk, dv, d_before = backward(c, broken, k, v, dout, log_decay, before, d_after)
+        spoilt(dq, "dq", (0, slice(0, 0)))
+        spoilt(dk, "dk", (0, slice(0, t0 + 1), 0, 5))
+        spoilt(dv, "dv", (0, slice(0, t0 + 1), 0))
+        spoilt(d_before, "d_before", (0, 0, 5))
+        broken = dout.clone()
+        broken[0, t0, 1, 5] = bad
+        dq, dk, dv, d_before = backward(c, q, k, v, broken, log_decay, before, d_after)
+        spoilt(dq, "dq", (0, t0, 1))
+        spoilt(dk, "dk", (0, slice(0, t0 + 1), 0))
+        spoilt(dv, "dv", (0, slice(0, t0 + 1), 0, 5))
+        spoilt(d_before, "d_before", (0, 0, slice(None), 5))
