@@ -362,11 +362,12 @@ __device__ __forceinline__ void enlarge(acc_t (&matrix)[K], float up) {
 #pragma unroll
         for (int k = 0; k < K; ++k) matrix[k] *= up;
 }
-// For outputs in half precision: by the largest value times the largest weight, and not by more than 2^30, which fp32 has room for.
+// For outputs in half precision: by the largest value times the largest weight, and not by more than 2^30, or than a state at the end of fp32's
+// range leaves: matrix_scale has brought the matrix below 2^15, and a group's heads add less than 2^92 where they are enlarged at all.
 template <typename T, int K>
-__device__ __forceinline__ float enlarge_by_values(acc_t (&matrix)[K], const Values<T>& values, float largest_weight) {
+__device__ __forceinline__ float enlarge_by_values(acc_t (&matrix)[K], float matrix_scale, const Values<T>& values, float largest_weight) {
     if constexpr (!kNarrow<T>) return 1.0f;
-    const float up = fminf(range_scale(values.largest() * largest_weight, 14, 15), 0x1p30f);
+    const float up = fminf(range_scale(values.largest() * largest_weight, 14, 15), fminf(0x1p110f * matrix_scale, 0x1p30f));
     enlarge<T, K>(matrix, up);
     return up;
 }
@@ -580,7 +581,7 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
     for (int step = 0; step < steps; ++step) {
         const int row0 = row_of(step), length = min(kChunk, tokens - row0);
         acc_t o, within;  // by what came before the chunk, and by its own tokens
-        float since;
+        float since, matrix_scale = 1.0f;
         for (int each = 0; each < heads_each; ++each) {
             const T* y_tile = y_tiles + buffer * kTile<T, W>;
             const bool last_each = each + 1 == heads_each, update = REVERSE || last_each, before = !REVERSE || each == 0;
@@ -649,7 +650,6 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
             if (before) {
                 constexpr int STEPS = W / 32;
                 const int rows_at = along<T>(at, mine * 16 * STEPS);
-                float matrix_scale = 1.0f;
                 if constexpr (kNarrow<T>) matrix_scale = range_scale(largest_of(matrix), -3, 15);
                 const float passed = update ? power(l, length) : 1.0f;
                 frag_t<T> xs[AHEAD + 1][2], m[2];
@@ -706,7 +706,7 @@ __device__ __forceinline__ void walk_segment(const LinearArgs& a, const Task<T>&
                 for (int n = 0; n < 3 * kPieces; ++n) fetch(n);
             }
             const bool finite = !__any(!values.finite());
-            const float up = update ? enlarge_by_values<T, K>(matrix, values, largest_weight) : 1.0f;
+            const float up = update ? enlarge_by_values<T, K>(matrix, matrix_scale, values, largest_weight) : 1.0f;
             if (kShares<T> && update)
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {

@@ -4,8 +4,9 @@ matrices by the largest there are, undecayed, which is loose over long sequences
 What half precision leaves of an operand, beside its half step u that linear_oracle.py counts: a tile's scores and a wavefront's part of the matrix C are
 brought to 2^-3 or more by their largest, so 2^-25 absolute is 2^-22 of that,
   2^-22 max|P| sum |z_r| over the chunk's tokens that are seen,  2^-22 max|C| sum |x_t| since;
-the weighted z are brought to 2^14 or more by the chunk's largest z times its largest weight, in two parts, by at most 2^30: 2^-39 of that
-largest, or 2^-55, times sum |y_r|, decaying with the matrix. All of it twice rounded: times 1 + 2^-6."""
+the weighted z are brought to 2^14 or more by the chunk's largest z times its largest weight, in two parts, by at most 2^30 and by no more than leaves
+2^110 (of a matrix at 2^14) for the matrix they are added to: 2^-39 of that largest, 2^-55, or 2^-149 of the matrix's largest, times sum |y_r|, decaying
+with the matrix. All of it twice rounded: times 1 + 2^-6."""
 import math
 
 import torch
@@ -47,7 +48,7 @@ def half_slack(x, y, z, carry, log_decay, scale, reverse):
         slack[:, :, rows] = 2.0 ** -22 * scores * product(seen.expand(*xs.shape[:2], n, n), zs) + of_matrix[..., None]
         weights = matrix_scale * decays(log_decay, at + 1 if reverse else CHUNK - at)[None, ..., None]
         passed = decays(log_decay, one * n).view(1, -1, 1)
-        left = 2.0 ** -39 * zs.amax((2, 3))[..., None] * (matrix_scale * g if reverse else 1.0) + 2.0 ** -55
+        left = 2.0 ** -39 * zs.amax((2, 3))[..., None] * (matrix_scale * g if reverse else 1.0) + 2.0 ** -55 + 2.0 ** -148 * largest
         lost = passed * lost + left * ys.sum(2)
         matrix = passed[..., None] * matrix + product(ys.transpose(2, 3), weights * zs)
     return slack * (1 + 2.0 ** -6)

@@ -112,3 +112,15 @@ def test_what_is_not_finite_and_has_decayed(device, t, decay, bad, dtype):
         spoilt(dk, "dk", (0, slice(0, t0 + 1), 0))
         spoilt(dv, "dv", (0, slice(0, t0 + 1), 0, 5))
         spoilt(d_before, "d_before", (0, 0, slice(None), 5))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=DTYPE_IDS)
+def test_states_at_the_end_of_the_range(device, dtype):
+    """A first state (and a last one's gradient) of 2^120, which 0.4 a token brings back to outputs that half precision holds behind 270 tokens of 400.
+    More sequences than compute units, so that none is cut."""
+    c = case(130, 400, 2, 2, 32, decay=[-0.4 * 0.6931471805599453])
+    q, k, v, dout, log_decay, before, d_after = inputs(c, dtype, device)
+    before, d_after = before.sign() * 2.0 ** 120, d_after.sign() * 2.0 ** 120
+    want = {**linear_forward(q, k, v, log_decay, before, 0.0), **linear_backward(q, k, v, log_decay, before, dout, d_after, 0.0)}
+    for name, got in zip(("out", "after", *GRADS), (*forward(c, q, k, v, log_decay, before), *backward(c, q, k, v, dout, log_decay, before, d_after))):
+        check(got, want[name], name)
