@@ -124,3 +124,19 @@ def test_states_at_the_end_of_the_range(device, dtype):
     want = {**linear_forward(q, k, v, log_decay, before, 0.0), **linear_backward(q, k, v, log_decay, before, dout, d_after, 0.0)}
     for name, got in zip(("out", "after", *GRADS), (*forward(c, q, k, v, log_decay, before), *backward(c, q, k, v, dout, log_decay, before, d_after))):
         check(got, want[name], name)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("t,hq,hkv,d,decay", [(4097, 2, 1, 64, -0.01), (1025, 4, 2, 128, -1e-3), (8000, 3, 1, 40, -0.1)], ids=str)
+def test_long_sequences_in_the_2_norm(device, t, hq, hkv, d, decay, dtype):
+    """Scores, the matrix and the result are rounded once, each by at most a half step u of terms whose signs are random, so that their sum's 2-norm is the
+    terms': 3 u, and the decayed values' 2^-16. What a chunk, a segment or a join adds wrongly would show at several per cent of an output."""
+    c = case(1, t, hq, hkv, d, decay=[decay])
+    q, k, v, dout, log_decay, before, d_after = inputs(c, dtype, device)
+    want = {**linear_forward(q, k, v, log_decay, before, 0.0), **linear_backward(q, k, v, log_decay, before, dout, d_after, 0.0)}
+    tolerance = 3 * torch.finfo(dtype).eps / 2 + 2.0 ** -16
+    for name, got in zip(("out", "after", *GRADS), (*forward(c, q, k, v, log_decay, before), *backward(c, q, k, v, dout, log_decay, before, d_after))):
+        check(got, want[name], name)
+        for rows in (slice(0, 64), slice(64, t // 2), slice(t // 2, None)) if got.shape[1] == t else (slice(None),):
+            off = (got[:, rows].double() - want[name].value[:, rows]).norm() / want[name].value[:, rows].norm()
+            assert off <= tolerance, f"{name}, {rows}: {off:.3g} of its norm, allowed {tolerance:.3g}"
