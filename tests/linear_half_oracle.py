@@ -6,13 +6,14 @@ brought to 2^-3 or more by their largest, so 2^-25 absolute is 2^-22 of that,
   2^-22 max|P| sum |z_r| over the chunk's tokens that are seen,  2^-22 max|C| sum |x_t| since;
 the weighted z are brought to 2^14 or more by the chunk's largest z times its largest weight, in two parts, by at most 2^30 and by no more than leaves
 2^110 (of a matrix at 2^14) for the matrix they are added to: 2^-39 of that largest, 2^-55, or 2^-149 of the matrix's largest, times sum |y_r|, decaying
-with the matrix. All of it twice rounded: times 1 + 2^-6."""
+with the matrix. Matrices that are stored: 2^-39 of the chunk's largest weighted z, or 2^-145 of what the matrix cannot exceed (2^22 times the sum of
+those largest), times sum |y_r|, decaying. All of it twice rounded: times 1 + 2^-6."""
 import math
 
 import torch
 
 from tests import linear_oracle
-from tests.linear_oracle import Sum, half_step, heads_first, pairs_sum, product, rows_of
+from tests.linear_oracle import Sum, half_step, heads_first, matrix_sum, pairs_sum, product, rows_of
 
 CHUNK = 64
 
@@ -64,13 +65,44 @@ def half_sum(x, y, z, carry, log_decay, group, scale, carry_scale, reverse, grou
     return Sum(sums.value, sums.error + (u * (1 + 2.0 ** -6) + 2.0 ** -22) * a + u * sums.value.abs() + 2.0 ** -25 + slack)
 
 
+def half_matrix(y, z, ahead, log_decay, group, scale, reverse):
+    """A stored matrix, of tokens and a group's heads; the bound is linear_oracle.matrix_sum's with these terms for its last one."""
+    tokens, device, more = y.shape[2], y.device, (log_decay, group, scale, reverse)
+    sums = matrix_sum(y, z, ahead, *more, torch.float32)
+    size = (y.abs(), z.abs(), None if ahead is None else ahead.abs())
+    a = matrix_sum(*size, *more, torch.float32).value
+    each = log_decay.repeat_interleave(group) if reverse else log_decay
+    lost = torch.zeros(y.shape[:2] + y.shape[3:], dtype=torch.float64, device=device)
+    room = torch.zeros((*y.shape[:2], 1), dtype=torch.float64, device=device)
+    starts = range(0, tokens, CHUNK)
+    for first in reversed(starts) if reverse else starts:
+        rows = slice(first, min(first + CHUNK, tokens))
+        ys, zs = size[0][:, :, rows], size[1][:, :, rows]
+        n = ys.shape[2]
+        at = torch.arange(n, device=device)
+        end = n - 1 if not reverse and rows.stop == tokens else n  # what is stored is the matrix as the last token sees it
+        w = (scale if reverse else 1.0) * decays(each, at + 1 if reverse else end - at)
+        largest = (w[None, ..., None] * zs).amax((2, 3))[..., None]
+        passed = decays(each, torch.full((1,), end, device=device)).view(1, -1, 1)
+        room = passed * room
+        if reverse:  # of the heads before, which are added to the same matrix
+            room = room.view(room.shape[0], -1, group, 1).sum(2).repeat_interleave(group, 1)
+        lost = passed * lost + (2.0 ** -39 * largest + 2.0 ** -145 * room) * ys.sum(2)
+        room = room / (group if reverse else 1) + 2.0 ** 22 * largest
+    if reverse:
+        lost = lost.view(lost.shape[0], -1, group, lost.shape[2]).sum(2)
+    return Sum(sums.value, sums.error + 2.0 ** -22 * a + (1 + 2.0 ** -6) * lost[..., None])
+
+
 def linear_forward(q, k, v, log_decay, before, scale):
     want = linear_oracle.linear_forward(q, k, v, log_decay, before, scale)
     if q.dtype == torch.float16:
         group = q.shape[2] // k.shape[2]
         scale = scale if scale > 0 else 1 / math.sqrt(q.shape[3])
-        each = None if before is None else before.double().repeat_interleave(group, dim=1)
+        state = None if before is None else before.double()
+        each = None if before is None else state.repeat_interleave(group, dim=1)
         want["out"] = rows_of(half_sum(heads_first(q), heads_first(k, group), heads_first(v, group), each, log_decay, group, scale, scale, False, False))
+        want["after"] = half_matrix(heads_first(k), heads_first(v), state, log_decay, group, 1.0, False)
     return want
 
 
@@ -92,4 +124,5 @@ def linear_backward(q, k, v, log_decay, before, dout, d_after, scale):
     want["dq"] = rows_of(half_sum(do, vh, kh, each(before, transposed=True), *more, scale, False, False))
     want["dv"] = rows_of(half_sum(kh, qh, do, each(d_after, group), *more, 1.0, True, True))
     want["dk"] = rows_of(half_sum(vh, do, qh, each(d_after, group, True), *more, 1.0, True, True))
+    want["d_before"] = half_matrix(qh, do, None if d_after is None else d_after.double(), *more, True)
     return want
