@@ -7,7 +7,10 @@ brought to 2^-3 or more by their largest, so 2^-25 absolute is 2^-22 of that,
 the weighted z are brought to 2^14 or more by the chunk's largest z times its largest weight, in two parts, by at most 2^30 and by no more than leaves
 2^110 (of a matrix at 2^14) for the matrix they are added to: 2^-39 of that largest, 2^-55, or 2^-149 of the matrix's largest, times sum |y_r|, decaying
 with the matrix. Matrices that are stored: 2^-39 of the chunk's largest weighted z, or 2^-145 of what the matrix cannot exceed (2^22 times the sum of
-those largest), times sum |y_r|, decaying. All of it twice rounded: times 1 + 2^-6."""
+those largest), times sum |y_r|, decaying. All of it twice rounded: times 1 + 2^-6.
+
+A matrix instruction aligns products by their operands' exponents, which of a number below 2^-14, half precision's smallest normal one, is that one's: to the
+fp32 terms such operands count as 2^-14."""
 import math
 
 import torch
@@ -20,6 +23,10 @@ CHUNK = 64
 
 def decays(log_decay, n):
     return torch.exp(torch.clamp(log_decay.double(), max=0.0, min=-1e4).view(-1, 1) * n.double())
+
+
+def magnitude(t):
+    return None if t is None else torch.where(t != 0, t.abs().clamp(min=2.0 ** -14), t.abs())
 
 
 def half_slack(x, y, z, carry, log_decay, scale, reverse):
@@ -58,19 +65,20 @@ def half_slack(x, y, z, carry, log_decay, scale, reverse):
 def half_sum(x, y, z, carry, log_decay, group, scale, carry_scale, reverse, grouped):
     more = (log_decay, group, scale, carry_scale, reverse, torch.float32, grouped)
     size = (x.abs(), y.abs(), z.abs(), None if carry is None else carry.abs())
-    sums, a, u = pairs_sum(x, y, z, carry, *more), pairs_sum(*size, *more).value, half_step(torch.float16)
+    value, a, u = pairs_sum(x, y, z, carry, *more).value, pairs_sum(*size, *more).value, half_step(torch.float16)
+    error = pairs_sum(*(magnitude(t) for t in (x, y, z)), size[3], *more).error
     slack = half_slack(*size, log_decay.repeat_interleave(group), scale, reverse)
     if grouped:
         slack = slack.view(x.shape[0], -1, group, *slack.shape[2:]).sum(2)
-    return Sum(sums.value, sums.error + (u * (1 + 2.0 ** -6) + 2.0 ** -22) * a + u * sums.value.abs() + 2.0 ** -25 + slack)
+    return Sum(value, error + (u * (1 + 2.0 ** -6) + 2.0 ** -22) * a + u * value.abs() + 2.0 ** -25 + slack)
 
 
 def half_matrix(y, z, ahead, log_decay, group, scale, reverse):
     """A stored matrix, of tokens and a group's heads; the bound is linear_oracle.matrix_sum's with these terms for its last one."""
     tokens, device, more = y.shape[2], y.device, (log_decay, group, scale, reverse)
-    sums = matrix_sum(y, z, ahead, *more, torch.float32)
     size = (y.abs(), z.abs(), None if ahead is None else ahead.abs())
-    a = matrix_sum(*size, *more, torch.float32).value
+    value, a = (matrix_sum(*t, *more, torch.float32).value for t in ((y, z, ahead), size))
+    error = matrix_sum(magnitude(y), magnitude(z), size[2], *more, torch.float32).error
     each = log_decay.repeat_interleave(group) if reverse else log_decay
     lost = torch.zeros(y.shape[:2] + y.shape[3:], dtype=torch.float64, device=device)
     room = torch.zeros((*y.shape[:2], 1), dtype=torch.float64, device=device)
@@ -91,7 +99,7 @@ def half_matrix(y, z, ahead, log_decay, group, scale, reverse):
         room = room / (group if reverse else 1) + 2.0 ** 22 * largest
     if reverse:
         lost = lost.view(lost.shape[0], -1, group, lost.shape[2]).sum(2)
-    return Sum(sums.value, sums.error + 2.0 ** -22 * a + (1 + 2.0 ** -6) * lost[..., None])
+    return Sum(value, error + 2.0 ** -22 * a + (1 + 2.0 ** -6) * lost[..., None])
 
 
 def linear_forward(q, k, v, log_decay, before, scale):
