@@ -10,7 +10,7 @@
 // so the matrix: for dk and dv a token counts once for every head of the group.
 //
 // A workgroup walks chunks of 64 tokens: in a chunk the pairs are a masked product of tiles, Z'P' with P = (X Y') g^|t-r|, and what came before
-// it is C' X'. The matrix stays in the accumulation registers from chunk to chunk, 32 of its columns a wavefront, and goes as an operand into its
+// it is C' X'. The matrix stays in registers from chunk to chunk, 32 of its columns a wavefront, and goes as an operand into its
 // product as it lies (the columns of Y are read in the order that makes it so). Where there are fewer sequences than compute units, they are cut into
 // segments that workgroups walk side by side: one launch leaves each segment's own matrix, one adds them up along the sequence, and the third starts
 // each segment from there.
@@ -19,6 +19,7 @@
 // brings them into its range where they leave it. The matrix in a walk is fed with the decayed Z in two parts, high and low,
 // and the matrices that are stored (fp32) with three in bfloat16.
 // An Inf or NaN reaches the tokens that see it and no others: chunks that hold one are added up token by token.
+// Times in the comments are medians of passes in a row over three sets of inputs, the variants in turn on one card.
 #include "attention_tiles.hpp"
 
 #include <cmath>
@@ -456,13 +457,14 @@ __device__ __forceinline__ int along(int offset, int columns) {
     return sizeof(T) == 2 ? offset ^ columns : offset + columns;
 }
 
-// The output of one head in one segment. Two wavefronts have the same 32 columns of Z, the matrix and the output, each half of the matrix's rows and half
-// of a chunk's tokens: W/2 x 32 and 32 x 32 in registers. In a chunk: scores of the pairs, by three wavefronts, and what came before it, where
-// each has half of both sums and leaves the other's to it | all is there, X and Z have been read, the next chunk's are on their way (Y has two
-// buffers in 16-bit storage) | products with Z, the matrix, the output | the next chunk is there. What bounds it is how long these steps wait for each
-// other: with a wavefront for both halves a chunk has half the instructions in all and takes as long where 16 chunks follow each other (32
-// sequences of 1024 tokens, heads of 128: 59 us forward, 162 backward; with two 58 and 167), and longer where there are few (77 tokens of
-// half precision: 11 us, with two 9; fp32, 2 x 333 tokens, backward: 37, with two 30).
+// The output of one head in one segment. Two wavefronts have the same 32 columns of Z, the matrix and the output, each half of the matrix's rows and
+// half of a chunk's tokens: W/2 x 32 and 32 x 32 in registers (fp32, whose operands are twice as large, spills 16 to 55 registers of 256). In a
+// chunk: scores of the pairs, by three wavefronts, and what came before it, where each has half of both sums and leaves the other's to it | all is
+// there, X and Z have been read, the next chunk's are on their way (Y has two buffers in 16-bit storage) | products with Z, the matrix, the output |
+// the next chunk is there. What bounds it is how long these steps wait for each other (32 sequences of 1024 tokens, 8 and 2 heads of 128: the matrix
+// cores are busy for 23 per cent of the launch, forward and backward). With a wavefront for both halves a chunk has half the instructions in all and
+// takes as long where 16 chunks follow each other (that case: 61 us forward, 148 backward; with two 62 and 143), and longer where there are few (77
+// tokens of half precision: 11.1 us, with two 9.1; fp32, 2 x 333 tokens, backward: 37, with two 31).
 template <typename T, int W>
 constexpr int kWalkThreads = W * 4;
 template <typename T>
@@ -1044,8 +1046,8 @@ __global__ __launch_bounds__(W * 2, 2) void linear_segments_kernel(LinearArgs a)
 }
 
 // The segments' matrices become what comes before each (blockIdx.y = 0) or behind it (1), in order along the sequence, a thread an element.
-// What it waits for is the loads: 32 at a time in workgroups of one wavefront (128 segments of 4 matrices of 64 x 64: the call takes 68 us, with
-// 8 at a time in workgroups of four 74, with 64 at a time 120).
+// What it waits for is the loads: 32 at a time in workgroups of one wavefront (128 segments of 4 matrices of 64 x 64: the call takes 66 us, with
+// 8 at a time in workgroups of four 71, with 64 at a time 117).
 constexpr int kAhead = 32, kJoinThreads = 64;
 __global__ __launch_bounds__(kJoinThreads) void linear_join_kernel(LinearArgs a) {
     const bool reverse = blockIdx.y == 1;
@@ -1216,12 +1218,14 @@ LinearArgs make_args(const Shape& s, const void* q, const void* k, const void* v
 
 // Cuts the sequences into at most `most` segments of whole chunks, and says how many of a group's query heads a workgroup takes one after the other.
 // Walks that give three compute units of four work are not cut: two segments each would need their matrices first (32 sequences of 1024 tokens,
-// 8 query and 2 kv heads of 128: 57 us forward and 173 backward, cut in two 96 and 235). Then every query head has a workgroup of its own;
+// 8 query and 2 kv heads of 128: 62 us forward and 143 backward, cut in two 94 and 228). Then every query head has a workgroup of its own;
 // where sequences have to be cut, a group's heads share what is done for k and v, unless that leaves units without work (backward has three
-// walks a segment then: 5 sequences of 1001 half precision tokens, 12 and 4 heads of 64: 46 us, heads apart 52). Segments are two chunks or
-// longer in 16-bit storage (of one chunk: 77 tokens 15 us instead of 9); in fp32, whose products take longer than what a segment costs, one
-// (2 sequences of 333 tokens, 4 heads of 40: 29 us forward, two chunks or longer 41). Two a unit where the tokens allow it (32768 tokens, 12 and 4
-// heads of 64, forward: 68 us, one a unit 72).
+// walks a segment then: 5 sequences of 1001 half precision tokens, 12 and 4 heads of 64: 45 us, heads apart 51). Segments are two chunks or
+// longer in 16-bit storage (of one chunk: 77 tokens 15.6 us instead of 9.1); in fp32, whose products take longer than what a segment costs, one
+// (2 sequences of 333 tokens, 4 heads of 40, backward: 31 us, two chunks or longer 44). Two a unit where the tokens allow it (32768 tokens, 12 and 4
+// heads of 64, forward: 66 us, one a unit 71).
+// Backward the rule goes by dq's walks. Those of dk and dv are as many times fewer and longer as a group has heads, and are not cut for that: 256 query heads
+// of 1024 tokens and 128 columns in all take 143 us in groups of four, 250 of eight, 477 of sixteen, 940 of 32.
 void cut(LinearArgs& a, int most, bool backward, bool fp32) {
     const int chunks = (a.tokens + kChunk - 1) / kChunk, group = a.hq / a.hkv;
     const long pairs = static_cast<long>(a.batch) * a.hkv, units = compute_units();

@@ -5,10 +5,10 @@
 //   G = dxs + rs (dy w - xs rs^2 mean(dy w xs)),   dx = a G,   h = gate u G,   df = rf (h - f rf^2 mean(h f)),
 //   dw = sum_rows dy xs rs,  du = sum_rows gate G f rf,  dgate = u sum_rows G f rf (over the rows of a gate)
 //
-// What bounds it is memory: two rows read and two written forward, four and two backward, where the operators one by one would read the
-// stream and the branch again for every norm, gate and sum. A row stays in registers between its sums and its stores (row_vectors.hpp);
-// forward the second norm's sum is taken from the stream as it is stored, backward both norms' first sums in one go and the branch norm's
-// second one when G is known. All sums are fp32; G is not rounded before either gradient.
+// What bounds it is memory: two rows read and two written forward, four and two backward, where the operators one by one would read the stream and
+// the branch again for every norm, gate and sum. A row stays in registers between its sums and its stores (row_vectors.hpp), backward with a part of
+// it in scratch memory where it is wide (see RowPlan); forward the second norm's sum is taken from the stream as it is stored, backward both norms'
+// first sums in one go and the branch norm's second one when G is known. All sums are fp32; G is not rounded before either gradient.
 // u and gate are constant over the rows of a gate, so one sum of G f rf stands for both their gradients. Workgroups have rows of one gate as
 // a rule (BY_BLOCK); where there are so many gates that most would have few rows, a row's lanes take whole gates one after the other
 // (BY_SLOT), and write the gate's gradient themselves. Per-workgroup partial sums go to scratch and a second launch adds them in a fixed order.
@@ -563,7 +563,11 @@ struct RowPlan {
         slots = L::kSlots;
         threads = L::kThreadsHere;
     }
-    // Up to 16 values of a row in a lane where one wavefront has it (backward holds eleven of each), 8 or 16 where several do.
+    // Up to 16 values of a row in a lane. Backward holds eleven of each: 250 registers at 16 values, two wavefronts a SIMD. With eight wavefronts a
+    // row (4097 to 8192 columns) up to 13 registers are spilled, with sixteen (8193 to 16384 in 16-bit storage), which leave a lane 128, 127 to 188:
+    // backward in bfloat16 with one gate, in TB/s of what is read and written, 5.0 at 32768 x 1024, 4.7 at 8192 x 4096, 4.1 at 4096 x 8192, 0.9 at
+    // 2730 x 12288, 1.1 at 2048 x 16384, and 1.7 with the kernels for rows of any length at 1638 x 20480; forward, which spills nothing, 5.4, 5.3,
+    // 5.7, 4.8, 5.1 and 3.8.
     explicit RowPlan(int hidden) {
         const int vectors = (hidden + kVec128<T> - 1) / kVec128<T>;
         if (vectors <= 16) take<16, 1, 1>();
@@ -576,7 +580,9 @@ struct RowPlan {
         else if (vectors <= 2048) take<64, sizeof(T) == 2 ? 16 : 8, sizeof(T) == 2 ? 2 : 4>();
     }
     // How a launch deals its rows out: its workgroups, and which kernel takes them. Lanes take whole gates where there are at least twice as many as
-    // the chip holds workgroups, or where a gate has fewer rows than a workgroup has slots.
+    // the chip holds workgroups, or where a gate has fewer rows than a workgroup has slots. Else a workgroup leaves three rows of partial sums,
+    // however few rows its gate has: many gates of few wide rows pay for that backward (bfloat16: 1000 rows of 4096 in 264 us with a gate each, in 21
+    // with one for all; 32768 of 1024 in 116 with 512 gates, in 84 with 32).
     int deal(Sizes& s, const void* by_block, const void* by_slot, bool* slot) const {
         *slot = s.gates > 1 && (s.per_gate < slots || s.gates >= 2 * resident_blocks(by_block, threads));
         if (*slot) return std::min((s.gates + slots - 1) / slots, resident_blocks(by_slot, threads));

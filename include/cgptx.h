@@ -439,11 +439,14 @@ int cgptx_differential_lambda_forward(float* lambda, const void* query1,
  *   S_t = exp(log_decay) S_{t-1} + k_t v_t',  output_t = s S_t' q_t.
  * log_decay: fp32 [kv_heads] on the device, at most 0 (larger values count as 0; -inf forgets all but the token itself). States are fp32
  * [batch, kv_heads, head_dim (k), head_dim (v)]; initial_state NULL: zeros; final_state, the matrix behind the last token, may be
- * NULL and must not be initial_state. Any head_dim up to 128; attention_scale <= 0 selects 1/sqrt(head_dim). What a token adds
- * to the final state is exact to 2^-22; for the output of 16-bit inputs, scores and states are rounded to 16 bits once where they enter a
- * product and decayed values kept to 2^-16. A token that
- * is not finite reaches itself and the tokens behind it. Long sequences are walked in parts side by side, as many as the scratch arena has room
- * for: recorded where it cannot grow, the call adds in another order. */
+ * NULL and must not be initial_state. head_dim up to 128, batch up to 65535, batch*query_heads up to 2^20, sequence up to 2^30; attention_scale <= 0
+ * selects 1/sqrt(head_dim).
+ * What a token adds to the final state n tokens further on is exact to 2^-22, and to 2^-21 (1 + |n log_decay|) for its weight, of itself. For the
+ * output of 16-bit inputs, scores and states are rounded to 16 bits once where they enter a product and decayed values kept to 2^-16. Half
+ * precision brings scores, states and decayed values into its range by a power of two for all of a tile's: each of them may also be off by 2^-22
+ * (scores, states) or 2^-39 (decayed values, also of the final state) of the tile's largest.
+ * A token that is not finite reaches itself and the tokens behind it. Long sequences are walked in parts side by side, as many as the scratch
+ * arena has room for: recorded where it cannot grow, the call adds in another order. */
 int cgptx_linear_attention_forward(
     void* output, float* final_state, const void* query, const void* key,
     const void* value, const float* log_decay, const float* initial_state,
