@@ -5,7 +5,7 @@ import torch
 
 from tests.linear_half_oracle import linear_backward, linear_forward
 from tests.linear_oracle import check
-from tests.test_gpu_linear_attention import GRADS, backward, case, forward, inputs
+from tests.test_gpu_linear_attention import CASES, GRADS, IDS, backward, case, forward, inputs
 from tests.util import DTYPE_IDS, DTYPES, randn
 
 pytestmark = pytest.mark.gpu
@@ -140,3 +140,11 @@ def test_long_sequences_in_the_2_norm(device, t, hq, hkv, d, decay, dtype):
         for rows in (slice(0, 64), slice(64, t // 2), slice(t // 2, None)) if got.shape[1] == t else (slice(None),):
             off = (got[:, rows].double() - want[name].value[:, rows]).norm() / want[name].value[:, rows].norm()
             assert off <= tolerance, f"{name}, {rows}: {off:.3g} of its norm, allowed {tolerance:.3g}"
+
+
+@pytest.mark.parametrize("c", CASES, ids=IDS)
+def test_half_precision_to_what_the_decays_leave(device, c):
+    q, k, v, dout, log_decay, before, d_after = inputs(c, torch.float16, device)
+    want = {**linear_forward(q, k, v, log_decay, before, c["scale"]), **linear_backward(q, k, v, log_decay, before, dout, d_after, c["scale"])}
+    for name, got in zip(("out", "after", *GRADS), (*forward(c, q, k, v, log_decay, before), *backward(c, q, k, v, dout, log_decay, before, d_after))):
+        check(got, want[name], name)
